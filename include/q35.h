@@ -316,6 +316,112 @@ int q35_attention_core_prefill(const q35_dims* d, const float* q_gate, int32_t l
                                void* stream);
 size_t q35_attention_prefill_ws_bytes(const q35_dims* d, int32_t T);
 
+/* ---------------------------------------------------------------- paged caches, token scores */
+
+/* No counterparts in the reference (one sequence, a cache that grows by concatenation, greedy argmax):
+ * for callers that serve several continuations of shared contexts (beam search, several samples of
+ * one prompt, checking drafted tokens, chunks of prompts beside decoding sequences).
+ *
+ * A pool of cache pages of `page` tokens (a power of two, 16..256) for n_layers attention layers:
+ *   data[n_layers][n_pages][2][kv_heads][page][head_dim], plane 0 the keys (after k_norm and RoPE),
+ *   plane 1 the values, 16-byte aligned, in f32, f16 or bf16 (values are rounded to nearest even
+ *   when they are appended; head_dim 256).
+ * A page table is int32 [B][ld_table]: entry c of row b is the page that holds tokens c*page .. of
+ * sequence b, or -1.  A page may stand in several rows (shared contexts); pages that a sequence is
+ * about to append to must stand in its row alone, which q35_pages_fork sees to.
+ *
+ * `status` (optional, NULL: not reported): a zero-initialised device word into which calls OR
+ *   Q35_STATUS_ARG   a device-resident index was out of range (a page, a position, a parent, a token
+ *                    id, a pair that q35_pages_copy refuses): nothing was read or written outside
+ *                    the buffers and what belongs to the index is as each entry point says;
+ *   Q35_STATUS_FULL  q35_pages_fork found no free page for an entry, which is left -1.
+ * q35_status_check synchronises `stream`, reads and clears it: Q35_E_RANGE for the first, Q35_E_NOMEM
+ * for the second alone. */
+enum { Q35_F32 = 0, Q35_F16 = 1, Q35_BF16 = 2 };
+enum { Q35_STATUS_ARG = 1, Q35_STATUS_FULL = 2 };
+typedef struct {
+  void* data;
+  int32_t dtype; /* Q35_F32, Q35_F16 or Q35_BF16 */
+  int32_t n_layers, n_pages, kv_heads, page, head_dim;
+} q35_pages;
+int q35_status_check(uint32_t* status, void* stream);
+
+/* The attention core (q35_attention_core_prefill's arithmetic) for the new tokens of B sequences over
+ * the paged cache of layer `layer`: rows seq_start[b] .. seq_start[b+1]-1 of the T rows are the new
+ * tokens of sequence b (none, one, or any number of them), at positions pos[b] .. ; seq_start is int32
+ * [B+1], non-decreasing from 0, and rows from seq_start[B] on are neither read nor written.  Keys
+ * and values are appended to the sequence's pages, then each new token attends to positions 0 .. its
+ * own.  q_gate [T][ld_qg] (per head [query | gate]), k_new and v_new [T][kv_ld], out [T][ld_out],
+ * f32, rows 16-byte aligned; rope_cos / rope_sin [rope_rows][rot_dim].  attn_heads / kv_heads at
+ * most 16.  A sequence whose positions leave [0, min(ld_table * page, rope_rows)) is skipped, its rows
+ * of out as they were; a page outside the pool is not appended to and its tokens count as page 0's
+ * (Q35_STATUS_ARG: the sequence's outputs are then invalid).  Keys and values in reach must be
+ * finite; what lies behind a sequence's last token in its last page may be anything.
+ * Products and sums are f32 or their equivalent: 16-bit caches are multiplied as they are with
+ * queries and weights carried whole; f32 caches with every value as two f16 halves (22 bits), under
+ * one power of two per group of keys.  The keys' norms are formed in f64, so that what a 16-bit cache
+ * holds does not hang on the order of a sum.
+ * ws: q35_attention_paged_ws_bytes(d, T, B) bytes of scratch, 16-byte aligned (no zeroing needed). */
+size_t q35_attention_paged_ws_bytes(const q35_dims* d, int32_t T, int32_t B);
+int q35_attention_core_paged(const q35_dims* d, q35_pages pool, int32_t layer, const float* q_gate, int32_t ld_qg,
+                             const float* k_new, const float* v_new, int32_t kv_ld, int32_t T,
+                             const int32_t* seq_start, const int32_t* pos, int32_t B, const int32_t* table,
+                             int32_t ld_table, const float* q_norm, const float* k_norm, const float* rope_cos,
+                             const float* rope_sin, int32_t rope_rows, float* out, int32_t ld_out, uint32_t* status,
+                             void* ws, size_t ws_bytes, void* stream);
+
+/* Copies page src_ids[i] of `src` to page dst_ids[i] of `dst`, i < n, in every layer.  The pools
+ * differ in n_pages at most; they may be one pool, else they must not overlap.  A pair with an id
+ * outside its pool, a destination that another pair names too, and in one pool a pair with a page that
+ * is both a source and a destination are not copied (Q35_STATUS_ARG).  ws:
+ * q35_pages_copy_ws_bytes(n) bytes of scratch. */
+size_t q35_pages_copy_ws_bytes(int32_t n);
+int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const int32_t* dst_ids, int32_t n,
+                   uint32_t* status, void* ws, size_t ws_bytes, void* stream);
+
+/* The next page table of a set of sequences: row j of table_out [B_out][ld_table] continues sequence
+ * parent[j] of table [B][ld_table] (len[b] tokens), or is empty for parent[j] = -1, with pages for grow[j]
+ * more tokens (grow NULL: none).  So one call forks (a parent named several times), drops (a
+ * parent not named), frees (-1) and reserves.  Full pages are shared; of a partly filled last page the
+ * first child keeps the page and every other gets a new one with a copy of its tokens, in every
+ * layer.  New pages are those that table_out's kept entries leave unnamed, the lowest first, dealt to
+ * the rows in order; entries behind a row's pages are -1.  len_out[j] is the parent's length, refs
+ * [n_pages] the number of rows of table_out that name each page.  Pages that no row names any more may
+ * be overwritten, the old table is otherwise as it was: table_out must be another buffer, and `table`
+ * must cover every sequence of the pool that is to live on.  A parent outside [-1, B), or one
+ * whose length is negative or more than its row can hold, counts as -1, a kept page outside the pool
+ * becomes -1 and a row is cut at ld_table entries (all Q35_STATUS_ARG); where no page is left the entry
+ * stays -1 (Q35_STATUS_FULL).  B, B_out <= 4096; n_pages <= 262144. */
+int q35_pages_fork(q35_pages pool, const int32_t* table, int32_t ld_table, const int32_t* len, int32_t B,
+                   const int32_t* parent, const int32_t* grow, int32_t B_out, int32_t* table_out, int32_t* len_out,
+                   int32_t* refs, uint32_t* status, void* stream);
+
+/* Moves the pages that `table` [B][ld_table] names to the pool's front, in every layer: with n of them,
+ * the i-th lowest named page >= n goes to the i-th lowest unnamed page < n, and the others stay.
+ * table_out (another buffer) is the table afterwards, refs [n_pages] its counts, *used = n: pages from n
+ * on are free.  An entry outside [-1, n_pages) becomes -1 (Q35_STATUS_ARG).  ws:
+ * q35_pages_compact_ws_bytes(n_pages) bytes of scratch.  n_pages <= 262144. */
+size_t q35_pages_compact_ws_bytes(int32_t n_pages);
+int q35_pages_compact(q35_pages pool, const int32_t* table, int32_t ld_table, int32_t B, int32_t* table_out,
+                      int32_t* refs, int32_t* used, uint32_t* status, void* ws, size_t ws_bytes, void* stream);
+
+/* Scores of M rows of logits [M][ld] over V values (dtype Q35_F32 / _F16 / _BF16; rows need no
+ * alignment beyond the type's), with lse = ln sum e^x:
+ *   logprob[m] = x[targets[m]] - lse;
+ *   rank[m]    = the number of tokens ranked before the target: larger logits, and equal ones of a
+ *                lower id;
+ *   entropy[m] = -sum p ln p (values of -inf contribute nothing);
+ *   top_ids / top_logprobs [M][top]: the `top` (0..64, at most V) highest logits, the lowest id first
+ *                among equal ones, and their x - lse.
+ * targets NULL: no logprob and rank (both may be NULL).  A negative target scores 0 with rank -1
+ * (padding); one >= V gives NaN with rank -1 (Q35_STATUS_ARG).  Rows of -inf alone: logprob -inf,
+ * entropy 0.  A NaN or +inf in a row makes its logprob, entropy and top_logprobs NaN; a NaN ranks
+ * behind every number.  ws: q35_token_logprobs_ws_bytes(M, V, top) bytes of scratch, 16-byte aligned. */
+size_t q35_token_logprobs_ws_bytes(int32_t M, int32_t V, int32_t top);
+int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, int64_t ld, const int32_t* targets,
+                       int32_t top, float* logprob, int32_t* rank, float* entropy, int32_t* top_ids,
+                       float* top_logprobs, uint32_t* status, void* ws, size_t ws_bytes, void* stream);
+
 /* ---------------------------------------------------------------- model level (model.rs, main.rs) */
 
 typedef struct q35_model q35_model;

@@ -1,0 +1,402 @@
+// Scores of rows of logits: log probability and rank of a given token, entropy, highest alternatives.
+//
+// One pass over each row.  With d = x - m (m the running maximum) a lane keeps S = sum e^d and
+// U = sum d e^d of what it has seen; when m rises by c, U becomes (U - c S) e^-c and S becomes S e^-c,
+// so that at the end lse = m + ln S and the entropy is -sum p ln p = ln S - U / S, both from numbers
+// of the size of the result (never as a difference of two lse-sized ones).  The rank of the
+// target counts the values ranked before it in the same pass; its logit is one load at the start.
+//
+// The alternatives: a value and its index make one 64-bit key (the value's bits in ascending order,
+// then the complement of the index), so "larger value, then lower index" is one unsigned comparison
+// and every choice below is exact whatever the order of the work.  A wave keeps its best 64 keys
+// sorted, one per lane; a chunk of values costs one comparison of each lane's maximum with the
+// last wanted key, and only values above it are inserted, one by one.  The first chunk would insert
+// almost everything: the last wanted key starts at the `top`-th of the 64 lanes' maxima instead (that many
+// values are at least as large).
+// Waves, then the splits of a row (blocks), are joined by ranks: a key's place is the number of larger
+// keys.
+#include "pages.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace q35 {
+
+namespace {
+
+constexpr int kT = 256;         // threads per block
+constexpr int kNW = kT / 64;
+constexpr int kPer = 16;        // values of a lane per chunk
+constexpr int kChunk = 64 * kPer;
+constexpr int kMaxSplit = 256;  // blocks per row: the joining block holds one head key per thread
+
+typedef unsigned long long key_t;
+
+struct ScoreArgs {
+  ScoreCall c;
+  int32_t nsplit, len;  // values per split
+  float* stat;          // [M][nsplit][4]: m, S, U, -
+  int32_t* cnt;         // [M][nsplit]: values ranked before the target
+  key_t* keys;          // [M][nsplit][top]
+};
+
+// a float's bits in ascending order; NaN below everything
+Q35_DEV uint32_t asc(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 is 0)
+  return x != x ? 0u : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+Q35_DEV float from_asc(uint32_t a) {
+  return a == 0 ? __uint_as_float(0x7fc00000u) : __uint_as_float((a & 0x80000000u) ? a & 0x7fffffffu : ~a);
+}
+Q35_DEV key_t key_of(float x, int i) { return ((key_t)asc(x) << 32) | (uint32_t)~i; }
+Q35_DEV int key_index(key_t k) { return (int)~(uint32_t)k; }
+
+Q35_DEV key_t lane_key(key_t k, int lane) {
+  return ((key_t)(uint32_t)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)k, lane);
+}
+
+template <int DT>
+Q35_DEV float value(const void* p, int64_t i) {
+  if constexpr (DT == Q35_F32) return ((const Q35_GLOBAL float*)p)[i];
+  if constexpr (DT == Q35_F16) return (float)((const Q35_GLOBAL _Float16*)p)[i];
+  return __uint_as_float((uint32_t)((const Q35_GLOBAL uint16_t*)p)[i] << 16);
+}
+template <int DT>
+Q35_DEV float half_of(uint32_t w, int h) {
+  if constexpr (DT == Q35_F16) return (float)__builtin_bit_cast(_Float16, (uint16_t)(h ? w >> 16 : w));
+  return __uint_as_float(h ? w & 0xffff0000u : w << 16);
+}
+
+// running maximum, sum and weighted sum of a lane
+struct Stat {
+  float m, s, u;
+};
+Q35_DEV float exp_d(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504088896341f); }
+Q35_DEV void stat_join(Stat& a, float m, float s, float u) {
+  const float mn = fmaxf(a.m, m);
+  const float r = mn == -INFINITY ? 0.f : mn;
+  const float da = fmaxf(a.m - r, -1e4f), db = fmaxf(m - r, -1e4f);
+  const float ea = exp_d(da), eb = exp_d(db);
+  a.u = (a.u + da * a.s) * ea + (u + db * s) * eb;
+  a.s = a.s * ea + s * eb;
+  a.m = mn;
+}
+
+// Final numbers of row m of the call.
+Q35_DEV void finish_row(const ScoreCall& c, int m, float mx, double S, double U, int cnt) {
+  const double l = log(S);
+  if (c.entropy) c.entropy[m] = S > 0.0 ? (float)fmax(l - U / S, 0.0) : S == 0.0 ? 0.f : NAN;
+  if (!c.targets) return;
+  const int t = c.targets[m];
+  if (t < 0 || t >= c.V) {
+    c.logprob[m] = t < 0 ? 0.f : NAN;
+    c.rank[m] = -1;
+    if (t >= c.V) raise_status(c.status, Q35_STATUS_ARG);
+    return;
+  }
+  const int64_t o = (int64_t)m * c.ld + t;
+  const float x = c.dtype == Q35_F32 ? value<Q35_F32>(c.x, o) : c.dtype == Q35_F16 ? value<Q35_F16>(c.x, o) : value<Q35_BF16>(c.x, o);
+  c.logprob[m] = mx == -INFINITY && S == 0.0 ? -INFINITY : (float)((double)(x - mx) - l);
+  c.rank[m] = cnt;
+}
+Q35_DEV void put_top(const ScoreCall& c, int m, int i, key_t k, float mx, double S) {
+  const int64_t o = (int64_t)m * c.top + i;
+  c.top_ids[o] = key_index(k);
+  const float x = from_asc((uint32_t)(k >> 32));
+  c.top_lp[o] = mx == -INFINITY && S == 0.0 ? -INFINITY : (float)((double)(x - mx) - log(S));
+}
+
+// Blocks (row, split).
+template <int DT>
+__global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
+  const ScoreCall& c = a.c;
+  __shared__ key_t lists[kNW][kMaxTop];
+  __shared__ float sm[kNW], ss[kNW], su[kNW];
+  __shared__ int sc[kNW];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int m = blockIdx.x / a.nsplit, sp = blockIdx.x % a.nsplit;
+  constexpr int kEs = DT == Q35_F32 ? 4 : 2, kVec = 16 / kEs;  // values of a 16-byte load
+  const char* row = static_cast<const char*>(c.x) + (int64_t)m * c.ld * kEs;
+  // index i of the row is value i + shift of the 16-byte words that begin at or before it
+  const int shift = (int)((reinterpret_cast<uintptr_t>(row) & 15) / kEs);
+  const char* base = row - shift * kEs;
+  const int i0 = sp * a.len, i1 = min(c.V, i0 + a.len);  // the split's values
+  int tgt = -1;
+  float xt = 0.f;
+  if (c.targets) {
+    tgt = c.targets[m];
+    if (tgt >= 0 && tgt < c.V) xt = value<DT>(row, tgt);
+    else tgt = -1;
+  }
+  Stat st = {-INFINITY, 0.f, 0.f};
+  int cnt = 0;
+  key_t best = 0, last = 0;  // the lane's key of the wave's list; the list's top-th key
+  const int top = c.top;
+  const int w_first = (i0 + shift) / kVec, w_end = (i1 + shift + kVec - 1) / kVec;  // words of the split
+  constexpr int kWords = kPer / kVec;
+  bool first = true;
+  for (int w0 = w_first + wid * (kChunk / kVec); w0 < w_end; w0 += kNW * (kChunk / kVec)) {
+    float x[kPer];
+    int idx0[kWords];
+    uint32_t ok = 0;  // which of the values belong to the split
+#pragma unroll
+    for (int g = 0; g < kWords; ++g) {
+      const int w = w0 + g * 64 + lane;
+      const int f = w * kVec - shift;
+      idx0[g] = f;
+      if (f >= i0 && f + kVec <= i1) {
+        const uint4 v = ldg16_nt(base + (int64_t)w * 16);
+        const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          x[g * kVec + j] = DT == Q35_F32 ? __uint_as_float(d[j & 3]) : half_of<DT>(d[(j >> 1) & 3], j & 1);
+        ok |= ((1u << kVec) - 1u) << (g * kVec);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const bool in = f + j >= i0 && f + j < i1;
+          x[g * kVec + j] = in ? value<DT>(row, f + j) : -INFINITY;
+          ok |= (in ? 1u : 0u) << (g * kVec + j);
+        }
+      }
+    }
+    float mx = x[0];
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) mx = fmaxf(mx, x[e]);
+    {
+      const float mn = fmaxf(st.m, mx);
+      const float r = mn == -INFINITY ? 0.f : mn;
+      const float dc = fmaxf(st.m - r, -1e4f), ec = exp_d(dc);
+      st.u = (st.u + dc * st.s) * ec;
+      st.s *= ec;
+      st.m = mn;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const float d = x[e] - r, p = exp_d(d);
+        st.s += p;
+        st.u += fmaxf(d, -1e4f) * p;
+      }
+    }
+    if (tgt >= 0) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) {
+        const int i = idx0[e / kVec] + e % kVec;
+        cnt += (x[e] > xt || (x[e] == xt && i < tgt)) && ((ok >> e) & 1u) ? 1 : 0;
+      }
+    }
+    if (top > 0) {
+      if (first) {  // (uniform in the wave)
+        first = false;
+        key_t lm = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const key_t k = (ok >> e) & 1u ? key_of(x[e], idx0[e / kVec] + e % kVec) : 0;
+          lm = k > lm ? k : lm;
+        }
+        int before = 0;
+        for (int l = 0; l < 64; ++l) before += lane_key(lm, l) > lm ? 1 : 0;
+        const unsigned long long at = __ballot(before == top - 1 && lm != 0);
+        if (at) last = lane_key(lm, (int)__builtin_ctzll(at)) - 1;
+      }
+      if (__ballot(asc(mx) >= (uint32_t)(last >> 32))) {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const key_t k = (ok >> e) & 1u ? key_of(x[e], idx0[e / kVec] + e % kVec) : 0;
+          unsigned long long todo = __ballot(k > last);
+          while (todo) {
+            const int l = (int)__builtin_ctzll(todo);
+            todo &= todo - 1;
+            const key_t cand = lane_key(k, l);
+            if (cand <= last) continue;
+            const int place = __popcll(__ballot(best > cand));
+            const key_t up = __shfl_up(best, 1, 64);
+            best = lane > place ? up : lane == place ? cand : best;
+            const key_t t = lane_key(best, top - 1);
+            last = t > last ? t : last;
+          }
+        }
+      }
+    }
+  }
+  // lanes, then waves
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float om = __shfl_xor(st.m, o, 64), os = __shfl_xor(st.s, o, 64), ou = __shfl_xor(st.u, o, 64);
+    stat_join(st, om, os, ou);
+    cnt += __shfl_xor(cnt, o, 64);
+  }
+  if (lane == 0) {
+    sm[wid] = st.m;
+    ss[wid] = st.s;
+    su[wid] = st.u;
+    sc[wid] = cnt;
+  }
+  if (top > 0) lists[wid][lane] = best;
+  __syncthreads();
+  Stat all = {sm[0], ss[0], su[0]};
+  int n = sc[0];
+#pragma unroll
+  for (int w = 1; w < kNW; ++w) {
+    stat_join(all, sm[w], ss[w], su[w]);
+    n += sc[w];
+  }
+  const int64_t slot = (int64_t)m * a.nsplit + sp;
+  if (tid == 0) {
+    if (a.nsplit == 1) {
+      finish_row(c, m, all.m, (double)all.s, (double)all.u, n);
+    } else {
+      float* o = a.stat + slot * 4;
+      o[0] = all.m;
+      o[1] = all.s;
+      o[2] = all.u;
+      a.cnt[slot] = n;
+    }
+  }
+  if (top > 0 && lane < top) {
+    // the key's place among the block's: its own list's keys before it, and the other lists' larger ones
+    int place = lane;
+    for (int w = 0; w < kNW; ++w) {
+      if (w == wid) continue;
+      int lo = 0, hi = top;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (lists[w][mid] > best) lo = mid + 1;
+        else hi = mid;
+      }
+      place += lo;
+    }
+    if (best != 0 && place < top) {
+      if (a.nsplit == 1) put_top(c, m, place, best, all.m, (double)all.s);
+      else a.keys[slot * top + place] = best;
+    }
+    // a split with fewer values than `top` leaves the rest of its list empty
+    const int have = min(top, i1 - i0);
+    if (a.nsplit > 1 && wid == 0 && lane >= have) a.keys[slot * top + lane] = 0;
+  }
+}
+
+// Block per row: joins its splits.
+__global__ __launch_bounds__(kT) void score_join_kernel(const ScoreArgs a) {
+  const ScoreCall& c = a.c;
+  extern __shared__ key_t cand[];
+  __shared__ key_t heads[kMaxSplit];
+  __shared__ float sm[kT];
+  __shared__ double sS[kNW], sU[kNW];
+  __shared__ int sn[kNW];
+  __shared__ key_t floor_key;
+  __shared__ int ncand;
+  const int m = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, ns = a.nsplit, top = c.top;
+  const float* stat = a.stat + (int64_t)m * ns * 4;
+  const bool in = tid < ns;
+  const float mi = in ? stat[tid * 4] : -INFINITY, si = in ? stat[tid * 4 + 1] : 0.f, ui = in ? stat[tid * 4 + 2] : 0.f;
+  int n = in ? a.cnt[(int64_t)m * ns + tid] : 0;
+  float mx = mi;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
+  if (lane == 0) sm[wid] = mx;
+  if (top > 0) heads[tid] = in ? a.keys[((int64_t)m * ns + tid) * top] : 0;
+  if (tid == 0) {
+    ncand = 0;
+    floor_key = 0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kNW; ++w) mx = fmaxf(mx, sm[w]);
+  const double r = mx == -INFINITY ? 0.0 : (double)mx;
+  const double d = fmax((double)mi - r, -1e4), e = exp(d);
+  double S = (double)si * e, U = ((double)ui + d * (double)si) * e;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    S += __shfl_xor(S, o, 64);
+    U += __shfl_xor(U, o, 64);
+    n += __shfl_xor(n, o, 64);
+  }
+  if (lane == 0) {
+    sS[wid] = S;
+    sU[wid] = U;
+    sn[wid] = n;
+  }
+  if (top > 0) {
+    // `top` of the splits' first keys are at least as large as the top-th of them: nothing below it counts
+    const key_t h = heads[tid];
+    int before = 0;
+    for (int s = 0; s < ns; ++s) before += heads[s] > h ? 1 : 0;
+    if (in && h != 0 && before == top - 1) floor_key = h;
+  }
+  __syncthreads();
+  S = (sS[0] + sS[1]) + (sS[2] + sS[3]);
+  U = (sU[0] + sU[1]) + (sU[2] + sU[3]);
+  n = (sn[0] + sn[1]) + (sn[2] + sn[3]);
+  if (tid == 0) finish_row(c, m, mx, S, U, n);
+  if (top == 0) return;
+  const key_t fl = floor_key;
+  const key_t* ks = a.keys + (int64_t)m * ns * top;
+  for (int q = tid; q < ns * top; q += kT) {
+    const key_t k = ks[q];
+    if (k != 0 && k >= fl) cand[atomicAdd(&ncand, 1)] = k;
+  }
+  __syncthreads();
+  const int nc = ncand;
+  for (int q = tid; q < nc; q += kT) {
+    const key_t k = cand[q];
+    int place = 0;
+    for (int s = 0; s < nc; ++s) place += cand[s] > k ? 1 : 0;
+    if (place < top) put_top(c, m, place, k, mx, S);
+  }
+}
+
+// Blocks per row: enough to fill the chip when rows are few, of one chunk per wave at least.
+int score_split(int M, int V) {
+  const int want = (4 * 256 + M - 1) / M, most = std::min(kMaxSplit, (V + kNW * kChunk - 1) / (kNW * kChunk));
+  return std::max(1, std::min(want, most));
+}
+
+struct ScoreLayout {
+  int nsplit;
+  size_t stat, cnt, keys;
+};
+ScoreLayout score_layout(int M, int V, int top) {
+  ScoreLayout L;
+  L.nsplit = score_split(M, V);
+  const size_t n = L.nsplit > 1 ? (size_t)M * L.nsplit : 0;
+  auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+  L.stat = up(n * 16);
+  L.cnt = up(n * 4);
+  L.keys = up(n * top * 8);
+  return L;
+}
+
+}  // namespace
+
+size_t token_logprobs_ws_bytes(int M, int V, int top) {
+  const ScoreLayout L = score_layout(M, V, top);
+  return L.stat + L.cnt + L.keys;
+}
+
+int token_logprobs_launch(const ScoreCall& c, hipStream_t st) {
+  const ScoreLayout L = score_layout(c.M, c.V, c.top);
+  ScoreArgs a;
+  a.c = c;
+  a.nsplit = L.nsplit;
+  a.len = (c.V + L.nsplit - 1) / L.nsplit;
+  char* ws = static_cast<char*>(c.ws);
+  a.stat = reinterpret_cast<float*>(ws);
+  a.cnt = reinterpret_cast<int32_t*>(ws + L.stat);
+  a.keys = reinterpret_cast<key_t*>(ws + L.stat + L.cnt);
+  const dim3 grid((uint32_t)c.M * L.nsplit);
+  if (c.dtype == Q35_F32) hipLaunchKernelGGL(score_kernel<Q35_F32>, grid, dim3(kT), 0, st, a);
+  else if (c.dtype == Q35_F16) hipLaunchKernelGGL(score_kernel<Q35_F16>, grid, dim3(kT), 0, st, a);
+  else hipLaunchKernelGGL(score_kernel<Q35_BF16>, grid, dim3(kT), 0, st, a);
+  Q35_HIP_TRY(hipGetLastError());
+  if (L.nsplit > 1) {
+    // keys that can reach the list: fewer than `top` splits give all of theirs, else at most `top`
+    // splits have a first key at or above the floor
+    const size_t nc = (size_t)std::min(L.nsplit, c.top) * c.top;
+    hipLaunchKernelGGL(score_join_kernel, dim3(c.M), dim3(kT), nc * sizeof(key_t), st, a);
+    Q35_HIP_TRY(hipGetLastError());
+  }
+  return Q35_OK;
+}
+
+}  // namespace q35

@@ -1,0 +1,415 @@
+// Pages of a cache: copies, forks, compaction.
+//
+// The bookkeeping of a fork or a compaction is whole-number work on tables of a few thousand entries:
+// one block does it with a bitmap of the pool's pages in LDS, so that it needs no host round trip
+// and no order among blocks; every choice (which page is new, which page moves where) is a rank among
+// bits, hence the same on every run.  The pages themselves are then moved by a second launch over
+// the whole chip; a page of one layer is one contiguous run.
+#include "pages.h"
+
+namespace q35 {
+
+namespace {
+
+constexpr int kCT = 256;        // threads of a copying block
+constexpr int kUnit = 16384;    // bytes a block copies at a time: 4 x 16 bytes per thread (the smallest page)
+constexpr int kPT = 1024;       // threads of a bookkeeping block
+constexpr int kPW = kPT / 64;
+
+Q35_DEV void copy_unit(char* dst, const char* src) {
+  const int o = threadIdx.x * 16;
+  uint4 v[kUnit / (16 * kCT)];
+#pragma unroll
+  for (int i = 0; i < kUnit / (16 * kCT); ++i) v[i] = ldg16_nt(src + o + i * 16 * kCT);
+#pragma unroll
+  for (int i = 0; i < kUnit / (16 * kCT); ++i) {
+    const q35_u32x4 w = {v[i].x, v[i].y, v[i].z, v[i].w};
+    __builtin_nontemporal_store(w, (Q35_GLOBAL q35_u32x4*)(dst + o + i * 16 * kCT));
+  }
+}
+
+// ---- copies
+struct CopyArgs {
+  char* src;
+  char* dst;
+  int64_t src_layer, dst_layer, page;  // bytes
+  int32_t src_pages, dst_pages, same, n, units;
+  const int32_t *sid, *did;
+  const uint8_t* ok;  // nullptr: the block checks its pair itself
+  uint32_t* status;
+};
+
+// Pair i is copied if both pages exist, no other pair names its destination and, in one pool, its
+// destination is nobody's source and its source nobody's destination.
+Q35_DEV bool pair_clash(int s, int d, int s2, int d2, int same) { return d2 == d || (same && (s2 == d || d2 == s)); }
+
+// Blocks (pair i, layer, unit of the page).
+__global__ __launch_bounds__(kCT) void pages_copy_kernel(const CopyArgs a) {
+  const int i = blockIdx.x / a.units, u = blockIdx.x % a.units, layer = blockIdx.y;
+  const int s = a.sid[i], d = a.did[i];
+  bool bad = (uint32_t)s >= (uint32_t)a.src_pages || (uint32_t)d >= (uint32_t)a.dst_pages;
+  if (a.ok) {
+    bad |= !a.ok[i];
+  } else {
+    bool clash = a.same && s == d;
+    for (int j = threadIdx.x; j < a.n; j += kCT)
+      if (j != i) clash |= pair_clash(s, d, a.sid[j], a.did[j], a.same);
+    bad = __syncthreads_or(bad || clash);
+  }
+  if (bad) {
+    if (threadIdx.x == 0 && u == 0 && layer == 0) raise_status(a.status, Q35_STATUS_ARG);
+    return;
+  }
+  const int64_t o = (int64_t)u * kUnit;
+  copy_unit(a.dst + layer * a.dst_layer + d * a.page + o, a.src + layer * a.src_layer + s * a.page + o);
+}
+
+// ok[i] for many pairs: bitmaps of the pages that are a source, a destination, a destination twice.
+__global__ __launch_bounds__(kPT) void pages_copy_check_kernel(const CopyArgs a, uint8_t* ok) {
+  extern __shared__ uint32_t bm[];
+  const int ws = (a.src_pages + 31) / 32, wd = (a.dst_pages + 31) / 32;
+  uint32_t *S = bm, *D = bm + ws, *DD = D + wd;
+  for (int e = threadIdx.x; e < ws + 2 * wd; e += kPT) bm[e] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n; i += kPT) {
+    const int s = a.sid[i], d = a.did[i];
+    if ((uint32_t)s < (uint32_t)a.src_pages) atomicOr(&S[s >> 5], 1u << (s & 31));
+    if ((uint32_t)d < (uint32_t)a.dst_pages) {
+      const uint32_t b = 1u << (d & 31);
+      if (atomicOr(&D[d >> 5], b) & b) atomicOr(&DD[d >> 5], b);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n; i += kPT) {
+    const int s = a.sid[i], d = a.did[i];
+    bool good = (uint32_t)s < (uint32_t)a.src_pages && (uint32_t)d < (uint32_t)a.dst_pages;
+    if (good) {
+      good = !((DD[d >> 5] >> (d & 31)) & 1u);
+      if (a.same) good = good && !((S[d >> 5] >> (d & 31)) & 1u) && !((D[s >> 5] >> (s & 31)) & 1u);
+    }
+    ok[i] = good ? 1 : 0;
+  }
+}
+
+// ---- block-wide helpers of the bookkeeping kernels
+// exclusive sum of v over the block's threads; *total = the sum.  sh: kPW ints.
+Q35_DEV int block_excl(int v, int* sh, int* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) sh[w] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kPW; ++i) {
+    before += i < w ? sh[i] : 0;
+    all += sh[i];
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// ---- fork
+struct ForkShared {
+  int first[kPageMaxSeqs];          // parent -> its first child
+  int kept[kPageMaxSeqs];           // entries that row j keeps
+  int base[kPageMaxSeqs + 1];       // new pages before row j
+  int sh[kPW];
+};
+
+Q35_DEV int fork_parent(const ForkCall& c, int j, int* n, bool* bad) {
+  const int p = c.parent[j];
+  *n = 0;
+  *bad = p < -1 || p >= c.B;
+  if (*bad || p < 0) return -1;
+  const int l = c.len[p];
+  if (l < 0 || l > (int64_t)c.ld * c.P.page) {
+    *bad = true;
+    return -1;
+  }
+  *n = l;
+  return p;
+}
+
+__global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
+  extern __shared__ uint32_t bits[];  // pages that a kept entry names
+  __shared__ ForkShared s;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int np = c.P.n_pages, words = (np + 31) / 32, page = c.P.page;
+  bool bad = false;
+  for (int e = tid; e < words; e += kPT) bits[e] = 0;
+  for (int e = tid; e < np; e += kPT) c.refs[e] = 0;
+  for (int e = tid; e < c.B; e += kPT) s.first[e] = INT32_MAX;
+  __syncthreads();
+  for (int j = tid; j < c.Bo; j += kPT) {
+    int n;
+    bool b;
+    const int p = fork_parent(c, j, &n, &b);
+    if (p >= 0) atomicMin(&s.first[p], j);
+    c.len_out[j] = n;
+    bad |= b;
+  }
+  __syncthreads();
+  int run = 0;  // new pages of the rows before this group of kPT
+  for (int j0 = 0; j0 < c.Bo; j0 += kPT) {
+    const int j = j0 + tid;
+    int need = 0;
+    if (j < c.Bo) {
+      int n;
+      bool b;
+      const int p = fork_parent(c, j, &n, &b);
+      int64_t g = c.grow ? c.grow[j] : 0;
+      if (g < 0) {
+        g = 0;
+        bad = true;
+      }
+      const int kept = n / page + (p >= 0 && n % page != 0 && s.first[p] == j ? 1 : 0);
+      int64_t total = ((int64_t)n + g + page - 1) / page;
+      if (total > c.ld) {
+        total = c.ld;
+        bad = true;
+      }
+      s.kept[j] = kept;
+      need = (int)total - kept;
+    }
+    int all;
+    const int b = block_excl(need, s.sh, &all);
+    if (j < c.Bo) s.base[j] = run + b;
+    run += all;
+    __syncthreads();
+  }
+  if (tid == 0) s.base[c.Bo] = run;
+  __syncthreads();
+  // kept entries and what lies behind each row's pages; a wave per row
+  for (int j = wid; j < c.Bo; j += kPW) {
+    const int kept = s.kept[j], end = kept + s.base[j + 1] - s.base[j];
+    const int32_t* old = c.table + (int64_t)max(c.parent[j], 0) * c.ld;
+    int32_t* row = c.table_out + (int64_t)j * c.ld;
+    for (int e = lane; e < c.ld; e += 64) {
+      if (e >= kept && e < end) continue;
+      int v = -1;
+      if (e < kept) {
+        v = old[e];
+        if ((uint32_t)v >= (uint32_t)np) {
+          v = -1;
+          bad = true;
+        } else {
+          atomicOr(&bits[v >> 5], 1u << (v & 31));
+          __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+      row[e] = v;
+    }
+  }
+  __syncthreads();
+  // the free pages in ascending order: thread t holds words [t per, (t + 1) per)
+  const int per = (words + kPT - 1) / kPT;
+  const int w0 = min(words, tid * per), w1 = min(words, w0 + per);
+  auto free_bits = [&](int w) {
+    uint32_t f = ~bits[w];
+    if (32 * w + 32 > np) f &= (1u << (np & 31)) - 1u;
+    return f;
+  };
+  int cnt = 0;
+  for (int w = w0; w < w1; ++w) cnt += __popc(free_bits(w));
+  int nfree;
+  int r = block_excl(cnt, s.sh, &nfree);
+  auto row_of = [&](int rank) {  // the row j with base[j] <= rank < base[j + 1]
+    int lo = 0, hi = c.Bo;
+    while (hi - lo > 1) {
+      const int m = (lo + hi) / 2;
+      if (s.base[m] <= rank) lo = m;
+      else hi = m;
+    }
+    return lo;
+  };
+  for (int w = w0; w < w1 && r < run; ++w) {
+    uint32_t f = free_bits(w);
+    while (f && r < run) {
+      const int e = 32 * w + __ffs(f) - 1;
+      f &= f - 1;
+      const int j = row_of(r);
+      c.table_out[(int64_t)j * c.ld + s.kept[j] + r - s.base[j]] = e;
+      c.refs[e] = 1;
+      ++r;
+    }
+  }
+  for (int q = nfree + tid; q < run; q += kPT) {
+    const int j = row_of(q);
+    c.table_out[(int64_t)j * c.ld + s.kept[j] + q - s.base[j]] = -1;
+  }
+  if (bad) raise_status(c.status, Q35_STATUS_ARG);
+  if (tid == 0 && run > nfree) raise_status(c.status, Q35_STATUS_FULL);
+}
+
+// The tokens of last pages that were not kept: blocks (row j, layer, plane and head).
+__global__ __launch_bounds__(kCT) void pages_fork_copy_kernel(const ForkCall c) {
+  const int j = blockIdx.x, layer = blockIdx.y, ph = blockIdx.z;
+  int n;
+  bool b;
+  const int p = fork_parent(c, j, &n, &b);
+  const int tail = n % c.P.page;
+  if (p < 0 || tail == 0) return;
+  const int at = n / c.P.page;
+  const int src = c.table[(int64_t)p * c.ld + at], dst = c.table_out[(int64_t)j * c.ld + at];
+  if (src == dst || (uint32_t)src >= (uint32_t)c.P.n_pages || (uint32_t)dst >= (uint32_t)c.P.n_pages) return;
+  const int rb = c.P.head_dim * (c.P.dtype == Q35_F32 ? 4 : 2);
+  const int64_t head = (int64_t)c.P.page * rb, pb = head * 2 * c.P.kv_heads;
+  char* base = static_cast<char*>(c.P.data) + (int64_t)layer * c.P.n_pages * pb + ph * head;
+  const char* f = base + src * pb;
+  char* t = base + dst * pb;
+  for (int o = threadIdx.x * 16; o < tail * rb; o += kCT * 16) {
+    const uint4 v = ldg16(f + o);
+    *reinterpret_cast<uint4*>(t + o) = v;
+  }
+}
+
+// ---- compaction
+__global__ __launch_bounds__(kPT) void pages_compact_kernel(const CompactCall c) {
+  extern __shared__ uint32_t bits[];  // pages in use, then the number of them before each word
+  __shared__ int sh[kPW];
+  const int tid = threadIdx.x;
+  const int np = c.P.n_pages, words = (np + 31) / 32;
+  int* before = reinterpret_cast<int*>(bits + words);
+  const int64_t ne = (int64_t)c.B * c.ld;
+  bool bad = false;
+  for (int e = tid; e < words; e += kPT) bits[e] = 0;
+  for (int e = tid; e < np; e += kPT) c.refs[e] = 0;
+  __syncthreads();
+  for (int64_t e = tid; e < ne; e += kPT) {
+    const int v = c.table[e];
+    if ((uint32_t)v < (uint32_t)np) atomicOr(&bits[v >> 5], 1u << (v & 31));
+    else bad |= v != -1;
+  }
+  __syncthreads();
+  const int per = (words + kPT - 1) / kPT;
+  const int w0 = min(words, tid * per), w1 = min(words, w0 + per);
+  int cnt = 0;
+  for (int w = w0; w < w1; ++w) cnt += __popc(bits[w]);
+  int n;
+  int r = block_excl(cnt, sh, &n);
+  for (int w = w0; w < w1; ++w) {
+    before[w] = r;
+    r += __popc(bits[w]);
+  }
+  __syncthreads();
+  auto rank = [&](int p) { return before[p >> 5] + __popc(bits[p >> 5] & ((1u << (p & 31)) - 1u)); };  // pages in use < p
+  const int low = n < np ? rank(n) : n;  // pages in use below n; n - low of them move
+  // hole h (the h-th unused page below n) and mover h (the h-th page in use from n on)
+  for (int p = tid; p < np; p += kPT) {
+    const bool live = (bits[p >> 5] >> (p & 31)) & 1u;
+    const int k = rank(p);
+    if (p < n && !live) c.moves[p - k] = p;
+    if (p >= n && live) c.moves[np + k - low] = p;
+  }
+  if (tid == 0) *c.used = n;
+  __syncthreads();
+  for (int64_t e = tid; e < ne; e += kPT) {
+    int v = c.table[e];
+    if ((uint32_t)v >= (uint32_t)np) v = -1;
+    else {
+      if (v >= n) v = c.moves[rank(v) - low];
+      __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    c.table_out[e] = v;
+  }
+  // the copying launch reads the number of moves behind the lists
+  if (tid == 0) c.moves[2 * (int64_t)np] = n - low;
+  if (bad) raise_status(c.status, Q35_STATUS_ARG);
+}
+
+// Any number of blocks: units of (move, layer, part of the page) dealt round.
+__global__ __launch_bounds__(kCT) void pages_compact_copy_kernel(const CompactCall c, int64_t pb, int units) {
+  const int np = c.P.n_pages;
+  const int64_t all = (int64_t)c.moves[2 * (int64_t)np] * c.P.n_layers * units;
+  char* base = static_cast<char*>(c.P.data);
+  for (int64_t e = blockIdx.x; e < all; e += gridDim.x) {
+    const int u = (int)(e % units), layer = (int)(e / units % c.P.n_layers);
+    const int m = (int)(e / units / c.P.n_layers);
+    const int64_t off = (int64_t)layer * np * pb + (int64_t)u * kUnit;
+    copy_unit(base + off + c.moves[m] * pb, base + off + c.moves[np + m] * pb);
+  }
+}
+
+// Launches with more than 64 KB of LDS (large pools' bitmaps) ask for it first.
+template <class K>
+void allow_lds(K kernel, size_t bytes) {
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+}  // namespace
+
+int check_pages(const q35_pages& P, const char* what) {
+  const std::string w(what);
+  if (!P.data) return fail(Q35_E_ARG, w + ": null pool");
+  if (P.dtype != Q35_F32 && P.dtype != Q35_F16 && P.dtype != Q35_BF16) return fail(Q35_E_ARG, w + ": bad pool dtype");
+  if (P.head_dim != kPageHd) return fail(Q35_E_SHAPE, w + ": head_dim must be 256");
+  if (P.page < 16 || P.page > 256 || (P.page & (P.page - 1)) != 0)
+    return fail(Q35_E_SHAPE, w + ": tokens per page must be a power of two in 16..256");
+  if (P.n_layers < 1 || P.n_layers > 65535 || P.n_pages < 1 || P.n_pages > kPageMaxPages || P.kv_heads < 1 || P.kv_heads > 1024)
+    return fail(Q35_E_SHAPE, w + ": layers, pages (at most 262144) and kv heads (at most 1024) must be positive");
+  if ((reinterpret_cast<uintptr_t>(P.data) & 15) != 0) return fail(Q35_E_ALIGN, w + ": pool not 16-byte aligned");
+  return Q35_OK;
+}
+
+int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t* sid, const int32_t* did, int n,
+                      uint32_t* status, uint8_t* ok, hipStream_t st) {
+  CopyArgs a;
+  const int64_t pb = (int64_t)page_bytes(src);
+  a.src = static_cast<char*>(src.data);
+  a.dst = static_cast<char*>(dst.data);
+  a.page = pb;
+  a.src_layer = pb * src.n_pages;
+  a.dst_layer = pb * dst.n_pages;
+  a.src_pages = src.n_pages;
+  a.dst_pages = dst.n_pages;
+  a.same = src.data == dst.data;
+  a.n = n;
+  a.units = (int)(pb / kUnit);
+  a.sid = sid;
+  a.did = did;
+  a.status = status;
+  a.ok = nullptr;
+  if (n > kCT) {
+    const size_t lds = ((src.n_pages + 31) / 32 + 2 * (size_t)((dst.n_pages + 31) / 32)) * 4;
+    if (lds > 48 * 1024) allow_lds(pages_copy_check_kernel, lds);
+    hipLaunchKernelGGL(pages_copy_check_kernel, dim3(1), dim3(kPT), lds, st, a, ok);
+    Q35_HIP_TRY(hipGetLastError());
+    a.ok = ok;
+  }
+  hipLaunchKernelGGL(pages_copy_kernel, dim3(n * a.units, src.n_layers), dim3(kCT), 0, st, a);
+  Q35_HIP_TRY(hipGetLastError());
+  return Q35_OK;
+}
+
+int pages_fork_launch(const ForkCall& c, hipStream_t st) {
+  const size_t lds = (size_t)((c.P.n_pages + 31) / 32) * 4;
+  if (lds > 8 * 1024) allow_lds(pages_fork_kernel, lds);
+  hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(kPT), lds, st, c);
+  Q35_HIP_TRY(hipGetLastError());
+  hipLaunchKernelGGL(pages_fork_copy_kernel, dim3(c.Bo, c.P.n_layers, 2 * c.P.kv_heads), dim3(kCT), 0, st, c);
+  Q35_HIP_TRY(hipGetLastError());
+  return Q35_OK;
+}
+
+int pages_compact_launch(const CompactCall& c, hipStream_t st) {
+  const int words = (c.P.n_pages + 31) / 32;
+  if (words * 8 > 48 * 1024) allow_lds(pages_compact_kernel, (size_t)words * 8);
+  hipLaunchKernelGGL(pages_compact_kernel, dim3(1), dim3(kPT), (size_t)words * 8, st, c);
+  Q35_HIP_TRY(hipGetLastError());
+  const int64_t pb = (int64_t)page_bytes(c.P);
+  const int units = (int)(pb / kUnit);
+  // at most half of the pages move
+  const int64_t most = (int64_t)(c.P.n_pages / 2) * c.P.n_layers * units;
+  const int grid = (int)(most < 1 ? 1 : most > 8 * device_cus() ? 8 * device_cus() : most);
+  hipLaunchKernelGGL(pages_compact_copy_kernel, dim3(grid), dim3(kCT), 0, st, c, pb, units);
+  Q35_HIP_TRY(hipGetLastError());
+  return Q35_OK;
+}
+
+}  // namespace q35

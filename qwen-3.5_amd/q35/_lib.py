@@ -14,6 +14,8 @@ Q35_OK, Q35_E_SHAPE, Q35_E_ALIGN, Q35_E_HIP, Q35_E_ARG, Q35_E_WS, Q35_E_NOMEM, Q
 Q35_KN, Q35_NK, Q35_KN_TILED, Q35_KN_PANEL, Q35_KN_MB = 0, 1, 2, 3, 4
 Q35_LAUNCH_STREAM, Q35_LAUNCH_GRAPH, Q35_LAUNCH_PERSISTENT = 0, 1, 2
 Q35_PREFILL_GEMM = 0x100
+Q35_F32, Q35_F16, Q35_BF16 = 0, 1, 2
+Q35_STATUS_ARG, Q35_STATUS_FULL = 1, 2
 Q35_MB_PLAIN, Q35_MB_RMS, Q35_MB_GATED, Q35_MB_SWIGLU = 0, 1, 2, 3
 ERROR_NAMES = {1: "Q35_E_SHAPE", 2: "Q35_E_ALIGN", 3: "Q35_E_HIP", 4: "Q35_E_ARG", 5: "Q35_E_WS", 6: "Q35_E_NOMEM",
                7: "Q35_E_RANGE"}
@@ -33,6 +35,10 @@ class Dims(ctypes.Structure):
 
     def as_dict(self):
         return {n: getattr(self, n) for n, _ in self._fields_}
+
+
+class Pages(ctypes.Structure):
+    _fields_ = [("data", c_vp)] + [(n, c_i32) for n in ("dtype", "n_layers", "n_pages", "kv_heads", "page", "head_dim")]
 
 
 class GdnWeights(ctypes.Structure):
@@ -87,6 +93,19 @@ PROTOTYPES = {
     "q35_attention_core_prefill": (ctypes.c_int, [ctypes.POINTER(Dims), c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_i32,
                                                   c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "q35_attention_prefill_ws_bytes": (c_sz, [ctypes.POINTER(Dims), c_i32]),
+    "q35_status_check": (ctypes.c_int, [c_vp, c_vp]),
+    "q35_attention_paged_ws_bytes": (c_sz, [ctypes.POINTER(Dims), c_i32, c_i32]),
+    "q35_attention_core_paged": (ctypes.c_int, [ctypes.POINTER(Dims), Pages, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32, c_i32,
+                                                c_vp, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp,
+                                                c_i32, c_vp, c_vp, c_sz, c_vp]),
+    "q35_pages_copy_ws_bytes": (c_sz, [c_i32]),
+    "q35_pages_copy": (ctypes.c_int, [Pages, Pages, c_vp, c_vp, c_i32, c_vp, c_vp, c_sz, c_vp]),
+    "q35_pages_fork": (ctypes.c_int, [Pages, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "q35_pages_compact_ws_bytes": (c_sz, [c_i32]),
+    "q35_pages_compact": (ctypes.c_int, [Pages, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "q35_token_logprobs_ws_bytes": (c_sz, [c_i32, c_i32, c_i32]),
+    "q35_token_logprobs": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i64, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                          c_vp, c_sz, c_vp]),
     "q35_model_create_synthetic": (ctypes.c_int, [ctypes.POINTER(Dims), c_u64, c_i32, ctypes.POINTER(c_vp)]),
     "q35_model_create_from_safetensors": (ctypes.c_int, [ctypes.POINTER(Dims), ctypes.c_char_p, c_i32,
                                                          ctypes.POINTER(c_vp)]),
