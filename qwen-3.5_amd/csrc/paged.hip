@@ -1,7 +1,11 @@
 // Attention of new tokens over a paged cache: q/k RMSNorm (1 + w), rotary, append of keys and values to
 // the sequences' pages, causal softmax(q K^T / 16) V with shared kv heads, sigmoid output gate.
+//
+// Launches: append (with the plan), the attention of the sequences with few new tokens, that of the
+// sequences with many, and the join of what the plan cut.
 #include "pages.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace q35 {
@@ -11,35 +15,182 @@ namespace {
 constexpr int kHd = kPageHd;
 constexpr int kT = 256;
 
-// The sequence of row t: b with start[b] <= t < start[b + 1]; false if there is none, or if its
-// positions leave the table or the rotary rows (reported).
+// Sequence b: its rows, and whether they lie in the call's rows and their positions in the table and the
+// rotary rows.
 struct Seq {
-  int b, i, n, p0;  // sequence, row within it, its rows, its cached tokens
+  int b, s0, n, p0;  // sequence, first row, rows, tokens cached before
 };
-Q35_DEV bool seq_ok(const PagedAttn& a, int n, int p0) {
+Q35_DEV bool load_seq(const PagedAttn& a, int b, Seq* s) {
+  s->b = b;
+  s->s0 = a.start[b];
+  const int s1 = a.start[b + 1];
+  s->n = s1 - s->s0;
+  s->p0 = a.pos[b];
   const int64_t cap = (int64_t)a.ld_table * a.P.page;
   const int64_t lim = cap < a.rope_rows ? cap : a.rope_rows;
-  return p0 >= 0 && (int64_t)p0 + n <= lim;
+  return s->s0 >= 0 && s1 >= s->s0 && s1 <= a.T && s->p0 >= 0 && (int64_t)s->p0 + s->n <= lim;
 }
-Q35_DEV bool find_seq(const PagedAttn& a, int t, Seq* s, bool report) {
+// The sequence of row t: b with start[b] <= t < start[b + 1]; false if there is none or it is refused.
+Q35_DEV bool find_seq(const PagedAttn& a, int t, Seq* s) {
   int lo = 0, hi = a.B;  // the last b with start[b] <= t
   while (hi - lo > 1) {
     const int m = (lo + hi) / 2;
     if (a.start[m] <= t) lo = m;
     else hi = m;
   }
-  const int s0 = a.start[lo], s1 = a.start[lo + 1];
-  if (t < s0 || t >= s1) return false;
-  s->b = lo;
-  s->i = t - s0;
-  s->n = s1 - s0;
-  s->p0 = a.pos[lo];
-  if (seq_ok(a, s->n, s->p0)) return true;
-  if (report) raise_status(a.status, Q35_STATUS_ARG);
-  return false;
+  return load_seq(a, lo, s) && t >= s->s0 && t < s->s0 + s->n;
 }
 
-// Byte offset of token p of row b's pages, plane 0, kv head 0; -1 if its page is not in the pool
+// ------------------------------------------------------------------ the plan
+// Work is dealt out in units of 32 cached tokens of one kv head for one tile of query rows, laid end to
+// end over all tiles of all sequences: block g of G takes the units [g W / G, (g + 1) W / G), whatever
+// tiles they belong to.  So ragged batches load every CU alike, and a few long sequences are split as
+// finely as many short ones are not.  Where a block's range cuts a tile, it leaves (max, sum, output)
+// of its part, and the merge kernel joins the parts; only the first and the last tile of a block can be
+// cut, so two slots per block hold them all.
+//
+// Two kinds of tiles: sequences of a token or two ("few": the cache's stream bounds them) and chunks
+// ("many": the matrix cores do).
+constexpr int kUnit = 32;      // tokens of a unit
+constexpr int kMinUnits = 4;   // units a block takes at least
+constexpr int kManyRows = 128; // query rows (token, head) of a "many" tile
+
+template <int DT>
+struct Kind {
+  // parts of a query value (and of a weight): f16 products take two f16 halves, bf16 three bf16 values,
+  // and f32 caches are split into three bf16 values themselves
+  static constexpr int kParts = DT == Q35_F16 ? 2 : 3;
+  static constexpr int kPairs = kParts == 2 ? 8 : 4;  // (token, head) pairs of a "few" tile: its parts share 16 columns
+};
+
+struct Tile {
+  int64_t u0;  // its first unit
+  int32_t b, i, units, pad;
+};
+struct PlanHead {
+  int64_t w[2];      // units: few, many
+  int32_t tiles[2], blocks[2];
+};
+
+struct AttnArgs {
+  PagedAttn c;
+  int32_t rep, tok_many;  // query heads per kv head; tokens of a "many" tile
+  int32_t max_tiles[2], max_blocks[2], part_rows[2];
+  PlanHead* head;
+  float* q;              // [T][heads][256] queries after norm and rotary
+  float* qmax;           // [T][heads] largest |value|
+  int32_t* tile0;        // [2][B] first tile of the sequence in the list of each kind
+  Tile* tiles[2];
+  float* part_ml[2];     // [2 max_blocks][part_rows][2]
+  float* part_o[2];      // [2 max_blocks][part_rows][256]
+};
+
+template <int DT>
+Q35_DEV int kind_of(const AttnArgs& A, int n) { return n == 1 || n * A.rep <= 2 * Kind<DT>::kPairs ? 0 : 1; }
+template <int DT>
+Q35_DEV int tiles_of(const AttnArgs& A, int n) {
+  if (n <= 0) return 0;
+  const int per = kind_of<DT>(A, n) ? A.tok_many : Kind<DT>::kPairs;
+  return ((kind_of<DT>(A, n) ? n : n * A.rep) + per - 1) / per;
+}
+// cached tokens that tile i of the sequence looks at
+template <int DT>
+Q35_DEV int tile_len(const AttnArgs& A, const Seq& s, int i) {
+  const int tok = kind_of<DT>(A, s.n) ? (i + 1) * A.tok_many - 1 : ((i + 1) * Kind<DT>::kPairs - 1) / A.rep;
+  return s.p0 + min(tok, s.n - 1) + 1;
+}
+// first unit of block g, and the block that holds unit u
+Q35_DEV int64_t block_u0(int64_t w, int blocks, int g) { return w * g / blocks; }
+Q35_DEV int unit_block(int64_t w, int blocks, int64_t u) { return (int)(((u + 1) * blocks - 1) / w); }
+
+// exclusive sum over the block's kT threads
+template <class V>
+Q35_DEV V plan_excl(V v, V* sh, V* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  V x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const V y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) sh[w] = x;
+  __syncthreads();
+  V before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kT / 64; ++i) {
+    before += i < w ? sh[i] : 0;
+    all += sh[i];
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// Made by one block: the sequences' tiles, then each tile's first unit.
+template <int DT>
+Q35_DEV void make_plan(const AttnArgs& A) {
+  const PagedAttn& a = A.c;
+  __shared__ int si[kT / 64];
+  __shared__ int64_t sl[kT / 64];
+  const int tid = threadIdx.x;
+  int count[2] = {0, 0};
+  bool bad = false, falls = false;
+  for (int b0 = 0; b0 < a.B; b0 += kT) {
+    const int b = b0 + tid;
+    int nt[2] = {0, 0};
+    if (b < a.B) {
+      Seq s;
+      if (load_seq(a, b, &s)) nt[kind_of<DT>(A, s.n)] = tiles_of<DT>(A, s.n);
+      else bad = true;
+      falls |= s.n < 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      int all;
+      const int t = plan_excl(nt[k], si, &all);
+      if (b < a.B) A.tile0[(int64_t)k * a.B + b] = count[k] + t;
+      count[k] += all;
+    }
+  }
+  if (bad) raise_status(a.status, Q35_STATUS_ARG);
+  // (starts that fall could name more rows than there are: nothing is done then)
+  if (__syncthreads_or(falls)) count[0] = count[1] = 0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int nt = min(count[k], A.max_tiles[k]);
+    const int32_t* tile0 = A.tile0 + (int64_t)k * a.B;
+    int64_t run = 0;
+    for (int x0 = 0; x0 < nt; x0 += kT) {
+      const int x = x0 + tid;
+      Tile t = {0, 0, 0, 0, 0};
+      if (x < nt) {
+        // the last sequence with tile0 <= x: those without tiles of this kind share the next one's number
+        int lo = 0, hi = a.B;
+        while (hi - lo > 1) {
+          const int m = (lo + hi) / 2;
+          if (tile0[m] <= x) lo = m;
+          else hi = m;
+        }
+        Seq s;
+        load_seq(a, lo, &s);
+        t.b = lo;
+        t.i = x - tile0[lo];
+        t.units = (tile_len<DT>(A, s, t.i) + kUnit - 1) / kUnit;
+      }
+      int64_t all;
+      t.u0 = run + plan_excl((int64_t)t.units * a.nkv, sl, &all);
+      if (x < nt) A.tiles[k][x] = t;
+      run += all;
+    }
+    if (tid == 0) {
+      A.head->w[k] = run;
+      A.head->tiles[k] = nt;
+      const int64_t most = (run + kMinUnits - 1) / kMinUnits;
+      A.head->blocks[k] = (int)(most < A.max_blocks[k] ? most : A.max_blocks[k]);
+    }
+  }
+}
+
 template <int DT>
 struct Elt;
 template <>
@@ -65,6 +216,13 @@ Q35_DEV double wave_sum64(double v) {
   return v;
 }
 
+// what one lane of a wave wrote to LDS is read by others of the same wave
+Q35_DEV void wave_lds_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+}
+
 // A key's value as the cache holds it: rounded to f32, then to the cache's type (both to nearest even).
 // The empty asm keeps the compiler from rounding f64 to f16 in one step, as it otherwise does.
 template <class E>
@@ -74,138 +232,855 @@ Q35_DEV E stored(double y) {
   return (E)f;
 }
 
-// Keys and values of the new tokens into their pages; a wave per (row, kv head).
+// Keys and values of the new tokens into their pages, and the normalised, rotated queries (with each one's
+// largest |value|) into the workspace; a wave per (row, kv head or query head).  Block 0 makes the plan.
 template <int DT>
-__global__ __launch_bounds__(kT) void paged_append_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
+  const PagedAttn& a = A.c;
   __shared__ double xs[kT / 64][kHd];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int64_t item = (int64_t)blockIdx.x * (kT / 64) + wid;
-  const int t = (int)(item / a.nkv), g = (int)(item % a.nkv);
+  if (blockIdx.x == 0) {
+    make_plan<DT>(A);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, per = a.nkv + a.nh;
+  const int64_t item = ((int64_t)blockIdx.x - 1) * (kT / 64) + wid;
+  const int64_t t = item / per;
+  const int hd = (int)(item % per), g = hd, h = hd - a.nkv;  // kv head g, or query head h
   Seq s;
-  const bool in = t < a.T && find_seq(a, t, &s, lane == 0);
-  int page = -1, p = 0;
-  if (in) {
-    p = s.p0 + s.i;
-    page = a.table[(int64_t)s.b * a.ld_table + p / a.P.page];
-    if ((uint32_t)page >= (uint32_t)a.P.n_pages) {
-      if (lane == 0) raise_status(a.status, Q35_STATUS_ARG);
-      page = -1;
+  if (t >= a.T || !find_seq(a, (int)t, &s)) return;
+  const int p = s.p0 + (int)t - s.s0, d = 4 * lane, half = a.rot / 2;
+  const float* cs = a.rcos + (int64_t)p * a.rot;
+  const float* sn = a.rsin + (int64_t)p * a.rot;
+  if (h >= 0) {
+    float* x = reinterpret_cast<float*>(xs[wid]);
+    const float4 q = *reinterpret_cast<const float4*>(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + d);
+    const float4 w = *reinterpret_cast<const float4*>(a.qnw + d);
+    const float r = rsqrt_f(wave_sum(q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w) / (float)kHd + a.eps);
+    float y[4] = {q.x * r * (1.0f + w.x), q.y * r * (1.0f + w.y), q.z * r * (1.0f + w.z), q.w * r * (1.0f + w.w)};
+    *reinterpret_cast<float4*>(x + d) = make_float4(y[0], y[1], y[2], y[3]);
+    wave_lds_sync();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = d + j;
+      if (i < a.rot) y[j] = y[j] * cs[i] + (i < half ? -x[i + half] : x[i - half]) * sn[i];
     }
+    const int64_t o = t * a.nh + h;
+    *reinterpret_cast<float4*>(A.q + o * kHd + d) = make_float4(y[0], y[1], y[2], y[3]);
+    float m = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+#pragma unroll
+    for (int e = 32; e > 0; e >>= 1) m = fmaxf(m, __shfl_xor(m, e, 64));
+    if (lane == 0) A.qmax[o] = m;
+    return;
   }
-  const int d = 4 * lane;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (page >= 0) {
-    const float4 k = *reinterpret_cast<const float4*>(a.k + (int64_t)t * a.ld_kv + (int64_t)g * kHd + d);
-    v = *reinterpret_cast<const float4*>(a.v + (int64_t)t * a.ld_kv + (int64_t)g * kHd + d);
-    const float4 w = *reinterpret_cast<const float4*>(a.knw + d);
-    const double x0 = k.x, x1 = k.y, x2 = k.z, x3 = k.w;
-    const double r = 1.0 / sqrt(wave_sum64((x0 * x0 + x1 * x1) + (x2 * x2 + x3 * x3)) / (double)kHd + (double)a.eps);
-    xs[wid][d] = x0 * r * (1.0 + (double)w.x);
-    xs[wid][d + 1] = x1 * r * (1.0 + (double)w.y);
-    xs[wid][d + 2] = x2 * r * (1.0 + (double)w.z);
-    xs[wid][d + 3] = x3 * r * (1.0 + (double)w.w);
+  const int page = a.table[(int64_t)s.b * a.ld_table + p / a.P.page];
+  if ((uint32_t)page >= (uint32_t)a.P.n_pages) {
+    if (lane == 0) raise_status(a.status, Q35_STATUS_ARG);
+    return;
   }
-  __syncthreads();
-  if (page < 0) return;
-  const int half = a.rot / 2;
+  const float4 k = *reinterpret_cast<const float4*>(a.k + t * a.ld_kv + (int64_t)g * kHd + d);
+  const float4 v = *reinterpret_cast<const float4*>(a.v + t * a.ld_kv + (int64_t)g * kHd + d);
+  const float4 w = *reinterpret_cast<const float4*>(a.knw + d);
+  const double x0 = k.x, x1 = k.y, x2 = k.z, x3 = k.w;
+  const double r = 1.0 / sqrt(wave_sum64((x0 * x0 + x1 * x1) + (x2 * x2 + x3 * x3)) / (double)kHd + (double)a.eps);
+  double y[4] = {x0 * r * (1.0 + (double)w.x), x1 * r * (1.0 + (double)w.y), x2 * r * (1.0 + (double)w.z), x3 * r * (1.0 + (double)w.w)};
+  double* x = xs[wid];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) x[d + j] = y[j];
+  wave_lds_sync();
   E* kr = static_cast<E*>(a.P.data) + ((int64_t)a.layer * a.P.n_pages + page) * page_elts(a) +
           ((int64_t)g * a.P.page + p % a.P.page) * kHd;
   E* vr = kr + plane_elts(a);
-  const float* cs = a.rcos + (int64_t)p * a.rot;
-  const float* sn = a.rsin + (int64_t)p * a.rot;
   const float vv[4] = {v.x, v.y, v.z, v.w};
+  E ko[4], vo[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int i = d + j;
-    double y = xs[wid][i];
-    if (i < a.rot) {
-      const double rh = i < half ? -xs[wid][i + half] : xs[wid][i - half];
-      y = y * (double)cs[i] + rh * (double)sn[i];
-    }
-    kr[i] = stored<E>(y);
-    vr[i] = (E)vv[j];
+    if (i < a.rot) y[j] = y[j] * (double)cs[i] + (i < half ? -x[i + half] : x[i - half]) * (double)sn[i];
+    ko[j] = stored<E>(y[j]);
+    vo[j] = (E)vv[j];
   }
+  typedef E E4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<E4*>(kr + d) = E4{ko[0], ko[1], ko[2], ko[3]};
+  *reinterpret_cast<E4*>(vr + d) = E4{vo[0], vo[1], vo[2], vo[3]};
 }
 
-// A wave per (row, query head), one key after another.
-template <int DT>
-__global__ __launch_bounds__(kT) void paged_attn_simple_kernel(const PagedAttn a) {
-  typedef typename Elt<DT>::T E;
-  __shared__ float xs[kT / 64][kHd];
-  const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6;
-  const int64_t item = (int64_t)blockIdx.x * (kT / 64) + wid;
-  const int t = (int)(item / a.nh), h = (int)(item % a.nh);
-  Seq s;
-  const bool in = t < a.T && find_seq(a, t, &s, false);
-  const int d = 4 * lane;
-  if (in) {
-    const float4 q = *reinterpret_cast<const float4*>(a.qg + (int64_t)t * a.ld_qg + (int64_t)h * 2 * kHd + d);
-    const float4 w = *reinterpret_cast<const float4*>(a.qnw + d);
-    const float r = rsqrt_f(wave_sum(q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w) / (float)kHd + a.eps);
-    xs[wid][d] = q.x * r * (1.0f + w.x);
-    xs[wid][d + 1] = q.y * r * (1.0f + w.y);
-    xs[wid][d + 2] = q.z * r * (1.0f + w.z);
-    xs[wid][d + 3] = q.w * r * (1.0f + w.w);
+// ------------------------------------------------------------------ shared by the attention kernels
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+Q35_DEV float max_x32(float v) {  // the larger of lanes l and l ^ 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+Q35_DEV float max_x16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+Q35_DEV float add_x32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+Q35_DEV float add_x16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// The tile that holds unit u: every thread looks at some (they are few and in order).
+Q35_DEV int find_tile(const AttnArgs& A, int k, int64_t u, int* sh) {
+  const int nt = A.head->tiles[k];
+  for (int x = threadIdx.x; x < nt; x += blockDim.x) {
+    const Tile t = A.tiles[k][x];
+    if (t.u0 <= u && u < t.u0 + (int64_t)t.units * A.c.nkv) *sh = x;
   }
   __syncthreads();
-  if (!in) return;
-  const int p = s.p0 + s.i, half = a.rot / 2, g = h / (a.nh / a.nkv);
-  float q[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = d + j;
-    q[j] = xs[wid][i];
-    if (i < a.rot) {
-      const float rh = i < half ? -xs[wid][i + half] : xs[wid][i - half];
-      q[j] = q[j] * a.rcos[(int64_t)p * a.rot + i] + rh * a.rsin[(int64_t)p * a.rot + i];
-    }
-  }
-  const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)g * a.P.page * kHd;
-  const int32_t* row = a.table + (int64_t)s.b * a.ld_table;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+  const int x = *sh;
+  __syncthreads();
+  return x;
+}
+
+// Page of tokens j0 .. (16 of them share one); pages outside the pool count as page 0.
+Q35_DEV int page_of(const PagedAttn& a, const int32_t* row, int j0, bool* bad) {
+  const int v = __builtin_amdgcn_readfirstlane(row[j0 / a.P.page]);  // (j0 is the wave's)
+  if ((uint32_t)v < (uint32_t)a.P.n_pages) return v;
+  *bad = true;
+  return 0;
+}
+
+// ------------------------------------------------------------------ few new tokens
+// A block takes one tile - up to 4 (8) pairs of token and query head of a kv head - over some units; its
+// 4 waves take every 4th unit, each with its own running softmax, and are joined at the end.
+//
+// The keys of a unit go from the cache straight into the operand registers of S^T = K Q^T (16x16x32
+// matrix products: keys in rows, pairs in columns), its values into those of O^T += V^T P^T: the scores
+// come out where the weights are needed as operands, a pair's maximum and sum stay in its lanes, and
+// nothing passes LDS between the two products.  The order of the summed index is free as long as both
+// operands share it: the k-slot (lane group g, j) of the second product stands for key 4 g + j (j < 4) or
+// 16 + 4 g + j - 4, the lanes that hold those scores; and a value row's 16-byte pieces are dealt to
+// lanes so that each holds 8 keys of the same 8 dims, which a byte permute turns into operands.
+// A query value is carried whole, as 2 f16 or 3 bf16 parts in 2 or 3 of the 16 columns: a tile of
+// 4 pairs fills the columns that its pairs alone would leave empty, and the parts' sums are added
+// by lane rotations (the scores) or once at the end (the outputs).  Weights are split the same way.
+// An f32 cache's values are split into three bf16 values as they arrive, so all products are f32's.
+template <int DT>
+__global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
+  typedef typename Elt<DT>::T E;
+  constexpr int kPairs = Kind<DT>::kPairs, kParts = Kind<DT>::kParts;
+  constexpr bool kWide = DT == Q35_F32;
+  constexpr int kLd = kHd + 4;
+  const PagedAttn& a = A.c;
+  __shared__ __align__(16) float os[4][kPairs][kLd];
+  __shared__ float ms[4][kPairs], ls[4][kPairs];
+  __shared__ int sh;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g = lane >> 4;
+  const int64_t W = A.head->w[0];
+  const int G = A.head->blocks[0];
+  if ((int)blockIdx.x >= G) return;
+  int64_t u = block_u0(W, G, blockIdx.x);
+  const int64_t u_end = block_u0(W, G, blockIdx.x + 1);
+  int x = find_tile(A, 0, u, &sh);
+  const int pair = c16 % kPairs, part = c16 / kPairs;  // (kPairs == 4: part 3 is an empty column)
   const float sl2 = a.scale * 1.44269504088896341f;
-  for (int j = 0; j <= p; ++j) {
-    int page = row[j / a.P.page];
-    if ((uint32_t)page >= (uint32_t)a.P.n_pages) {
-      if (lane == 0) raise_status(a.status, Q35_STATUS_ARG);
-      page = 0;
+  bool bad = false;
+  for (int seg = 0; u < u_end; ++seg) {
+    const Tile t = A.tiles[0][x];
+    const int64_t off = u - t.u0;
+    const int gk = (int)(off / t.units), k0 = (int)(off % t.units);
+    const int k1 = (int)min((int64_t)t.units, k0 + (u_end - u));
+    Seq s;
+    load_seq(a, t.b, &s);
+    const int npair = min(kPairs, s.n * A.rep - t.i * kPairs);
+    auto token = [&](int pr) { return (t.i * kPairs + min(pr, npair - 1)) / A.rep; };
+    auto head = [&](int pr) { return gk * A.rep + (t.i * kPairs + min(pr, npair - 1)) % A.rep; };
+    q35_u32x4 qb[8];
+    float qscale = sl2;
+    {  // (pairs past the last one repeat it; their columns are not written anywhere)
+      const int64_t qi = (int64_t)(s.s0 + token(pair)) * a.nh + head(pair);
+      float fq = 1.f;
+      if constexpr (DT == Q35_F16) {  // a power of two per query brings its largest value to 2^14
+        float inv;
+        split_scale(A.qmax[qi], fq, inv);
+        qscale = sl2 * inv;
+      }
+#pragma unroll
+      for (int st = 0; st < 8; ++st) {
+        const float* qp = A.q + qi * kHd + 32 * st + 8 * g;
+        const f4 v0 = *(const Q35_GLOBAL f4*)qp, v1 = *(const Q35_GLOBAL f4*)(qp + 4);
+        const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p0, p1, p2 = 0;
+          if constexpr (DT == Q35_F16) split2(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
+          else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
+          qb[st][j] = part == 0 ? p0 : part == 1 ? p1 : part == 2 ? p2 : 0u;
+        }
+      }
     }
-    const E* kr = base + (int64_t)page * page_elts(a) + (int64_t)(j % a.P.page) * kHd + d;
-    const E* vr = kr + plane_elts(a);
-    float x = 0.f;
+    const int lim = s.p0 + token(pair);  // the last token the lane's pair sees
+    const int end = s.p0 + s.n;          // tokens from here on do not exist
+    const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
+    const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
+    // pages of the unit's two halves
+    auto pages = [&](int k, int& pa, int& pb) {
+      const int j0 = k * kUnit;
+      pa = page_of(a, row, j0, &bad);
+      pb = a.P.page > 16 || j0 + 16 >= end ? pa : page_of(a, row, j0 + 16, &bad);
+    };
+    constexpr int kW = kWide ? 2 : 1;  // 16-byte words of 8 values
+    q35_u32x4 kr[2][8 * kW], vr[8][2 * kW];
+    auto load_k = [&](int k, int pa, int pb) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x += q[e] * (float)kr[e];
-    x = wave_sum(x) * sl2;
-    const float mn = fmaxf(m, x);
-    const float f = __builtin_amdgcn_exp2f(m - mn), pr = __builtin_amdgcn_exp2f(x - mn);
-    m = mn;
-    l = l * f + pr;
+      for (int hf = 0; hf < 2; ++hf) {
+        const int slot = (k * kUnit + 16 * hf + c16) & (a.P.page - 1);
+        const E* p = base + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + 8 * g;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * f + pr * (float)vr[e];
+        for (int st = 0; st < 8; ++st)
+#pragma unroll
+          for (int w = 0; w < kW; ++w)
+            kr[hf][st * kW + w] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + 32 * st) + w);
+      }
+    };
+    auto load_v = [&](int k, int pa, int pb) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int slot = (k * kUnit + 16 * (j >> 2) + 4 * g + (j & 3)) & (a.P.page - 1);
+        const E* p = base + plane_elts(a) + (int64_t)(j >> 2 ? pb : pa) * page_elts(a) + (int64_t)slot * kHd;
+#pragma unroll
+        for (int w = 0; w < 2 * kW; ++w)
+          vr[j][w] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + w * (128 / kW)) + c16);
+      }
+    };
+    f4 o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    int k = k0 + wid, pa = 0, pb = 0;
+    if (k < k1) {
+      pages(k, pa, pb);
+      load_k(k, pa, pb);
+      load_v(k, pa, pb);
+    }
+    for (; k < k1; k += 4) {
+      const bool more = k + 4 < k1;
+      if (more) pages(k + 4, pa, pb);
+      f4 sc[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        f4 acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
+#pragma unroll
+        for (int st = 0; st < 8; ++st) {
+          if constexpr (DT == Q35_F16) {
+            f4& c = st & 1 ? acc2 : acc;
+            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, kr[hf][st]), __builtin_bit_cast(q35_h8, qb[st]), c, 0, 0, 0);
+          } else if constexpr (DT == Q35_BF16) {
+            f4& c = st & 1 ? acc2 : acc;
+            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, kr[hf][st]), __builtin_bit_cast(q35_b8, qb[st]), c, 0, 0, 0);
+          } else {
+            q35_u32x4 hi, mid, lo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t a0, a1, a2;
+              split3(__uint_as_float(kr[hf][2 * st + (j >> 1)][2 * (j & 1)]), __uint_as_float(kr[hf][2 * st + (j >> 1)][2 * (j & 1) + 1]), a0, a1, a2);
+              hi[j] = a0;
+              mid[j] = a1;
+              lo[j] = a2;
+            }
+            const q35_b8 q = __builtin_bit_cast(q35_b8, qb[st]);
+            acc2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, lo), q, acc2, 0, 0, 0);
+            acc2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, mid), q, acc2, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, hi), q, acc, 0, 0, 0);
+          }
+        }
+        sc[hf] = acc + acc2;
+      }
+      const int j0 = k * kUnit;
+      if (more) load_k(k + 4, pa, pb);
+      asm volatile("" ::: "memory");
+      float sv[8], bm = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v = sc[j >> 2][j & 3];
+        v += row_ror<8>(v);
+        if constexpr (kParts == 3) v += row_ror<4>(v);
+        const int key = j0 + 16 * (j >> 2) + 4 * g + (j & 3);
+        sv[j] = key <= lim ? v * qscale : -INFINITY;
+        bm = fmaxf(bm, sv[j]);
+      }
+      bm = max_x32(max_x16(bm));
+      const float mn = fmaxf(m, bm);
+      if (__ballot(mn > m)) {
+        const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= al;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] *= al;
+        m = mn;
+      }
+      // f16 weights are kept 2^12 times larger (at most 4096), so that their halves hold 22 bits down to 2^-26
+      const float mr = (m == -INFINITY ? 0.f : m) - (DT == Q35_F16 ? 12.f : 0.f);
+      q35_u32x4 pw;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float p0 = __builtin_amdgcn_exp2f(sv[2 * j] - mr), p1 = __builtin_amdgcn_exp2f(sv[2 * j + 1] - mr);
+        l += p0 + p1;
+        uint32_t w0, w1, w2 = 0;
+        if constexpr (DT == Q35_F16) split2(p0, p1, w0, w1);
+        else split3(p0, p1, w0, w1, w2);
+        pw[j] = part == 0 ? w0 : part == 1 ? w1 : part == 2 ? w2 : 0u;
+      }
+      if (j0 + kUnit > end) {  // (uniform) rows behind the sequence's last token may hold anything
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j0 + 16 * (j >> 2) + 4 * g + (j & 3) >= end) {
+#pragma unroll
+            for (int w = 0; w < 2 * kW; ++w) vr[j][w] = q35_u32x4{0, 0, 0, 0};
+          }
+      }
+#pragma unroll
+      for (int w = 0; w < 2 * kW; ++w) {
+#pragma unroll
+        for (int e = 0; e < 8 / kW; ++e) {
+          const int i = w * (8 / kW) + e;
+          if constexpr (kWide) {
+            q35_u32x4 hi, mid, lo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t a0, a1, a2;
+              split3(__uint_as_float(vr[2 * j][w][e]), __uint_as_float(vr[2 * j + 1][w][e]), a0, a1, a2);
+              hi[j] = a0;
+              mid[j] = a1;
+              lo[j] = a2;
+            }
+            const q35_b8 p = __builtin_bit_cast(q35_b8, pw);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, lo), p, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, mid), p, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, hi), p, o[i], 0, 0, 0);
+          } else {
+            q35_u32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              v[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w][e >> 1], vr[2 * j][w][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+            if constexpr (DT == Q35_F16)
+              o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, v), __builtin_bit_cast(q35_h8, pw), o[i], 0, 0, 0);
+            else
+              o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, v), __builtin_bit_cast(q35_b8, pw), o[i], 0, 0, 0);
+          }
+        }
+      }
+      if (more) load_v(k + 4, pa, pb);
+      asm volatile("" ::: "memory");
+    }
+    // the parts' columns together; tile i = w (8 / kW) + e, row 4 g + r: dim w (128 / kW) + (8 / kW)(4 g + r) + e
+    l = add_x32(add_x16(l));
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float v = o[i][r];
+        v += row_ror<8>(v);
+        if constexpr (kParts == 3) v += row_ror<4>(v);
+        constexpr int kE = 8 / kW;
+        if (part == (r & 1)) os[wid][pair][(i / kE) * (128 / kW) + kE * (4 * g + r) + i % kE] = v;
+      }
+    if (g == 0 && part == 0) {
+      ms[wid][pair] = m;
+      ls[wid][pair] = l;
+    }
+    __syncthreads();
+    // pairs wid, wid + 4: 4 dims per lane
+    const bool whole = k0 == 0 && k1 == t.units;
+    const int slot = 2 * blockIdx.x + (seg == 0 ? 0 : 1);
+    for (int pr = wid; pr < npair; pr += 4) {
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, ms[w][pr]);
+      float L = 0.f;
+      f4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = ms[w][pr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[w][pr] - M);
+        L += ls[w][pr] * f;
+        r += *(const f4*)&os[w][pr][4 * lane] * f;
+      }
+      if (whole) {
+        const int64_t tr = s.s0 + token(pr);
+        const f4 gv = *(const f4*)(a.qg + tr * a.ld_qg + (int64_t)head(pr) * 2 * kHd + kHd + 4 * lane);
+        f4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = r[e] / L * sigmoid_f(gv[e]);
+        *(f4*)(a.out + tr * a.ld_out + (int64_t)head(pr) * kHd + 4 * lane) = y;
+      } else {
+        const int64_t pi = (int64_t)slot * A.part_rows[0] + pr;
+        *(f4*)(A.part_o[0] + pi * kHd + 4 * lane) = r;
+        if (lane == 0) {
+          A.part_ml[0][2 * pi] = M;
+          A.part_ml[0][2 * pi + 1] = L;
+        }
+      }
+    }
+    __syncthreads();
+    u += k1 - k0;
+    if (u == t.u0 + (int64_t)t.units * a.nkv) ++x;
   }
-  const float4 gv = *reinterpret_cast<const float4*>(a.qg + (int64_t)t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + d);
-  float* dst = a.out + (int64_t)t * a.ld_out + (int64_t)h * kHd + d;
-  *reinterpret_cast<float4*>(dst) = make_float4(o[0] / l * sigmoid_f(gv.x), o[1] / l * sigmoid_f(gv.y),
-                                                o[2] / l * sigmoid_f(gv.z), o[3] / l * sigmoid_f(gv.w));
+  if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
+}
+
+// ------------------------------------------------------------------ many new tokens
+// A block takes one tile of up to 128 rows (token, query head of one kv head), 32 per wave, over some
+// units.  A unit's keys and values pass LDS, where all four waves read them: 4 waves with 32 columns of
+// queries each use every operand read from LDS for 128 columns, a quarter of the LDS's rate, and one wave
+// per SIMD has the registers for its queries (128 or 192) and outputs (128).  As above, S^T = K Q^T and
+// O^T += V^T P^T (32x32x16 products) keep a row's statistics in its lane pair and turn scores into
+// operands in place: score register i of lane half h is key 8 (i / 4) + 4 h + i % 4, so V^T's rows
+// list the keys in that order and eight consecutive registers are one operand.
+// While a unit is multiplied, the next one is on its way into registers; it is then laid out in the
+// other LDS buffer, so one barrier per unit is enough.
+// LDS: keys [key][32 pieces of 8 dims], piece c at c ^ (key & 7); values [dim][4 pieces of 8 keys], dim
+// d's row at d ^ ((d / 8) % 4) and piece c at c ^ ((d / 4 ^ d / 16) % 4): reads touch every bank once.
+// f16 caches are multiplied with 2 f16 halves of a query or weight, bf16 ones with 3 bf16 parts; f32
+// caches as 2 f16 halves with 2 (three products; what is dropped is 2^-22 of a term), under a power of
+// two for every 8 keys (a wave's share of the unit) and one for 8 values, whose inverse goes into the weights.
+constexpr int kRowsW = 32;
+constexpr int kPlane = 16384;  // bytes of a unit's keys (or values) of one part
+template <int DT>
+constexpr int many_lds() { return 2 * 2 * kPlane * (DT == Q35_F32 ? 2 : 1); }
+
+template <int DT>
+__global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
+  typedef typename Elt<DT>::T E;
+  constexpr bool kWide = DT == Q35_F32;
+  constexpr int kQ = DT == Q35_BF16 ? 3 : 2;  // parts of a query or weight
+  constexpr int kKV = kWide ? 2 : 1;          // parts of a key or value
+  // how far (log2) a score may pass the running maximum before the sums are rescaled: f16 weights
+  // are kept 2^12 times larger and must stay below 2^16
+  constexpr float kSlack = DT == Q35_BF16 ? 8.f : 3.f;
+  const PagedAttn& a = A.c;
+  extern __shared__ __align__(16) char lds[];  // [2 buffers][keys, values][part]
+  __shared__ float scl[2][2][4];               // [buffer][keys, values][group of 8 keys]
+  __shared__ int sh;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, hf = lane >> 5;
+  const int64_t W = A.head->w[1];
+  const int G = A.head->blocks[1];
+  if ((int)blockIdx.x >= G) return;
+  int64_t u = block_u0(W, G, blockIdx.x);
+  const int64_t u_end = block_u0(W, G, blockIdx.x + 1);
+  int x = find_tile(A, 1, u, &sh);
+  const float sl2 = a.scale * 1.44269504088896341f;
+  bool bad = false;
+  for (int seg = 0; u < u_end; ++seg) {
+    const Tile t = A.tiles[1][x];
+    const int64_t off = u - t.u0;
+    const int gk = (int)(off / t.units), k0 = (int)(off % t.units);
+    const int k1 = (int)min((int64_t)t.units, k0 + (u_end - u));
+    Seq s;
+    load_seq(a, t.b, &s);
+    const int tok0 = t.i * A.tok_many, rows = min(A.tok_many, s.n - tok0) * A.rep;
+    const int r = min(wid * kRowsW + n, rows - 1);  // the lane's row (past the last one: repeated, not written)
+    const int tok = tok0 + r / A.rep, h = gk * A.rep + r % A.rep;
+    const int lim = s.p0 + tok;
+    const bool wave_on = wid * kRowsW < rows;
+    // the first and the last token that a row of the wave sees
+    const int lim0 = s.p0 + tok0 + min(wid * kRowsW, rows - 1) / A.rep;
+    const int lim1 = s.p0 + tok0 + min(wid * kRowsW + kRowsW - 1, rows - 1) / A.rep;
+    const int end = s.p0 + s.n;
+    const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
+    const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
+    // staging registers: keys 8 wid + 2 i + hf, dims 8 n ..; values: keys 8 wid + 4 hf + i, dims 8 n ..
+    q35_u32x4 kr[4][kKV], vr[4][kKV];
+    auto load_unit = [&](int k) {
+      const int j0 = k * kUnit + 8 * wid;  // (8 keys lie in one page)
+      const int pg = j0 < end ? page_of(a, row, j0, &bad) : page_of(a, row, k * kUnit, &bad);
+      const E* p = base + (int64_t)pg * page_elts(a) + (int64_t)(j0 & (a.P.page - 1)) * kHd + 8 * n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < kKV; ++w) kr[i][w] = *((const Q35_GLOBAL q35_u32x4*)(p + (2 * i + hf) * kHd) + w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < kKV; ++w) vr[i][w] = *((const Q35_GLOBAL q35_u32x4*)(p + plane_elts(a) + (4 * hf + i) * kHd) + w);
+    };
+    const int vpiece = ((wid >> 1) * 2 + hf), vhalf = wid & 1;
+    auto store_unit = [&](int k, int buf) {
+      if (k * kUnit + kUnit > end) {  // (uniform) rows behind the last token may hold anything
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (k * kUnit + 8 * wid + 2 * i + hf >= end) {
+#pragma unroll
+            for (int w = 0; w < kKV; ++w) kr[i][w] = q35_u32x4{0, 0, 0, 0};
+          }
+          if (k * kUnit + 8 * wid + 4 * hf + i >= end) {
+#pragma unroll
+            for (int w = 0; w < kKV; ++w) vr[i][w] = q35_u32x4{0, 0, 0, 0};
+          }
+        }
+      }
+      char* kb = lds + buf * 2 * kKV * kPlane;
+      char* vb = kb + kKV * kPlane;
+      float fk = 1.f, fv = 1.f;
+      if constexpr (kWide) {
+        float mk = 0.f, mv = 0.f, ik, iv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              mk = fmaxf(mk, fabsf(__uint_as_float(kr[i][w][e])));
+              mv = fmaxf(mv, fabsf(__uint_as_float(vr[i][w][e])));
+            }
+        mk = fmaxf(mk, row_ror<8>(mk)); mv = fmaxf(mv, row_ror<8>(mv));
+        mk = fmaxf(mk, row_ror<4>(mk)); mv = fmaxf(mv, row_ror<4>(mv));
+        mk = fmaxf(mk, row_ror<2>(mk)); mv = fmaxf(mv, row_ror<2>(mv));
+        mk = fmaxf(mk, row_ror<1>(mk)); mv = fmaxf(mv, row_ror<1>(mv));
+        split_scale(max_x32(max_x16(mk)), fk, ik);
+        mv = max_x32(max_x16(mv));
+        split_scale(mv, fv, iv);
+        iv = mv > 0.f ? fmaxf(iv, 7.888609e-31f) : 7.888609e-31f;  // (2^-100: zeros ask for no room)
+        if (lane == 0) {
+          scl[buf][0][wid] = ik;
+          scl[buf][1][wid] = iv;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 8 * wid + 2 * i + hf;
+        char* dst = kb + key * 512 + (n ^ (key & 7)) * 16;
+        if constexpr (kWide) {
+          q35_u32x4 hi, lo;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t a0, a1;
+            split2(__uint_as_float(kr[i][j >> 1][2 * (j & 1)]) * fk, __uint_as_float(kr[i][j >> 1][2 * (j & 1) + 1]) * fk, a0, a1);
+            hi[j] = a0;
+            lo[j] = a1;
+          }
+          *(q35_u32x4*)dst = hi;
+          *(q35_u32x4*)(dst + kPlane) = lo;
+        } else {
+          *(q35_u32x4*)dst = kr[i][0];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int d = 8 * n + e;
+        char* dst = vb + (d ^ (n & 3)) * 64 + ((vpiece ^ ((d >> 2) ^ (d >> 4))) & 3) * 16 + vhalf * 8;
+        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+        if constexpr (kWide) {
+          const float v0 = __uint_as_float(vr[0][e >> 2][e & 3]) * fv, v1 = __uint_as_float(vr[1][e >> 2][e & 3]) * fv;
+          const float v2 = __uint_as_float(vr[2][e >> 2][e & 3]) * fv, v3 = __uint_as_float(vr[3][e >> 2][e & 3]) * fv;
+          uint32_t a0, a1, b0, b1;
+          split2(v0, v1, a0, a1);
+          split2(v2, v3, b0, b1);
+          *(u2*)dst = u2{a0, b0};
+          *(u2*)(dst + kPlane) = u2{a1, b1};
+        } else {
+          const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+          *(u2*)dst = u2{__builtin_amdgcn_perm(vr[1][0][e >> 1], vr[0][0][e >> 1], sel),
+                         __builtin_amdgcn_perm(vr[3][0][e >> 1], vr[2][0][e >> 1], sel)};
+        }
+      }
+    };
+    load_unit(k0);
+    // queries: column n, dims 16 st + 8 hf ..
+    q35_u32x4 qb[kQ][16];
+    float qscale = sl2;
+    {
+      const int64_t qi = (int64_t)(s.s0 + tok) * a.nh + h;
+      float fq = 1.f;
+      if constexpr (DT != Q35_BF16) {
+        float inv;
+        split_scale(A.qmax[qi], fq, inv);
+        qscale = sl2 * inv;
+      }
+#pragma unroll
+      for (int st = 0; st < 16; ++st) {
+        const float* qp = A.q + qi * kHd + 16 * st + 8 * hf;
+        const f4 v0 = *(const Q35_GLOBAL f4*)qp, v1 = *(const Q35_GLOBAL f4*)(qp + 4);
+        const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t p0, p1, p2 = 0;
+          if constexpr (kQ == 2) split2(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
+          else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
+          qb[0][st][j] = p0;
+          qb[1][st][j] = p1;
+          if constexpr (kQ == 3) qb[2][st][j] = p2;
+        }
+      }
+    }
+    f16v o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    float ov = DT == Q35_BF16 ? 1.f : 4096.f;  // o is kept this much larger (f32 caches: a power of two below the values')
+    bool fresh = true;
+    for (int k = k0; k < k1; ++k) {
+      const int buf = (k - k0) & 1;
+      store_unit(k, buf);
+      if (k + 1 < k1) load_unit(k + 1);
+      __syncthreads();
+      const int j0 = k * kUnit;
+      if (!wave_on || j0 > lim1) continue;  // (uniform in the wave; the barrier above is passed by all)
+      const char* kb = lds + buf * 2 * kKV * kPlane;
+      const char* vb = kb + kKV * kPlane;
+      f16v sc;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+#pragma unroll
+      for (int st = 0; st < 16; ++st) {
+        const char* src = kb + n * 512 + ((2 * st + hf) ^ (n & 7)) * 16;
+        const q35_u32x4 ka = *(const q35_u32x4*)src;
+        if constexpr (DT == Q35_BF16) {
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(q35_b8, ka), __builtin_bit_cast(q35_b8, qb[q][st]), sc, 0, 0, 0);
+        } else {
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[0][st]), sc, 0, 0, 0);
+          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[1][st]), sc, 0, 0, 0);
+          if constexpr (kWide) {
+            const q35_u32x4 kl = *(const q35_u32x4*)(src + kPlane);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, kl), __builtin_bit_cast(q35_h8, qb[0][st]), sc, 0, 0, 0);
+          }
+        }
+      }
+      float fk[4], fp[4];
+      float vscale = ov;
+      if constexpr (kWide) {
+        // the outputs' power of two: 2^12 over the largest values so far
+        float iv = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          fk[q] = scl[buf][0][q] * qscale;
+          fp[q] = scl[buf][1][q];
+          iv = fmaxf(iv, fp[q]);
+        }
+        vscale = 4096.f * __uint_as_float((254u << 23) - __float_as_uint(iv));  // 2^12 / iv
+        if (!fresh) vscale = fminf(vscale, ov);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) fp[q] *= vscale;  // 2^12 at most
+      }
+      float bm = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        sc[e] *= kWide ? fk[e >> 2] : qscale;
+        if (j0 + kUnit - 1 > lim0) sc[e] = j0 + 8 * (e >> 2) + 4 * hf + (e & 3) <= lim ? sc[e] : -INFINITY;
+        bm = fmaxf(bm, sc[e]);
+      }
+      bm = max_x32(bm);
+      if (__ballot(bm > m + kSlack || (m == -INFINITY && bm > m)) || (kWide && vscale != ov)) {
+        const float mn = fmaxf(m, bm);
+        float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= al;
+        m = mn;
+        if (!fresh) {
+          if constexpr (kWide) al *= vscale / ov;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] *= al;
+        }
+        ov = vscale;
+      }
+      fresh = false;
+      const float mr = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int th = 0; th < 2; ++th) {
+        q35_u32x4 pw[kQ];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int e = 8 * th + 2 * j;
+          float p0 = __builtin_amdgcn_exp2f(sc[e] - mr), p1 = __builtin_amdgcn_exp2f(sc[e + 1] - mr);
+          l += p0 + p1;
+          if constexpr (kWide) {
+            p0 *= fp[e >> 2];
+            p1 *= fp[e >> 2];
+          } else if constexpr (DT == Q35_F16) {
+            p0 *= 4096.f;
+            p1 *= 4096.f;
+          }
+          uint32_t w0, w1, w2 = 0;
+          if constexpr (kQ == 2) split2(p0, p1, w0, w1);
+          else split3(p0, p1, w0, w1, w2);
+          pw[0][j] = w0;
+          pw[1][j] = w1;
+          if constexpr (kQ == 3) pw[2][j] = w2;
+        }
+#pragma unroll
+        for (int dt = 0; dt < 8; ++dt) {
+          const int d = 32 * dt + n;
+          const char* src = vb + (d ^ ((d >> 3) & 3)) * 64 + (((2 * th + hf) ^ ((d >> 2) ^ (d >> 4))) & 3) * 16;
+          const q35_u32x4 va = *(const q35_u32x4*)src;
+          if constexpr (DT == Q35_BF16) {
+#pragma unroll
+            for (int q = 0; q < 3; ++q)
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(q35_b8, va), __builtin_bit_cast(q35_b8, pw[q]), o[dt], 0, 0, 0);
+          } else {
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[1]), o[dt], 0, 0, 0);
+            if constexpr (kWide) {
+              const q35_u32x4 vl = *(const q35_u32x4*)(src + kPlane);
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, vl), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
+            }
+          }
+        }
+      }
+    }
+    // register 4 q + e of o[dt] is dim 32 dt + 8 q + 4 hf + e
+    l = add_x32(l);
+    const bool whole = k0 == 0 && k1 == t.units;
+    if (wid * kRowsW + n < rows) {
+      const float f = (whole ? 1.f / l : 1.f) / ov;
+      const int64_t tr = s.s0 + tok;
+      const float* gate = a.qg + tr * a.ld_qg + (int64_t)h * 2 * kHd + kHd;
+      const int64_t pi = (int64_t)(2 * blockIdx.x + (seg == 0 ? 0 : 1)) * A.part_rows[1] + r;
+      float* dst = whole ? a.out + tr * a.ld_out + (int64_t)h * kHd : A.part_o[1] + pi * kHd;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = 32 * dt + 8 * q + 4 * hf;
+          f4 y = {o[dt][4 * q] * f, o[dt][4 * q + 1] * f, o[dt][4 * q + 2] * f, o[dt][4 * q + 3] * f};
+          if (whole) {
+            const f4 gv = *(const f4*)(gate + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] *= sigmoid_f(gv[e]);
+          }
+          *(f4*)(dst + d) = y;
+        }
+      if (!whole && hf == 0) {
+        A.part_ml[1][2 * pi] = m;
+        A.part_ml[1][2 * pi + 1] = l;
+      }
+    }
+    __syncthreads();  // (the buffers are the next segment's)
+    u += k1 - k0;
+    if (u == t.u0 + (int64_t)t.units * a.nkv) ++x;
+  }
+  if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
+}
+
+// A wave per (row, query head): joins the parts of its tile, if the plan cut it.
+template <int DT>
+__global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
+  const PagedAttn& a = A.c;
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * (kT / 64) + (threadIdx.x >> 6);
+  const int64_t t = item / a.nh;
+  const int h = (int)(item % a.nh);
+  Seq s;
+  if (t >= a.T || !find_seq(a, (int)t, &s)) return;
+  const int kind = kind_of<DT>(A, s.n), gk = h / A.rep, hr = h % A.rep, tok = (int)t - s.s0;
+  const int pair = tok * A.rep + hr;
+  const int i = kind ? tok / A.tok_many : pair / Kind<DT>::kPairs;
+  const int r = kind ? pair - i * A.tok_many * A.rep : pair % Kind<DT>::kPairs;
+  const int x = A.tile0[(int64_t)kind * a.B + s.b] + i;
+  if (x >= A.head->tiles[kind]) return;
+  const Tile tl = A.tiles[kind][x];
+  const int64_t W = A.head->w[kind], u0 = tl.u0 + (int64_t)gk * tl.units;
+  const int G = A.head->blocks[kind];
+  const int g0 = unit_block(W, G, u0), g1 = unit_block(W, G, u0 + tl.units - 1);
+  if (g0 == g1) return;
+  const int first = block_u0(W, G, g0) == u0 ? 0 : 1;
+  float M = -INFINITY;
+  for (int gb = g0; gb <= g1; ++gb) {
+    const int64_t pi = (int64_t)(2 * gb + (gb == g0 ? first : 0)) * A.part_rows[kind] + r;
+    M = fmaxf(M, A.part_ml[kind][2 * pi]);
+  }
+  float L = 0.f;
+  f4 y = {0.f, 0.f, 0.f, 0.f};
+  for (int gb = g0; gb <= g1; ++gb) {
+    const int64_t pi = (int64_t)(2 * gb + (gb == g0 ? first : 0)) * A.part_rows[kind] + r;
+    const float mg = A.part_ml[kind][2 * pi];
+    if (mg == -INFINITY) continue;  // (nothing of that part was in sight of this row)
+    const float f = __builtin_amdgcn_exp2f(mg - M);
+    L += A.part_ml[kind][2 * pi + 1] * f;
+    y += *(const f4*)(A.part_o[kind] + pi * kHd + 4 * lane) * f;
+  }
+  const f4 gv = *(const f4*)(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + 4 * lane);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = y[e] / L * sigmoid_f(gv[e]);
+  *(f4*)(a.out + t * a.ld_out + (int64_t)h * kHd + 4 * lane) = y;
+}
+
+
+struct PagedLayout {
+  int32_t max_tiles[2], max_blocks[2], part_rows[2];
+  size_t head, tile0, q, qmax, tiles[2], ml[2], o[2];  // byte sizes
+  size_t bytes;
+};
+PagedLayout paged_layout(int nh, int nkv, int T, int B) {
+  PagedLayout L;
+  const int rep = nh / nkv, tok_many = kManyRows / rep;
+  auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+  // (4 pairs per tile at least, whatever the cache's type)
+  L.max_tiles[0] = (int)(((int64_t)T * rep + 3) / 4 + std::min(B, T));
+  const bool many = T > 1 && T * rep > 8;
+  L.max_tiles[1] = many ? T / tok_many + std::min(B, T) : 0;
+  const int cus = device_cus();
+  L.max_blocks[0] = 2 * cus;
+  L.max_blocks[1] = many ? cus : 0;
+  L.part_rows[0] = 8;
+  L.part_rows[1] = (int)std::min<int64_t>(kManyRows, (int64_t)T * rep);
+  L.head = up(sizeof(PlanHead));
+  L.tile0 = up((size_t)2 * B * 4);
+  L.q = up((size_t)T * nh * kHd * 4);
+  L.qmax = up((size_t)T * nh * 4);
+  L.bytes = L.head + L.tile0 + L.q + L.qmax;
+  for (int k = 0; k < 2; ++k) {
+    const size_t rows = (size_t)2 * L.max_blocks[k] * L.part_rows[k];
+    L.tiles[k] = up((size_t)L.max_tiles[k] * sizeof(Tile));
+    L.ml[k] = up(rows * 8);
+    L.o[k] = up(rows * kHd * 4);
+    L.bytes += L.tiles[k] + L.ml[k] + L.o[k];
+  }
+  return L;
 }
 
 template <int DT>
 int launch(const PagedAttn& a, hipStream_t st) {
-  const int64_t ka = (int64_t)a.T * a.nkv, qa = (int64_t)a.T * a.nh;
-  hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((uint32_t)((ka + 3) / 4)), dim3(kT), 0, st, a);
+  const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B);
+  AttnArgs A;
+  A.c = a;
+  A.rep = a.nh / a.nkv;
+  A.tok_many = kManyRows / A.rep;
+  char* p = static_cast<char*>(a.ws);
+  A.head = reinterpret_cast<PlanHead*>(p);
+  p += L.head;
+  A.tile0 = reinterpret_cast<int32_t*>(p);
+  p += L.tile0;
+  A.q = reinterpret_cast<float*>(p);
+  p += L.q;
+  A.qmax = reinterpret_cast<float*>(p);
+  p += L.qmax;
+  for (int k = 0; k < 2; ++k) {
+    A.max_tiles[k] = L.max_tiles[k];
+    A.max_blocks[k] = L.max_blocks[k];
+    A.part_rows[k] = L.part_rows[k];
+    A.tiles[k] = reinterpret_cast<Tile*>(p);
+    p += L.tiles[k];
+    A.part_ml[k] = reinterpret_cast<float*>(p);
+    p += L.ml[k];
+    A.part_o[k] = reinterpret_cast<float*>(p);
+    p += L.o[k];
+  }
+  const int64_t ka = (int64_t)a.T * (a.nkv + a.nh), qa = (int64_t)a.T * a.nh;
+  hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((uint32_t)((ka + 3) / 4 + 1)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(paged_attn_simple_kernel<DT>, dim3((uint32_t)((qa + 3) / 4)), dim3(kT), 0, st, a);
+  hipLaunchKernelGGL(paged_few_kernel<DT>, dim3(A.max_blocks[0]), dim3(kT), 0, st, A);
+  Q35_HIP_TRY(hipGetLastError());
+  if (A.max_blocks[1] > 0) {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, many_lds<DT>());
+    hipLaunchKernelGGL(paged_many_kernel<DT>, dim3(A.max_blocks[1]), dim3(kT), many_lds<DT>(), st, A);
+    Q35_HIP_TRY(hipGetLastError());
+  }
+  hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((uint32_t)((qa + 3) / 4)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
   return Q35_OK;
 }
 
 }  // namespace
 
-size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) {
-  (void)nh; (void)nkv; (void)T; (void)B;
-  return 256;
-}
+size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) { return paged_layout(nh, nkv, T, B).bytes; }
 
 int paged_attn_launch(const PagedAttn& a, hipStream_t st) {
   return a.P.dtype == Q35_F32 ? launch<Q35_F32>(a, st) : a.P.dtype == Q35_F16 ? launch<Q35_F16>(a, st) : launch<Q35_BF16>(a, st);
