@@ -74,6 +74,7 @@ struct PlanHead {
 
 struct AttnArgs {
   PagedAttn c;
+  int32_t page_shift;     // log2 of the tokens per page
   int32_t rep, tok_many;  // query heads per kv head; tokens of a "many" tile
   int32_t max_tiles[2], max_blocks[2], part_rows[2];
   PlanHead* head;
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
     if (lane == 0) A.qmax[o] = m;
     return;
   }
-  const int page = a.table[(int64_t)s.b * a.ld_table + p / a.P.page];
+  const int page = a.table[(int64_t)s.b * a.ld_table + (p >> A.page_shift)];
   if ((uint32_t)page >= (uint32_t)a.P.n_pages) {
     if (lane == 0) raise_status(a.status, Q35_STATUS_ARG);
     return;
@@ -289,7 +290,7 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
   for (int j = 0; j < 4; ++j) x[d + j] = y[j];
   wave_lds_sync();
   E* kr = static_cast<E*>(a.P.data) + ((int64_t)a.layer * a.P.n_pages + page) * page_elts(a) +
-          ((int64_t)g * a.P.page + p % a.P.page) * kHd;
+          ((int64_t)g * a.P.page + (p & (a.P.page - 1))) * kHd;
   E* vr = kr + plane_elts(a);
   const float vv[4] = {v.x, v.y, v.z, v.w};
   E ko[4], vo[4];
@@ -307,7 +308,6 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
 
 // ------------------------------------------------------------------ shared by the attention kernels
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef float f16v __attribute__((ext_vector_type(16)));
 
 Q35_DEV float max_x32(float v) {  // the larger of lanes l and l ^ 32
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -339,8 +339,9 @@ Q35_DEV int find_tile(const AttnArgs& A, int k, int64_t u, int* sh) {
 }
 
 // Page of tokens j0 .. (16 of them share one); pages outside the pool count as page 0.
-Q35_DEV int page_of(const PagedAttn& a, const int32_t* row, int j0, bool* bad) {
-  const int v = __builtin_amdgcn_readfirstlane(row[j0 / a.P.page]);  // (j0 is the wave's)
+Q35_DEV int page_of(const AttnArgs& A, const int32_t* row, int j0, bool* bad) {
+  const PagedAttn& a = A.c;
+  const int v = __builtin_amdgcn_readfirstlane(row[j0 >> A.page_shift]);  // (j0 is the wave's)
   if ((uint32_t)v < (uint32_t)a.P.n_pages) return v;
   *bad = true;
   return 0;
@@ -422,8 +423,8 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
     // pages of the unit's two halves
     auto pages = [&](int k, int& pa, int& pb) {
       const int j0 = k * kUnit;
-      pa = page_of(a, row, j0, &bad);
-      pb = a.P.page > 16 || j0 + 16 >= end ? pa : page_of(a, row, j0 + 16, &bad);
+      pa = page_of(A, row, j0, &bad);
+      pb = a.P.page > 16 || j0 + 16 >= end ? pa : page_of(A, row, j0 + 16, &bad);
     };
     constexpr int kW = kWide ? 2 : 1;  // 16-byte words of 8 values
     q35_u32x4 kr[2][8 * kW], vr[8][2 * kW];
@@ -624,27 +625,28 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
 }
 
 // ------------------------------------------------------------------ many new tokens
-// A block takes one tile of up to 128 rows (token, query head of one kv head), 32 per wave, over some
-// units.  A unit's keys and values pass LDS, where all four waves read them: 4 waves with 32 columns of
-// queries each use every operand read from LDS for 128 columns, a quarter of the LDS's rate, and one wave
-// per SIMD has the registers for its queries (128 or 192) and outputs (128).  As above, S^T = K Q^T and
-// O^T += V^T P^T (32x32x16 products) keep a row's statistics in its lane pair and turn scores into
-// operands in place: score register i of lane half h is key 8 (i / 4) + 4 h + i % 4, so V^T's rows
-// list the keys in that order and eight consecutive registers are one operand.
+// A block takes one tile of up to 128 rows (token, query head of one kv head), 16 per wave, over some
+// units.  A unit's keys and values pass LDS, where all eight waves read them.  As above, S^T = K Q^T and
+// O^T += V^T P^T (16x16x32 products) keep a row's statistics in its lanes and turn scores into
+// operands in place.  16 rows are what leaves two waves a SIMD: a wave's queries (64 or 96 registers)
+// and outputs (64) stay in registers that the vector ALU reaches too (with 32 rows per wave, half the
+// LDS reads, and one wave per SIMD they did not: 2.5 ms instead of XX for 2048 tokens behind 14336).
 // While a unit is multiplied, the next one is on its way into registers; it is then laid out in the
 // other LDS buffer, so one barrier per unit is enough.
-// LDS: keys [key][32 pieces of 8 dims], piece c at c ^ (key & 7); values [dim][4 pieces of 8 keys], dim
-// d's row at d ^ ((d / 8) % 4) and piece c at c ^ ((d / 4 ^ d / 16) % 4): reads touch every bank once.
+// LDS: keys [key][32 pieces of 8 dims], piece c at c ^ (key & 7); values [dim][4 pieces of 8 keys], the keys
+// in the order of the weights' registers, dim d's row at d ^ (d / 16 % 4), piece c at c ^ (d / 4 % 4): what
+// lanes read or write at a time lies in different banks.
 // f16 caches are multiplied with 2 f16 halves of a query or weight, bf16 ones with 3 bf16 parts; f32
 // caches as 2 f16 halves with 2 (three products; what is dropped is 2^-22 of a term), under a power of
-// two for every 8 keys (a wave's share of the unit) and one for 8 values, whose inverse goes into the weights.
-constexpr int kRowsW = 32;
+// two for every 4 keys (a wave's share of the unit) and one for 4 values, whose inverse goes into the weights.
+constexpr int kMT = 512;       // threads
+constexpr int kRowsW = 16;     // rows of a wave
 constexpr int kPlane = 16384;  // bytes of a unit's keys (or values) of one part
 template <int DT>
 constexpr int many_lds() { return 2 * 2 * kPlane * (DT == Q35_F32 ? 2 : 1); }
 
 template <int DT>
-__global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
   constexpr bool kWide = DT == Q35_F32;
   constexpr int kQ = DT == Q35_BF16 ? 3 : 2;  // parts of a query or weight
@@ -652,12 +654,13 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
   // how far (log2) a score may pass the running maximum before the sums are rescaled: f16 weights
   // are kept 2^12 times larger and must stay below 2^16
   constexpr float kSlack = DT == Q35_BF16 ? 8.f : 3.f;
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
   const PagedAttn& a = A.c;
   extern __shared__ __align__(16) char lds[];  // [2 buffers][keys, values][part]
-  __shared__ float scl[2][2][4];               // [buffer][keys, values][group of 8 keys]
+  __shared__ float scl[2][2][8];               // [buffer][keys, values][group of 4 keys]
   __shared__ int sh;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 31, hf = lane >> 5;
+  const int n = lane & 15, g = lane >> 4, n32 = lane & 31, hf = lane >> 5;
   const int64_t W = A.head->w[1];
   const int G = A.head->blocks[1];
   if ((int)blockIdx.x >= G) return;
@@ -684,35 +687,32 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
     const int end = s.p0 + s.n;
     const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
     const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
-    // staging registers: keys 8 wid + 2 i + hf, dims 8 n ..; values: keys 8 wid + 4 hf + i, dims 8 n ..
-    q35_u32x4 kr[4][kKV], vr[4][kKV];
+    // staging registers: keys 4 wid + 2 i + hf, dims 8 n32 ..; values: keys 4 wid + i, dims 4 lane ..
+    q35_u32x4 kr[2][kKV];
+    typedef typename std::conditional<kWide, q35_u32x4, u2>::type VW;
+    VW vr[4];
     auto load_unit = [&](int k) {
-      const int j0 = k * kUnit + 8 * wid;  // (8 keys lie in one page)
-      const int pg = j0 < end ? page_of(a, row, j0, &bad) : page_of(a, row, k * kUnit, &bad);
-      const E* p = base + (int64_t)pg * page_elts(a) + (int64_t)(j0 & (a.P.page - 1)) * kHd + 8 * n;
+      const int j0 = k * kUnit + 4 * wid;  // (4 keys lie in one page)
+      const int pg = page_of(A, row, j0 < end ? j0 : k * kUnit, &bad);
+      const E* p = base + (int64_t)pg * page_elts(a) + (int64_t)(j0 & (a.P.page - 1)) * kHd;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int w = 0; w < kKV; ++w) kr[i][w] = *((const Q35_GLOBAL q35_u32x4*)(p + (2 * i + hf) * kHd) + w);
+        for (int w = 0; w < kKV; ++w) kr[i][w] = *((const Q35_GLOBAL q35_u32x4*)(p + (2 * i + hf) * kHd + 8 * n32) + w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int w = 0; w < kKV; ++w) vr[i][w] = *((const Q35_GLOBAL q35_u32x4*)(p + plane_elts(a) + (4 * hf + i) * kHd) + w);
+      for (int i = 0; i < 4; ++i) vr[i] = *(const Q35_GLOBAL VW*)(p + plane_elts(a) + i * kHd + 4 * lane);
     };
-    const int vpiece = ((wid >> 1) * 2 + hf), vhalf = wid & 1;
     auto store_unit = [&](int k, int buf) {
       if (k * kUnit + kUnit > end) {  // (uniform) rows behind the last token may hold anything
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (k * kUnit + 8 * wid + 2 * i + hf >= end) {
+        for (int i = 0; i < 2; ++i)
+          if (k * kUnit + 4 * wid + 2 * i + hf >= end) {
 #pragma unroll
             for (int w = 0; w < kKV; ++w) kr[i][w] = q35_u32x4{0, 0, 0, 0};
           }
-          if (k * kUnit + 8 * wid + 4 * hf + i >= end) {
 #pragma unroll
-            for (int w = 0; w < kKV; ++w) vr[i][w] = q35_u32x4{0, 0, 0, 0};
-          }
-        }
+        for (int i = 0; i < 4; ++i)
+          if (k * kUnit + 4 * wid + i >= end) vr[i] = VW(0);
       }
       char* kb = lds + buf * 2 * kKV * kPlane;
       char* vb = kb + kKV * kPlane;
@@ -722,18 +722,16 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int w = 0; w < 2; ++w)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              mk = fmaxf(mk, fabsf(__uint_as_float(kr[i][w][e])));
-              mv = fmaxf(mv, fabsf(__uint_as_float(vr[i][w][e])));
-            }
+          for (int e = 0; e < 4; ++e) {
+            mk = fmaxf(mk, fabsf(__uint_as_float(kr[i >> 1][i & 1][e])));
+            mv = fmaxf(mv, fabsf(__uint_as_float(vr[i][e])));
+          }
         mk = fmaxf(mk, row_ror<8>(mk)); mv = fmaxf(mv, row_ror<8>(mv));
         mk = fmaxf(mk, row_ror<4>(mk)); mv = fmaxf(mv, row_ror<4>(mv));
         mk = fmaxf(mk, row_ror<2>(mk)); mv = fmaxf(mv, row_ror<2>(mv));
         mk = fmaxf(mk, row_ror<1>(mk)); mv = fmaxf(mv, row_ror<1>(mv));
-        split_scale(max_x32(max_x16(mk)), fk, ik);
         mv = max_x32(max_x16(mv));
+        split_scale(max_x32(max_x16(mk)), fk, ik);
         split_scale(mv, fv, iv);
         iv = mv > 0.f ? fmaxf(iv, 7.888609e-31f) : 7.888609e-31f;  // (2^-100: zeros ask for no room)
         if (lane == 0) {
@@ -742,9 +740,9 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 8 * wid + 2 * i + hf;
-        char* dst = kb + key * 512 + (n ^ (key & 7)) * 16;
+      for (int i = 0; i < 2; ++i) {
+        const int key = 4 * wid + 2 * i + hf;
+        char* dst = kb + key * 512 + (n32 ^ (key & 7)) * 16;
         if constexpr (kWide) {
           q35_u32x4 hi, lo;
 #pragma unroll
@@ -760,29 +758,25 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
           *(q35_u32x4*)dst = kr[i][0];
         }
       }
+      // keys 4 wid .. of dim d: piece wid % 4 (the keys of the weights' lane group), half wid / 4
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int d = 8 * n + e;
-        char* dst = vb + (d ^ (n & 3)) * 64 + ((vpiece ^ ((d >> 2) ^ (d >> 4))) & 3) * 16 + vhalf * 8;
-        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+      for (int e = 0; e < 4; ++e) {
+        char* dst = vb + (4 * lane + (e ^ ((lane >> 2) & 3))) * 64 + (((wid ^ lane) & 3) * 16) + (wid >> 2) * 8;
         if constexpr (kWide) {
-          const float v0 = __uint_as_float(vr[0][e >> 2][e & 3]) * fv, v1 = __uint_as_float(vr[1][e >> 2][e & 3]) * fv;
-          const float v2 = __uint_as_float(vr[2][e >> 2][e & 3]) * fv, v3 = __uint_as_float(vr[3][e >> 2][e & 3]) * fv;
           uint32_t a0, a1, b0, b1;
-          split2(v0, v1, a0, a1);
-          split2(v2, v3, b0, b1);
+          split2(__uint_as_float(vr[0][e]) * fv, __uint_as_float(vr[1][e]) * fv, a0, a1);
+          split2(__uint_as_float(vr[2][e]) * fv, __uint_as_float(vr[3][e]) * fv, b0, b1);
           *(u2*)dst = u2{a0, b0};
           *(u2*)(dst + kPlane) = u2{a1, b1};
         } else {
           const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-          *(u2*)dst = u2{__builtin_amdgcn_perm(vr[1][0][e >> 1], vr[0][0][e >> 1], sel),
-                         __builtin_amdgcn_perm(vr[3][0][e >> 1], vr[2][0][e >> 1], sel)};
+          *(u2*)dst = u2{__builtin_amdgcn_perm(vr[1][e >> 1], vr[0][e >> 1], sel), __builtin_amdgcn_perm(vr[3][e >> 1], vr[2][e >> 1], sel)};
         }
       }
     };
     load_unit(k0);
-    // queries: column n, dims 16 st + 8 hf ..
-    q35_u32x4 qb[kQ][16];
+    // queries: column n, dims 32 st + 8 g ..
+    q35_u32x4 qb[kQ][8];
     float qscale = sl2;
     {
       const int64_t qi = (int64_t)(s.s0 + tok) * a.nh + h;
@@ -793,8 +787,8 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
         qscale = sl2 * inv;
       }
 #pragma unroll
-      for (int st = 0; st < 16; ++st) {
-        const float* qp = A.q + qi * kHd + 16 * st + 8 * hf;
+      for (int st = 0; st < 8; ++st) {
+        const float* qp = A.q + qi * kHd + 32 * st + 8 * g;
         const f4 v0 = *(const Q35_GLOBAL f4*)qp, v1 = *(const Q35_GLOBAL f4*)(qp + 4);
         const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
 #pragma unroll
@@ -808,14 +802,14 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
         }
       }
     }
-    f16v o[8];
+    f4 o[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    for (int i = 0; i < 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    float ov = DT == Q35_BF16 ? 1.f : 4096.f;  // o is kept this much larger (f32 caches: a power of two below the values')
+    float ov = DT == Q35_BF16 ? 1.f : 4096.f;  // o is kept this much larger (f32 caches: 2^12 over the values' powers of two)
     bool fresh = true;
+    // reads: key n (+ 16), pieces 4 st + g; dim 16 dt + n, piece g
+    const int ka_off = n * 512, kx = n & 7, va_off = n * 64 + ((g ^ (n >> 2)) & 3) * 16;
     for (int k = k0; k < k1; ++k) {
       const int buf = (k - k0) & 1;
       store_unit(k, buf);
@@ -825,108 +819,100 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
       if (!wave_on || j0 > lim1) continue;  // (uniform in the wave; the barrier above is passed by all)
       const char* kb = lds + buf * 2 * kKV * kPlane;
       const char* vb = kb + kKV * kPlane;
-      f16v sc;
+      f4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
+      for (int st = 0; st < 8; ++st) {
+        const char* src = kb + ka_off + ((4 * st + g) ^ kx) * 16;
 #pragma unroll
-      for (int st = 0; st < 16; ++st) {
-        const char* src = kb + n * 512 + ((2 * st + hf) ^ (n & 7)) * 16;
-        const q35_u32x4 ka = *(const q35_u32x4*)src;
-        if constexpr (DT == Q35_BF16) {
+        for (int tl = 0; tl < 2; ++tl) {
+          const q35_u32x4 ka = *(const q35_u32x4*)(src + tl * 16 * 512);
+          if constexpr (DT == Q35_BF16) {
 #pragma unroll
-          for (int q = 0; q < 3; ++q)
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(q35_b8, ka), __builtin_bit_cast(q35_b8, qb[q][st]), sc, 0, 0, 0);
-        } else {
-          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[0][st]), sc, 0, 0, 0);
-          sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[1][st]), sc, 0, 0, 0);
-          if constexpr (kWide) {
-            const q35_u32x4 kl = *(const q35_u32x4*)(src + kPlane);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, kl), __builtin_bit_cast(q35_h8, qb[0][st]), sc, 0, 0, 0);
+            for (int q = 0; q < 3; ++q)
+              sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, ka), __builtin_bit_cast(q35_b8, qb[q][st]), sc[tl], 0, 0, 0);
+          } else {
+            sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[0][st]), sc[tl], 0, 0, 0);
+            sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[1][st]), sc[tl], 0, 0, 0);
+            if constexpr (kWide) {
+              const q35_u32x4 kl = *(const q35_u32x4*)(src + tl * 16 * 512 + kPlane);
+              sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, kl), __builtin_bit_cast(q35_h8, qb[0][st]), sc[tl], 0, 0, 0);
+            }
           }
         }
       }
-      float fk[4], fp[4];
+      float fk[2] = {qscale, qscale}, fp[2] = {4096.f, 4096.f};
       float vscale = ov;
       if constexpr (kWide) {
         // the outputs' power of two: 2^12 over the largest values so far
         float iv = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          fk[q] = scl[buf][0][q] * qscale;
-          fp[q] = scl[buf][1][q];
-          iv = fmaxf(iv, fp[q]);
-        }
+        for (int q = 0; q < 8; ++q) iv = fmaxf(iv, scl[buf][1][q]);
         vscale = 4096.f * __uint_as_float((254u << 23) - __float_as_uint(iv));  // 2^12 / iv
         if (!fresh) vscale = fminf(vscale, ov);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) fp[q] *= vscale;  // 2^12 at most
+        for (int tl = 0; tl < 2; ++tl) {
+          fk[tl] = scl[buf][0][4 * tl + g] * qscale;
+          fp[tl] = scl[buf][1][4 * tl + g] * vscale;  // 2^12 at most
+        }
       }
       float bm = -INFINITY;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sc[e] *= kWide ? fk[e >> 2] : qscale;
-        if (j0 + kUnit - 1 > lim0) sc[e] = j0 + 8 * (e >> 2) + 4 * hf + (e & 3) <= lim ? sc[e] : -INFINITY;
-        bm = fmaxf(bm, sc[e]);
+      for (int e = 0; e < 8; ++e) {
+        float v = sc[e >> 2][e & 3] * fk[e >> 2];
+        if (j0 + kUnit - 1 > lim0) v = j0 + 16 * (e >> 2) + 4 * g + (e & 3) <= lim ? v : -INFINITY;
+        sc[e >> 2][e & 3] = v;
+        bm = fmaxf(bm, v);
       }
-      bm = max_x32(bm);
+      bm = max_x32(max_x16(bm));
       if (__ballot(bm > m + kSlack || (m == -INFINITY && bm > m)) || (kWide && vscale != ov)) {
         const float mn = fmaxf(m, bm);
         float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
         l *= al;
         m = mn;
-        if (!fresh) {
-          if constexpr (kWide) al *= vscale / ov;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) o[i] *= al;
-        }
+        if constexpr (kWide) al *= vscale / ov;
         ov = vscale;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] *= al;
       }
       fresh = false;
       const float mr = m == -INFINITY ? 0.f : m;
+      q35_u32x4 pw[kQ];
 #pragma unroll
-      for (int th = 0; th < 2; ++th) {
-        q35_u32x4 pw[kQ];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int e = 8 * th + 2 * j;
-          float p0 = __builtin_amdgcn_exp2f(sc[e] - mr), p1 = __builtin_amdgcn_exp2f(sc[e + 1] - mr);
-          l += p0 + p1;
-          if constexpr (kWide) {
-            p0 *= fp[e >> 2];
-            p1 *= fp[e >> 2];
-          } else if constexpr (DT == Q35_F16) {
-            p0 *= 4096.f;
-            p1 *= 4096.f;
-          }
-          uint32_t w0, w1, w2 = 0;
-          if constexpr (kQ == 2) split2(p0, p1, w0, w1);
-          else split3(p0, p1, w0, w1, w2);
-          pw[0][j] = w0;
-          pw[1][j] = w1;
-          if constexpr (kQ == 3) pw[2][j] = w2;
+      for (int j = 0; j < 4; ++j) {
+        const int e = 2 * j;
+        float p0 = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - mr), p1 = __builtin_amdgcn_exp2f(sc[e >> 2][(e & 3) + 1] - mr);
+        l += p0 + p1;
+        if constexpr (DT != Q35_BF16) {
+          p0 *= fp[e >> 2];
+          p1 *= fp[e >> 2];
         }
+        uint32_t w0, w1, w2 = 0;
+        if constexpr (kQ == 2) split2(p0, p1, w0, w1);
+        else split3(p0, p1, w0, w1, w2);
+        pw[0][j] = w0;
+        pw[1][j] = w1;
+        if constexpr (kQ == 3) pw[2][j] = w2;
+      }
 #pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          const int d = 32 * dt + n;
-          const char* src = vb + (d ^ ((d >> 3) & 3)) * 64 + (((2 * th + hf) ^ ((d >> 2) ^ (d >> 4))) & 3) * 16;
-          const q35_u32x4 va = *(const q35_u32x4*)src;
-          if constexpr (DT == Q35_BF16) {
+      for (int dt = 0; dt < 16; ++dt) {
+        const char* src = vb + (va_off ^ ((dt & 3) * 64)) + dt * 1024;
+        const q35_u32x4 va = *(const q35_u32x4*)src;
+        if constexpr (DT == Q35_BF16) {
 #pragma unroll
-            for (int q = 0; q < 3; ++q)
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(q35_b8, va), __builtin_bit_cast(q35_b8, pw[q]), o[dt], 0, 0, 0);
-          } else {
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
-            o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[1]), o[dt], 0, 0, 0);
-            if constexpr (kWide) {
-              const q35_u32x4 vl = *(const q35_u32x4*)(src + kPlane);
-              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(q35_h8, vl), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
-            }
+          for (int q = 0; q < 3; ++q)
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, va), __builtin_bit_cast(q35_b8, pw[q]), o[dt], 0, 0, 0);
+        } else {
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
+          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[1]), o[dt], 0, 0, 0);
+          if constexpr (kWide) {
+            const q35_u32x4 vl = *(const q35_u32x4*)(src + kPlane);
+            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, vl), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
           }
         }
       }
     }
-    // register 4 q + e of o[dt] is dim 32 dt + 8 q + 4 hf + e
-    l = add_x32(l);
+    // register e of o[dt] is dim 16 dt + 4 g + e
+    l = add_x32(add_x16(l));
     const bool whole = k0 == 0 && k1 == t.units;
     if (wid * kRowsW + n < rows) {
       const float f = (whole ? 1.f / l : 1.f) / ov;
@@ -935,19 +921,17 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
       const int64_t pi = (int64_t)(2 * blockIdx.x + (seg == 0 ? 0 : 1)) * A.part_rows[1] + r;
       float* dst = whole ? a.out + tr * a.ld_out + (int64_t)h * kHd : A.part_o[1] + pi * kHd;
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt)
+      for (int dt = 0; dt < 16; ++dt) {
+        const int d = 16 * dt + 4 * g;
+        f4 y = o[dt] * f;
+        if (whole) {
+          const f4 gv = *(const f4*)(gate + d);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int d = 32 * dt + 8 * q + 4 * hf;
-          f4 y = {o[dt][4 * q] * f, o[dt][4 * q + 1] * f, o[dt][4 * q + 2] * f, o[dt][4 * q + 3] * f};
-          if (whole) {
-            const f4 gv = *(const f4*)(gate + d);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] *= sigmoid_f(gv[e]);
-          }
-          *(f4*)(dst + d) = y;
+          for (int e = 0; e < 4; ++e) y[e] *= sigmoid_f(gv[e]);
         }
-      if (!whole && hf == 0) {
+        *(f4*)(dst + d) = y;
+      }
+      if (!whole && g == 0) {
         A.part_ml[1][2 * pi] = m;
         A.part_ml[1][2 * pi + 1] = l;
       }
@@ -959,15 +943,19 @@ __global__ __launch_bounds__(kT, 1) void paged_many_kernel(const AttnArgs A) {
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
 }
 
-// A wave per (row, query head): joins the parts of its tile, if the plan cut it.
-template <int DT>
+// Joins the parts of a row's tile, if the plan cut it: kJW waves per (row, query head), each taking every
+// kJW-th part, eight of them in flight.
+template <int DT, int kJW>
 __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
   const PagedAttn& a = A.c;
-  const int lane = threadIdx.x & 63;
-  const int64_t item = (int64_t)blockIdx.x * (kT / 64) + (threadIdx.x >> 6);
+  __shared__ __align__(16) float ys[kJW > 1 ? kT / 64 : 1][kHd];
+  __shared__ float ls[kT / 64];
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), jw = wid % kJW;
+  const int64_t item = (int64_t)blockIdx.x * (kT / 64 / kJW) + wid / kJW;
   const int64_t t = item / a.nh;
   const int h = (int)(item % a.nh);
   Seq s;
+  // (kJW > 1: the block's waves share their item, and leave together)
   if (t >= a.T || !find_seq(a, (int)t, &s)) return;
   const int kind = kind_of<DT>(A, s.n), gk = h / A.rep, hr = h % A.rep, tok = (int)t - s.s0;
   const int pair = tok * A.rep + hr;
@@ -978,30 +966,51 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
   const Tile tl = A.tiles[kind][x];
   const int64_t W = A.head->w[kind], u0 = tl.u0 + (int64_t)gk * tl.units;
   const int G = A.head->blocks[kind];
-  const int g0 = unit_block(W, G, u0), g1 = unit_block(W, G, u0 + tl.units - 1);
-  if (g0 == g1) return;
+  const int g0 = unit_block(W, G, u0), np = unit_block(W, G, u0 + tl.units - 1) - g0 + 1;
+  if (np == 1) return;
   const int first = block_u0(W, G, g0) == u0 ? 0 : 1;
+  auto slot = [&](int q) { return (int64_t)(2 * (g0 + q) + (q == 0 ? first : 0)) * A.part_rows[kind] + r; };
+  const float* ml = A.part_ml[kind];
+  const f4 gv = *(const f4*)(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + 4 * lane);
   float M = -INFINITY;
-  for (int gb = g0; gb <= g1; ++gb) {
-    const int64_t pi = (int64_t)(2 * gb + (gb == g0 ? first : 0)) * A.part_rows[kind] + r;
-    M = fmaxf(M, A.part_ml[kind][2 * pi]);
-  }
+  for (int q = lane; q < np; q += 64) M = fmaxf(M, ml[2 * slot(q)]);
+#pragma unroll
+  for (int e = 32; e > 0; e >>= 1) M = fmaxf(M, __shfl_xor(M, e, 64));
   float L = 0.f;
   f4 y = {0.f, 0.f, 0.f, 0.f};
-  for (int gb = g0; gb <= g1; ++gb) {
-    const int64_t pi = (int64_t)(2 * gb + (gb == g0 ? first : 0)) * A.part_rows[kind] + r;
-    const float mg = A.part_ml[kind][2 * pi];
-    if (mg == -INFINITY) continue;  // (nothing of that part was in sight of this row)
-    const float f = __builtin_amdgcn_exp2f(mg - M);
-    L += A.part_ml[kind][2 * pi + 1] * f;
-    y += *(const f4*)(A.part_o[kind] + pi * kHd + 4 * lane) * f;
+  for (int q0 = jw; q0 < np; q0 += 8 * kJW) {
+    f4 v[8];
+    float w[8], lw[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int64_t o = slot(min(q0 + e * kJW, np - 1));
+      v[e] = *(const Q35_GLOBAL f4*)(A.part_o[kind] + o * kHd + 4 * lane);
+      w[e] = ml[2 * o];
+      lw[e] = ml[2 * o + 1];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      // (a part none of whose tokens the row sees has the maximum -inf and zeros)
+      const float f = q0 + e * kJW < np ? __builtin_amdgcn_exp2f(w[e] - M) : 0.f;
+      L += lw[e] * f;
+      y += v[e] * f;
+    }
   }
-  const f4 gv = *(const f4*)(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + 4 * lane);
+  if constexpr (kJW > 1) {
+    *(f4*)&ys[wid][4 * lane] = y;
+    if (lane == 0) ls[wid] = L;
+    __syncthreads();
+    if (wid != 0) return;
+#pragma unroll
+    for (int w = 1; w < kJW; ++w) {
+      y += *(const f4*)&ys[w][4 * lane];
+      L += ls[w];
+    }
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = y[e] / L * sigmoid_f(gv[e]);
   *(f4*)(a.out + t * a.ld_out + (int64_t)h * kHd + 4 * lane) = y;
 }
-
 
 struct PagedLayout {
   int32_t max_tiles[2], max_blocks[2], part_rows[2];
@@ -1041,6 +1050,7 @@ int launch(const PagedAttn& a, hipStream_t st) {
   const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B);
   AttnArgs A;
   A.c = a;
+  A.page_shift = __builtin_ctz((unsigned)a.P.page);
   A.rep = a.nh / a.nkv;
   A.tok_many = kManyRows / A.rep;
   char* p = static_cast<char*>(a.ws);
@@ -1070,10 +1080,12 @@ int launch(const PagedAttn& a, hipStream_t st) {
   Q35_HIP_TRY(hipGetLastError());
   if (A.max_blocks[1] > 0) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, many_lds<DT>());
-    hipLaunchKernelGGL(paged_many_kernel<DT>, dim3(A.max_blocks[1]), dim3(kT), many_lds<DT>(), st, A);
+    hipLaunchKernelGGL(paged_many_kernel<DT>, dim3(A.max_blocks[1]), dim3(kMT), many_lds<DT>(), st, A);
     Q35_HIP_TRY(hipGetLastError());
   }
-  hipLaunchKernelGGL(paged_join_kernel<DT>, dim3((uint32_t)((qa + 3) / 4)), dim3(kT), 0, st, A);
+  // few rows: their parts are many, or the chip is empty
+  if (qa <= 4096) hipLaunchKernelGGL((paged_join_kernel<DT, 4>), dim3((uint32_t)qa), dim3(kT), 0, st, A);
+  else hipLaunchKernelGGL((paged_join_kernel<DT, 1>), dim3((uint32_t)((qa + 3) / 4)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
   return Q35_OK;
 }
