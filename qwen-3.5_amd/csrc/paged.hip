@@ -633,9 +633,10 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
 // LDS reads, and one wave per SIMD they did not: 2.5 ms instead of XX for 2048 tokens behind 14336).
 // While a unit is multiplied, the next one is on its way into registers; it is then laid out in the
 // other LDS buffer, so one barrier per unit is enough.
-// LDS: keys [key][32 pieces of 8 dims], piece c at c ^ (key & 7); values [dim][4 pieces of 8 keys], the keys
-// in the order of the weights' registers, dim d's row at d ^ (d / 16 % 4), piece c at c ^ (d / 4 % 4): what
-// lanes read or write at a time lies in different banks.
+// LDS: keys [key][32 pieces of 8 dims], piece c at c ^ (key & 15); values [dim][4 pieces of 8 keys], the keys
+// in the order of the weights' registers, dim d's row at d ^ (d / 16 % 4), piece c at c ^ (-(d / 4) % 4): a
+// 16-byte read serves lanes 0-3, 12-15, 20-23, 24-27 at a time, then 4-11, 16-19, 28-31, and so does the
+// upper half; these places lie in different banks each time.
 // f16 caches are multiplied with 2 f16 halves of a query or weight, bf16 ones with 3 bf16 parts; f32
 // caches as 2 f16 halves with 2 (three products; what is dropped is 2^-22 of a term), under a power of
 // two for every 4 keys (a wave's share of the unit) and one for 4 values, whose inverse goes into the weights.
@@ -646,7 +647,13 @@ template <int DT>
 constexpr int many_lds() { return 2 * 2 * kPlane * (DT == Q35_F32 ? 2 : 1); }
 
 template <int DT>
-__global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
+Q35_DEV f4 mma(q35_u32x4 x, q35_u32x4 y, f4 c) {
+  if constexpr (DT == Q35_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, x), __builtin_bit_cast(q35_b8, y), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, x), __builtin_bit_cast(q35_h8, y), c, 0, 0, 0);
+}
+
+template <int DT>
+__global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_many_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
   constexpr bool kWide = DT == Q35_F32;
   constexpr int kQ = DT == Q35_BF16 ? 3 : 2;  // parts of a query or weight
@@ -742,7 +749,7 @@ __global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int key = 4 * wid + 2 * i + hf;
-        char* dst = kb + key * 512 + (n32 ^ (key & 7)) * 16;
+        char* dst = kb + key * 512 + (n32 ^ (key & 15)) * 16;
         if constexpr (kWide) {
           q35_u32x4 hi, lo;
 #pragma unroll
@@ -761,7 +768,7 @@ __global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
       // keys 4 wid .. of dim d: piece wid % 4 (the keys of the weights' lane group), half wid / 4
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        char* dst = vb + (4 * lane + (e ^ ((lane >> 2) & 3))) * 64 + (((wid ^ lane) & 3) * 16) + (wid >> 2) * 8;
+        char* dst = vb + (4 * lane + (e ^ ((lane >> 2) & 3))) * 64 + (((wid ^ -lane) & 3) * 16) + (wid >> 2) * 8;
         if constexpr (kWide) {
           uint32_t a0, a1, b0, b1;
           split2(__uint_as_float(vr[0][e]) * fv, __uint_as_float(vr[1][e]) * fv, a0, a1);
@@ -809,7 +816,10 @@ __global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
     float ov = DT == Q35_BF16 ? 1.f : 4096.f;  // o is kept this much larger (f32 caches: 2^12 over the values' powers of two)
     bool fresh = true;
     // reads: key n (+ 16), pieces 4 st + g; dim 16 dt + n, piece g
-    const int ka_off = n * 512, kx = n & 7, va_off = n * 64 + ((g ^ (n >> 2)) & 3) * 16;
+    int ka_off[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ka_off[i] = n * 512 + ((4 * i + g) ^ n) * 16;
+    const int va_off = n * 64 + ((g ^ -(n >> 2)) & 3) * 16;
     for (int k = k0; k < k1; ++k) {
       const int buf = (k - k0) & 1;
       store_unit(k, buf);
@@ -822,24 +832,34 @@ __global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
       f4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
       for (int st = 0; st < 8; ++st) {
-        const char* src = kb + ka_off + ((4 * st + g) ^ kx) * 16;
+        const char* src = kb + ka_off[st & 3] + (st >> 2) * 256;
+        q35_u32x4 ka[2][kKV];
 #pragma unroll
-        for (int tl = 0; tl < 2; ++tl) {
-          const q35_u32x4 ka = *(const q35_u32x4*)(src + tl * 16 * 512);
-          if constexpr (DT == Q35_BF16) {
+        for (int w = 0; w < kKV; ++w)
 #pragma unroll
-            for (int q = 0; q < 3; ++q)
-              sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, ka), __builtin_bit_cast(q35_b8, qb[q][st]), sc[tl], 0, 0, 0);
-          } else {
-            sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[0][st]), sc[tl], 0, 0, 0);
-            sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, ka), __builtin_bit_cast(q35_h8, qb[1][st]), sc[tl], 0, 0, 0);
-            if constexpr (kWide) {
-              const q35_u32x4 kl = *(const q35_u32x4*)(src + tl * 16 * 512 + kPlane);
-              sc[tl] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, kl), __builtin_bit_cast(q35_h8, qb[0][st]), sc[tl], 0, 0, 0);
-            }
-          }
+          for (int tl = 0; tl < 2; ++tl) ka[tl][w] = *(const q35_u32x4*)(src + tl * 16 * 512 + w * kPlane);
+        // (the two tiles in turn: a product does not wait for the one before it)
+#pragma unroll
+        for (int q = 0; q < kQ; ++q)
+#pragma unroll
+          for (int tl = 0; tl < 2; ++tl) sc[tl] = mma<DT>(ka[tl][0], qb[q][st], sc[tl]);
+        if constexpr (kWide) {
+#pragma unroll
+          for (int tl = 0; tl < 2; ++tl) sc[tl] = mma<DT>(ka[tl][1], qb[0][st], sc[tl]);
         }
       }
+      // operands are read kAhead steps before their products
+      constexpr int kAhead = kWide ? 1 : 2;
+      constexpr int kKr = 2 * kKV, kKm = 2 * (kWide ? 3 : kQ);  // reads and products of a step
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead * kKr, 0);
+#pragma unroll
+      for (int st = 0; st < 8 - kAhead; ++st) {
+        __builtin_amdgcn_sched_group_barrier(0x008, kKm / 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kKr / 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, kKm / 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kKr / 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kKm, 0);
       float fk[2] = {qscale, qscale}, fp[2] = {4096.f, 4096.f};
       float vscale = ov;
       if constexpr (kWide) {
@@ -894,22 +914,32 @@ __global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
         if constexpr (kQ == 3) pw[2][j] = w2;
       }
 #pragma unroll
-      for (int dt = 0; dt < 16; ++dt) {
-        const char* src = vb + (va_off ^ ((dt & 3) * 64)) + dt * 1024;
-        const q35_u32x4 va = *(const q35_u32x4*)src;
-        if constexpr (DT == Q35_BF16) {
+      for (int dt = 0; dt < 16; dt += 2) {
+        q35_u32x4 va[2][kKV];
 #pragma unroll
-          for (int q = 0; q < 3; ++q)
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, va), __builtin_bit_cast(q35_b8, pw[q]), o[dt], 0, 0, 0);
-        } else {
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
-          o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, va), __builtin_bit_cast(q35_h8, pw[1]), o[dt], 0, 0, 0);
-          if constexpr (kWide) {
-            const q35_u32x4 vl = *(const q35_u32x4*)(src + kPlane);
-            o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, vl), __builtin_bit_cast(q35_h8, pw[0]), o[dt], 0, 0, 0);
-          }
+        for (int w = 0; w < kKV; ++w)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            va[i][w] = *(const q35_u32x4*)(vb + (va_off ^ (((dt + i) & 3) * 64)) + (dt + i) * 1024 + w * kPlane);
+#pragma unroll
+        for (int q = 0; q < kQ; ++q)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) o[dt + i] = mma<DT>(va[i][0], pw[q], o[dt + i]);
+        if constexpr (kWide) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) o[dt + i] = mma<DT>(va[i][1], pw[0], o[dt + i]);
         }
       }
+      constexpr int kVm = 2 * (kWide ? 3 : kQ), kVr = 2 * kKV, kAheadV = kWide ? 1 : 2;  // of two dims' tiles
+      __builtin_amdgcn_sched_group_barrier(0x100, kAheadV * kVr, 0);
+#pragma unroll
+      for (int dt = 0; dt < 8 - kAheadV; ++dt) {
+        __builtin_amdgcn_sched_group_barrier(0x008, kVm / 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kVr / 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, kVm / 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kVr / 2, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kAheadV * kVm, 0);
     }
     // register e of o[dt] is dim 16 dt + 4 g + e
     l = add_x32(add_x16(l));
@@ -920,16 +950,24 @@ __global__ __launch_bounds__(kMT, 2) void paged_many_kernel(const AttnArgs A) {
       const float* gate = a.qg + tr * a.ld_qg + (int64_t)h * 2 * kHd + kHd;
       const int64_t pi = (int64_t)(2 * blockIdx.x + (seg == 0 ? 0 : 1)) * A.part_rows[1] + r;
       float* dst = whole ? a.out + tr * a.ld_out + (int64_t)h * kHd : A.part_o[1] + pi * kHd;
+      // (the empty asm keeps these addresses from being formed before the loop, where they cost its operands
+      // their registers)
+      int ge = 4 * g;
+      asm volatile("" : "+v"(ge));
+      gate += ge;
+      dst += ge;
+      if (whole) {
 #pragma unroll
-      for (int dt = 0; dt < 16; ++dt) {
-        const int d = 16 * dt + 4 * g;
-        f4 y = o[dt] * f;
-        if (whole) {
-          const f4 gv = *(const f4*)(gate + d);
+        for (int dt = 0; dt < 16; ++dt) {
+          const f4 gv = *(const f4*)(gate + 16 * dt);
+          f4 y = o[dt] * f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) y[e] *= sigmoid_f(gv[e]);
+          *(f4*)(dst + 16 * dt) = y;
         }
-        *(f4*)(dst + d) = y;
+      } else {
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt) *(f4*)(dst + 16 * dt) = o[dt] * f;
       }
       if (!whole && g == 0) {
         A.part_ml[1][2 * pi] = m;
