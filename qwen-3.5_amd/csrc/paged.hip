@@ -49,35 +49,31 @@ Q35_DEV bool find_seq(const PagedAttn& a, int t, Seq* s) {
 // of its part, and the merge kernel joins the parts; only the first and the last tile of a block can be
 // cut, so two slots per block hold them all.
 //
-// Two kinds of tiles: sequences of a token or two ("few": the cache's stream bounds them) and chunks
-// ("many": the matrix cores do).
-constexpr int kUnit = 32;      // tokens of a unit
-constexpr int kMinUnits = 4;   // units a block takes at least
-constexpr int kManyRows = 128; // query rows (token, head) of a "many" tile
+// Two kinds of tiles: sequences of few rows ("few": the cache's stream bounds them) and chunks ("many":
+// the matrix cores do).
+constexpr int kUnit = 32;       // tokens of a unit
+constexpr int kFewRows = 16;    // query rows (token, head) of a "few" tile
+constexpr int kManyRows = 128;  // of a "many" tile
+constexpr int kFewMost = 2 * kFewRows;  // sequences of at most this many rows (or one token) are "few"
 
-template <int DT>
-struct Kind {
-  // parts of a query value (and of a weight): f16 products take two f16 halves, bf16 three bf16 values,
-  // and f32 caches are split into three bf16 values themselves
-  static constexpr int kParts = DT == Q35_F16 ? 2 : 3;
-  static constexpr int kPairs = kParts == 2 ? 8 : 4;  // (token, head) pairs of a "few" tile: its parts share 16 columns
-};
-
+// All that a block needs to know of a tile, in one load
 struct Tile {
-  int64_t u0;  // its first unit
-  int32_t b, i, units, pad;
+  int64_t u0;                       // its first unit
+  int32_t units, b, i, s0, n, p0;   // units per kv head; sequence, tile of it, its first row, rows, cached tokens
 };
+// The plan of one kind: block g starts at unit g q + min(g, r)
 struct PlanHead {
-  int64_t w[2];      // units: few, many
-  int32_t tiles[2], blocks[2];
+  int64_t w, q;  // units of all tiles
+  int32_t r, tiles, blocks, pad;
 };
 
 struct AttnArgs {
   PagedAttn c;
   int32_t page_shift;     // log2 of the tokens per page
   int32_t rep, tok_many;  // query heads per kv head; tokens of a "many" tile
+  uint32_t rep_inv;
   int32_t max_tiles[2], max_blocks[2], part_rows[2];
-  PlanHead* head;
+  PlanHead* head;        // [2]
   float* q;              // [T][heads][256] queries after norm and rotary
   float* qmax;           // [T][heads] largest |value|
   int32_t* tile0;        // [2][B] first tile of the sequence in the list of each kind
@@ -86,23 +82,28 @@ struct AttnArgs {
   float* part_o[2];      // [2 max_blocks][part_rows][256]
 };
 
-template <int DT>
-Q35_DEV int kind_of(const AttnArgs& A, int n) { return n == 1 || n * A.rep <= 2 * Kind<DT>::kPairs ? 0 : 1; }
-template <int DT>
+Q35_DEV int kind_of(const AttnArgs& A, int n) { return n == 1 || n * A.rep <= kFewMost ? 0 : 1; }
+// x / rep for x < 2^28 (rep_inv = 2^32 / rep + 1)
+Q35_DEV int div_rep(const AttnArgs& A, int x) { return A.rep == 1 ? x : (int)__umulhi((uint32_t)x, A.rep_inv); }
 Q35_DEV int tiles_of(const AttnArgs& A, int n) {
   if (n <= 0) return 0;
-  const int per = kind_of<DT>(A, n) ? A.tok_many : Kind<DT>::kPairs;
-  return ((kind_of<DT>(A, n) ? n : n * A.rep) + per - 1) / per;
+  return kind_of(A, n) ? (n + A.tok_many - 1) / A.tok_many : (n * A.rep + kFewRows - 1) / kFewRows;
 }
 // cached tokens that tile i of the sequence looks at
-template <int DT>
 Q35_DEV int tile_len(const AttnArgs& A, const Seq& s, int i) {
-  const int tok = kind_of<DT>(A, s.n) ? (i + 1) * A.tok_many - 1 : ((i + 1) * Kind<DT>::kPairs - 1) / A.rep;
+  const int tok = kind_of(A, s.n) ? (i + 1) * A.tok_many - 1 : div_rep(A, (i + 1) * kFewRows - 1);
   return s.p0 + min(tok, s.n - 1) + 1;
 }
 // first unit of block g, and the block that holds unit u
-Q35_DEV int64_t block_u0(int64_t w, int blocks, int g) { return w * g / blocks; }
-Q35_DEV int unit_block(int64_t w, int blocks, int64_t u) { return (int)(((u + 1) * blocks - 1) / w); }
+Q35_DEV int64_t block_u0(const PlanHead& h, int g) { return h.q * g + min(g, h.r); }
+Q35_DEV int unit_block(const PlanHead& h, int64_t u) {
+  const int64_t big = h.r * (h.q + 1);  // the first r blocks take q + 1 units
+  const int64_t x = u < big ? u : u - h.r, y = u < big ? h.q + 1 : h.q;
+  int64_t g = (int64_t)((double)x / (double)y);
+  if (g * y > x) --g;
+  else if ((g + 1) * y <= x) ++g;
+  return (int)g;
+}
 
 // exclusive sum over the block's kT threads
 template <class V>
@@ -128,7 +129,6 @@ Q35_DEV V plan_excl(V v, V* sh, V* total) {
 }
 
 // Made by one block: the sequences' tiles, then each tile's first unit.
-template <int DT>
 Q35_DEV void make_plan(const AttnArgs& A) {
   const PagedAttn& a = A.c;
   __shared__ int si[kT / 64];
@@ -141,7 +141,7 @@ Q35_DEV void make_plan(const AttnArgs& A) {
     int nt[2] = {0, 0};
     if (b < a.B) {
       Seq s;
-      if (load_seq(a, b, &s)) nt[kind_of<DT>(A, s.n)] = tiles_of<DT>(A, s.n);
+      if (load_seq(a, b, &s)) nt[kind_of(A, s.n)] = tiles_of(A, s.n);
       else bad = true;
       falls |= s.n < 0;
     }
@@ -163,7 +163,7 @@ Q35_DEV void make_plan(const AttnArgs& A) {
     int64_t run = 0;
     for (int x0 = 0; x0 < nt; x0 += kT) {
       const int x = x0 + tid;
-      Tile t = {0, 0, 0, 0, 0};
+      Tile t = {0, 0, 0, 0, 0, 0, 0};
       if (x < nt) {
         // the last sequence with tile0 <= x: those without tiles of this kind share the next one's number
         int lo = 0, hi = a.B;
@@ -176,7 +176,10 @@ Q35_DEV void make_plan(const AttnArgs& A) {
         load_seq(a, lo, &s);
         t.b = lo;
         t.i = x - tile0[lo];
-        t.units = (tile_len<DT>(A, s, t.i) + kUnit - 1) / kUnit;
+        t.units = (tile_len(A, s, t.i) + kUnit - 1) / kUnit;
+        t.s0 = s.s0;
+        t.n = s.n;
+        t.p0 = s.p0;
       }
       int64_t all;
       t.u0 = run + plan_excl((int64_t)t.units * a.nkv, sl, &all);
@@ -184,10 +187,10 @@ Q35_DEV void make_plan(const AttnArgs& A) {
       run += all;
     }
     if (tid == 0) {
-      A.head->w[k] = run;
-      A.head->tiles[k] = nt;
-      const int64_t most = (run + kMinUnits - 1) / kMinUnits;
-      A.head->blocks[k] = (int)(most < A.max_blocks[k] ? most : A.max_blocks[k]);
+      // (a "many" block takes four units at least: what it leaves to the join costs about one)
+      const int64_t least = k ? 4 : 1, most = (run + least - 1) / least;
+      const int64_t blocks = most < A.max_blocks[k] ? most : A.max_blocks[k];
+      A.head[k] = PlanHead{run, blocks ? run / blocks : 0, blocks ? (int)(run % blocks) : 0, nt, (int)blocks, 0};
     }
   }
 }
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
   const PagedAttn& a = A.c;
   __shared__ double xs[kT / 64][kHd];
   if (blockIdx.x == 0) {
-    make_plan<DT>(A);
+    make_plan(A);
     return;
   }
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, per = a.nkv + a.nh;
@@ -325,17 +328,28 @@ Q35_DEV float add_x16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// The tile that holds unit u: every thread looks at some (they are few and in order).
-Q35_DEV int find_tile(const AttnArgs& A, int k, int64_t u, int* sh) {
-  const int nt = A.head->tiles[k];
-  for (int x = threadIdx.x; x < nt; x += blockDim.x) {
-    const Tile t = A.tiles[k][x];
-    if (t.u0 <= u && u < t.u0 + (int64_t)t.units * A.c.nkv) *sh = x;
+// The block's first tile, the one that holds unit u: every thread looks at some (they are few).  The first
+// ones are asked for before the plan's head has arrived.
+struct Start {
+  Tile t;
+  int x;
+};
+Q35_DEV bool block_start(const AttnArgs& A, int k, PlanHead* head, Start* sh) {
+  const int x0 = threadIdx.x;
+  Tile t;
+  if (x0 < A.max_tiles[k]) t = A.tiles[k][x0];
+  *head = A.head[k];
+  if ((int)blockIdx.x >= head->blocks) return false;
+  const int64_t u = block_u0(*head, blockIdx.x);
+  for (int x = x0; x < head->tiles; x += blockDim.x) {
+    if (x != x0) t = A.tiles[k][x];
+    if (t.u0 <= u && u < t.u0 + (int64_t)t.units * A.c.nkv) {
+      sh->t = t;
+      sh->x = x;
+    }
   }
   __syncthreads();
-  const int x = *sh;
-  __syncthreads();
-  return x;
+  return true;
 }
 
 // Page of tokens j0 .. (16 of them share one); pages outside the pool count as page 0.
@@ -348,76 +362,58 @@ Q35_DEV int page_of(const AttnArgs& A, const int32_t* row, int j0, bool* bad) {
 }
 
 // ------------------------------------------------------------------ few new tokens
-// A block takes one tile - up to 4 (8) pairs of token and query head of a kv head - over some units; its
-// 4 waves take every 4th unit, each with its own running softmax, and are joined at the end.
+// A block takes one tile - up to 16 rows (token, query head) of a kv head - over some units; its 4 waves
+// take every 4th unit, each with its own running softmax, and are joined at the end.
 //
-// The keys of a unit go from the cache straight into the operand registers of S^T = K Q^T (16x16x32
-// matrix products: keys in rows, pairs in columns), its values into those of O^T += V^T P^T: the scores
-// come out where the weights are needed as operands, a pair's maximum and sum stay in its lanes, and
-// nothing passes LDS between the two products.  The order of the summed index is free as long as both
-// operands share it: the k-slot (lane group g, j) of the second product stands for key 4 g + j (j < 4) or
-// 16 + 4 g + j - 4, the lanes that hold those scores; and a value row's 16-byte pieces are dealt to
-// lanes so that each holds 8 keys of the same 8 dims, which a byte permute turns into operands.
-// A query value is carried whole, as 2 f16 or 3 bf16 parts in 2 or 3 of the 16 columns: a tile of
-// 4 pairs fills the columns that its pairs alone would leave empty, and the parts' sums are added
-// by lane rotations (the scores) or once at the end (the outputs).  Weights are split the same way.
-// An f32 cache's values are split into three bf16 values as they arrive, so all products are f32's.
+// The keys of a unit go from the cache straight into the operand registers of S^T = K Q^T (keys in rows,
+// query rows in columns), its values into those of O^T += V^T P^T: the scores come out where the weights
+// are needed as operands, a row's maximum and sum stay in its lanes, and nothing passes LDS between the
+// two products.  The order of the summed index is free as long as both operands share it: with 16-bit
+// caches the k-slot (lane group g, j) of the second product (16x16x32) stands for key 4 g + j (j < 4) or
+// 16 + 4 g + j - 4, the lanes that hold those scores, and a value row's 16-byte pieces are dealt to
+// lanes so that each holds 8 keys of the same 8 dims, which a byte permute turns into operands.  f32
+// caches are multiplied in f32 (16x16x4).
+// A query value and a weight are carried whole, as 2 f16 or 3 bf16 parts with a product each; the matrix
+// cores have time for that: the bound is the cache's stream.
+// A block's first unit waits for the instructions too: code that runs once is fetched at about 64 bytes
+// in 35 ns, so the loops' bodies are kept short.
+template <int DT>
+Q35_DEV f4 mma(q35_u32x4 x, q35_u32x4 y, f4 c) {
+  if constexpr (DT == Q35_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, x), __builtin_bit_cast(q35_b8, y), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, x), __builtin_bit_cast(q35_h8, y), c, 0, 0, 0);
+}
+constexpr int kFewLd = kHd + 4;
+constexpr int kFewLds = 4 * kFewRows * kFewLd * 4;
+
 template <int DT>
 __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
-  constexpr int kPairs = Kind<DT>::kPairs, kParts = Kind<DT>::kParts;
   constexpr bool kWide = DT == Q35_F32;
-  constexpr int kLd = kHd + 4;
+  constexpr int kQ = kWide ? 1 : DT == Q35_F16 ? 2 : 3;  // parts of a query or weight
+  constexpr int kW = kWide ? 2 : 1;                       // 16-byte words of 8 values
   const PagedAttn& a = A.c;
-  __shared__ __align__(16) float os[4][kPairs][kLd];
-  __shared__ float ms[4][kPairs], ls[4][kPairs];
-  __shared__ int sh;
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), c16 = lane & 15, g = lane >> 4;
-  const int64_t W = A.head->w[0];
-  const int G = A.head->blocks[0];
-  if ((int)blockIdx.x >= G) return;
-  int64_t u = block_u0(W, G, blockIdx.x);
-  const int64_t u_end = block_u0(W, G, blockIdx.x + 1);
-  int x = find_tile(A, 0, u, &sh);
-  const int pair = c16 % kPairs, part = c16 / kPairs;  // (kPairs == 4: part 3 is an empty column)
+  extern __shared__ __align__(16) float os[];  // [wave][row][kFewLd]
+  __shared__ float ms[4][kFewRows], ls[4][kFewRows];
+  __shared__ Start sh;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
+  PlanHead H;
+  if (!block_start(A, 0, &H, &sh)) return;
+  int64_t u = block_u0(H, blockIdx.x);
+  const int64_t u_end = block_u0(H, blockIdx.x + 1);
+  Tile t = sh.t;
+  int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
   bool bad = false;
+#pragma unroll 1
   for (int seg = 0; u < u_end; ++seg) {
-    const Tile t = A.tiles[0][x];
-    const int64_t off = u - t.u0;
-    const int gk = (int)(off / t.units), k0 = (int)(off % t.units);
-    const int k1 = (int)min((int64_t)t.units, k0 + (u_end - u));
-    Seq s;
-    load_seq(a, t.b, &s);
-    const int npair = min(kPairs, s.n * A.rep - t.i * kPairs);
-    auto token = [&](int pr) { return (t.i * kPairs + min(pr, npair - 1)) / A.rep; };
-    auto head = [&](int pr) { return gk * A.rep + (t.i * kPairs + min(pr, npair - 1)) % A.rep; };
-    q35_u32x4 qb[8];
-    float qscale = sl2;
-    {  // (pairs past the last one repeat it; their columns are not written anywhere)
-      const int64_t qi = (int64_t)(s.s0 + token(pair)) * a.nh + head(pair);
-      float fq = 1.f;
-      if constexpr (DT == Q35_F16) {  // a power of two per query brings its largest value to 2^14
-        float inv;
-        split_scale(A.qmax[qi], fq, inv);
-        qscale = sl2 * inv;
-      }
-#pragma unroll
-      for (int st = 0; st < 8; ++st) {
-        const float* qp = A.q + qi * kHd + 32 * st + 8 * g;
-        const f4 v0 = *(const Q35_GLOBAL f4*)qp, v1 = *(const Q35_GLOBAL f4*)(qp + 4);
-        const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t p0, p1, p2 = 0;
-          if constexpr (DT == Q35_F16) split2(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
-          else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
-          qb[st][j] = part == 0 ? p0 : part == 1 ? p1 : part == 2 ? p2 : 0u;
-        }
-      }
-    }
-    const int lim = s.p0 + token(pair);  // the last token the lane's pair sees
-    const int end = s.p0 + s.n;          // tokens from here on do not exist
+    int gk = 0;
+    int64_t off = u - t.u0;
+    for (; off >= t.units; off -= t.units) ++gk;
+    const int k0 = (int)off, k1 = (int)min((int64_t)t.units, k0 + (u_end - u));
+    const int rows = min(kFewRows, t.n * A.rep - t.i * kFewRows);
+    const int pr = t.i * kFewRows + min(n, rows - 1), tok = div_rep(A, pr), h = gk * A.rep + pr - tok * A.rep;
+    const int lim = t.p0 + tok;   // the last token the lane's row sees (rows past the last one repeat it)
+    const int end = t.p0 + t.n;   // tokens from here on do not exist
     const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
     const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
     // pages of the unit's two halves
@@ -426,85 +422,101 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
       pa = page_of(A, row, j0, &bad);
       pb = a.P.page > 16 || j0 + 16 >= end ? pa : page_of(A, row, j0 + 16, &bad);
     };
-    constexpr int kW = kWide ? 2 : 1;  // 16-byte words of 8 values
     q35_u32x4 kr[2][8 * kW], vr[8][2 * kW];
     auto load_k = [&](int k, int pa, int pb) {
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const int slot = (k * kUnit + 16 * hf + c16) & (a.P.page - 1);
-        const E* p = base + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + 8 * g;
+        const int slot = (k * kUnit + 16 * hf + n) & (a.P.page - 1);
+        const E* p = base + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * g;
 #pragma unroll
-        for (int st = 0; st < 8; ++st)
-#pragma unroll
-          for (int w = 0; w < kW; ++w)
-            kr[hf][st * kW + w] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + 32 * st) + w);
+        for (int i = 0; i < 8 * kW; ++i)
+          kr[hf][i] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + (kWide ? 16 : 32) * i));
       }
     };
     auto load_v = [&](int k, int pa, int pb) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int slot = (k * kUnit + 16 * (j >> 2) + 4 * g + (j & 3)) & (a.P.page - 1);
-        const E* p = base + plane_elts(a) + (int64_t)(j >> 2 ? pb : pa) * page_elts(a) + (int64_t)slot * kHd;
+      for (int hf = 0; hf < 2; ++hf) {
+        const int slot = (k * kUnit + 16 * hf + 4 * g) & (a.P.page - 1);  // 4 keys of one page
+        const E* p = base + plane_elts(a) + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * n;
 #pragma unroll
-        for (int w = 0; w < 2 * kW; ++w)
-          vr[j][w] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + w * (128 / kW)) + c16);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int w = 0; w < 2 * kW; ++w)
+            vr[4 * hf + j][w] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + j * kHd + w * (128 / kW)));
       }
     };
-    f4 o[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
     int k = k0 + wid, pa = 0, pb = 0;
     if (k < k1) {
       pages(k, pa, pb);
       load_k(k, pa, pb);
       load_v(k, pa, pb);
     }
+    // queries: column n; dims 32 st + 8 g .. (16-bit), 16 st + 4 g .. (f32)
+    q35_u32x4 qb[kQ][8 * kW];
+    float qscale = sl2;
+    {
+      const int64_t qi = (int64_t)(t.s0 + tok) * a.nh + h;
+      const float* qp = A.q + qi * kHd;
+      if constexpr (kWide) {
+#pragma unroll
+        for (int st = 0; st < 16; ++st) qb[0][st] = *(const Q35_GLOBAL q35_u32x4*)(qp + 16 * st + 4 * g);
+      } else {
+        float fq = 1.f;
+        if constexpr (DT == Q35_F16) {  // a power of two per query brings its largest value to 2^14
+          float inv;
+          split_scale(A.qmax[qi], fq, inv);
+          qscale = sl2 * inv;
+        }
+#pragma unroll
+        for (int st = 0; st < 8; ++st) {
+          const f4 v0 = *(const Q35_GLOBAL f4*)(qp + 32 * st + 8 * g), v1 = *(const Q35_GLOBAL f4*)(qp + 32 * st + 8 * g + 4);
+          const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t p0, p1, p2 = 0;
+            if constexpr (DT == Q35_F16) split2(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
+            else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
+            qb[0][st][j] = p0;
+            if constexpr (kQ > 1) qb[1][st][j] = p1;
+            if constexpr (kQ > 2) qb[2][st][j] = p2;
+          }
+        }
+      }
+    }
+    f4 o[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
     for (; k < k1; k += 4) {
       const bool more = k + 4 < k1;
       if (more) pages(k + 4, pa, pb);
-      f4 sc[2];
+      f4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      // (the two halves in turn: a product does not wait for the one before it)
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        f4 acc = {0.f, 0.f, 0.f, 0.f}, acc2 = acc;
+      for (int st = 0; st < 8 * kW; ++st) {
+        if constexpr (kWide) {
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {
-          if constexpr (DT == Q35_F16) {
-            f4& c = st & 1 ? acc2 : acc;
-            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, kr[hf][st]), __builtin_bit_cast(q35_h8, qb[st]), c, 0, 0, 0);
-          } else if constexpr (DT == Q35_BF16) {
-            f4& c = st & 1 ? acc2 : acc;
-            c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, kr[hf][st]), __builtin_bit_cast(q35_b8, qb[st]), c, 0, 0, 0);
-          } else {
-            q35_u32x4 hi, mid, lo;
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t a0, a1, a2;
-              split3(__uint_as_float(kr[hf][2 * st + (j >> 1)][2 * (j & 1)]), __uint_as_float(kr[hf][2 * st + (j >> 1)][2 * (j & 1) + 1]), a0, a1, a2);
-              hi[j] = a0;
-              mid[j] = a1;
-              lo[j] = a2;
-            }
-            const q35_b8 q = __builtin_bit_cast(q35_b8, qb[st]);
-            acc2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, lo), q, acc2, 0, 0, 0);
-            acc2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, mid), q, acc2, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, hi), q, acc, 0, 0, 0);
-          }
+            for (int hf = 0; hf < 2; ++hf)
+              sc[hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[hf][st][e]), __uint_as_float(qb[0][st][e]), sc[hf], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int q = 0; q < kQ; ++q)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) sc[hf] = mma<DT>(kr[hf][st], qb[q][st], sc[hf]);
         }
-        sc[hf] = acc + acc2;
       }
       const int j0 = k * kUnit;
       if (more) load_k(k + 4, pa, pb);
       asm volatile("" ::: "memory");
-      float sv[8], bm = -INFINITY;
+      float bm = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        float v = sc[j >> 2][j & 3];
-        v += row_ror<8>(v);
-        if constexpr (kParts == 3) v += row_ror<4>(v);
-        const int key = j0 + 16 * (j >> 2) + 4 * g + (j & 3);
-        sv[j] = key <= lim ? v * qscale : -INFINITY;
-        bm = fmaxf(bm, sv[j]);
+        const float v = j0 + 16 * (j >> 2) + 4 * g + (j & 3) <= lim ? sc[j >> 2][j & 3] * qscale : -INFINITY;
+        sc[j >> 2][j & 3] = v;
+        bm = fmaxf(bm, v);
       }
       bm = max_x32(max_x16(bm));
       const float mn = fmaxf(m, bm);
@@ -517,15 +529,23 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
       }
       // f16 weights are kept 2^12 times larger (at most 4096), so that their halves hold 22 bits down to 2^-26
       const float mr = (m == -INFINITY ? 0.f : m) - (DT == Q35_F16 ? 12.f : 0.f);
-      q35_u32x4 pw;
+      q35_u32x4 pw[kQ];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float p0 = __builtin_amdgcn_exp2f(sv[2 * j] - mr), p1 = __builtin_amdgcn_exp2f(sv[2 * j + 1] - mr);
-        l += p0 + p1;
-        uint32_t w0, w1, w2 = 0;
-        if constexpr (DT == Q35_F16) split2(p0, p1, w0, w1);
-        else split3(p0, p1, w0, w1, w2);
-        pw[j] = part == 0 ? w0 : part == 1 ? w1 : part == 2 ? w2 : 0u;
+      for (int j = 0; j < 8; ++j) {
+        sc[j >> 2][j & 3] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - mr);
+        l += sc[j >> 2][j & 3];
+      }
+      if constexpr (!kWide) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float p0 = sc[j >> 1][2 * (j & 1)], p1 = sc[j >> 1][2 * (j & 1) + 1];
+          uint32_t w0, w1, w2 = 0;
+          if constexpr (DT == Q35_F16) split2(p0, p1, w0, w1);
+          else split3(p0, p1, w0, w1, w2);
+          pw[0][j] = w0;
+          if constexpr (kQ > 1) pw[1][j] = w1;
+          if constexpr (kQ > 2) pw[2][j] = w2;
+        }
       }
       if (j0 + kUnit > end) {  // (uniform) rows behind the sequence's last token may hold anything
 #pragma unroll
@@ -535,91 +555,88 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
             for (int w = 0; w < 2 * kW; ++w) vr[j][w] = q35_u32x4{0, 0, 0, 0};
           }
       }
+      // tile i = w (8 / kW) + e: dims w (128 / kW) + (8 / kW) (4 g + r) + e in register r
 #pragma unroll
       for (int w = 0; w < 2 * kW; ++w) {
+        if constexpr (kWide) {
 #pragma unroll
-        for (int e = 0; e < 8 / kW; ++e) {
-          const int i = w * (8 / kW) + e;
-          if constexpr (kWide) {
-            q35_u32x4 hi, mid, lo;
+          for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][w][e]), sc[j >> 2][j & 3], o[4 * w + e], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            q35_u32x4 v[2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              uint32_t a0, a1, a2;
-              split3(__uint_as_float(vr[2 * j][w][e]), __uint_as_float(vr[2 * j + 1][w][e]), a0, a1, a2);
-              hi[j] = a0;
-              mid[j] = a1;
-              lo[j] = a2;
+              v[0][j] = __builtin_amdgcn_perm(vr[2 * j + 1][w][e >> 1], vr[2 * j][w][e >> 1], 0x05040100u);
+              v[1][j] = __builtin_amdgcn_perm(vr[2 * j + 1][w][e >> 1], vr[2 * j][w][e >> 1], 0x07060302u);
             }
-            const q35_b8 p = __builtin_bit_cast(q35_b8, pw);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, lo), p, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, mid), p, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, hi), p, o[i], 0, 0, 0);
-          } else {
-            q35_u32x4 v;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              v[j] = __builtin_amdgcn_perm(vr[2 * j + 1][w][e >> 1], vr[2 * j][w][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-            if constexpr (DT == Q35_F16)
-              o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, v), __builtin_bit_cast(q35_h8, pw), o[i], 0, 0, 0);
-            else
-              o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, v), __builtin_bit_cast(q35_b8, pw), o[i], 0, 0, 0);
+            for (int q = 0; q < kQ; ++q)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) o[8 * w + e + i] = mma<DT>(v[i], pw[q], o[8 * w + e + i]);
           }
         }
       }
       if (more) load_v(k + 4, pa, pb);
       asm volatile("" ::: "memory");
     }
-    // the parts' columns together; tile i = w (8 / kW) + e, row 4 g + r: dim w (128 / kW) + (8 / kW)(4 g + r) + e
     l = add_x32(add_x16(l));
+    if (n < rows) {
+      float* dst = os + (wid * kFewRows + n) * kFewLd + (8 / kW) * 4 * g;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
+      for (int w = 0; w < 2 * kW; ++w)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v = o[i][r];
-        v += row_ror<8>(v);
-        if constexpr (kParts == 3) v += row_ror<4>(v);
-        constexpr int kE = 8 / kW;
-        if (part == (r & 1)) os[wid][pair][(i / kE) * (128 / kW) + kE * (4 * g + r) + i % kE] = v;
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < 8 / kW; e += 4) {
+            const int i = w * (8 / kW) + e;
+            *(f4*)(dst + w * (128 / kW) + (8 / kW) * r + e) = f4{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]};
+          }
+      if (g == 0) {
+        ms[wid][n] = m;
+        ls[wid][n] = l;
       }
-    if (g == 0 && part == 0) {
-      ms[wid][pair] = m;
-      ls[wid][pair] = l;
     }
     __syncthreads();
-    // pairs wid, wid + 4: 4 dims per lane
+    // rows wid, wid + 4, ..: 4 dims per lane
     const bool whole = k0 == 0 && k1 == t.units;
     const int slot = 2 * blockIdx.x + (seg == 0 ? 0 : 1);
-    for (int pr = wid; pr < npair; pr += 4) {
+#pragma unroll 1
+    for (int r = wid; r < rows; r += 4) {
       float M = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, ms[w][pr]);
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, ms[w][r]);
       float L = 0.f;
-      f4 r = {0.f, 0.f, 0.f, 0.f};
+      f4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
-        const float f = ms[w][pr] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[w][pr] - M);
-        L += ls[w][pr] * f;
-        r += *(const f4*)&os[w][pr][4 * lane] * f;
+        const float f = ms[w][r] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[w][r] - M);
+        L += ls[w][r] * f;
+        y += *(const f4*)(os + (w * kFewRows + r) * kFewLd + 4 * lane) * f;
       }
       if (whole) {
-        const int64_t tr = s.s0 + token(pr);
-        const f4 gv = *(const f4*)(a.qg + tr * a.ld_qg + (int64_t)head(pr) * 2 * kHd + kHd + 4 * lane);
-        f4 y;
+        const int p2 = t.i * kFewRows + r, tk = div_rep(A, p2), h2 = gk * A.rep + p2 - tk * A.rep;
+        const int64_t tr = t.s0 + tk;
+        const f4 gv = *(const f4*)(a.qg + tr * a.ld_qg + (int64_t)h2 * 2 * kHd + kHd + 4 * lane);
+        const float f = 1.f / L;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = r[e] / L * sigmoid_f(gv[e]);
-        *(f4*)(a.out + tr * a.ld_out + (int64_t)head(pr) * kHd + 4 * lane) = y;
+        for (int e = 0; e < 4; ++e) y[e] = y[e] * f * sigmoid_f(gv[e]);
+        *(f4*)(a.out + tr * a.ld_out + (int64_t)h2 * kHd + 4 * lane) = y;
       } else {
-        const int64_t pi = (int64_t)slot * A.part_rows[0] + pr;
-        *(f4*)(A.part_o[0] + pi * kHd + 4 * lane) = r;
+        const int64_t pi = (int64_t)slot * A.part_rows[0] + r;
+        *(f4*)(A.part_o[0] + pi * kHd + 4 * lane) = y;
         if (lane == 0) {
           A.part_ml[0][2 * pi] = M;
           A.part_ml[0][2 * pi + 1] = L;
         }
       }
     }
-    __syncthreads();
     u += k1 - k0;
-    if (u == t.u0 + (int64_t)t.units * a.nkv) ++x;
+    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = A.tiles[0][++x];
+    __syncthreads();
   }
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
 }
@@ -647,12 +664,6 @@ template <int DT>
 constexpr int many_lds() { return 2 * 2 * kPlane * (DT == Q35_F32 ? 2 : 1); }
 
 template <int DT>
-Q35_DEV f4 mma(q35_u32x4 x, q35_u32x4 y, f4 c) {
-  if constexpr (DT == Q35_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, x), __builtin_bit_cast(q35_b8, y), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, x), __builtin_bit_cast(q35_h8, y), c, 0, 0, 0);
-}
-
-template <int DT>
 __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_many_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
   constexpr bool kWide = DT == Q35_F32;
@@ -665,33 +676,31 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const PagedAttn& a = A.c;
   extern __shared__ __align__(16) char lds[];  // [2 buffers][keys, values][part]
   __shared__ float scl[2][2][8];               // [buffer][keys, values][group of 4 keys]
-  __shared__ int sh;
+  __shared__ Start sh;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4, n32 = lane & 31, hf = lane >> 5;
-  const int64_t W = A.head->w[1];
-  const int G = A.head->blocks[1];
-  if ((int)blockIdx.x >= G) return;
-  int64_t u = block_u0(W, G, blockIdx.x);
-  const int64_t u_end = block_u0(W, G, blockIdx.x + 1);
-  int x = find_tile(A, 1, u, &sh);
+  PlanHead H;
+  if (!block_start(A, 1, &H, &sh)) return;
+  int64_t u = block_u0(H, blockIdx.x);
+  const int64_t u_end = block_u0(H, blockIdx.x + 1);
+  Tile t = sh.t;
+  int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
   bool bad = false;
   for (int seg = 0; u < u_end; ++seg) {
-    const Tile t = A.tiles[1][x];
-    const int64_t off = u - t.u0;
-    const int gk = (int)(off / t.units), k0 = (int)(off % t.units);
-    const int k1 = (int)min((int64_t)t.units, k0 + (u_end - u));
-    Seq s;
-    load_seq(a, t.b, &s);
-    const int tok0 = t.i * A.tok_many, rows = min(A.tok_many, s.n - tok0) * A.rep;
+    int gk = 0;
+    int64_t off = u - t.u0;
+    for (; off >= t.units; off -= t.units) ++gk;
+    const int k0 = (int)off, k1 = (int)min((int64_t)t.units, k0 + (u_end - u));
+    const int tok0 = t.i * A.tok_many, rows = min(A.tok_many, t.n - tok0) * A.rep;
     const int r = min(wid * kRowsW + n, rows - 1);  // the lane's row (past the last one: repeated, not written)
-    const int tok = tok0 + r / A.rep, h = gk * A.rep + r % A.rep;
-    const int lim = s.p0 + tok;
+    const int tok = tok0 + div_rep(A, r), h = gk * A.rep + r - (tok - tok0) * A.rep;
+    const int lim = t.p0 + tok;
     const bool wave_on = wid * kRowsW < rows;
     // the first and the last token that a row of the wave sees
-    const int lim0 = s.p0 + tok0 + min(wid * kRowsW, rows - 1) / A.rep;
-    const int lim1 = s.p0 + tok0 + min(wid * kRowsW + kRowsW - 1, rows - 1) / A.rep;
-    const int end = s.p0 + s.n;
+    const int lim0 = t.p0 + tok0 + div_rep(A, min(wid * kRowsW, rows - 1));
+    const int lim1 = t.p0 + tok0 + div_rep(A, min(wid * kRowsW + kRowsW - 1, rows - 1));
+    const int end = t.p0 + t.n;
     const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
     const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
     // staging registers: keys 4 wid + 2 i + hf, dims 8 n32 ..; values: keys 4 wid + i, dims 4 lane ..
@@ -786,7 +795,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     q35_u32x4 qb[kQ][8];
     float qscale = sl2;
     {
-      const int64_t qi = (int64_t)(s.s0 + tok) * a.nh + h;
+      const int64_t qi = (int64_t)(t.s0 + tok) * a.nh + h;
       float fq = 1.f;
       if constexpr (DT != Q35_BF16) {
         float inv;
@@ -946,7 +955,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const bool whole = k0 == 0 && k1 == t.units;
     if (wid * kRowsW + n < rows) {
       const float f = (whole ? 1.f / l : 1.f) / ov;
-      const int64_t tr = s.s0 + tok;
+      const int64_t tr = t.s0 + tok;
       const float* gate = a.qg + tr * a.ld_qg + (int64_t)h * 2 * kHd + kHd;
       const int64_t pi = (int64_t)(2 * blockIdx.x + (seg == 0 ? 0 : 1)) * A.part_rows[1] + r;
       float* dst = whole ? a.out + tr * a.ld_out + (int64_t)h * kHd : A.part_o[1] + pi * kHd;
@@ -974,16 +983,16 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         A.part_ml[1][2 * pi + 1] = l;
       }
     }
-    __syncthreads();  // (the buffers are the next segment's)
     u += k1 - k0;
-    if (u == t.u0 + (int64_t)t.units * a.nkv) ++x;
+    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = A.tiles[1][++x];
+    __syncthreads();  // (the buffers are the next segment's)
   }
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
 }
 
 // Joins the parts of a row's tile, if the plan cut it: kJW waves per (row, query head), each taking every
 // kJW-th part, eight of them in flight.
-template <int DT, int kJW>
+template <int kJW>
 __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
   const PagedAttn& a = A.c;
   __shared__ __align__(16) float ys[kJW > 1 ? kT / 64 : 1][kHd];
@@ -995,18 +1004,18 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
   Seq s;
   // (kJW > 1: the block's waves share their item, and leave together)
   if (t >= a.T || !find_seq(a, (int)t, &s)) return;
-  const int kind = kind_of<DT>(A, s.n), gk = h / A.rep, hr = h % A.rep, tok = (int)t - s.s0;
+  const int kind = kind_of(A, s.n), gk = div_rep(A, h), hr = h - gk * A.rep, tok = (int)t - s.s0;
   const int pair = tok * A.rep + hr;
-  const int i = kind ? tok / A.tok_many : pair / Kind<DT>::kPairs;
-  const int r = kind ? pair - i * A.tok_many * A.rep : pair % Kind<DT>::kPairs;
+  const int i = kind ? tok / A.tok_many : pair / kFewRows;
+  const int r = kind ? pair - i * A.tok_many * A.rep : pair % kFewRows;
+  const PlanHead H = A.head[kind];
   const int x = A.tile0[(int64_t)kind * a.B + s.b] + i;
-  if (x >= A.head->tiles[kind]) return;
+  if (x >= H.tiles) return;
   const Tile tl = A.tiles[kind][x];
-  const int64_t W = A.head->w[kind], u0 = tl.u0 + (int64_t)gk * tl.units;
-  const int G = A.head->blocks[kind];
-  const int g0 = unit_block(W, G, u0), np = unit_block(W, G, u0 + tl.units - 1) - g0 + 1;
+  const int64_t u0 = tl.u0 + (int64_t)gk * tl.units;
+  const int g0 = unit_block(H, u0), np = unit_block(H, u0 + tl.units - 1) - g0 + 1;
   if (np == 1) return;
-  const int first = block_u0(W, G, g0) == u0 ? 0 : 1;
+  const int first = block_u0(H, g0) == u0 ? 0 : 1;
   auto slot = [&](int q) { return (int64_t)(2 * (g0 + q) + (q == 0 ? first : 0)) * A.part_rows[kind] + r; };
   const float* ml = A.part_ml[kind];
   const f4 gv = *(const f4*)(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + 4 * lane);
@@ -1059,16 +1068,15 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B) {
   PagedLayout L;
   const int rep = nh / nkv, tok_many = kManyRows / rep;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-  // (4 pairs per tile at least, whatever the cache's type)
-  L.max_tiles[0] = (int)(((int64_t)T * rep + 3) / 4 + std::min(B, T));
-  const bool many = T > 1 && T * rep > 8;
+  L.max_tiles[0] = (int)(((int64_t)T * rep + kFewRows - 1) / kFewRows + std::min(B, T));
+  const bool many = T > 1 && (int64_t)T * rep > kFewMost;
   L.max_tiles[1] = many ? T / tok_many + std::min(B, T) : 0;
   const int cus = device_cus();
-  L.max_blocks[0] = 2 * cus;
+  L.max_blocks[0] = cus;
   L.max_blocks[1] = many ? cus : 0;
-  L.part_rows[0] = 8;
+  L.part_rows[0] = (int)std::min<int64_t>(kFewRows, (int64_t)T * rep);
   L.part_rows[1] = (int)std::min<int64_t>(kManyRows, (int64_t)T * rep);
-  L.head = up(sizeof(PlanHead));
+  L.head = up(2 * sizeof(PlanHead));
   L.tile0 = up((size_t)2 * B * 4);
   L.q = up((size_t)T * nh * kHd * 4);
   L.qmax = up((size_t)T * nh * 4);
@@ -1090,6 +1098,7 @@ int launch(const PagedAttn& a, hipStream_t st) {
   A.c = a;
   A.page_shift = __builtin_ctz((unsigned)a.P.page);
   A.rep = a.nh / a.nkv;
+  A.rep_inv = A.rep > 1 ? (uint32_t)(0x100000000ull / (uint32_t)A.rep) + 1u : 0u;
   A.tok_many = kManyRows / A.rep;
   char* p = static_cast<char*>(a.ws);
   A.head = reinterpret_cast<PlanHead*>(p);
@@ -1114,7 +1123,8 @@ int launch(const PagedAttn& a, hipStream_t st) {
   const int64_t ka = (int64_t)a.T * (a.nkv + a.nh), qa = (int64_t)a.T * a.nh;
   hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((uint32_t)((ka + 3) / 4 + 1)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
-  hipLaunchKernelGGL(paged_few_kernel<DT>, dim3(A.max_blocks[0]), dim3(kT), 0, st, A);
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_few_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
+  hipLaunchKernelGGL(paged_few_kernel<DT>, dim3(A.max_blocks[0]), dim3(kT), kFewLds, st, A);
   Q35_HIP_TRY(hipGetLastError());
   if (A.max_blocks[1] > 0) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, many_lds<DT>());
@@ -1122,8 +1132,8 @@ int launch(const PagedAttn& a, hipStream_t st) {
     Q35_HIP_TRY(hipGetLastError());
   }
   // few rows: their parts are many, or the chip is empty
-  if (qa <= 4096) hipLaunchKernelGGL((paged_join_kernel<DT, 4>), dim3((uint32_t)qa), dim3(kT), 0, st, A);
-  else hipLaunchKernelGGL((paged_join_kernel<DT, 1>), dim3((uint32_t)((qa + 3) / 4)), dim3(kT), 0, st, A);
+  if (qa <= 4096) hipLaunchKernelGGL(paged_join_kernel<4>, dim3((uint32_t)qa), dim3(kT), 0, st, A);
+  else hipLaunchKernelGGL(paged_join_kernel<1>, dim3((uint32_t)((qa + 3) / 4)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
   return Q35_OK;
 }
