@@ -386,13 +386,14 @@ constexpr int kFewLd = kHd + 4;
 constexpr int kFewLds = 4 * kFewRows * kFewLd * 4;
 
 template <int DT>
-__global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
+__global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
   constexpr bool kWide = DT == Q35_F32;
   constexpr int kQ = kWide ? 1 : DT == Q35_F16 ? 2 : 3;  // parts of a query or weight
   constexpr int kW = kWide ? 2 : 1;                       // 16-byte words of 8 values
+  constexpr int kH = kWide ? 1 : 2, kS = 16 * kH;          // keys of a wave's step
   const PagedAttn& a = A.c;
-  extern __shared__ __align__(16) float os[];  // [wave][row][kFewLd]
+  extern __shared__ __align__(16) float os[];  // the queries' operands, then the waves' outputs [wave][row][kFewLd]
   __shared__ float ms[4][kFewRows], ls[4][kFewRows];
   __shared__ Start sh;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
@@ -403,6 +404,7 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
   Tile t = sh.t;
   int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
+  q35_u32x4* const qs = reinterpret_cast<q35_u32x4*>(os);  // [part][step][lane]
   bool bad = false;
 #pragma unroll 1
   for (int seg = 0; u < u_end; ++seg) {
@@ -416,27 +418,26 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
     const int end = t.p0 + t.n;   // tokens from here on do not exist
     const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
     const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
-    // pages of the unit's two halves
-    auto pages = [&](int k, int& pa, int& pb) {
-      const int j0 = k * kUnit;
+    // pages of the step's 16-key halves
+    auto pages = [&](int j0, int& pa, int& pb) {
       pa = page_of(A, row, j0, &bad);
-      pb = a.P.page > 16 || j0 + 16 >= end ? pa : page_of(A, row, j0 + 16, &bad);
+      pb = kH == 1 || a.P.page > 16 || j0 + 16 >= end ? pa : page_of(A, row, j0 + 16, &bad);
     };
-    q35_u32x4 kr[2][8 * kW], vr[8][2 * kW];
-    auto load_k = [&](int k, int pa, int pb) {
+    q35_u32x4 kr[kH][8 * kW], vr[4 * kH][2 * kW];
+    auto load_k = [&](int j0, int pa, int pb) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int slot = (k * kUnit + 16 * hf + n) & (a.P.page - 1);
+      for (int hf = 0; hf < kH; ++hf) {
+        const int slot = (j0 + 16 * hf + n) & (a.P.page - 1);
         const E* p = base + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * g;
 #pragma unroll
         for (int i = 0; i < 8 * kW; ++i)
           kr[hf][i] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + (kWide ? 16 : 32) * i));
       }
     };
-    auto load_v = [&](int k, int pa, int pb) {
+    auto load_v = [&](int j0, int pa, int pb) {
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const int slot = (k * kUnit + 16 * hf + 4 * g) & (a.P.page - 1);  // 4 keys of one page
+      for (int hf = 0; hf < kH; ++hf) {
+        const int slot = (j0 + 16 * hf + 4 * g) & (a.P.page - 1);  // 4 keys of one page
         const E* p = base + plane_elts(a) + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * n;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -445,75 +446,80 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
             vr[4 * hf + j][w] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + j * kHd + w * (128 / kW)));
       }
     };
-    int k = k0 + wid, pa = 0, pb = 0;
-    if (k < k1) {
-      pages(k, pa, pb);
-      load_k(k, pa, pb);
-      load_v(k, pa, pb);
+    int j0 = k0 * kUnit + wid * kS, pa = 0, pb = 0;
+    const int j1 = min(k1 * kUnit, end);
+    if (j0 < j1) {
+      pages(j0, pa, pb);
+      load_k(j0, pa, pb);
+      load_v(j0, pa, pb);
     }
-    // queries: column n; dims 32 st + 8 g .. (16-bit), 16 st + 4 g .. (f32)
-    q35_u32x4 qb[kQ][8 * kW];
+    // queries: column n; dims 32 st + 8 g .. (16-bit), 16 st + 4 g .. (f32); each wave lays out a quarter
     float qscale = sl2;
     {
       const int64_t qi = (int64_t)(t.s0 + tok) * a.nh + h;
       const float* qp = A.q + qi * kHd;
-      if constexpr (kWide) {
+      float fq = 1.f;
+      if constexpr (DT == Q35_F16) {  // a power of two per query brings its largest value to 2^14
+        float inv;
+        split_scale(A.qmax[qi], fq, inv);
+        qscale = sl2 * inv;
+      }
 #pragma unroll
-        for (int st = 0; st < 16; ++st) qb[0][st] = *(const Q35_GLOBAL q35_u32x4*)(qp + 16 * st + 4 * g);
-      } else {
-        float fq = 1.f;
-        if constexpr (DT == Q35_F16) {  // a power of two per query brings its largest value to 2^14
-          float inv;
-          split_scale(A.qmax[qi], fq, inv);
-          qscale = sl2 * inv;
-        }
-#pragma unroll
-        for (int st = 0; st < 8; ++st) {
+      for (int i = 0; i < 2 * kW; ++i) {
+        const int st = 2 * kW * wid + i;
+        if constexpr (kWide) {
+          qs[st * 64 + lane] = *(const Q35_GLOBAL q35_u32x4*)(qp + 16 * st + 4 * g);
+        } else {
           const f4 v0 = *(const Q35_GLOBAL f4*)(qp + 32 * st + 8 * g), v1 = *(const Q35_GLOBAL f4*)(qp + 32 * st + 8 * g + 4);
           const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          q35_u32x4 qb[3];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t p0, p1, p2 = 0;
             if constexpr (DT == Q35_F16) split2(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
             else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
-            qb[0][st][j] = p0;
-            if constexpr (kQ > 1) qb[1][st][j] = p1;
-            if constexpr (kQ > 2) qb[2][st][j] = p2;
+            qb[0][j] = p0;
+            qb[1][j] = p1;
+            qb[2][j] = p2;
           }
+#pragma unroll
+          for (int q = 0; q < kQ; ++q) qs[(q * 8 + st) * 64 + lane] = qb[q];
         }
       }
     }
+    __syncthreads();
     f4 o[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-    for (; k < k1; k += 4) {
-      const bool more = k + 4 < k1;
-      if (more) pages(k + 4, pa, pb);
+    for (; j0 < j1; j0 += 4 * kS) {
+      const bool more = j0 + 4 * kS < j1;
+      if (more) pages(j0 + 4 * kS, pa, pb);
       f4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      // (the two halves in turn: a product does not wait for the one before it)
+      // (two sums in turn, the halves' or even and odd dims': a product does not wait for the one before it)
 #pragma unroll
       for (int st = 0; st < 8 * kW; ++st) {
         if constexpr (kWide) {
+          const q35_u32x4 qv = qs[st * 64 + lane];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-              sc[hf] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[hf][st][e]), __uint_as_float(qb[0][st][e]), sc[hf], 0, 0, 0);
+            sc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[0][st][e]), __uint_as_float(qv[e]), sc[e & 1], 0, 0, 0);
         } else {
 #pragma unroll
-          for (int q = 0; q < kQ; ++q)
+          for (int q = 0; q < kQ; ++q) {
+            const q35_u32x4 qv = qs[(q * 8 + st) * 64 + lane];
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) sc[hf] = mma<DT>(kr[hf][st], qb[q][st], sc[hf]);
+            for (int hf = 0; hf < kH; ++hf) sc[hf] = mma<DT>(kr[hf][st], qv, sc[hf]);
+          }
         }
       }
-      const int j0 = k * kUnit;
-      if (more) load_k(k + 4, pa, pb);
+      if (more) load_k(j0 + 4 * kS, pa, pb);
       asm volatile("" ::: "memory");
+      if constexpr (kWide) sc[0] += sc[1];
       float bm = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4 * kH; ++j) {
         const float v = j0 + 16 * (j >> 2) + 4 * g + (j & 3) <= lim ? sc[j >> 2][j & 3] * qscale : -INFINITY;
         sc[j >> 2][j & 3] = v;
         bm = fmaxf(bm, v);
@@ -531,7 +537,7 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
       const float mr = (m == -INFINITY ? 0.f : m) - (DT == Q35_F16 ? 12.f : 0.f);
       q35_u32x4 pw[kQ];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4 * kH; ++j) {
         sc[j >> 2][j & 3] = __builtin_amdgcn_exp2f(sc[j >> 2][j & 3] - mr);
         l += sc[j >> 2][j & 3];
       }
@@ -547,9 +553,9 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
           if constexpr (kQ > 2) pw[2][j] = w2;
         }
       }
-      if (j0 + kUnit > end) {  // (uniform) rows behind the sequence's last token may hold anything
+      if (j0 + kS > end) {  // (uniform) rows behind the sequence's last token may hold anything
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 4 * kH; ++j)
           if (j0 + 16 * (j >> 2) + 4 * g + (j & 3) >= end) {
 #pragma unroll
             for (int w = 0; w < 2 * kW; ++w) vr[j][w] = q35_u32x4{0, 0, 0, 0};
@@ -560,10 +566,10 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
       for (int w = 0; w < 2 * kW; ++w) {
         if constexpr (kWide) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+          for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              o[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][w][e]), sc[j >> 2][j & 3], o[4 * w + e], 0, 0, 0);
+              o[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[j][w][e]), sc[0][j], o[4 * w + e], 0, 0, 0);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; e += 2) {
@@ -580,9 +586,10 @@ __global__ __launch_bounds__(kT, 1) void paged_few_kernel(const AttnArgs A) {
           }
         }
       }
-      if (more) load_v(k + 4, pa, pb);
+      if (more) load_v(j0 + 4 * kS, pa, pb);
       asm volatile("" ::: "memory");
     }
+    __syncthreads();  // (the queries' operands are done with)
     l = add_x32(add_x16(l));
     if (n < rows) {
       float* dst = os + (wid * kFewRows + n) * kFewLd + (8 / kW) * 4 * g;
@@ -1072,7 +1079,7 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B) {
   const bool many = T > 1 && (int64_t)T * rep > kFewMost;
   L.max_tiles[1] = many ? T / tok_many + std::min(B, T) : 0;
   const int cus = device_cus();
-  L.max_blocks[0] = cus;
+  L.max_blocks[0] = 2 * cus;
   L.max_blocks[1] = many ? cus : 0;
   L.part_rows[0] = (int)std::min<int64_t>(kFewRows, (int64_t)T * rep);
   L.part_rows[1] = (int)std::min<int64_t>(kManyRows, (int64_t)T * rep);
