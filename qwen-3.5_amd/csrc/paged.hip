@@ -6,6 +6,7 @@
 #include "pages.h"
 
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 namespace q35 {
@@ -30,13 +31,17 @@ Q35_DEV bool load_seq(const PagedAttn& a, int b, Seq* s) {
   const int64_t lim = cap < a.rope_rows ? cap : a.rope_rows;
   return s->s0 >= 0 && s1 >= s->s0 && s1 <= a.T && s->p0 >= 0 && (int64_t)s->p0 + s->n <= lim;
 }
-// The sequence of row t: b with start[b] <= t < start[b + 1]; false if there is none or it is refused.
+// The sequence of the wave's row t: b with start[b] <= t < start[b + 1]; false if there is none or it is
+// refused.  The lanes look at 64 starts at a time.
 Q35_DEV bool find_seq(const PagedAttn& a, int t, Seq* s) {
-  int lo = 0, hi = a.B;  // the last b with start[b] <= t
-  while (hi - lo > 1) {
-    const int m = (lo + hi) / 2;
-    if (a.start[m] <= t) lo = m;
-    else hi = m;
+  const int lane = threadIdx.x & 63;
+  int lo = 0, len = a.B;  // the last b in [lo, lo + len) with start[b] <= t
+  while (len > 1) {
+    const int step = (len + 63) / 64, off = lane * step;
+    const int c = __popcll(__ballot(off < len && a.start[lo + min(off, len - 1)] <= t));
+    if (c == 0) return false;
+    lo += (c - 1) * step;
+    len = min(step, len - (c - 1) * step);
   }
   return load_seq(a, lo, s) && t >= s->s0 && t < s->s0 + s->n;
 }
@@ -54,7 +59,6 @@ Q35_DEV bool find_seq(const PagedAttn& a, int t, Seq* s) {
 constexpr int kUnit = 32;       // tokens of a unit
 constexpr int kFewRows = 16;    // query rows (token, head) of a "few" tile
 constexpr int kManyRows = 128;  // of a "many" tile
-constexpr int kFewMost = 2 * kFewRows;  // sequences of at most this many rows (or one token) are "few"
 
 // All that a block needs to know of a tile, in one load
 struct Tile {
@@ -72,6 +76,7 @@ struct AttnArgs {
   int32_t page_shift;     // log2 of the tokens per page
   int32_t rep, tok_many;  // query heads per kv head; tokens of a "many" tile
   uint32_t rep_inv;
+  int32_t few_most;       // sequences of at most this many new tokens are "few"
   int32_t max_tiles[2], max_blocks[2], part_rows[2];
   PlanHead* head;        // [2]
   float* q;              // [T][heads][256] queries after norm and rotary
@@ -82,7 +87,7 @@ struct AttnArgs {
   float* part_o[2];      // [2 max_blocks][part_rows][256]
 };
 
-Q35_DEV int kind_of(const AttnArgs& A, int n) { return n == 1 || n * A.rep <= kFewMost ? 0 : 1; }
+Q35_DEV int kind_of(const AttnArgs& A, int n) { return n <= A.few_most ? 0 : 1; }
 // x / rep for x < 2^28 (rep_inv = 2^32 / rep + 1)
 Q35_DEV int div_rep(const AttnArgs& A, int x) { return A.rep == 1 ? x : (int)__umulhi((uint32_t)x, A.rep_inv); }
 Q35_DEV int tiles_of(const AttnArgs& A, int n) {
@@ -1067,7 +1072,7 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
 }
 
 struct PagedLayout {
-  int32_t max_tiles[2], max_blocks[2], part_rows[2];
+  int32_t max_tiles[2], max_blocks[2], part_rows[2], few_most;
   size_t head, tile0, q, qmax, tiles[2], ml[2], o[2];  // byte sizes
   size_t bytes;
 };
@@ -1075,12 +1080,19 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B) {
   PagedLayout L;
   const int rep = nh / nkv, tok_many = kManyRows / rep;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-  L.max_tiles[0] = (int)(((int64_t)T * rep + kFewRows - 1) / kFewRows + std::min(B, T));
-  const bool many = T > 1 && (int64_t)T * rep > kFewMost;
-  L.max_tiles[1] = many ? T / tok_many + std::min(B, T) : 0;
+  // Which kinds there are is the device's knowledge; what a call cannot or need not have gets no launch (an
+  // empty one takes 4 us).  Up to two tokens per sequence on average: all are "few" (one that is longer then
+  // costs its own stream again for every 16 rows, a fraction of the batch's).  One sequence: its rows decide,
+  // if all rows are its.  Else a sequence of two tiles of "few" rows, or of one token, is "few": 5 drafted
+  // tokens of 4 heads (20 rows) behind 100 take 9.4 us there and 17.8 as a chunk.
+  const bool few_only = T <= 2 * B || (int64_t)T * rep <= 2 * kFewRows, many_only = !few_only && B == 1;
+  L.few_most = few_only ? INT_MAX : many_only ? 0 : std::max(1, 2 * kFewRows / rep);
+  const int seqs = std::min(B, T);
+  L.max_tiles[0] = many_only ? 0 : (int)(((int64_t)T * rep + kFewRows - 1) / kFewRows + seqs);
+  L.max_tiles[1] = few_only ? 0 : T / tok_many + seqs;
   const int cus = device_cus();
-  L.max_blocks[0] = 2 * cus;
-  L.max_blocks[1] = many ? cus : 0;
+  L.max_blocks[0] = many_only ? 0 : 2 * cus;
+  L.max_blocks[1] = few_only ? 0 : cus;
   L.part_rows[0] = (int)std::min<int64_t>(kFewRows, (int64_t)T * rep);
   L.part_rows[1] = (int)std::min<int64_t>(kManyRows, (int64_t)T * rep);
   L.head = up(2 * sizeof(PlanHead));
@@ -1107,6 +1119,7 @@ int launch(const PagedAttn& a, hipStream_t st) {
   A.rep = a.nh / a.nkv;
   A.rep_inv = A.rep > 1 ? (uint32_t)(0x100000000ull / (uint32_t)A.rep) + 1u : 0u;
   A.tok_many = kManyRows / A.rep;
+  A.few_most = L.few_most;
   char* p = static_cast<char*>(a.ws);
   A.head = reinterpret_cast<PlanHead*>(p);
   p += L.head;
@@ -1130,9 +1143,11 @@ int launch(const PagedAttn& a, hipStream_t st) {
   const int64_t ka = (int64_t)a.T * (a.nkv + a.nh), qa = (int64_t)a.T * a.nh;
   hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((uint32_t)((ka + 3) / 4 + 1)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
-  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_few_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
-  hipLaunchKernelGGL(paged_few_kernel<DT>, dim3(A.max_blocks[0]), dim3(kT), kFewLds, st, A);
-  Q35_HIP_TRY(hipGetLastError());
+  if (A.max_blocks[0] > 0) {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_few_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
+    hipLaunchKernelGGL(paged_few_kernel<DT>, dim3(A.max_blocks[0]), dim3(kT), kFewLds, st, A);
+    Q35_HIP_TRY(hipGetLastError());
+  }
   if (A.max_blocks[1] > 0) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, many_lds<DT>());
     hipLaunchKernelGGL(paged_many_kernel<DT>, dim3(A.max_blocks[1]), dim3(kMT), many_lds<DT>(), st, A);
