@@ -8,11 +8,11 @@
 //
 // The alternatives: a value and its index make one 64-bit key (the value's bits in ascending order,
 // then the complement of the index), so "larger value, then lower index" is one unsigned comparison
-// and every choice below is exact whatever the order of the work.  A wave keeps its best 64 keys
+// and every choice below is exact whatever the order of the work.  A wave keeps its best `top` keys
 // sorted, one per lane; a chunk of values costs one comparison of each lane's maximum with the
-// last wanted key, and only values above it are inserted, one by one.  The first chunk would insert
-// almost everything: the last wanted key starts at the `top`-th of the 64 lanes' maxima instead (that many
-// values are at least as large).
+// last wanted key, and only values above it are put aside and joined with the list, up to 64 at a time.  The
+// first chunk would put almost everything aside: the last wanted key starts at the `top`-th of the 64
+// lanes' maxima instead (that many values are at least as large).
 // Waves, then the splits of a row (blocks), are joined by ranks: a key's place is the number of larger
 // keys.
 #include "pages.h"
@@ -83,6 +83,48 @@ Q35_DEV void stat_join(Stat& a, float m, float s, float u) {
   a.m = mn;
 }
 
+// What one lane of the wave wrote to LDS is read by others of the same wave.
+Q35_DEV void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+}
+// The lanes' keys with `take` set behind the n of buf
+Q35_DEV void push_keys(key_t* buf, int& n, key_t k, bool take) {
+  const unsigned long long mask = __ballot(take);
+  if (!mask) return;
+  const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+  if (take) buf[at] = k;
+  n += __popcll(mask);
+}
+// Joins the n <= 64 keys of buf with the sorted list that the lanes hold: a key's new place is the number of
+// larger keys in both.  last becomes the list's top-th key.
+Q35_DEV void merge_keys(key_t* buf, int n, key_t& best, key_t& last, int top) {
+  const int lane = threadIdx.x & 63;
+  wave_sync();
+  const key_t c = lane < n ? buf[lane] : 0;
+  int pc = 0, pb = lane;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) {
+    const key_t k = lane_key(c, j);
+    pc += k > c ? 1 : 0;
+    pb += k > best ? 1 : 0;
+  }
+#pragma unroll 4
+  for (int j = 0; j < top; ++j) pc += lane_key(best, j) > c ? 1 : 0;
+  wave_sync();
+  buf[lane] = 0;
+  wave_sync();
+  // (empty places hold 0 and stay behind every key; only the first `top` places count)
+  if (best != 0 && pb < top) buf[pb] = best;
+  if (c != 0 && pc < top) buf[pc] = c;
+  wave_sync();
+  best = buf[lane];
+  wave_sync();
+  const key_t t = lane_key(best, top - 1);
+  last = t > last ? t : last;
+}
+
 // Final numbers of row m of the call.
 Q35_DEV void finish_row(const ScoreCall& c, int m, float mx, double S, double U, int cnt) {
   const double l = log(S);
@@ -112,6 +154,8 @@ template <int DT>
 __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   const ScoreCall& c = a.c;
   __shared__ key_t lists[kNW][kMaxTop];
+  __shared__ key_t buf[kNW][64];
+  __shared__ float stage[kNW][kPer][64];
   __shared__ float sm[kNW], ss[kNW], su[kNW];
   __shared__ int sc[kNW];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
@@ -131,7 +175,8 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   }
   Stat st = {-INFINITY, 0.f, 0.f};
   int cnt = 0;
-  key_t best = 0, last = 0;  // the lane's key of the wave's list; the list's top-th key
+  key_t best = 0, last = 0;  // the lane's key of the wave's list; what a value must pass to get in
+  int n = 0;                 // keys in buf
   const int top = c.top;
   const int w_first = (i0 + shift) / kVec, w_end = (i1 + shift + kVec - 1) / kVec;  // words of the split
   constexpr int kWords = kPer / kVec;
@@ -152,11 +197,12 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
         for (int j = 0; j < kVec; ++j)
           x[g * kVec + j] = DT == Q35_F32 ? __uint_as_float(d[j & 3]) : half_of<DT>(d[(j >> 1) & 3], j & 1);
         ok |= ((1u << kVec) - 1u) << (g * kVec);
-      } else {
+      } else {  // (the word holds others' values too)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
+          const float v = value<DT>(row, min(max(f + j, i0), i1 - 1));
           const bool in = f + j >= i0 && f + j < i1;
-          x[g * kVec + j] = in ? value<DT>(row, f + j) : -INFINITY;
+          x[g * kVec + j] = in ? v : -INFINITY;
           ok |= (in ? 1u : 0u) << (g * kVec + j);
         }
       }
@@ -188,32 +234,44 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
     if (top > 0) {
       if (first) {  // (uniform in the wave)
         first = false;
-        key_t lm = 0;
+        int im = -1;  // the lane's first largest value (lanes without values, or with NaN alone, have none)
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const key_t k = (ok >> e) & 1u ? key_of(x[e], idx0[e / kVec] + e % kVec) : 0;
-          lm = k > lm ? k : lm;
-        }
+        for (int e = kPer - 1; e >= 0; --e) im = x[e] == mx && ((ok >> e) & 1u) ? idx0[e / kVec] + e % kVec : im;
+        const key_t lm = im >= 0 ? key_of(mx, im) : 0;
         int before = 0;
+#pragma unroll 4
         for (int l = 0; l < 64; ++l) before += lane_key(lm, l) > lm ? 1 : 0;
         const unsigned long long at = __ballot(before == top - 1 && lm != 0);
         if (at) last = lane_key(lm, (int)__builtin_ctzll(at)) - 1;
       }
       if (__ballot(asc(mx) >= (uint32_t)(last >> 32))) {
+        // values at or above the last wanted one (all, while that is nothing or NaN)
+        const float lf = from_asc((uint32_t)(last >> 32));
+        const bool open = (uint32_t)(last >> 32) == 0;
+        int total = 0;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          const key_t k = (ok >> e) & 1u ? key_of(x[e], idx0[e / kVec] + e % kVec) : 0;
-          unsigned long long todo = __ballot(k > last);
-          while (todo) {
-            const int l = (int)__builtin_ctzll(todo);
-            todo &= todo - 1;
-            const key_t cand = lane_key(k, l);
-            if (cand <= last) continue;
-            const int place = __popcll(__ballot(best > cand));
-            const key_t up = __shfl_up(best, 1, 64);
-            best = lane > place ? up : lane == place ? cand : best;
-            const key_t t = lane_key(best, top - 1);
-            last = t > last ? t : last;
+        for (int e = 0; e < kPer; ++e) total += __popcll(__ballot(x[e] >= lf || open));
+        if (total <= 64) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) {
+            if (__ballot(x[e] >= lf || open)) {
+              const key_t k = (ok >> e) & 1u ? key_of(x[e], idx0[e / kVec] + e % kVec) : 0;
+              push_keys(buf[wid], n, k, k > last);
+            }
+          }
+          if (n > 0) merge_keys(buf[wid], n, best, last, top);
+          n = 0;
+        } else {  // more than fit: one value of every lane at a time
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) stage[wid][e][lane] = x[e];
+          wave_sync();
+#pragma unroll 1
+          for (int e = 0; e < kPer; ++e) {
+            const int f = (w0 + (e / kVec) * 64 + lane) * kVec - shift + e % kVec;
+            const key_t k = (ok >> e) & 1u ? key_of(stage[wid][e][lane], f) : 0;
+            push_keys(buf[wid], n, k, k > last);
+            if (n > 0) merge_keys(buf[wid], n, best, last, top);
+            n = 0;
           }
         }
       }
@@ -235,22 +293,22 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   if (top > 0) lists[wid][lane] = best;
   __syncthreads();
   Stat all = {sm[0], ss[0], su[0]};
-  int n = sc[0];
+  int before = sc[0];
 #pragma unroll
   for (int w = 1; w < kNW; ++w) {
     stat_join(all, sm[w], ss[w], su[w]);
-    n += sc[w];
+    before += sc[w];
   }
   const int64_t slot = (int64_t)m * a.nsplit + sp;
   if (tid == 0) {
     if (a.nsplit == 1) {
-      finish_row(c, m, all.m, (double)all.s, (double)all.u, n);
+      finish_row(c, m, all.m, (double)all.s, (double)all.u, before);
     } else {
       float* o = a.stat + slot * 4;
       o[0] = all.m;
       o[1] = all.s;
       o[2] = all.u;
-      a.cnt[slot] = n;
+      a.cnt[slot] = before;
     }
   }
   if (top > 0 && lane < top) {
