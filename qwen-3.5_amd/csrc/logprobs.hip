@@ -173,6 +173,9 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
     if (tgt >= 0 && tgt < c.V) xt = value<DT>(row, tgt);
     else tgt = -1;
   }
+  // the next float above it (NaN above +inf: nothing is >= that)
+  const uint32_t xb = __float_as_uint(xt + 0.0f);
+  const float above = __uint_as_float(xt == 0.f ? 1u : (xb & 0x80000000u) ? xb - 1u : xb + 1u);
   Stat st = {-INFINITY, 0.f, 0.f};
   int cnt = 0;
   key_t best = 0, last = 0;  // the lane's key of the wave's list; what a value must pass to get in
@@ -180,6 +183,7 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   const int top = c.top;
   const int w_first = (i0 + shift) / kVec, w_end = (i1 + shift + kVec - 1) / kVec;  // words of the split
   constexpr int kWords = kPer / kVec;
+  constexpr uint32_t kAll = (1u << kPer) - 1u;
   bool first = true;
   for (int w0 = w_first + wid * (kChunk / kVec); w0 < w_end; w0 += kNW * (kChunk / kVec)) {
     float x[kPer];
@@ -225,10 +229,22 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
       }
     }
     if (tgt >= 0) {
+      // a word of values whose indices all lie before the target's counts what is >= it, one behind it what
+      // is >= the next float; the word in which it lies, words with others' values and a NaN go by the keys
+      bool mixed = xt != xt || ok != kAll;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) {
-        const int i = idx0[e / kVec] + e % kVec;
-        cnt += (x[e] > xt || (x[e] == xt && i < tgt)) && ((ok >> e) & 1u) ? 1 : 0;
+      for (int g = 0; g < kWords; ++g) mixed |= (uint32_t)(tgt - idx0[g]) < (uint32_t)kVec;
+      if (__ballot(mixed)) {
+        const key_t kt = key_of(xt, tgt);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) cnt += key_of(x[e], idx0[e / kVec] + e % kVec) > kt && ((ok >> e) & 1u) ? 1 : 0;
+      } else {
+#pragma unroll
+        for (int g = 0; g < kWords; ++g) {
+          const float from = idx0[g] < tgt ? xt : above;
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) cnt += x[g * kVec + j] >= from ? 1 : 0;
+        }
       }
     }
     if (top > 0) {
@@ -404,9 +420,10 @@ __global__ __launch_bounds__(kT) void score_join_kernel(const ScoreArgs a) {
   }
 }
 
+constexpr int kBlocks = 4 * 256;
 // Blocks per row: enough to fill the chip when rows are few, of one chunk per wave at least.
 int score_split(int M, int V) {
-  const int want = (4 * 256 + M - 1) / M, most = std::min(kMaxSplit, (V + kNW * kChunk - 1) / (kNW * kChunk));
+  const int want = (kBlocks + M - 1) / M, most = std::min(kMaxSplit, (V + kNW * kChunk - 1) / (kNW * kChunk));
   return std::max(1, std::min(want, most));
 }
 
