@@ -114,14 +114,24 @@ Q35_DEV int block_excl(int v, int* sh, int* total) {
   return before + x - v;
 }
 
-// ---- fork
-struct ForkShared {
-  int first[kPageMaxSeqs];          // parent -> its first child
-  int kept[kPageMaxSeqs];           // entries that row j keeps
-  int base[kPageMaxSeqs + 1];       // new pages before row j
-  int sh[kPW];
-};
+// before[w] = bits set in the words before w; returns the number of all.  Every thread holds a run of words.
+Q35_DEV int count_before(const uint32_t* bits, int* before, int words, int* sh) {
+  const int per = (words + kPT - 1) / kPT;
+  const int w0 = min(words, (int)threadIdx.x * per), w1 = min(words, w0 + per);
+  int cnt = 0;
+  for (int w = w0; w < w1; ++w) cnt += __popc(bits[w]);
+  int n;
+  int r = block_excl(cnt, sh, &n);
+  for (int w = w0; w < w1; ++w) {
+    before[w] = r;
+    r += __popc(bits[w]);
+  }
+  __syncthreads();
+  return n;
+}
 
+// ---- fork
+// The parent of row j and its length; -1 for an empty row or a refused parent
 Q35_DEV int fork_parent(const ForkCall& c, int j, int* n, bool* bad) {
   const int p = c.parent[j];
   *n = 0;
@@ -136,115 +146,134 @@ Q35_DEV int fork_parent(const ForkCall& c, int j, int* n, bool* bad) {
   return p;
 }
 
+// LDS of the bookkeeping, in ints
+struct ForkLds {
+  int words, first, len, par, base, refs, total;
+};
+// Counts of up to this many pages are kept in LDS (64 KB); a shared prefix's counts, added to from every
+// row, otherwise wait for each other in the cache (that case: 15.8 us, 10.5 so).
+constexpr int kLdsRefs = 16384;
+__host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo) {
+  ForkLds L;
+  L.words = (n_pages + 31) / 32;
+  L.first = 2 * L.words;      // [words] pages that a kept entry names, [words] pages in use before the word
+  L.len = L.first + B;        // parent -> its first child
+  L.par = L.len + Bo;         // row -> its length
+  L.base = L.par + Bo;        // row -> its parent
+  L.refs = L.base + Bo + 1;   // row -> new pages before it
+  L.total = L.refs + (n_pages <= kLdsRefs ? n_pages : 0);
+  return L;
+}
+
+// Every step spreads its entries over all threads (a wave per row waited for its row's loads in turn: 35
+// instead of 17 us for 200 rows of 36 entries).
 __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
-  extern __shared__ uint32_t bits[];  // pages that a kept entry names
-  __shared__ ForkShared s;
-  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int np = c.P.n_pages, words = (np + 31) / 32, page = c.P.page;
+  extern __shared__ int lds[];
+  __shared__ int sh[kPW];
+  const int tid = threadIdx.x, np = c.P.n_pages, page = c.P.page, shift = __ffs(page) - 1;  // (a power of two)
+  const ForkLds L = fork_lds(np, c.B, c.Bo);
+  const int words = L.words;
+  uint32_t* bits = reinterpret_cast<uint32_t*>(lds);
+  int *before = lds + words, *first = lds + L.first, *len = lds + L.len, *par = lds + L.par, *base = lds + L.base;
   bool bad = false;
   for (int e = tid; e < words; e += kPT) bits[e] = 0;
-  for (int e = tid; e < np; e += kPT) c.refs[e] = 0;
-  for (int e = tid; e < c.B; e += kPT) s.first[e] = INT32_MAX;
+  int* refs = lds + L.refs;
+  const bool counted = np <= kLdsRefs;
+  for (int e = tid; e < np; e += kPT) (counted ? refs : c.refs)[e] = 0;
+  for (int e = tid; e < c.B; e += kPT) first[e] = INT32_MAX;
   __syncthreads();
   for (int j = tid; j < c.Bo; j += kPT) {
     int n;
     bool b;
     const int p = fork_parent(c, j, &n, &b);
-    if (p >= 0) atomicMin(&s.first[p], j);
+    if (p >= 0) atomicMin(&first[p], j);
     c.len_out[j] = n;
+    len[j] = n;
+    par[j] = p;
     bad |= b;
   }
   __syncthreads();
+  // entries that row j keeps
+  auto kept_of = [&](int j) {
+    const int n = len[j], p = par[j];
+    return (n >> shift) + (p >= 0 && (n & (page - 1)) != 0 && first[p] == j ? 1 : 0);
+  };
   int run = 0;  // new pages of the rows before this group of kPT
   for (int j0 = 0; j0 < c.Bo; j0 += kPT) {
     const int j = j0 + tid;
     int need = 0;
     if (j < c.Bo) {
-      int n;
-      bool b;
-      const int p = fork_parent(c, j, &n, &b);
       int64_t g = c.grow ? c.grow[j] : 0;
       if (g < 0) {
         g = 0;
         bad = true;
       }
-      const int kept = n / page + (p >= 0 && n % page != 0 && s.first[p] == j ? 1 : 0);
-      int64_t total = ((int64_t)n + g + page - 1) / page;
+      int64_t total = ((int64_t)len[j] + g + page - 1) >> shift;
       if (total > c.ld) {
         total = c.ld;
         bad = true;
       }
-      s.kept[j] = kept;
-      need = (int)total - kept;
+      need = (int)total - kept_of(j);
     }
     int all;
-    const int b = block_excl(need, s.sh, &all);
-    if (j < c.Bo) s.base[j] = run + b;
+    const int b = block_excl(need, sh, &all);
+    if (j < c.Bo) base[j] = run + b;
     run += all;
-    __syncthreads();
   }
-  if (tid == 0) s.base[c.Bo] = run;
+  if (tid == 0) base[c.Bo] = run;
   __syncthreads();
-  // kept entries and what lies behind each row's pages; a wave per row
-  for (int j = wid; j < c.Bo; j += kPW) {
-    const int kept = s.kept[j], end = kept + s.base[j + 1] - s.base[j];
-    const int32_t* old = c.table + (int64_t)max(c.parent[j], 0) * c.ld;
-    int32_t* row = c.table_out + (int64_t)j * c.ld;
-    for (int e = lane; e < c.ld; e += 64) {
-      if (e >= kept && e < end) continue;
-      int v = -1;
-      if (e < kept) {
-        v = old[e];
-        if ((uint32_t)v >= (uint32_t)np) {
-          v = -1;
+  // kept entries, and -1 behind each row's pages
+  const int ne = c.Bo * c.ld;  // (at most 2^28)
+  constexpr int kU = 4;  // entries of a thread in flight
+  for (int e0 = tid; e0 < ne; e0 += kU * kPT) {
+    int v[kU], kind[kU];  // kind: 0 not written here, 1 behind the row's pages, 2 kept
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+      const int x = min(e0 + i * kPT, ne - 1);
+      const int j = x / c.ld, e = x - j * c.ld, kept = kept_of(j);
+      kind[i] = e < kept ? 2 : e < kept + base[j + 1] - base[j] ? 0 : 1;
+      if (e0 + i * kPT >= ne) kind[i] = 0;
+      v[i] = kind[i] == 2 ? c.table[(int64_t)par[j] * c.ld + e] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+      if (kind[i] == 0) continue;
+      if (kind[i] == 2) {
+        if ((uint32_t)v[i] >= (uint32_t)np) {
+          v[i] = -1;
           bad = true;
         } else {
-          atomicOr(&bits[v >> 5], 1u << (v & 31));
-          __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          atomicOr(&bits[v[i] >> 5], 1u << (v[i] & 31));
+          if (counted) atomicAdd(&refs[v[i]], 1);
+          else __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v[i]], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
       }
-      row[e] = v;
+      c.table_out[e0 + i * kPT] = v[i];
     }
   }
   __syncthreads();
-  // the free pages in ascending order: thread t holds words [t per, (t + 1) per)
-  const int per = (words + kPT - 1) / kPT;
-  const int w0 = min(words, tid * per), w1 = min(words, w0 + per);
-  auto free_bits = [&](int w) {
-    uint32_t f = ~bits[w];
-    if (32 * w + 32 > np) f &= (1u << (np & 31)) - 1u;
-    return f;
-  };
-  int cnt = 0;
-  for (int w = w0; w < w1; ++w) cnt += __popc(free_bits(w));
-  int nfree;
-  int r = block_excl(cnt, s.sh, &nfree);
-  auto row_of = [&](int rank) {  // the row j with base[j] <= rank < base[j + 1]
-    int lo = 0, hi = c.Bo;
+  const int used = count_before(bits, before, words, sh);
+  // the r-th free page is the r-th new entry
+  auto place = [&](int r, int page_id) {
+    int lo = 0, hi = c.Bo;  // the row j with base[j] <= r < base[j + 1]
     while (hi - lo > 1) {
       const int m = (lo + hi) / 2;
-      if (s.base[m] <= rank) lo = m;
+      if (base[m] <= r) lo = m;
       else hi = m;
     }
-    return lo;
+    c.table_out[(int64_t)lo * c.ld + kept_of(lo) + r - base[lo]] = page_id;
   };
-  for (int w = w0; w < w1 && r < run; ++w) {
-    uint32_t f = free_bits(w);
-    while (f && r < run) {
-      const int e = 32 * w + __ffs(f) - 1;
-      f &= f - 1;
-      const int j = row_of(r);
-      c.table_out[(int64_t)j * c.ld + s.kept[j] + r - s.base[j]] = e;
-      c.refs[e] = 1;
-      ++r;
-    }
+  for (int p = tid; p < np; p += kPT) {
+    const uint32_t w = bits[p >> 5], below = (1u << (p & 31)) - 1u;
+    const int r = p - (before[p >> 5] + __popc(w & below));
+    const bool fresh = !((w >> (p & 31)) & 1u) && r < run;
+    if (fresh) place(r, p);
+    if (counted) c.refs[p] = fresh ? 1 : refs[p];
+    else if (fresh) c.refs[p] = 1;
   }
-  for (int q = nfree + tid; q < run; q += kPT) {
-    const int j = row_of(q);
-    c.table_out[(int64_t)j * c.ld + s.kept[j] + q - s.base[j]] = -1;
-  }
+  for (int r = np - used + tid; r < run; r += kPT) place(r, -1);
   if (bad) raise_status(c.status, Q35_STATUS_ARG);
-  if (tid == 0 && run > nfree) raise_status(c.status, Q35_STATUS_FULL);
+  if (tid == 0 && run > np - used) raise_status(c.status, Q35_STATUS_FULL);
 }
 
 // The tokens of last pages that were not kept: blocks (row j, layer, plane and head).
@@ -287,17 +316,7 @@ __global__ __launch_bounds__(kPT) void pages_compact_kernel(const CompactCall c)
     else bad |= v != -1;
   }
   __syncthreads();
-  const int per = (words + kPT - 1) / kPT;
-  const int w0 = min(words, tid * per), w1 = min(words, w0 + per);
-  int cnt = 0;
-  for (int w = w0; w < w1; ++w) cnt += __popc(bits[w]);
-  int n;
-  int r = block_excl(cnt, sh, &n);
-  for (int w = w0; w < w1; ++w) {
-    before[w] = r;
-    r += __popc(bits[w]);
-  }
-  __syncthreads();
+  const int n = count_before(bits, before, words, sh);
   auto rank = [&](int p) { return before[p >> 5] + __popc(bits[p >> 5] & ((1u << (p & 31)) - 1u)); };  // pages in use < p
   const int low = n < np ? rank(n) : n;  // pages in use below n; n - low of them move
   // hole h (the h-th unused page below n) and mover h (the h-th page in use from n on)
@@ -388,8 +407,8 @@ int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t*
 }
 
 int pages_fork_launch(const ForkCall& c, hipStream_t st) {
-  const size_t lds = (size_t)((c.P.n_pages + 31) / 32) * 4;
-  if (lds > 8 * 1024) allow_lds(pages_fork_kernel, lds);
+  const size_t lds = (size_t)fork_lds(c.P.n_pages, c.B, c.Bo).total * 4;
+  if (lds > 48 * 1024) allow_lds(pages_fork_kernel, lds);
   hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(kPT), lds, st, c);
   Q35_HIP_TRY(hipGetLastError());
   hipLaunchKernelGGL(pages_fork_copy_kernel, dim3(c.Bo, c.P.n_layers, 2 * c.P.kv_heads), dim3(kCT), 0, st, c);
