@@ -83,6 +83,7 @@ struct AttnArgs {
   float* qmax;           // [T][heads] largest |value|
   int32_t* tile0;        // [2][B] first tile of the sequence in the list of each kind
   Tile* tiles[2];
+  int4* cut;             // [T][heads] where the parts of a cut tile lie (cut_record)
   float* part_ml[2];     // [2 max_blocks][part_rows][2]
   float* part_o[2];      // [2 max_blocks][part_rows][256]
 };
@@ -256,17 +257,28 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
   const int64_t item = ((int64_t)blockIdx.x - 1) * (kT / 64) + wid;
   const int64_t t = item / per;
   const int hd = (int)(item % per), g = hd, h = hd - a.nkv;  // kv head g, or query head h
+  if (t >= a.T) return;
+  // (the row's values are asked for before its sequence is known: it lies in the call's rows either way)
+  const int d = 4 * lane, half = a.rot / 2;
+  const bool query = h >= 0;
+  const float4 in = *reinterpret_cast<const float4*>(query ? a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + d
+                                                           : a.k + t * a.ld_kv + (int64_t)g * kHd + d);
+  const float4 w = *reinterpret_cast<const float4*>((query ? a.qnw : a.knw) + d);
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (query) {
+    if (lane == 0) A.cut[t * a.nh + h] = make_int4(0, 0, 0, 0);
+  } else {
+    v = *reinterpret_cast<const float4*>(a.v + t * a.ld_kv + (int64_t)g * kHd + d);
+  }
   Seq s;
-  if (t >= a.T || !find_seq(a, (int)t, &s)) return;
-  const int p = s.p0 + (int)t - s.s0, d = 4 * lane, half = a.rot / 2;
+  if (!find_seq(a, (int)t, &s)) return;
+  const int p = s.p0 + (int)t - s.s0;
   const float* cs = a.rcos + (int64_t)p * a.rot;
   const float* sn = a.rsin + (int64_t)p * a.rot;
-  if (h >= 0) {
+  if (query) {
     float* x = reinterpret_cast<float*>(xs[wid]);
-    const float4 q = *reinterpret_cast<const float4*>(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + d);
-    const float4 w = *reinterpret_cast<const float4*>(a.qnw + d);
-    const float r = rsqrt_f(wave_sum(q.x * q.x + q.y * q.y + q.z * q.z + q.w * q.w) / (float)kHd + a.eps);
-    float y[4] = {q.x * r * (1.0f + w.x), q.y * r * (1.0f + w.y), q.z * r * (1.0f + w.z), q.w * r * (1.0f + w.w)};
+    const float r = rsqrt_f(wave_sum(in.x * in.x + in.y * in.y + in.z * in.z + in.w * in.w) / (float)kHd + a.eps);
+    float y[4] = {in.x * r * (1.0f + w.x), in.y * r * (1.0f + w.y), in.z * r * (1.0f + w.z), in.w * r * (1.0f + w.w)};
     *reinterpret_cast<float4*>(x + d) = make_float4(y[0], y[1], y[2], y[3]);
     wave_lds_sync();
 #pragma unroll
@@ -287,10 +299,7 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
     if (lane == 0) raise_status(a.status, Q35_STATUS_ARG);
     return;
   }
-  const float4 k = *reinterpret_cast<const float4*>(a.k + t * a.ld_kv + (int64_t)g * kHd + d);
-  const float4 v = *reinterpret_cast<const float4*>(a.v + t * a.ld_kv + (int64_t)g * kHd + d);
-  const float4 w = *reinterpret_cast<const float4*>(a.knw + d);
-  const double x0 = k.x, x1 = k.y, x2 = k.z, x3 = k.w;
+  const double x0 = in.x, x1 = in.y, x2 = in.z, x3 = in.w;
   const double r = 1.0 / sqrt(wave_sum64((x0 * x0 + x1 * x1) + (x2 * x2 + x3 * x3)) / (double)kHd + (double)a.eps);
   double y[4] = {x0 * r * (1.0 + (double)w.x), x1 * r * (1.0 + (double)w.y), x2 * r * (1.0 + (double)w.z), x3 * r * (1.0 + (double)w.w)};
   double* x = xs[wid];
@@ -357,10 +366,21 @@ Q35_DEV bool block_start(const AttnArgs& A, int k, PlanHead* head, Start* sh) {
   return true;
 }
 
-// Page of tokens j0 .. (16 of them share one); pages outside the pool count as page 0.
+// Where the parts of a cut tile lie: block g's slots are 2 g (its first segment) and 2 g + 1.  Written for the part
+// that holds the tile's first unit u0: its slot + 1 (0: not cut), the row in its slots (-1 - row for "many"),
+// the tile's last unit.
+Q35_DEV int4 cut_record(int slot, int row, int64_t u0, int units) {
+  const int64_t last = u0 + units - 1;
+  return make_int4(slot + 1, row, (int)(uint32_t)last, (int)(last >> 32));
+}
+
+// Page of tokens j0 .. (16 of them share one); pages outside the pool count as page 0.  The table is read
+// through the constant address space and j0 is the wave's: a scalar load, which waits for nothing else (as a
+// vector load it waited for every key and value under way).
 Q35_DEV int page_of(const AttnArgs& A, const int32_t* row, int j0, bool* bad) {
   const PagedAttn& a = A.c;
-  const int v = __builtin_amdgcn_readfirstlane(row[j0 >> A.page_shift]);  // (j0 is the wave's)
+  typedef __attribute__((address_space(4))) const int32_t cint;
+  const int v = ((cint*)row)[__builtin_amdgcn_readfirstlane(j0 >> A.page_shift)];
   if ((uint32_t)v < (uint32_t)a.P.n_pages) return v;
   *bad = true;
   return 0;
@@ -643,6 +663,10 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
         if (lane == 0) {
           A.part_ml[0][2 * pi] = M;
           A.part_ml[0][2 * pi + 1] = L;
+          if (k0 == 0) {
+            const int p2 = t.i * kFewRows + r, tk = div_rep(A, p2);
+            A.cut[(int64_t)(t.s0 + tk) * a.nh + gk * A.rep + p2 - tk * A.rep] = cut_record(slot, r, u, t.units);
+          }
         }
       }
     }
@@ -659,7 +683,7 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
 // O^T += V^T P^T (16x16x32 products) keep a row's statistics in its lanes and turn scores into
 // operands in place.  16 rows are what leaves two waves a SIMD: a wave's queries (64 or 96 registers)
 // and outputs (64) stay in registers that the vector ALU reaches too (with 32 rows per wave, half the
-// LDS reads, and one wave per SIMD they did not: 2.5 ms instead of XX for 2048 tokens behind 14336).
+// LDS reads, and one wave per SIMD they did not: 2.5 ms instead of 1.15 for 2048 tokens behind 14336).
 // While a unit is multiplied, the next one is on its way into registers; it is then laid out in the
 // other LDS buffer, so one barrier per unit is enough.
 // LDS: keys [key][32 pieces of 8 dims], piece c at c ^ (key & 15); values [dim][4 pieces of 8 keys], the keys
@@ -674,6 +698,25 @@ constexpr int kRowsW = 16;     // rows of a wave
 constexpr int kPlane = 16384;  // bytes of a unit's keys (or values) of one part
 template <int DT>
 constexpr int many_lds() { return 2 * 2 * kPlane * (DT == Q35_F32 ? 2 : 1); }
+
+// m = max(m, |x|, |y|) of f32 bits (fmaxf quiets its arguments first, an instruction each)
+Q35_DEV void max3_abs(float& m, uint32_t x, uint32_t y) { asm("v_max3_f32 %0, |%1|, |%2|, %0" : "+v"(m) : "v"(x), "v"(y)); }
+// larger of each 16-bit half
+Q35_DEV uint32_t pk_max(uint32_t x, uint32_t y) {
+  typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, y)));
+}
+// f y (f a power of two, y as f32 bits) as f16 halves hi + lo, to nearest: v_fma_mixlo / mixhi multiply in f32, add
+// an f16 and round to f16 in one instruction, so a value takes two
+Q35_DEV void split2_scaled(uint32_t y0, uint32_t y1, float f, uint32_t& hi, uint32_t& lo) {
+  uint32_t h, l;
+  asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(h) : "v"(y0), "v"(f));
+  asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(h) : "v"(y1), "v"(f));
+  asm("v_fma_mixlo_f16 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(l) : "v"(y0), "v"(f), "v"(h));
+  asm("v_fma_mixhi_f16 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(l) : "v"(y1), "v"(f), "v"(h));
+  hi = h;
+  lo = l;
+}
 
 template <int DT>
 __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_many_kernel(const AttnArgs A) {
@@ -693,7 +736,8 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int n = lane & 15, g = lane >> 4, n32 = lane & 31, hf = lane >> 5;
   PlanHead H;
   if (!block_start(A, 1, &H, &sh)) return;
-  int64_t u = block_u0(H, blockIdx.x);
+  const int64_t u_begin = block_u0(H, blockIdx.x);
+  int64_t u = u_begin;
   const int64_t u_end = block_u0(H, blockIdx.x + 1);
   Tile t = sh.t;
   int x = sh.x;
@@ -719,9 +763,12 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     q35_u32x4 kr[2][kKV];
     typedef typename std::conditional<kWide, q35_u32x4, u2>::type VW;
     VW vr[4];
-    auto load_unit = [&](int k) {
-      const int j0 = k * kUnit + 4 * wid;  // (4 keys lie in one page)
-      const int pg = page_of(A, row, j0 < end ? j0 : k * kUnit, &bad);
+    auto unit_page = [&](int k) {  // of the wave's 4 keys
+      const int j0 = k * kUnit + 4 * wid;
+      return page_of(A, row, j0 < end ? j0 : k * kUnit, &bad);
+    };
+    auto load_unit = [&](int k, int pg) {
+      const int j0 = k * kUnit + 4 * wid;
       const E* p = base + (int64_t)pg * page_elts(a) + (int64_t)(j0 & (a.P.page - 1)) * kHd;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -746,22 +793,27 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       char* vb = kb + kKV * kPlane;
       float fk = 1.f, fv = 1.f;
       if constexpr (kWide) {
+        // the largest |key| and |value| of the wave's 4 rows, as the upper halves of their bits, in one word
         float mk = 0.f, mv = 0.f, ik, iv;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            mk = fmaxf(mk, fabsf(__uint_as_float(kr[i >> 1][i & 1][e])));
-            mv = fmaxf(mv, fabsf(__uint_as_float(vr[i][e])));
+          for (int e = 0; e < 4; e += 2) {
+            max3_abs(mk, kr[i >> 1][i & 1][e], kr[i >> 1][i & 1][e + 1]);
+            max3_abs(mv, vr[i][e], vr[i][e + 1]);
           }
-        mk = fmaxf(mk, row_ror<8>(mk)); mv = fmaxf(mv, row_ror<8>(mv));
-        mk = fmaxf(mk, row_ror<4>(mk)); mv = fmaxf(mv, row_ror<4>(mv));
-        mk = fmaxf(mk, row_ror<2>(mk)); mv = fmaxf(mv, row_ror<2>(mv));
-        mk = fmaxf(mk, row_ror<1>(mk)); mv = fmaxf(mv, row_ror<1>(mv));
-        mv = max_x32(max_x16(mv));
-        split_scale(max_x32(max_x16(mk)), fk, ik);
-        split_scale(mv, fv, iv);
-        iv = mv > 0.f ? fmaxf(iv, 7.888609e-31f) : 7.888609e-31f;  // (2^-100: zeros ask for no room)
+        uint32_t m2 = __builtin_amdgcn_perm(__float_as_uint(mv), __float_as_uint(mk), 0x07060302u);
+        m2 = pk_max(m2, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m2, 0x128, 0xf, 0xf, false));
+        m2 = pk_max(m2, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m2, 0x124, 0xf, 0xf, false));
+        m2 = pk_max(m2, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m2, 0x122, 0xf, 0xf, false));
+        m2 = pk_max(m2, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m2, 0x121, 0xf, 0xf, false));
+        const auto r16 = __builtin_amdgcn_permlane16_swap(m2, m2, false, false);
+        m2 = pk_max(r16[0], r16[1]);
+        const auto r32 = __builtin_amdgcn_permlane32_swap(m2, m2, false, false);
+        m2 = pk_max(r32[0], r32[1]);
+        split_scale(__uint_as_float(m2 << 16), fk, ik);  // (the exponent is all that counts)
+        split_scale(__uint_as_float(m2 & 0xffff0000u), fv, iv);
+        iv = m2 >> 16 ? fmaxf(iv, 7.888609e-31f) : 7.888609e-31f;  // (2^-100: zeros ask for no room)
         if (lane == 0) {
           scl[buf][0][wid] = ik;
           scl[buf][1][wid] = iv;
@@ -776,7 +828,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t a0, a1;
-            split2(__uint_as_float(kr[i][j >> 1][2 * (j & 1)]) * fk, __uint_as_float(kr[i][j >> 1][2 * (j & 1) + 1]) * fk, a0, a1);
+            split2_scaled(kr[i][j >> 1][2 * (j & 1)], kr[i][j >> 1][2 * (j & 1) + 1], fk, a0, a1);
             hi[j] = a0;
             lo[j] = a1;
           }
@@ -792,8 +844,8 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         char* dst = vb + (4 * lane + (e ^ ((lane >> 2) & 3))) * 64 + (((wid ^ -lane) & 3) * 16) + (wid >> 2) * 8;
         if constexpr (kWide) {
           uint32_t a0, a1, b0, b1;
-          split2(__uint_as_float(vr[0][e]) * fv, __uint_as_float(vr[1][e]) * fv, a0, a1);
-          split2(__uint_as_float(vr[2][e]) * fv, __uint_as_float(vr[3][e]) * fv, b0, b1);
+          split2_scaled(vr[0][e], vr[1][e], fv, a0, a1);
+          split2_scaled(vr[2][e], vr[3][e], fv, b0, b1);
           *(u2*)dst = u2{a0, b0};
           *(u2*)(dst + kPlane) = u2{a1, b1};
         } else {
@@ -802,7 +854,16 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
       }
     };
-    load_unit(k0);
+    // The blocks' ranges begin anywhere in their tiles.  The units of a range may come in any order, so a block
+    // begins where its unit's number is that of its own steps so far, modulo the units of a block, and goes
+    // round: all blocks then look at the same few places of the context at about the same time, and
+    // find in the L2 what another has read (2048 tokens behind 14336: 3.5 -> 1.75 GB from behind the L2s).
+    const int round = (int)min(H.q, (int64_t)INT32_MAX);
+    int ks = k0 + (int)(((u - u_begin - k0) % round + round) % round);
+    if (ks >= k1) ks = k0;
+    int kn = ks + 1 < k1 ? ks + 1 : k0;  // the next unit
+    int pg = unit_page(kn);              // and its page, asked for a unit ahead
+    load_unit(ks, unit_page(ks));
     // queries: column n, dims 32 st + 8 g ..
     q35_u32x4 qb[kQ][8];
     float qscale = sl2;
@@ -841,12 +902,16 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int i = 0; i < 4; ++i) ka_off[i] = n * 512 + ((4 * i + g) ^ n) * 16;
     const int va_off = n * 64 + ((g ^ -(n >> 2)) & 3) * 16;
-    for (int k = k0; k < k1; ++k) {
-      const int buf = (k - k0) & 1;
+    int k = ks;
+    for (int i = 0; i < k1 - k0; ++i) {
+      const int buf = i & 1;
       store_unit(k, buf);
-      if (k + 1 < k1) load_unit(k + 1);
-      __syncthreads();
       const int j0 = k * kUnit;
+      k = kn;
+      if (i + 1 < k1 - k0) load_unit(k, pg);
+      kn = k + 1 < k1 ? k + 1 : k0;
+      pg = unit_page(kn);
+      __syncthreads();
       if (!wave_on || j0 > lim1) continue;  // (uniform in the wave; the barrier above is passed by all)
       const char* kb = lds + buf * 2 * kKV * kPlane;
       const char* vb = kb + kKV * kPlane;
@@ -993,6 +1058,8 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       if (!whole && g == 0) {
         A.part_ml[1][2 * pi] = m;
         A.part_ml[1][2 * pi + 1] = l;
+        if (k0 == 0)
+          A.cut[tr * a.nh + h] = cut_record(2 * blockIdx.x + (seg == 0 ? 0 : 1), -1 - r, u, t.units);
       }
     }
     u += k1 - k0;
@@ -1013,22 +1080,12 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
   const int64_t item = (int64_t)blockIdx.x * (kT / 64 / kJW) + wid / kJW;
   const int64_t t = item / a.nh;
   const int h = (int)(item % a.nh);
-  Seq s;
-  // (kJW > 1: the block's waves share their item, and leave together)
-  if (t >= a.T || !find_seq(a, (int)t, &s)) return;
-  const int kind = kind_of(A, s.n), gk = div_rep(A, h), hr = h - gk * A.rep, tok = (int)t - s.s0;
-  const int pair = tok * A.rep + hr;
-  const int i = kind ? tok / A.tok_many : pair / kFewRows;
-  const int r = kind ? pair - i * A.tok_many * A.rep : pair % kFewRows;
-  const PlanHead H = A.head[kind];
-  const int x = A.tile0[(int64_t)kind * a.B + s.b] + i;
-  if (x >= H.tiles) return;
-  const Tile tl = A.tiles[kind][x];
-  const int64_t u0 = tl.u0 + (int64_t)gk * tl.units;
-  const int g0 = unit_block(H, u0), np = unit_block(H, u0 + tl.units - 1) - g0 + 1;
-  if (np == 1) return;
-  const int first = block_u0(H, g0) == u0 ? 0 : 1;
-  auto slot = [&](int q) { return (int64_t)(2 * (g0 + q) + (q == 0 ? first : 0)) * A.part_rows[kind] + r; };
+  if (t >= a.T) return;
+  const int4 c = A.cut[t * a.nh + h];
+  if (c.x == 0) return;  // (kJW > 1: the block's waves share their item, and leave together)
+  const int kind = c.y < 0 ? 1 : 0, r = kind ? -1 - c.y : c.y, g0 = (c.x - 1) >> 1;
+  const int np = unit_block(A.head[kind], (int64_t)c.w << 32 | (uint32_t)c.z) - g0 + 1;
+  auto slot = [&](int q) { return (int64_t)(q == 0 ? c.x - 1 : 2 * (g0 + q)) * A.part_rows[kind] + r; };
   const float* ml = A.part_ml[kind];
   const f4 gv = *(const f4*)(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + 4 * lane);
   float M = -INFINITY;
@@ -1073,7 +1130,7 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
 
 struct PagedLayout {
   int32_t max_tiles[2], max_blocks[2], part_rows[2], few_most;
-  size_t head, tile0, q, qmax, tiles[2], ml[2], o[2];  // byte sizes
+  size_t head, tile0, q, qmax, cut, tiles[2], ml[2], o[2];  // byte sizes
   size_t bytes;
 };
 PagedLayout paged_layout(int nh, int nkv, int T, int B) {
@@ -1099,7 +1156,8 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B) {
   L.tile0 = up((size_t)2 * B * 4);
   L.q = up((size_t)T * nh * kHd * 4);
   L.qmax = up((size_t)T * nh * 4);
-  L.bytes = L.head + L.tile0 + L.q + L.qmax;
+  L.cut = up((size_t)T * nh * sizeof(int4));
+  L.bytes = L.head + L.tile0 + L.q + L.qmax + L.cut;
   for (int k = 0; k < 2; ++k) {
     const size_t rows = (size_t)2 * L.max_blocks[k] * L.part_rows[k];
     L.tiles[k] = up((size_t)L.max_tiles[k] * sizeof(Tile));
@@ -1129,6 +1187,8 @@ int launch(const PagedAttn& a, hipStream_t st) {
   p += L.q;
   A.qmax = reinterpret_cast<float*>(p);
   p += L.qmax;
+  A.cut = reinterpret_cast<int4*>(p);
+  p += L.cut;
   for (int k = 0; k < 2; ++k) {
     A.max_tiles[k] = L.max_tiles[k];
     A.max_blocks[k] = L.max_blocks[k];
