@@ -61,7 +61,7 @@ constexpr int kFewRows = 16;    // query rows (token, head) of a "few" tile
 constexpr int kManyRows = 128;  // of a "many" tile
 
 // All that a block needs to know of a tile, in one load
-struct Tile {
+struct alignas(16) Tile {
   int64_t u0;                       // its first unit
   int32_t units, b, i, s0, n, p0;   // units per kv head; sequence, tile of it, its first row, rows, cached tokens
 };
@@ -342,6 +342,14 @@ Q35_DEV float add_x16(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
+Q35_DEV Tile load_tile(const Tile* p) {  // (two 16-byte loads; a copy of the structure goes through private memory)
+  const int4 a = reinterpret_cast<const int4*>(p)[0], b = reinterpret_cast<const int4*>(p)[1];
+  Tile t;
+  t.u0 = (int64_t)a.y << 32 | (uint32_t)a.x;
+  t.units = a.z; t.b = a.w; t.i = b.x; t.s0 = b.y; t.n = b.z; t.p0 = b.w;
+  return t;
+}
+
 // The block's first tile, the one that holds unit u: every thread looks at some (they are few).  The first
 // ones are asked for before the plan's head has arrived.
 struct Start {
@@ -351,12 +359,12 @@ struct Start {
 Q35_DEV bool block_start(const AttnArgs& A, int k, PlanHead* head, Start* sh) {
   const int x0 = threadIdx.x;
   Tile t;
-  if (x0 < A.max_tiles[k]) t = A.tiles[k][x0];
+  if (x0 < A.max_tiles[k]) t = load_tile(&A.tiles[k][x0]);
   *head = A.head[k];
   if ((int)blockIdx.x >= head->blocks) return false;
   const int64_t u = block_u0(*head, blockIdx.x);
   for (int x = x0; x < head->tiles; x += blockDim.x) {
-    if (x != x0) t = A.tiles[k][x];
+    if (x != x0) t = load_tile(&A.tiles[k][x]);
     if (t.u0 <= u && u < t.u0 + (int64_t)t.units * A.c.nkv) {
       sh->t = t;
       sh->x = x;
@@ -411,22 +419,26 @@ constexpr int kFewLd = kHd + 4;
 constexpr int kFewLds = 4 * kFewRows * kFewLd * 4;
 
 template <int DT>
-__global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
+constexpr int elt_bytes() { return DT == Q35_F32 ? 4 : 2; }
+template <bool kStream>
+Q35_DEV q35_u32x4 ldg16_if(const void* p) {
+  if constexpr (kStream) return __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)p);
+  else return *(const Q35_GLOBAL q35_u32x4*)p;
+}
+// os: the queries' operands, then the waves' outputs [wave][row][kFewLd]
+template <int DT, bool kStream>
+Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, float* os, float (&ms)[4][kFewRows],
+                     float (&ls)[4][kFewRows]) {
   typedef typename Elt<DT>::T E;
   constexpr bool kWide = DT == Q35_F32;
   constexpr int kQ = kWide ? 1 : DT == Q35_F16 ? 2 : 3;  // parts of a query or weight
   constexpr int kW = kWide ? 2 : 1;                       // 16-byte words of 8 values
   constexpr int kH = kWide ? 1 : 2, kS = 16 * kH;          // keys of a wave's step
   const PagedAttn& a = A.c;
-  extern __shared__ __align__(16) float os[];  // the queries' operands, then the waves' outputs [wave][row][kFewLd]
-  __shared__ float ms[4][kFewRows], ls[4][kFewRows];
-  __shared__ Start sh;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
-  PlanHead H;
-  if (!block_start(A, 0, &H, &sh)) return;
   int64_t u = block_u0(H, blockIdx.x);
   const int64_t u_end = block_u0(H, blockIdx.x + 1);
-  Tile t = sh.t;
+  Tile t = load_tile(&sh.t);
   int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
   q35_u32x4* const qs = reinterpret_cast<q35_u32x4*>(os);  // [part][step][lane]
@@ -455,8 +467,7 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
         const int slot = (j0 + 16 * hf + n) & (a.P.page - 1);
         const E* p = base + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * g;
 #pragma unroll
-        for (int i = 0; i < 8 * kW; ++i)
-          kr[hf][i] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + (kWide ? 16 : 32) * i));
+        for (int i = 0; i < 8 * kW; ++i) kr[hf][i] = ldg16_if<kStream>(p + (kWide ? 16 : 32) * i);
       }
     };
     auto load_v = [&](int j0, int pa, int pb) {
@@ -467,8 +478,7 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-          for (int w = 0; w < 2 * kW; ++w)
-            vr[4 * hf + j][w] = __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)(p + j * kHd + w * (128 / kW)));
+          for (int w = 0; w < 2 * kW; ++w) vr[4 * hf + j][w] = ldg16_if<kStream>(p + j * kHd + w * (128 / kW));
       }
     };
     int j0 = k0 * kUnit + wid * kS, pa = 0, pb = 0;
@@ -671,10 +681,24 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
       }
     }
     u += k1 - k0;
-    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = A.tiles[0][++x];
+    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = load_tile(&A.tiles[0][++x]);
     __syncthreads();
   }
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
+}
+
+template <int DT>
+__global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
+  extern __shared__ __align__(16) float os[];
+  __shared__ float ms[4][kFewRows], ls[4][kFewRows];
+  __shared__ Start sh;
+  PlanHead H;
+  if (!block_start(A, 0, &H, &sh)) return;
+  // What the tiles read in all, against the 256 MB of the last-level cache: a larger stream passes it by
+  // (33 tokens over 958 MB: 179 us, 206 through it), a smaller one is found there again by sequences that
+  // share pages and by second tiles (54 tiles over 229 MB: 40 us, 53 past it).
+  if (H.w > (int64_t)(256u << 20) / (kUnit * 2 * kHd * elt_bytes<DT>())) few_run<DT, true>(A, H, sh, os, ms, ls);
+  else few_run<DT, false>(A, H, sh, os, ms, ls);
 }
 
 // ------------------------------------------------------------------ many new tokens
@@ -739,7 +763,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int64_t u_begin = block_u0(H, blockIdx.x);
   int64_t u = u_begin;
   const int64_t u_end = block_u0(H, blockIdx.x + 1);
-  Tile t = sh.t;
+  Tile t = load_tile(&sh.t);
   int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
   bool bad = false;
@@ -1063,7 +1087,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
     u += k1 - k0;
-    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = A.tiles[1][++x];
+    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = load_tile(&A.tiles[1][++x]);
     __syncthreads();  // (the buffers are the next segment's)
   }
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
