@@ -1228,12 +1228,12 @@ int launch(const PagedAttn& a, hipStream_t st) {
   hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((uint32_t)((ka + 3) / 4 + 1)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
   if (A.max_blocks[0] > 0) {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_few_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds);
+    allow_lds<paged_few_kernel<DT>>(kFewLds);
     hipLaunchKernelGGL(paged_few_kernel<DT>, dim3(A.max_blocks[0]), dim3(kT), kFewLds, st, A);
     Q35_HIP_TRY(hipGetLastError());
   }
   if (A.max_blocks[1] > 0) {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(paged_many_kernel<DT>), hipFuncAttributeMaxDynamicSharedMemorySize, many_lds<DT>());
+    allow_lds<paged_many_kernel<DT>>(many_lds<DT>());
     hipLaunchKernelGGL(paged_many_kernel<DT>, dim3(A.max_blocks[1]), dim3(kMT), many_lds<DT>(), st, A);
     Q35_HIP_TRY(hipGetLastError());
   }

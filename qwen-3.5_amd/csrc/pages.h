@@ -1,5 +1,7 @@
 // Paged caches and token scores: calls between the C ABI (capi_paged.cpp) and the kernels.
 #pragma once
+#include <atomic>
+
 #include "q35_internal.h"
 
 namespace q35 {
@@ -8,6 +10,7 @@ constexpr int kPageHd = 256;            // head_dim
 constexpr int kPageMaxPages = 1 << 18;  // pages of a pool that fork / compact / copy keep in LDS bitmaps
 constexpr int kPageMaxSeqs = 4096;      // rows of a table in fork
 constexpr int kPageMaxRep = 16;         // query heads per kv head
+constexpr int kMaxLds = 150 * 1024;     // dynamic LDS that the kernels here ask for at most
 constexpr int kMaxTop = 64;             // alternatives per row of token_logprobs
 
 inline int elt_size(int dtype) { return dtype == Q35_F32 ? 4 : 2; }
@@ -15,6 +18,19 @@ inline int elt_size(int dtype) { return dtype == Q35_F32 ? 4 : 2; }
 // bytes of one page of one layer
 inline size_t page_bytes(const q35_pages& P) {
   return (size_t)2 * P.kv_heads * P.page * P.head_dim * elt_size(P.dtype);
+}
+
+// Lets a kernel's launches use more than 64 KB of dynamic LDS; asked once per kernel and device (the call
+// takes as long as a third of a launch).
+template <auto kKernel>
+void allow_lds(size_t bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  if (bytes <= 48 * 1024 || hipGetDevice(&dev) != hipSuccess) return;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  if (hipFuncSetAttribute(reinterpret_cast<const void*>(kKernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds) == hipSuccess)
+    done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 int check_pages(const q35_pages& P, const char* what);

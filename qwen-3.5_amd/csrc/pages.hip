@@ -355,12 +355,6 @@ __global__ __launch_bounds__(kCT) void pages_compact_copy_kernel(const CompactCa
   }
 }
 
-// Launches with more than 64 KB of LDS (large pools' bitmaps) ask for it first.
-template <class K>
-void allow_lds(K kernel, size_t bytes) {
-  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-}
-
 }  // namespace
 
 int check_pages(const q35_pages& P, const char* what) {
@@ -396,7 +390,7 @@ int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t*
   a.ok = nullptr;
   if (n > kCT) {
     const size_t lds = ((src.n_pages + 31) / 32 + 2 * (size_t)((dst.n_pages + 31) / 32)) * 4;
-    if (lds > 48 * 1024) allow_lds(pages_copy_check_kernel, lds);
+    allow_lds<pages_copy_check_kernel>(lds);
     hipLaunchKernelGGL(pages_copy_check_kernel, dim3(1), dim3(kPT), lds, st, a, ok);
     Q35_HIP_TRY(hipGetLastError());
     a.ok = ok;
@@ -408,7 +402,7 @@ int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t*
 
 int pages_fork_launch(const ForkCall& c, hipStream_t st) {
   const size_t lds = (size_t)fork_lds(c.P.n_pages, c.B, c.Bo).total * 4;
-  if (lds > 48 * 1024) allow_lds(pages_fork_kernel, lds);
+  allow_lds<pages_fork_kernel>(lds);
   hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(kPT), lds, st, c);
   Q35_HIP_TRY(hipGetLastError());
   hipLaunchKernelGGL(pages_fork_copy_kernel, dim3(c.Bo, c.P.n_layers, 2 * c.P.kv_heads), dim3(kCT), 0, st, c);
@@ -418,7 +412,7 @@ int pages_fork_launch(const ForkCall& c, hipStream_t st) {
 
 int pages_compact_launch(const CompactCall& c, hipStream_t st) {
   const int words = (c.P.n_pages + 31) / 32;
-  if (words * 8 > 48 * 1024) allow_lds(pages_compact_kernel, (size_t)words * 8);
+  allow_lds<pages_compact_kernel>((size_t)words * 8);
   hipLaunchKernelGGL(pages_compact_kernel, dim3(1), dim3(kPT), (size_t)words * 8, st, c);
   Q35_HIP_TRY(hipGetLastError());
   const int64_t pb = (int64_t)page_bytes(c.P);

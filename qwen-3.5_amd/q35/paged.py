@@ -19,6 +19,7 @@ torch's allocator call by call, so calls on several streams and captured graphs 
 import collections
 import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -33,19 +34,28 @@ PagesCompact = collections.namedtuple("PagesCompact", "table refs used")
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprob rank entropy top_ids top_logprobs")
 
 
-def _on(*tensors):
+def _on(first, *tensors):
     """The tensors' device as the current one (they must share it)."""
-    dev = tensors[0].device
+    dev = first.device
+    assert dev.type == "cuda", "tensors must be on the GPU"
     for t in tensors:
         assert t is None or t.device == dev, "tensors on different devices"
-    assert dev.type == "cuda", "tensors must be on the GPU"
     return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _ints(t, *shape):
     """An int32 tensor of the shape, contiguous."""
-    assert t.dtype == torch.int32 and tuple(t.shape) == shape, (t.dtype, tuple(t.shape), shape)
-    return t.contiguous()
+    assert t.dtype is torch.int32 and t.shape == shape, (t.dtype, tuple(t.shape), shape)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=1024)
+def _score_ws_bytes(M, V, top):
+    return L.lib().q35_token_logprobs_ws_bytes(M, V, top)
 
 
 class PagePool:
@@ -85,32 +95,32 @@ def attention_core_paged(dims, pool, layer, q_gate, k_new, v_new, seq_start, pos
     [T, kv_heads*256]; rotary tables [rows, rot_dim]; returns [T, heads*256] (rows of no sequence are left
     as they are in `out`).  check=True synchronises and raises as PagePool.check does."""
     T, B = q_gate.shape[0], pos.shape[0]
-    H, KV = dims.attn_heads, dims.kv_heads
-    for x, n in ((q_gate, 2 * H * dims.head_dim), (k_new, KV * dims.head_dim), (v_new, KV * dims.head_dim)):
-        assert x.dtype == torch.float32 and x.dim() == 2 and x.shape == (T, n) and (x.stride(1) == 1 or n == 1), \
-            (tuple(x.shape), x.dtype, x.stride())
-    assert T <= 1 or k_new.stride(0) == v_new.stride(0), "k_new and v_new must have one row stride"
-    for w, n in ((q_norm, (dims.head_dim,)), (k_norm, (dims.head_dim,)), (rope_cos, (rope_cos.shape[0], dims.rot_dim)),
-                 (rope_sin, (rope_cos.shape[0], dims.rot_dim))):
-        assert w.dtype == torch.float32 and tuple(w.shape) == n and w.is_contiguous(), (tuple(w.shape), n)
+    H, KV, hd, rot, f32 = dims.attn_heads, dims.kv_heads, dims.head_dim, dims.rot_dim, torch.float32
+    for x, n in ((q_gate, 2 * H * hd), (k_new, KV * hd), (v_new, KV * hd)):
+        assert x.dtype is f32 and x.shape == (T, n) and x.stride(1) == 1, (tuple(x.shape), x.dtype, x.stride())
+    # (the stride of a single row says nothing)
+    ld_q, ld_k, ld_v = (q_gate.stride(0), k_new.stride(0), v_new.stride(0)) if T > 1 else (2 * H * hd, KV * hd, KV * hd)
+    assert ld_k == ld_v, "k_new and v_new must have one row stride"
+    rows = rope_cos.shape[0]
+    assert q_norm.shape == (hd,) == k_norm.shape and rope_cos.shape == (rows, rot) == rope_sin.shape
+    for w in (q_norm, k_norm, rope_cos, rope_sin):
+        assert w.dtype is f32 and w.is_contiguous(), (w.dtype, w.stride())
     if out is None:
-        out = torch.empty((T, H * dims.head_dim), dtype=torch.float32, device=q_gate.device)
-    assert out.dtype == torch.float32 and tuple(out.shape) == (T, H * dims.head_dim) and out.stride(1) == 1
-    seq_start, pos, table = _ints(seq_start, B + 1), _ints(pos, B), _ints(table, B, table.shape[1])
+        out = torch.empty((T, H * hd), dtype=f32, device=q_gate.device)
+    assert out.dtype is f32 and out.shape == (T, H * hd) and out.stride(1) == 1, (tuple(out.shape), out.dtype, out.stride())
+    width = table.shape[1]
+    seq_start, pos, table = _ints(seq_start, B + 1), _ints(pos, B), _ints(table, B, width)
     if T == 0 or B == 0:
         return out
-
-    def ld(x):  # (the stride of a single row says nothing)
-        return x.stride(0) if T > 1 else x.shape[1]
-
-    with _on(pool.data, q_gate, k_new, v_new, seq_start, pos, table, q_norm, k_norm, rope_cos, rope_sin, out):
-        nbytes = L.lib().q35_attention_paged_ws_bytes(ctypes.byref(dims), T, B)
+    lib, d = L.lib(), ctypes.byref(dims)
+    with _on(q_gate, pool.data, k_new, v_new, seq_start, pos, table, q_norm, k_norm, rope_cos, rope_sin, out):
+        nbytes = lib.q35_attention_paged_ws_bytes(d, T, B)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q_gate.device)
-        L.check(L.lib().q35_attention_core_paged(
-            ctypes.byref(dims), pool.desc(), int(layer), q_gate.data_ptr(), ld(q_gate), k_new.data_ptr(), v_new.data_ptr(),
-            ld(k_new), T, seq_start.data_ptr(), pos.data_ptr(), B, table.data_ptr(), table.shape[1], q_norm.data_ptr(),
-            k_norm.data_ptr(), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], out.data_ptr(), ld(out),
-            pool.status.data_ptr(), ws.data_ptr(), nbytes, _stream()))
+        L.check(lib.q35_attention_core_paged(
+            d, pool.desc(), layer, q_gate.data_ptr(), ld_q, k_new.data_ptr(), v_new.data_ptr(), ld_k, T, seq_start.data_ptr(),
+            pos.data_ptr(), B, table.data_ptr(), width, q_norm.data_ptr(), k_norm.data_ptr(), rope_cos.data_ptr(),
+            rope_sin.data_ptr(), rows, out.data_ptr(), out.stride(0) if T > 1 else H * hd, pool.status.data_ptr(), ws.data_ptr(),
+            nbytes, _stream()))
     if check:
         pool.check()
     return out
@@ -181,32 +191,29 @@ def token_logprobs(logits, targets=None, top=0, check=False):
     rank counts the tokens before the target in that order.  check=True synchronises and raises Q35Error
     (Q35_E_RANGE) for a target >= V, which otherwise scores NaN with rank -1."""
     V, lead = logits.shape[-1], logits.shape[:-1]
-    assert logits.dtype in _DTYPES, logits.dtype
+    dtype, dev, f32, i32 = _DTYPES.get(logits.dtype), logits.device, torch.float32, torch.int32
+    assert dtype is not None, logits.dtype
     x = logits if logits.dim() == 2 and logits.stride(1) == 1 and logits.stride(0) >= V else logits.reshape(-1, V).contiguous()
     M = x.shape[0]
-    dev = x.device
     if targets is not None:
         targets = _ints(targets, *lead)
-    top = int(top)
     with _on(x, targets):
-        def new(dt, *shape):
-            return torch.empty((*lead, *shape), dtype=dt, device=dev)
-
-        res = TokenLogprobs(new(torch.float32) if targets is not None else None,
-                            new(torch.int32) if targets is not None else None, new(torch.float32),
-                            new(torch.int32, top) if top else None, new(torch.float32, top) if top else None)
+        logprob = rank = ids = lps = status = None
+        if targets is not None:
+            logprob, rank = torch.empty(lead, dtype=f32, device=dev), torch.empty(lead, dtype=i32, device=dev)
+        if top:
+            k = (*lead, top)
+            ids, lps = torch.empty(k, dtype=i32, device=dev), torch.empty(k, dtype=f32, device=dev)
+        res = TokenLogprobs(logprob, rank, torch.empty(lead, dtype=f32, device=dev), ids, lps)
         if M == 0:
             return res
-        status = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
-        nbytes = L.lib().q35_token_logprobs_ws_bytes(M, V, top)
+        if check:
+            status = torch.zeros(1, dtype=i32, device=dev)
+        nbytes = _score_ws_bytes(M, V, top)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-
-        def p(t):
-            return t.data_ptr() if t is not None else None
-
-        L.check(L.lib().q35_token_logprobs(x.data_ptr(), _DTYPES[x.dtype], M, V, x.stride(0) if M > 1 else V, p(targets), top,
-                                           p(res.logprob), p(res.rank), res.entropy.data_ptr(), p(res.top_ids),
-                                           p(res.top_logprobs), p(status), ws.data_ptr(), nbytes, _stream()))
+        L.check(L.lib().q35_token_logprobs(x.data_ptr(), dtype, M, V, x.stride(0) if M > 1 else V, _ptr(targets), top, _ptr(logprob),
+                                           _ptr(rank), res.entropy.data_ptr(), _ptr(ids), _ptr(lps), _ptr(status), ws.data_ptr(),
+                                           nbytes, _stream()))
         if check:
             L.check(L.lib().q35_status_check(status.data_ptr(), _stream()))
     return res
