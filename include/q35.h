@@ -355,12 +355,13 @@ int q35_status_check(uint32_t* status, void* stream);
  * f32, rows 16-byte aligned; rope_cos / rope_sin [rope_rows][rot_dim].  attn_heads / kv_heads at
  * most 16.  A sequence whose positions leave [0, min(ld_table * page, rope_rows)) is skipped, its rows
  * of out as they were; a page outside the pool is not appended to and its tokens count as page 0's
- * (Q35_STATUS_ARG: the sequence's outputs are then invalid).  Keys and values in reach must be
+ * (Q35_STATUS_ARG: the sequence's outputs are then invalid).  A sequence's keys and values must be
  * finite; what lies behind a sequence's last token in its last page may be anything.
  * Products and sums are f32 or their equivalent: 16-bit caches are multiplied as they are with
- * queries and weights carried whole; f32 caches with every value as two f16 halves (22 bits), under
- * one power of two per group of keys.  The keys' norms are formed in f64, so that what a 16-bit cache
- * holds does not hang on the order of a sum.
+ * queries and weights carried whole, f32 caches in f32 or, for chunks of tokens, with every number as two
+ * f16 halves (22 bits) under a power of two for every 4 keys or values: a value's error is then up to 2^-37 of
+ * the largest value its chunk has met.  The keys' norms are formed in f64, so that what a 16-bit cache holds
+ * does not hang on the order of a sum.
  * ws: q35_attention_paged_ws_bytes(d, T, B) bytes of scratch, 16-byte aligned (no zeroing needed). */
 size_t q35_attention_paged_ws_bytes(const q35_dims* d, int32_t T, int32_t B);
 int q35_attention_core_paged(const q35_dims* d, q35_pages pool, int32_t layer, const float* q_gate, int32_t ld_qg,
@@ -391,7 +392,7 @@ int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const i
  * must cover every sequence of the pool that is to live on.  A parent outside [-1, B), or one
  * whose length is negative or more than its row can hold, counts as -1, a kept page outside the pool
  * becomes -1 and a row is cut at ld_table entries (all Q35_STATUS_ARG); where no page is left the entry
- * stays -1 (Q35_STATUS_FULL).  B, B_out <= 4096; n_pages <= 262144. */
+ * stays -1 (Q35_STATUS_FULL).  B, B_out <= 4096; n_pages <= 262144; at most 2^26 entries. */
 int q35_pages_fork(q35_pages pool, const int32_t* table, int32_t ld_table, const int32_t* len, int32_t B,
                    const int32_t* parent, const int32_t* grow, int32_t B_out, int32_t* table_out, int32_t* len_out,
                    int32_t* refs, uint32_t* status, void* stream);
@@ -400,7 +401,7 @@ int q35_pages_fork(q35_pages pool, const int32_t* table, int32_t ld_table, const
  * the i-th lowest named page >= n goes to the i-th lowest unnamed page < n, and the others stay.
  * table_out (another buffer) is the table afterwards, refs [n_pages] its counts, *used = n: pages from n
  * on are free.  An entry outside [-1, n_pages) becomes -1 (Q35_STATUS_ARG).  ws:
- * q35_pages_compact_ws_bytes(n_pages) bytes of scratch.  n_pages <= 262144. */
+ * q35_pages_compact_ws_bytes(n_pages) bytes of scratch.  n_pages <= 262144; at most 2^26 entries. */
 size_t q35_pages_compact_ws_bytes(int32_t n_pages);
 int q35_pages_compact(q35_pages pool, const int32_t* table, int32_t ld_table, int32_t B, int32_t* table_out,
                       int32_t* refs, int32_t* used, uint32_t* status, void* ws, size_t ws_bytes, void* stream);

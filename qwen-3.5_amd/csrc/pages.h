@@ -9,6 +9,8 @@ namespace q35 {
 constexpr int kPageHd = 256;            // head_dim
 constexpr int kPageMaxPages = 1 << 18;  // pages of a pool that fork / compact / copy keep in LDS bitmaps
 constexpr int kPageMaxSeqs = 4096;      // rows of a table in fork
+constexpr int kPageMaxEntries = 1 << 26;  // of a page table in fork / compact (one block goes over them)
+constexpr int kPageMaxHeads = 1024;     // query heads
 constexpr int kPageMaxRep = 16;         // query heads per kv head
 constexpr int kMaxLds = 150 * 1024;     // dynamic LDS that the kernels here ask for at most
 constexpr int kMaxTop = 64;             // alternatives per row of token_logprobs

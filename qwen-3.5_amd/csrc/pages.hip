@@ -358,15 +358,15 @@ __global__ __launch_bounds__(kCT) void pages_compact_copy_kernel(const CompactCa
 }  // namespace
 
 int check_pages(const q35_pages& P, const char* what) {
-  const std::string w(what);
-  if (!P.data) return fail(Q35_E_ARG, w + ": null pool");
-  if (P.dtype != Q35_F32 && P.dtype != Q35_F16 && P.dtype != Q35_BF16) return fail(Q35_E_ARG, w + ": bad pool dtype");
-  if (P.head_dim != kPageHd) return fail(Q35_E_SHAPE, w + ": head_dim must be 256");
+  auto no = [&](int code, const char* why) { return fail(code, std::string(what) + why); };
+  if (!P.data) return no(Q35_E_ARG, ": null pool");
+  if (P.dtype != Q35_F32 && P.dtype != Q35_F16 && P.dtype != Q35_BF16) return no(Q35_E_ARG, ": bad pool dtype");
+  if (P.head_dim != kPageHd) return no(Q35_E_SHAPE, ": head_dim must be 256");
   if (P.page < 16 || P.page > 256 || (P.page & (P.page - 1)) != 0)
-    return fail(Q35_E_SHAPE, w + ": tokens per page must be a power of two in 16..256");
+    return no(Q35_E_SHAPE, ": tokens per page must be a power of two in 16..256");
   if (P.n_layers < 1 || P.n_layers > 65535 || P.n_pages < 1 || P.n_pages > kPageMaxPages || P.kv_heads < 1 || P.kv_heads > 1024)
-    return fail(Q35_E_SHAPE, w + ": layers, pages (at most 262144) and kv heads (at most 1024) must be positive");
-  if ((reinterpret_cast<uintptr_t>(P.data) & 15) != 0) return fail(Q35_E_ALIGN, w + ": pool not 16-byte aligned");
+    return no(Q35_E_SHAPE, ": layers, pages (at most 262144) and kv heads (at most 1024) must be positive");
+  if ((reinterpret_cast<uintptr_t>(P.data) & 15) != 0) return no(Q35_E_ALIGN, ": pool not 16-byte aligned");
   return Q35_OK;
 }
 

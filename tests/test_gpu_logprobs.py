@@ -132,9 +132,25 @@ def test_nan_and_infinity():
         assert r.logprob[:3].isnan().all() and r.entropy[:3].isnan().all() and r.top_logprobs[:3].isnan().all()
         assert 17 not in r.top_ids[0].tolist() and r.top_ids[1].tolist() == list(range(40)) and r.top_ids[2, 0] == 40
         assert r.logprob[3].isfinite()
+        for tt in ([17, 2, 40, 3], [18, V - 1, 41, 0]):  # targets that are a NaN, lie among NaN, are the infinity
+            tt = torch.tensor(tt, dtype=torch.int32, device="cuda")
+            want = R.scores(x.double().cpu().numpy(), tt.cpu().numpy(), 1)[1]
+            assert q35.token_logprobs(x, tt).rank.tolist() == want.tolist()
         x[0, :V - 5] = nan
         ids = q35.token_logprobs(x, top=10).top_ids[0].tolist()
         assert sorted(ids[:5]) == list(range(V - 5, V)) and ids[5:] == list(range(5))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_ranks_at_every_place(dtype):
+    """The target is each value of a row with ties in turn: words before, around and behind it; zeros of both signs."""
+    V = 97
+    x = (logits(8, 1, V, sigma=1.5).round() * torch.where(torch.arange(V, device="cuda") % 2 == 0, 1.0, -1.0)).to(DT[dtype]).repeat(V, 1)
+    t = torch.arange(V, dtype=torch.int32, device="cuda")
+    r = check(x, t, 5)
+    assert sorted(r.rank.tolist()) == list(range(V))
+    y = torch.cat([logits(9, V, 4000, dtype), x], 1)
+    check(y, t + 4000, 5)
 
 
 def test_targets_outside():

@@ -112,6 +112,112 @@ def test_attention_matches_64bit(dtype, page, heads, kv, seqs):
     check_attention(c, out, pool)
 
 
+LARGER = [
+    # chunks whose tiles are cut by several blocks; several tiles; more than 64 and more than 256 sequences
+    ("f32", 64, 8, 2, [(300, 900)]),
+    ("bf16", 32, 8, 2, [(200, 1500), (90, 0), (1, 2000)]),
+    ("f16", 16, 8, 2, [(150, 700), (40, 1200)] + [(1, 37 * i) for i in range(20)]),
+    ("f32", 16, 4, 1, [(1, 11 * i % 200) for i in range(70)]),
+    ("bf16", 16, 2, 1, [(i % 3, (7 * i) % 90) for i in range(330)]),
+    ("f32", 32, 8, 2, [(1, 50)] * 30 + [(28, 400)]),      # up to two tokens a sequence on average, one long
+    ("f16", 32, 16, 1, [(1, 300), (2, 30), (3, 170)]),
+]
+
+
+@pytest.mark.parametrize("dtype,page,heads,kv,seqs", LARGER)
+def test_attention_larger_batches(dtype, page, heads, kv, seqs):
+    print(dtype, page, heads, kv, seqs[:6], len(seqs), flush=True)
+    c = make_attention(31, dtype, page, heads, kv, seqs)
+    check_attention(c, *run_attention(c))
+
+
+@pytest.mark.parametrize("dtype,scale", [("f32", 1e-12), ("f32", 1e12), ("f16", 2.0 ** -20), ("f16", 2.0 ** 9), ("bf16", 1e-30), ("bf16", 1e30)])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_values_of_any_size(dtype, scale, n):
+    """Values of the cache and the new ones all scaled; f16 reaches its subnormal numbers."""
+    c = make_attention(32, dtype, 32, 8, 2, [(n, 200)])
+    c["pool"][:, :, 1] = (c["pool"][:, :, 1].double() * scale).to(c["pool"].dtype)
+    c["v"] = (c["v"] * np.float32(scale)).astype(np.float32)
+    check_attention(c, *run_attention(c))
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_values_zero_in_places(n):
+    """Pages of zeros beside small values (f32: the zeros must not set the values' power of two), uneven rows."""
+    c = make_attention(33, "f32", 16, 8, 2, [(n, 150)])
+    c["pool"] *= 1e-6
+    for p in c["table"][0][1:9:2]:
+        c["pool"][:, p] = 0.0
+    c["v"][:] *= 1e-6
+    check_attention(c, *run_attention(c))
+    # every 4 tokens' values two thousand times the 4 before: an error of 2^-37 of the largest is allowed
+    c = make_attention(34, "f32", 16, 8, 2, [(n, 60)])
+    c["v"][:] *= 1e-3
+    for t in range(60):
+        c["pool"][:, c["table"][0][t // 16], 1, :, t % 16] *= 2000.0 ** (t // 4 % 3)
+    check_attention(c, *run_attention(c))
+
+
+def test_attention_stream_larger_than_the_last_level_cache():
+    """70000 tokens of two f32 heads: the loads that pass the caches by, against the contiguous kernel."""
+    ctx, page = 70000, 64
+    dims = q35.dims_2b()
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    rnd = lambda *s, f=1.0: torch.randn(s, generator=g, device="cuda") * f
+    n = -(-(ctx + 1) // page)
+    pool = q35.PagePool(torch.randn((1, n, 2, 2, page, HD), generator=g, device="cuda"))
+    table = torch.randperm(n, generator=torch.Generator().manual_seed(1)).int().cuda()[None]
+    kc, vc = (pool.data[0, table[0].long(), i].permute(1, 0, 2, 3).reshape(1, 2, -1, HD).contiguous() for i in (0, 1))
+    qg, k, v, qw, kw = rnd(1, 4096), rnd(1, 512), rnd(1, 512), rnd(HD, f=0.2) + 0.5, rnd(HD, f=0.2)
+    cos, sin = (torch.from_numpy(a).cuda() for a in q35.rope_tables(dims, kc.shape[2]))
+    out = q35.attention_core_paged(dims, pool, 0, qg, k, v, i32([0, 1]), i32([ctx]), table, qw, kw, cos, sin, check=True)
+    want = q35.attention_core_decode(dims, qg, k, v, qw, kw, kc, vc, i32([ctx]), cos, sin, check=True)
+    # both sum 70001 f32 terms of weight 1 in all, off by a few 2^-20 of the scores' size (tests/paged_ref.py)
+    torch.testing.assert_close(out, want, rtol=0, atol=4 * 12 * 2.0 ** -20 * float(vc.abs().max()))
+    assert float((out - want).abs().max()) < 1e-5
+    p = int(table[0, ctx // page])
+    torch.testing.assert_close(pool.data[0, p, 0, :, ctx % page], kc[0, :, ctx], rtol=2e-6, atol=1e-6)
+    assert torch.equal(pool.data[0, p, 1, :, ctx % page], v.view(2, HD))
+
+
+def test_attention_one_sequence_in_a_padded_call():
+    """One sequence whose rows are fewer than the call's (a captured chunk's shape), down to none."""
+    for n in (0, 1, 9, 60):
+        c = make_attention(35, "bf16", 32, 8, 2, [(60, 70)])
+        c["start"] = np.array([0, n])
+        full = torch.full((60, 2048), 4.0, device="cuda")
+        out, pool = run_attention(c, out=full)
+        assert (out[n:] == 4.0).all()
+        cut = dict(c, qg=c["qg"][:n], k=c["k"][:n], v=c["v"][:n])
+        check_attention(cut, out[:n], pool)
+
+
+def test_attention_starts_that_fall_are_refused():
+    c = make_attention(36, "f32", 32, 8, 2, [(5, 40), (40, 20), (3, 9)])
+    bad = dict(c, start=np.array([0, 45, 5, 48]))
+    out, pool = run_attention(bad, out=torch.full((48, 2048), 6.0, device="cuda"))
+    assert (out == 6.0).all()
+    with pytest.raises(q35.Q35Error, match="Q35_E_RANGE"):
+        pool.check()
+    for start in ([0, 5, 45, 49], [-1, 5, 45, 48], [3, 5, 45, 48]):  # past the rows, before them, rows without a sequence
+        out, pool = run_attention(dict(c, start=np.array(start)), out=torch.full((48, 2048), 6.0, device="cuda"))
+        if start[0] == 3:
+            assert (out[:3] == 6.0).all() and not (out[3:] == 6.0).any()
+            pool.check()
+        else:
+            with pytest.raises(q35.Q35Error, match="Q35_E_RANGE"):
+                pool.check()
+            assert (out[45:] == 6.0).all() if start[0] == 0 else (out[:5] == 6.0).all()
+
+
+def test_attention_same_bits_on_every_run():
+    c = make_attention(37, "f16", 16, 8, 2, [(1, 700), (90, 333), (5, 100), (1, 0)])
+    first = run_attention(c)[0]
+    for _ in range(3):
+        assert torch.equal(run_attention(c)[0], first)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("fill", [float("nan"), float("inf"), -float("inf")])
 def test_attention_ignores_what_no_token_occupies(dtype, fill):
