@@ -346,14 +346,16 @@ typedef struct {
 } q35_pages;
 int q35_status_check(uint32_t* status, void* stream);
 
-/* The attention core (q35_attention_core_prefill's arithmetic) for the new tokens of B sequences over
- * the paged cache of layer `layer`: rows seq_start[b] .. seq_start[b+1]-1 of the T rows are the new
- * tokens of sequence b (none, one, or any number of them), at positions pos[b] .. ; seq_start is int32
- * [B+1], non-decreasing from 0, and rows from seq_start[B] on are neither read nor written.  Keys
- * and values are appended to the sequence's pages, then each new token attends to positions 0 .. its
- * own.  q_gate [T][ld_qg] (per head [query | gate]), k_new and v_new [T][kv_ld], out [T][ld_out],
- * f32, rows 16-byte aligned; rope_cos / rope_sin [rope_rows][rot_dim].  attn_heads / kv_heads at
- * most 16.  A sequence whose positions leave [0, min(ld_table * page, rope_rows)) is skipped, its rows
+/* The attention core (q35_attention_core_prefill's arithmetic) for the new tokens of B sequences
+ * over the paged cache of layer `layer`: rows seq_start[b] .. seq_start[b+1]-1 of the T rows are the
+ * new tokens of sequence b (none, one, or any number of them), at positions pos[b] .. ; seq_start is
+ * int32 [B+1], non-decreasing from 0 (where it falls, Q35_STATUS_ARG: no row of out is written and
+ * what is appended is undefined), and rows from seq_start[B] on count for nothing and stay in out as
+ * they were.  Keys and values are appended to the sequence's pages, then each new token attends to
+ * positions 0 .. its own.  q_gate [T][ld_qg] (per head [query | gate]), k_new and v_new [T][kv_ld],
+ * out [T][ld_out], f32, rows 16-byte aligned; rope_cos / rope_sin [rope_rows][rot_dim].  attn_heads
+ * / kv_heads at most 16; T and B at most 2^20, T (attn_heads + kv_heads) < 2^25; out overlaps no
+ * input.  A sequence whose positions leave [0, min(ld_table * page, rope_rows)) is skipped, its rows
  * of out as they were; a page outside the pool is not appended to and its tokens count as page 0's
  * (Q35_STATUS_ARG: the sequence's outputs are then invalid).  A sequence's keys and values must be
  * finite; what lies behind a sequence's last token in its last page may be anything.
@@ -407,7 +409,7 @@ int q35_pages_compact(q35_pages pool, const int32_t* table, int32_t ld_table, in
                       int32_t* refs, int32_t* used, uint32_t* status, void* ws, size_t ws_bytes, void* stream);
 
 /* Scores of M rows of logits [M][ld] over V values (dtype Q35_F32 / _F16 / _BF16; rows need no
- * alignment beyond the type's), with lse = ln sum e^x:
+ * alignment beyond the type's; M < 2^24, V at most 2^30), with lse = ln sum e^x:
  *   logprob[m] = x[targets[m]] - lse;
  *   rank[m]    = the number of tokens ranked before the target: larger logits, and equal ones of a
  *                lower id;

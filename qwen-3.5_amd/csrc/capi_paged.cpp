@@ -3,7 +3,6 @@
 #include "pages.h"
 
 #include <algorithm>
-#include <climits>
 #include <cmath>
 
 namespace q35 {
@@ -23,6 +22,10 @@ inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
   const char *x = static_cast<const char*>(a), *y = static_cast<const char*>(b);
   return x < y + nb && y < x + na;
 }
+// A launch has fewer than 2^32 threads along x: so many blocks of 256.
+constexpr int kMaxGrid = 1 << 24;
+// The paged attention's append has one block for 4 (row, query or kv head)s and one more.
+inline bool rows_fit(const q35_dims* d, int32_t T) { return (int64_t)T * (d->attn_heads + d->kv_heads) < (1 << 25); }
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace
@@ -49,7 +52,7 @@ int q35_status_check(uint32_t* status, void* stream) {
 
 size_t q35_attention_paged_ws_bytes(const q35_dims* d, int32_t T, int32_t B) {
   if (!d || T < 1 || B < 1 || T > (1 << 20) || B > (1 << 20) || d->kv_heads < 1 || d->attn_heads < d->kv_heads ||
-      d->attn_heads > kPageMaxHeads || d->attn_heads / d->kv_heads > kPageMaxRep)
+      d->attn_heads > kPageMaxHeads || d->attn_heads / d->kv_heads > kPageMaxRep || !rows_fit(d, T))
     return 0;
   return paged_attn_ws_bytes(d->attn_heads, d->kv_heads, T, B);
 }
@@ -74,6 +77,7 @@ int q35_attention_core_paged(const q35_dims* d, q35_pages pool, int32_t layer, c
     if (layer < 0 || layer >= pool.n_layers) return fail(Q35_E_SHAPE, "attention_paged: no such layer in the pool");
     if (T < 1 || B < 1 || T > (1 << 20) || B > (1 << 20) || ld_table < 1 || rope_rows < 1 || rope_rows > (1 << 30))
       return fail(Q35_E_SHAPE, "attention_paged: T and B in 1..2^20, ld_table >= 1 and rope_rows in 1..2^30 required");
+    if (!rows_fit(d, T)) return fail(Q35_E_SHAPE, "attention_paged: T (heads + kv heads) < 2^25 required");
     if (ld_qg < 2 * d->attn_heads * kPageHd || kv_ld < d->kv_heads * kPageHd || ld_out < d->attn_heads * kPageHd)
       return fail(Q35_E_SHAPE, "attention_paged: row strides too small");
     if (ld_qg % 4 || kv_ld % 4 || ld_out % 4 || !aligned(q_gate, 16) || !aligned(k_new, 16) || !aligned(v_new, 16) ||
@@ -116,7 +120,7 @@ int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const i
       return fail(Q35_E_ARG, "pages_copy: two pools that overlap");
     if (n == 0) return Q35_OK;
     if (!src_ids || !dst_ids) return fail(Q35_E_ARG, "pages_copy: null pointer");
-    if ((int64_t)n * (int64_t)(pb / 16384) > INT_MAX) return fail(Q35_E_SHAPE, "pages_copy: too many pages for one call");
+    if ((int64_t)n * (int64_t)(pb / 16384) >= kMaxGrid) return fail(Q35_E_SHAPE, "pages_copy: too many pages for one call");
     if (!ws || ws_bytes < q35_pages_copy_ws_bytes(n)) return fail(Q35_E_WS, "pages_copy: workspace too small");
     return pages_copy_launch(src, dst, src_ids, dst_ids, n, status, static_cast<uint8_t*>(ws), S(stream));
   });
@@ -184,7 +188,7 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
     if (targets && (!logprob || !rank)) return fail(Q35_E_ARG, "token_logprobs: targets need logprob and rank");
     if (dtype != Q35_F32 && dtype != Q35_F16 && dtype != Q35_BF16) return fail(Q35_E_ARG, "token_logprobs: bad dtype");
     // (indices shifted by up to 8 values stay below 2^31)
-    if (M < 1 || M > (1 << 24) || V < 1 || V > (1 << 30) || ld < V) return fail(Q35_E_SHAPE, "token_logprobs: 1 <= M <= 2^24, 1 <= V <= 2^30 and ld >= V required");
+    if (M < 1 || M >= kMaxGrid || V < 1 || V > (1 << 30) || ld < V) return fail(Q35_E_SHAPE, "token_logprobs: 1 <= M < 2^24, 1 <= V <= 2^30 and ld >= V required");
     if (top < 0 || top > kMaxTop || top > V) return fail(Q35_E_SHAPE, "token_logprobs: top must be in 0..64 and at most V");
     if (top > 0 && (!top_ids || !top_logprobs)) return fail(Q35_E_ARG, "token_logprobs: top needs top_ids and top_logprobs");
     if (!aligned(logits, elt_size(dtype))) return fail(Q35_E_ALIGN, "token_logprobs: logits not aligned to their type");

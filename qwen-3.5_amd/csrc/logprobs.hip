@@ -104,14 +104,19 @@ Q35_DEV void merge_keys(key_t* buf, int n, key_t& best, key_t& last, int top) {
   wave_sync();
   const key_t c = lane < n ? buf[lane] : 0;
   int pc = 0, pb = lane;
-#pragma unroll 4
-  for (int j = 0; j < n; ++j) {
-    const key_t k = lane_key(c, j);
-    pc += k > c ? 1 : 0;
-    pb += k > best ? 1 : 0;
+  // (four at a time: the places behind the n and behind the list's `top` hold 0, which is larger than nothing)
+  for (int j = 0; j < n; j += 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const key_t k = lane_key(c, j + e);
+      pc += k > c ? 1 : 0;
+      pb += k > best ? 1 : 0;
+    }
   }
-#pragma unroll 4
-  for (int j = 0; j < top; ++j) pc += lane_key(best, j) > c ? 1 : 0;
+  for (int j = 0; j < top; j += 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) pc += lane_key(best, j + e) > c ? 1 : 0;
+  }
   wave_sync();
   buf[lane] = 0;
   wave_sync();

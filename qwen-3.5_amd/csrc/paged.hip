@@ -1161,13 +1161,17 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B) {
   PagedLayout L;
   const int rep = nh / nkv, tok_many = kManyRows / rep;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+  // A sequence of two tiles of "few" rows, or of one token, is "few": 5 drafted tokens of 4 heads (20 rows) behind
+  // 100 take 9.4 us there and 17.8 as a chunk.  16 tokens (4 tiles) take 20 us behind 200 and 98 behind 30000 in
+  // f32, 32 and 47 as a chunk: every tile reads the context again.
   // Which kinds there are is the device's knowledge; what a call cannot or need not have gets no launch (an
-  // empty one takes 4 us).  Up to two tokens per sequence on average: all are "few" (one that is longer then
-  // costs its own stream again for every 16 rows, a fraction of the batch's).  One sequence: its rows decide,
-  // if all rows are its.  Else a sequence of two tiles of "few" rows, or of one token, is "few": 5 drafted
-  // tokens of 4 heads (20 rows) behind 100 take 9.4 us there and 17.8 as a chunk.
-  const bool few_only = T <= 2 * B || (int64_t)T * rep <= 2 * kFewRows, many_only = !few_only && B == 1;
-  L.few_most = few_only ? INT_MAX : many_only ? 0 : std::max(1, 2 * kFewRows / rep);
+  // empty one takes 4 us).  If no sequence is empty, the longest has T - B + 1 tokens at most: where that is
+  // "few", all are (were all "few" up to two tokens per sequence, 63 of one token behind 2000 and one of 64
+  // behind 30000 would take 207 us, 133 so).  One sequence: its rows decide, if all rows are its.
+  L.few_most = std::max(1, 2 * kFewRows / rep);
+  const bool few_only = T - B + 1 <= L.few_most, many_only = !few_only && B == 1;
+  if (few_only) L.few_most = INT_MAX;
+  if (many_only) L.few_most = 0;
   const int seqs = std::min(B, T);
   L.max_tiles[0] = many_only ? 0 : (int)(((int64_t)T * rep + kFewRows - 1) / kFewRows + seqs);
   L.max_tiles[1] = few_only ? 0 : T / tok_many + seqs;

@@ -223,7 +223,7 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
   if (tid == 0) base[c.Bo] = run;
   __syncthreads();
   // kept entries, and -1 behind each row's pages
-  const int ne = c.Bo * c.ld;  // (at most 2^28)
+  const int ne = c.Bo * c.ld;  // (at most 2^26)
   constexpr int kU = 4;  // entries of a thread in flight
   for (int e0 = tid; e0 < ne; e0 += kU * kPT) {
     int v[kU], kind[kU];  // kind: 0 not written here, 1 behind the row's pages, 2 kept

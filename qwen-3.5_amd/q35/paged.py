@@ -193,7 +193,9 @@ def token_logprobs(logits, targets=None, top=0, check=False):
     V, lead = logits.shape[-1], logits.shape[:-1]
     dtype, dev, f32, i32 = _DTYPES.get(logits.dtype), logits.device, torch.float32, torch.int32
     assert dtype is not None, logits.dtype
-    x = logits if logits.dim() == 2 and logits.stride(1) == 1 and logits.stride(0) >= V else logits.reshape(-1, V).contiguous()
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)  # (a view where the rows have one stride)
+    if x.stride(1) != 1 or x.stride(0) < V:
+        x = x.contiguous()
     M = x.shape[0]
     if targets is not None:
         targets = _ints(targets, *lead)

@@ -81,6 +81,23 @@ def test_strided_and_unaligned_rows(V, off, dtype):
     check(wide[:, off:off + V], targets_of(V, 4, V), min(V, 11))
 
 
+def test_padded_vocabulary_is_not_copied():
+    """Rows [B, T, V] cut out of wider ones have one stride: they are read where they are."""
+    V, wide = 20001, 20032
+    x = logits(9, 6, wide, "bf16").view(2, 3, wide)
+    x[..., V:] = float("nan")
+    t = targets_of(10, 6, V)
+    q35.token_logprobs(x[..., :V], t.view(2, 3), top=5)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    r = q35.token_logprobs(x[..., :V], t.view(2, 3), top=5)
+    assert torch.cuda.max_memory_allocated() - before < x.numel() * 2
+    want = check(x.view(6, wide)[:, :V], t, 5)  # (a copy's rows begin elsewhere in their 16-byte words: sums in another order)
+    for u, v in zip(r, want):
+        assert torch.equal(u.flatten(), v.flatten())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_ties_go_to_the_lowest_id(dtype):
     for V in (100, 3000, 60000):

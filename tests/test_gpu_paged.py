@@ -131,6 +131,20 @@ def test_attention_larger_batches(dtype, page, heads, kv, seqs):
     check_attention(c, *run_attention(c))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv,seqs", [
+    (8, 2, [(1, 60)] * 7 + [(8, 300)]),     # two tiles beside single tokens, and a token more
+    (8, 2, [(1, 60)] * 7 + [(9, 300)]),
+    (8, 2, [(0, 5)] * 20 + [(25, 400)]),    # a long one among empty ones, fewer tokens than sequences
+    (16, 1, [(1, 60), (0, 3), (3, 200)]),
+    (2, 2, [(32, 40), (33, 90), (1, 7)]),   # one head per kv head: 32 tokens are two tiles
+])
+def test_attention_few_and_many_tokens_meet(dtype, heads, kv, seqs):
+    print(dtype, heads, kv, seqs, flush=True)
+    c = make_attention(77, dtype, 32, heads, kv, seqs)
+    check_attention(c, *run_attention(c))
+
+
 @pytest.mark.parametrize("dtype,scale", [("f32", 1e-12), ("f32", 1e12), ("f16", 2.0 ** -20), ("f16", 2.0 ** 9), ("bf16", 1e-30), ("bf16", 1e30)])
 @pytest.mark.parametrize("n", [1, 40])
 def test_attention_values_of_any_size(dtype, scale, n):

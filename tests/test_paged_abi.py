@@ -172,3 +172,23 @@ def test_plain_attention_against_an_independent_one():
     want = np.cumsum(v, 0) / np.arange(1, 4)[:, None] / 2
     np.testing.assert_allclose(out, np.concatenate([want, want], 1), atol=1e-6)
     assert torch.equal(pool[0, 2, 1, 0, :3], torch.from_numpy(v)) and (pool[0, :2] == 0).all() and tol.min() > 0
+
+
+def test_limits():
+    """Heads, rotary rows, table entries and launch sizes beyond what the kernels index."""
+    assert attention(attn_heads=2048, kv_heads=128, pool=pages(kv_heads=128), ld_qg=1 << 20, kv_ld=1 << 15, ld_out=1 << 19) == L.Q35_E_SHAPE
+    assert attention(rows=(1 << 30) + 1) == L.Q35_E_SHAPE
+    wide = dict(attn_heads=64, kv_heads=16)
+    big = dict(wide, pool=pages(kv_heads=16), T=1 << 20, ld_qg=1 << 15, kv_ld=1 << 12, ld_out=1 << 14)  # T (heads + kv heads) > 2^25
+    assert attention(**big) == L.Q35_E_SHAPE
+    ws = L.lib().q35_attention_paged_ws_bytes
+    assert ws(ctypes.byref(q35.make_dims(**wide)), 1 << 20, 4) == 0
+    for bad in (dict(kv_heads=0), dict(attn_heads=0), dict(attn_heads=1, kv_heads=2), dict(attn_heads=-8), dict(attn_heads=2048, kv_heads=128), dict(attn_heads=34)):
+        assert ws(ctypes.byref(q35.make_dims(**bad)), 4, 4) == 0, bad
+    assert ws(ctypes.byref(q35.dims_2b()), (1 << 20) + 1, 4) == 0 and ws(ctypes.byref(q35.dims_2b()), 4, (1 << 20) + 1) == 0
+    assert fork(ld=65536, B=1, B_out=1025, out=A + (1 << 28)) == L.Q35_E_SHAPE
+    assert fork(len_out=A + 8) == L.Q35_E_ARG  # the last of len's three
+    assert compact(ld=65536, B=1025, out=A + (1 << 30)) == L.Q35_E_SHAPE
+    one = pages(n_layers=1, kv_heads=1, page=256, dtype=L.Q35_F32)  # 32 units of 16 KB per page
+    assert L.lib().q35_pages_copy(one, one, A, A, 1 << 19, None, A, 1 << 40, None) == L.Q35_E_SHAPE
+    assert score(M=1 << 24, top=0) == L.Q35_E_SHAPE
