@@ -12,7 +12,8 @@
 // sorted, one per lane; a chunk of values costs one comparison of each lane's maximum with the
 // last wanted key, and only values above it are put aside and joined with the list, up to 64 at a time.  The
 // first chunk would put almost everything aside: the last wanted key starts at the `top`-th of the 64
-// lanes' maxima instead (that many values are at least as large).
+// lanes' maxima instead (that many values are at least as large), or, for more than 32, the (top / 2)-th of
+// their second largest values.
 // Waves, then the splits of a row (blocks), are joined by ranks: a key's place is the number of larger
 // keys.
 #include "pages.h"
@@ -28,7 +29,9 @@ constexpr int kT = 256;         // threads per block
 constexpr int kNW = kT / 64;
 constexpr int kPer = 16;        // values of a lane per chunk
 constexpr int kChunk = 64 * kPer;
-constexpr int kMaxSplit = 256;  // blocks per row: the joining block holds one head key per thread
+constexpr int kMaxSplit = 256;  // blocks per row: the joining block holds one part's sums per thread
+constexpr int kLevels = 7;      // of the join's floors: 2^6 = kMaxTop
+constexpr int kMaxCand = kLevels * kMaxTop;  // sum over i of 2^i ceil(top / 2^i), 2^i <= top
 
 typedef unsigned long long key_t;
 
@@ -113,9 +116,11 @@ Q35_DEV void merge_keys(key_t* buf, int n, key_t& best, key_t& last, int top) {
       pb += k > best ? 1 : 0;
     }
   }
-  for (int j = 0; j < top; j += 4) {
+  if (lane_key(best, 0) != 0) {  // (the first time there is no list)
+    for (int j = 0; j < top; j += 4) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) pc += lane_key(best, j + e) > c ? 1 : 0;
+      for (int e = 0; e < 4; ++e) pc += lane_key(best, j + e) > c ? 1 : 0;
+    }
   }
   wave_sync();
   buf[lane] = 0;
@@ -130,10 +135,30 @@ Q35_DEV void merge_keys(key_t* buf, int n, key_t& best, key_t& last, int top) {
   last = t > last ? t : last;
 }
 
-// Final numbers of row m of the call.
-Q35_DEV void finish_row(const ScoreCall& c, int m, float mx, double S, double U, int cnt) {
-  const double l = log(S);
-  if (c.entropy) c.entropy[m] = S > 0.0 ? (float)fmax(l - U / S, 0.0) : S == 0.0 ? 0.f : NAN;
+// What a key must pass, from one value of every lane (-inf or NaN: none): the r-th largest of them, without its
+// lowest 6 bits (the lane's number takes their place, so that no two are equal); that many keys do.  0 if
+// fewer lanes have one.
+Q35_DEV key_t seed_key(float v, int r) {
+  const uint32_t a = (v > -INFINITY ? asc(v) & ~63u : 0u) | (threadIdx.x & 63);
+  int before = 0;
+#pragma unroll 8
+  for (int l = 0; l < 64; ++l) before += (uint32_t)__builtin_amdgcn_readlane((int)a, l) > a ? 1 : 0;
+  const unsigned long long at = __ballot(before == r - 1);
+  const uint32_t t = (uint32_t)__builtin_amdgcn_readlane((int)a, (int)__builtin_ctzll(at)) & ~63u;
+  return t == 0 ? 0 : ((key_t)t << 32) - 1;
+}
+
+// ln S, S a normal number: the exponent apart from the rest, whose logarithm is off by a few 2^-24 at most.
+// (With the f64 functions, whose code every block fetches, and the lists asked for only when wanted, the join
+// took 7.2 us; 5.1 so.)
+Q35_DEV double ln_sum(double S) {
+  int e;
+  const float f = (float)frexp(S, &e);
+  return (double)e * 0.693147180559945309 + (double)(__builtin_amdgcn_logf(f) * 0.693147180559945309f);
+}
+// Final numbers of row m of the call; l = ln S.
+Q35_DEV void finish_row(const ScoreCall& c, int m, float mx, double S, double U, double l, int cnt) {
+  if (c.entropy) c.entropy[m] = S > 0.0 ? fmaxf((float)l - (float)U / (float)S, 0.f) : S == 0.0 ? 0.f : NAN;
   if (!c.targets) return;
   const int t = c.targets[m];
   if (t < 0 || t >= c.V) {
@@ -147,11 +172,11 @@ Q35_DEV void finish_row(const ScoreCall& c, int m, float mx, double S, double U,
   c.logprob[m] = mx == -INFINITY && S == 0.0 ? -INFINITY : (float)((double)(x - mx) - l);
   c.rank[m] = cnt;
 }
-Q35_DEV void put_top(const ScoreCall& c, int m, int i, key_t k, float mx, double S) {
+Q35_DEV void put_top(const ScoreCall& c, int m, int i, key_t k, float mx, double S, double l) {
   const int64_t o = (int64_t)m * c.top + i;
   c.top_ids[o] = key_index(k);
   const float x = from_asc((uint32_t)(k >> 32));
-  c.top_lp[o] = mx == -INFINITY && S == 0.0 ? -INFINITY : (float)((double)(x - mx) - log(S));
+  c.top_lp[o] = mx == -INFINITY && S == 0.0 ? -INFINITY : (float)((double)(x - mx) - l);
 }
 
 // Blocks (row, split).
@@ -255,46 +280,50 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
     if (top > 0) {
       if (first) {  // (uniform in the wave)
         first = false;
-        int im = -1;  // the lane's first largest value (lanes without values, or with NaN alone, have none)
+        last = seed_key(mx, top);
+        if (top > 32) {  // second largest values: half of the lanes are enough
+          float m1 = -INFINITY, m2 = -INFINITY;
 #pragma unroll
-        for (int e = kPer - 1; e >= 0; --e) im = x[e] == mx && ((ok >> e) & 1u) ? idx0[e / kVec] + e % kVec : im;
-        const key_t lm = im >= 0 ? key_of(mx, im) : 0;
-        int before = 0;
-#pragma unroll 4
-        for (int l = 0; l < 64; ++l) before += lane_key(lm, l) > lm ? 1 : 0;
-        const unsigned long long at = __ballot(before == top - 1 && lm != 0);
-        if (at) last = lane_key(lm, (int)__builtin_ctzll(at)) - 1;
+          for (int e = 0; e < kPer; ++e) {
+            const float v = x[e] == x[e] ? x[e] : -INFINITY;  // (the smaller of a number and NaN is the number)
+            m2 = fmaxf(m2, fminf(m1, v));
+            m1 = fmaxf(m1, v);
+          }
+          const key_t l2 = seed_key(m2, (top + 1) / 2);
+          last = l2 > last ? l2 : last;
+        }
       }
       if (__ballot(asc(mx) >= (uint32_t)(last >> 32))) {
         // values at or above the last wanted one (all, while that is nothing or NaN)
         const float lf = from_asc((uint32_t)(last >> 32));
         const bool open = (uint32_t)(last >> 32) == 0;
-        int total = 0;
+        uint32_t left = 0;  // the lane's values to look at
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) total += __popcll(__ballot(x[e] >= lf || open));
-        if (total <= 64) {
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) {
-            if (__ballot(x[e] >= lf || open)) {
-              const key_t k = (ok >> e) & 1u ? key_of(x[e], idx0[e / kVec] + e % kVec) : 0;
-              push_keys(buf[wid], n, k, k > last);
-            }
-          }
-          if (n > 0) merge_keys(buf[wid], n, best, last, top);
-          n = 0;
-        } else {  // more than fit: one value of every lane at a time
-#pragma unroll
-          for (int e = 0; e < kPer; ++e) stage[wid][e][lane] = x[e];
-          wave_sync();
+        for (int e = 0; e < kPer; ++e) {
+          left |= (x[e] >= lf || open ? 1u : 0u) << e;
+          stage[wid][e][lane] = x[e];
+        }
+        left &= ok;
+        wave_sync();
+        // one of every lane at a time (a loop: written out for each of the 16 values, its code, which every
+        // block fetches, took 0.6 us); joined with the list whenever 64 are full
 #pragma unroll 1
-          for (int e = 0; e < kPer; ++e) {
-            const int f = (w0 + (e / kVec) * 64 + lane) * kVec - shift + e % kVec;
-            const key_t k = (ok >> e) & 1u ? key_of(stage[wid][e][lane], f) : 0;
+        for (;;) {
+          const unsigned long long any = __ballot(left != 0);
+          const int e = left != 0 ? __ffs(left) - 1 : 0;
+          const int f = (w0 + e / kVec * 64 + lane) * kVec - shift + e % kVec;
+          const key_t k = left != 0 ? key_of(stage[wid][e][lane], f) : 0;
+          const unsigned long long take = __ballot(k > last);
+          if (any ? n + __popcll(take) > 64 : n > 0) {
+            merge_keys(buf[wid], n, best, last, top);
+            n = 0;  // (the same values again: fewer pass the list now)
+          } else {
+            if (!any) break;
             push_keys(buf[wid], n, k, k > last);
-            if (n > 0) merge_keys(buf[wid], n, best, last, top);
-            n = 0;
+            left &= left - 1;
           }
         }
+        wave_sync();
       }
     }
   }
@@ -323,7 +352,7 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   const int64_t slot = (int64_t)m * a.nsplit + sp;
   if (tid == 0) {
     if (a.nsplit == 1) {
-      finish_row(c, m, all.m, (double)all.s, (double)all.u, before);
+      finish_row(c, m, all.m, (double)all.s, (double)all.u, ln_sum((double)all.s), before);
     } else {
       float* o = a.stat + slot * 4;
       o[0] = all.m;
@@ -334,19 +363,18 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   }
   if (top > 0 && lane < top) {
     // the key's place among the block's: its own list's keys before it, and the other lists' larger ones
-    int place = lane;
-    for (int w = 0; w < kNW; ++w) {
-      if (w == wid) continue;
-      int lo = 0, hi = top;
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (lists[w][mid] > best) lo = mid + 1;
-        else hi = mid;
-      }
-      place += lo;
+    int at[kNW] = {};
+#pragma unroll 1
+    for (int step = 1 << (31 - __clz(top)); step > 0; step >>= 1) {  // (the lists' searches side by side)
+#pragma unroll
+      for (int w = 0; w < kNW; ++w)
+        if (at[w] + step <= top && lists[w][at[w] + step - 1] > best) at[w] += step;
     }
+    int place = 0;  // (its own list's larger keys are those of the lanes before it)
+#pragma unroll
+    for (int w = 0; w < kNW; ++w) place += at[w];
     if (best != 0 && place < top) {
-      if (a.nsplit == 1) put_top(c, m, place, best, all.m, (double)all.s);
+      if (a.nsplit == 1) put_top(c, m, place, best, all.m, (double)all.s, ln_sum((double)all.s));
       else a.keys[slot * top + place] = best;
     }
     // a split with fewer values than `top` leaves the rest of its list empty
@@ -358,33 +386,40 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
 // Block per row: joins its splits.
 __global__ __launch_bounds__(kT) void score_join_kernel(const ScoreArgs a) {
   const ScoreCall& c = a.c;
-  extern __shared__ key_t cand[];
-  __shared__ key_t heads[kMaxSplit];
+  __shared__ key_t cand[kMaxCand];
+  __shared__ key_t heads[kLevels * kMaxSplit];
+  __shared__ key_t floors[kLevels];
   __shared__ float sm[kT];
   __shared__ double sS[kNW], sU[kNW];
   __shared__ int sn[kNW];
-  __shared__ key_t floor_key;
   __shared__ int ncand;
   const int m = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, ns = a.nsplit, top = c.top;
   const float* stat = a.stat + (int64_t)m * ns * 4;
   const bool in = tid < ns;
+  // (the lists' first keys are asked for with everything else)
+  const key_t* ks = a.keys + (int64_t)m * ns * top;
+  constexpr int kFirst = 8;
+  key_t kf[kFirst];
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i) kf[i] = tid + i * kT < ns * top ? ks[tid + i * kT] : 0;
   const float mi = in ? stat[tid * 4] : -INFINITY, si = in ? stat[tid * 4 + 1] : 0.f, ui = in ? stat[tid * 4 + 2] : 0.f;
   int n = in ? a.cnt[(int64_t)m * ns + tid] : 0;
   float mx = mi;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o, 64));
   if (lane == 0) sm[wid] = mx;
-  if (top > 0) heads[tid] = in ? a.keys[((int64_t)m * ns + tid) * top] : 0;
-  if (tid == 0) {
-    ncand = 0;
-    floor_key = 0;
-  }
+  // level i: the 2^i-th key of every split
+  const int levels = top > 0 ? 32 - __clz(top) : 0;
+  const int lg = ns <= 64 ? 6 : 8, sp = tid & ((1 << lg) - 1);  // (a wave per level, or the block)
+  for (int i = tid >> lg; i < levels; i += kT >> lg) heads[i << lg | sp] = sp < ns ? ks[sp * top + (1 << i) - 1] : 0;
+  if (tid < kLevels) floors[tid] = 0;
+  if (tid == 0) ncand = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kNW; ++w) mx = fmaxf(mx, sm[w]);
-  const double r = mx == -INFINITY ? 0.0 : (double)mx;
-  const double d = fmax((double)mi - r, -1e4), e = exp(d);
-  double S = (double)si * e, U = ((double)ui + d * (double)si) * e;
+  const float r = mx == -INFINITY ? 0.f : mx;
+  const float d = fmaxf(mi - r, -1e4f), e = exp_d(d);
+  double S = (double)si * (double)e, U = ((double)ui + (double)d * (double)si) * (double)e;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     S += __shfl_xor(S, o, 64);
@@ -396,22 +431,34 @@ __global__ __launch_bounds__(kT) void score_join_kernel(const ScoreArgs a) {
     sU[wid] = U;
     sn[wid] = n;
   }
-  if (top > 0) {
-    // `top` of the splits' first keys are at least as large as the top-th of them: nothing below it counts
-    const key_t h = heads[tid];
+  // If r splits have 2^i keys at or above k, and 2^i r >= top, nothing below k counts; the largest such k of all
+  // levels leaves few: of the 2^i-th keys at most ceil(top / 2^i) pass, each with at most 2^i keys of its list
+  // down to the next level's, so kMaxCand in all, wherever in the row the largest values lie.
+  for (int i = tid >> lg; i < levels; i += kT >> lg) {
+    const key_t* row = heads + (i << lg);
+    const key_t h = row[sp];
     int before = 0;
-    for (int s = 0; s < ns; ++s) before += heads[s] > h ? 1 : 0;
-    if (in && h != 0 && before == top - 1) floor_key = h;
+#pragma unroll 8
+    for (int s = 0; s < 64; ++s) before += row[s] > h ? 1 : 0;
+    if (lg > 6) {
+      for (int s = 64; s < ns; ++s) before += row[s] > h ? 1 : 0;
+    }
+    if (h != 0 && before == (top - 1) >> i) floors[i] = h;
   }
   __syncthreads();
   S = (sS[0] + sS[1]) + (sS[2] + sS[3]);
   U = (sU[0] + sU[1]) + (sU[2] + sU[3]);
   n = (sn[0] + sn[1]) + (sn[2] + sn[3]);
-  if (tid == 0) finish_row(c, m, mx, S, U, n);
+  const double l = ln_sum(S);
+  if (tid == 0) finish_row(c, m, mx, S, U, l, n);
   if (top == 0) return;
-  const key_t fl = floor_key;
-  const key_t* ks = a.keys + (int64_t)m * ns * top;
-  for (int q = tid; q < ns * top; q += kT) {
+  key_t fl = 0;
+#pragma unroll
+  for (int i = 0; i < kLevels; ++i) fl = floors[i] > fl ? floors[i] : fl;
+#pragma unroll
+  for (int i = 0; i < kFirst; ++i)
+    if (kf[i] != 0 && kf[i] >= fl) cand[atomicAdd(&ncand, 1)] = kf[i];
+  for (int q = tid + kFirst * kT; q < ns * top; q += kT) {
     const key_t k = ks[q];
     if (k != 0 && k >= fl) cand[atomicAdd(&ncand, 1)] = k;
   }
@@ -421,7 +468,7 @@ __global__ __launch_bounds__(kT) void score_join_kernel(const ScoreArgs a) {
     const key_t k = cand[q];
     int place = 0;
     for (int s = 0; s < nc; ++s) place += cand[s] > k ? 1 : 0;
-    if (place < top) put_top(c, m, place, k, mx, S);
+    if (place < top) put_top(c, m, place, k, mx, S, l);
   }
 }
 
@@ -470,10 +517,7 @@ int token_logprobs_launch(const ScoreCall& c, hipStream_t st) {
   else hipLaunchKernelGGL(score_kernel<Q35_BF16>, grid, dim3(kT), 0, st, a);
   Q35_HIP_TRY(hipGetLastError());
   if (L.nsplit > 1) {
-    // keys that can reach the list: fewer than `top` splits give all of theirs, else at most `top`
-    // splits have a first key at or above the floor
-    const size_t nc = (size_t)std::min(L.nsplit, c.top) * c.top;
-    hipLaunchKernelGGL(score_join_kernel, dim3(c.M), dim3(kT), nc * sizeof(key_t), st, a);
+    hipLaunchKernelGGL(score_join_kernel, dim3(c.M), dim3(kT), 0, st, a);
     Q35_HIP_TRY(hipGetLastError());
   }
   return Q35_OK;

@@ -117,6 +117,28 @@ def test_ascending_and_descending_rows():
     check(x, targets_of(1, 2, V), 64)
 
 
+@pytest.mark.parametrize("top", [1, 2, 20, 33, 63, 64])
+def test_largest_values_anywhere(top):
+    """The highest alternatives in one part of a long row, in a few, one in each, spread thinner and thinner; among
+    them NaN, and rows of few different values."""
+    V = 248320
+    g = np.random.default_rng(top)
+    x = g.standard_normal((8, V)).astype(np.float32)
+    x[0, 100000:100064] += 50                    # one part
+    x[1, np.arange(64) * 3881] += 50             # everywhere
+    x[2, 5000:5040] += 50                        # two parts
+    x[2, 240000:240030] += 49
+    for i in range(6):                           # 32 here, 16 there, ..
+        x[3, 20000 * i:20000 * i + (32 >> i)] += 60 - i
+    x[4] = np.sort(x[4])
+    x[5] = np.sort(x[5])[::-1]
+    x[6] = np.round(x[6])
+    x[7, g.permutation(V)[:V // 2]] = np.nan
+    for rows in (x, x[:1], x[4:5], x[7:]):
+        t = torch.from_numpy(np.full(len(rows), 100003, np.int32)).cuda()
+        check(torch.from_numpy(np.ascontiguousarray(rows)).cuda(), t, top)
+
+
 def test_masked_rows():
     """-inf, the type's lowest value, a single open token, rows with nothing open."""
     inf = float("inf")
