@@ -105,7 +105,7 @@ Q35_DEV int64_t block_u0(const PlanHead& h, int g) { return h.q * g + min(g, h.r
 Q35_DEV int unit_block(const PlanHead& h, int64_t u) {
   const int64_t big = h.r * (h.q + 1);  // the first r blocks take q + 1 units
   const int64_t x = u < big ? u : u - h.r, y = u < big ? h.q + 1 : h.q;
-  int64_t g = (int64_t)((double)x / (double)y);
+  int64_t g = (int64_t)((float)x * __builtin_amdgcn_rcpf((float)y));  // (at most 512: off by one at most)
   if (g * y > x) --g;
   else if ((g + 1) * y <= x) ++g;
   return (int)g;
@@ -1105,22 +1105,18 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
   const int64_t t = item / a.nh;
   const int h = (int)(item % a.nh);
   if (t >= a.T) return;
+  // (asked for together: the record, the plan's heads and the gate, then the statistics and the first parts)
   const int4 c = A.cut[t * a.nh + h];
+  const PlanHead head[2] = {A.head[0], A.head[1]};
   if (c.x == 0) return;  // (kJW > 1: the block's waves share their item, and leave together)
+  const f4 gv = *(const f4*)(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + 4 * lane);
   const int kind = c.y < 0 ? 1 : 0, r = kind ? -1 - c.y : c.y, g0 = (c.x - 1) >> 1;
-  const int np = unit_block(A.head[kind], (int64_t)c.w << 32 | (uint32_t)c.z) - g0 + 1;
+  const int np = unit_block(kind ? head[1] : head[0], (int64_t)c.w << 32 | (uint32_t)c.z) - g0 + 1;
   auto slot = [&](int q) { return (int64_t)(q == 0 ? c.x - 1 : 2 * (g0 + q)) * A.part_rows[kind] + r; };
   const float* ml = A.part_ml[kind];
-  const f4 gv = *(const f4*)(a.qg + t * a.ld_qg + (int64_t)h * 2 * kHd + kHd + 4 * lane);
-  float M = -INFINITY;
-  for (int q = lane; q < np; q += 64) M = fmaxf(M, ml[2 * slot(q)]);
-#pragma unroll
-  for (int e = 32; e > 0; e >>= 1) M = fmaxf(M, __shfl_xor(M, e, 64));
-  float L = 0.f;
-  f4 y = {0.f, 0.f, 0.f, 0.f};
-  for (int q0 = jw; q0 < np; q0 += 8 * kJW) {
-    f4 v[8];
-    float w[8], lw[8];
+  f4 v[8];
+  float w[8], lw[8];
+  auto load = [&](int q0) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int64_t o = slot(min(q0 + e * kJW, np - 1));
@@ -1128,6 +1124,16 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
       w[e] = ml[2 * o];
       lw[e] = ml[2 * o + 1];
     }
+  };
+  load(jw);
+  float M = -INFINITY;
+  for (int q = lane; q < np; q += 64) M = fmaxf(M, ml[2 * slot(q)]);
+#pragma unroll
+  for (int e = 32; e > 0; e >>= 1) M = fmaxf(M, __shfl_xor(M, e, 64));
+  float L = 0.f;
+  f4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int q0 = jw; q0 < np; q0 += 8 * kJW) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       // (a part none of whose tokens the row sees has the maximum -inf and zeros)
@@ -1135,6 +1141,7 @@ __global__ __launch_bounds__(kT) void paged_join_kernel(const AttnArgs A) {
       L += lw[e] * f;
       y += v[e] * f;
     }
+    if (q0 + 8 * kJW < np) load(q0 + 8 * kJW);
   }
   if constexpr (kJW > 1) {
     *(f4*)&ys[wid][4 * lane] = y;
