@@ -390,7 +390,7 @@ int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const i
  * layer.  New pages are those that table_out's kept entries leave unnamed, the lowest first, dealt to
  * the rows in order; entries behind a row's pages are -1.  len_out[j] is the parent's length, refs
  * [n_pages] the number of rows of table_out that name each page.  Pages that no row names any more may
- * be overwritten, the old table is otherwise as it was: table_out must be another buffer, and `table`
+ * be overwritten, the old table is otherwise as it was: no output overlaps an input, and `table`
  * must cover every sequence of the pool that is to live on.  A parent outside [-1, B), or one
  * whose length is negative or more than its row can hold, counts as -1, a kept page outside the pool
  * becomes -1 and a row is cut at ld_table entries (all Q35_STATUS_ARG); where no page is left the entry
@@ -401,7 +401,7 @@ int q35_pages_fork(q35_pages pool, const int32_t* table, int32_t ld_table, const
 
 /* Moves the pages that `table` [B][ld_table] names to the pool's front, in every layer: with n of them,
  * the i-th lowest named page >= n goes to the i-th lowest unnamed page < n, and the others stay.
- * table_out (another buffer) is the table afterwards, refs [n_pages] its counts, *used = n: pages from n
+ * table_out (no output overlaps the input) is the table afterwards, refs [n_pages] its counts, *used = n: pages from n
  * on are free.  An entry outside [-1, n_pages) becomes -1 (Q35_STATUS_ARG).  ws:
  * q35_pages_compact_ws_bytes(n_pages) bytes of scratch.  n_pages <= 262144; at most 2^26 entries. */
 size_t q35_pages_compact_ws_bytes(int32_t n_pages);

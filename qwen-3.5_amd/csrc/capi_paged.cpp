@@ -139,6 +139,8 @@ int q35_pages_fork(q35_pages pool, const int32_t* table, int32_t ld_table, const
     if ((int64_t)B_out * ld_table > kPageMaxEntries) return fail(Q35_E_SHAPE, "pages_fork: at most 2^26 entries");
     if (overlap(table, B * row, table_out, B_out * row)) return fail(Q35_E_ARG, "pages_fork: table_out must be another buffer");
     if (overlap(len, B * sizeof(int32_t), len_out, B_out * sizeof(int32_t))) return fail(Q35_E_ARG, "pages_fork: len_out must be another buffer");
+    const size_t n = B_out * sizeof(int32_t);
+    if (overlap(parent, n, len_out, n) || (grow && overlap(grow, n, len_out, n))) return fail(Q35_E_ARG, "pages_fork: len_out must be another buffer");
     ForkCall c;
     c.P = pool;
     c.table = table; c.len = len; c.parent = parent; c.grow = grow;

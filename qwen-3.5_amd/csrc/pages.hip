@@ -7,6 +7,8 @@
 // the whole chip; a page of one layer is one contiguous run.
 #include "pages.h"
 
+#include <algorithm>
+
 namespace q35 {
 
 namespace {
@@ -16,8 +18,9 @@ constexpr int kUnit = 16384;    // bytes a block copies at a time: 4 x 16 bytes 
 constexpr int kPT = 1024;       // threads of a bookkeeping block
 constexpr int kPW = kPT / 64;
 
-Q35_DEV void copy_unit(char* dst, const char* src) {
-  const int o = threadIdx.x * 16;
+// by kCT threads, thread t of them
+Q35_DEV void copy_unit(char* dst, const char* src, int t) {
+  const int o = t * 16;
   uint4 v[kUnit / (16 * kCT)];
 #pragma unroll
   for (int i = 0; i < kUnit / (16 * kCT); ++i) v[i] = ldg16_nt(src + o + i * 16 * kCT);
@@ -61,7 +64,7 @@ __global__ __launch_bounds__(kCT) void pages_copy_kernel(const CopyArgs a) {
     return;
   }
   const int64_t o = (int64_t)u * kUnit;
-  copy_unit(a.dst + layer * a.dst_layer + d * a.page + o, a.src + layer * a.src_layer + s * a.page + o);
+  copy_unit(a.dst + layer * a.dst_layer + d * a.page + o, a.src + layer * a.src_layer + s * a.page + o, threadIdx.x);
 }
 
 // ok[i] for many pairs: bitmaps of the pages that are a source, a destination, a destination twice.
@@ -146,14 +149,30 @@ Q35_DEV int fork_parent(const ForkCall& c, int j, int* n, bool* bad) {
   return p;
 }
 
+// The first `tail` tokens of page src to page dst, in one (layer, plane and head), by a block of nt threads; pages
+// outside the pool are left alone
+Q35_DEV void copy_tail(const ForkCall& c, int part, int src, int dst, int tail, int nt) {
+  if (src == dst || (uint32_t)src >= (uint32_t)c.P.n_pages || (uint32_t)dst >= (uint32_t)c.P.n_pages) return;
+  const int rb = c.P.head_dim * (c.P.dtype == Q35_F32 ? 4 : 2), planes = 2 * c.P.kv_heads;
+  const int64_t head = (int64_t)c.P.page * rb, pb = head * planes;
+  const int layer = part / planes, ph = part - layer * planes;
+  char* base = static_cast<char*>(c.P.data) + (int64_t)layer * c.P.n_pages * pb + ph * head;
+  const char* f = base + src * pb;
+  char* t = base + dst * pb;
+  for (int o = threadIdx.x * 16; o < tail * rb; o += nt * 16) {
+    const uint4 v = ldg16(f + o);
+    *reinterpret_cast<uint4*>(t + o) = v;
+  }
+}
+
 // LDS of the bookkeeping, in ints
 struct ForkLds {
-  int words, first, len, par, base, refs, total;
+  int words, first, len, par, base, refs, fresh, total;
 };
 // Counts of up to this many pages are kept in LDS (64 KB); a shared prefix's counts, added to from every
 // row, otherwise wait for each other in the cache (that case: 15.8 us, 10.5 so).
 constexpr int kLdsRefs = 16384;
-__host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo) {
+__host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo, bool one) {
   ForkLds L;
   L.words = (n_pages + 31) / 32;
   L.first = 2 * L.words;      // [words] pages that a kept entry names, [words] pages in use before the word
@@ -161,20 +180,25 @@ __host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo) {
   L.par = L.len + Bo;         // row -> its length
   L.base = L.par + Bo;        // row -> its parent
   L.refs = L.base + Bo + 1;   // row -> new pages before it
-  L.total = L.refs + (n_pages <= kLdsRefs ? n_pages : 0);
+  L.fresh = L.refs + (n_pages <= kLdsRefs ? n_pages : 0);  // row -> its first new page, if the launch copies too
+  L.total = L.fresh + (one ? Bo : 0);
   return L;
 }
 
 // Every step spreads its entries over all threads (a wave per row waited for its row's loads in turn: 35
 // instead of 17 us for 200 rows of 36 entries).
+// kOne: any number of blocks, which all do the bookkeeping, each for itself; the first writes it down, and then each
+// copies its share of the last pages' tokens.  That saves a launch, and a wait for it.
+template <bool kOne>
 __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
   extern __shared__ int lds[];
   __shared__ int sh[kPW];
   const int tid = threadIdx.x, np = c.P.n_pages, page = c.P.page, shift = __ffs(page) - 1;  // (a power of two)
-  const ForkLds L = fork_lds(np, c.B, c.Bo);
+  const ForkLds L = fork_lds(np, c.B, c.Bo, kOne);
   const int words = L.words;
+  const bool lead = !kOne || blockIdx.x == 0;
   uint32_t* bits = reinterpret_cast<uint32_t*>(lds);
-  int *before = lds + words, *first = lds + L.first, *len = lds + L.len, *par = lds + L.par, *base = lds + L.base;
+  int *before = lds + words, *first = lds + L.first, *len = lds + L.len, *par = lds + L.par, *base = lds + L.base, *fresh = lds + L.fresh;
   bool bad = false;
   for (int e = tid; e < words; e += kPT) bits[e] = 0;
   int* refs = lds + L.refs;
@@ -187,7 +211,7 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
     bool b;
     const int p = fork_parent(c, j, &n, &b);
     if (p >= 0) atomicMin(&first[p], j);
-    c.len_out[j] = n;
+    if (lead) c.len_out[j] = n;
     len[j] = n;
     par[j] = p;
     bad |= b;
@@ -244,11 +268,12 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
           bad = true;
         } else {
           atomicOr(&bits[v[i] >> 5], 1u << (v[i] & 31));
+          if (kOne && !lead) continue;
           if (counted) atomicAdd(&refs[v[i]], 1);
           else __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v[i]], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
       }
-      c.table_out[e0 + i * kPT] = v[i];
+      if (lead) c.table_out[e0 + i * kPT] = v[i];
     }
   }
   __syncthreads();
@@ -261,54 +286,71 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
       if (base[m] <= r) lo = m;
       else hi = m;
     }
-    c.table_out[(int64_t)lo * c.ld + kept_of(lo) + r - base[lo]] = page_id;
+    if (lead) c.table_out[(int64_t)lo * c.ld + kept_of(lo) + r - base[lo]] = page_id;
+    if (kOne && r == base[lo]) fresh[lo] = page_id;
   };
   for (int p = tid; p < np; p += kPT) {
     const uint32_t w = bits[p >> 5], below = (1u << (p & 31)) - 1u;
     const int r = p - (before[p >> 5] + __popc(w & below));
-    const bool fresh = !((w >> (p & 31)) & 1u) && r < run;
-    if (fresh) place(r, p);
-    if (counted) c.refs[p] = fresh ? 1 : refs[p];
-    else if (fresh) c.refs[p] = 1;
+    const bool dealt = !((w >> (p & 31)) & 1u) && r < run;
+    if (dealt) place(r, p);
+    if (counted) {
+      if (lead) c.refs[p] = dealt ? 1 : refs[p];
+    } else if (dealt) {
+      c.refs[p] = 1;
+    }
   }
   for (int r = np - used + tid; r < run; r += kPT) place(r, -1);
-  if (bad) raise_status(c.status, Q35_STATUS_ARG);
-  if (tid == 0 && run > np - used) raise_status(c.status, Q35_STATUS_FULL);
+  if (bad && lead) raise_status(c.status, Q35_STATUS_ARG);
+  if (tid == 0 && lead && run > np - used) raise_status(c.status, Q35_STATUS_FULL);
+  if constexpr (kOne) {
+    __syncthreads();
+    const int planes = 2 * c.P.kv_heads, parts = c.P.n_layers * planes;
+    for (int i = blockIdx.x; i < c.Bo * parts; i += gridDim.x) {
+      const int j = i / parts, p = par[j], n = len[j];
+      // (a row that keeps its last page has no copy: its first new page, if any, is behind its tokens)
+      if (p < 0 || (n & (page - 1)) == 0 || first[p] == j) continue;
+      copy_tail(c, i - j * parts, c.table[(int64_t)p * c.ld + (n >> shift)], fresh[j], n & (page - 1), kPT);
+    }
+  }
 }
 
 // The tokens of last pages that were not kept: blocks (row j, layer, plane and head).
 __global__ __launch_bounds__(kCT) void pages_fork_copy_kernel(const ForkCall c) {
-  const int j = blockIdx.x, layer = blockIdx.y, ph = blockIdx.z;
+  const int j = blockIdx.x;
   int n;
   bool b;
   const int p = fork_parent(c, j, &n, &b);
   const int tail = n % c.P.page;
   if (p < 0 || tail == 0) return;
   const int at = n / c.P.page;
-  const int src = c.table[(int64_t)p * c.ld + at], dst = c.table_out[(int64_t)j * c.ld + at];
-  if (src == dst || (uint32_t)src >= (uint32_t)c.P.n_pages || (uint32_t)dst >= (uint32_t)c.P.n_pages) return;
-  const int rb = c.P.head_dim * (c.P.dtype == Q35_F32 ? 4 : 2);
-  const int64_t head = (int64_t)c.P.page * rb, pb = head * 2 * c.P.kv_heads;
-  char* base = static_cast<char*>(c.P.data) + (int64_t)layer * c.P.n_pages * pb + ph * head;
-  const char* f = base + src * pb;
-  char* t = base + dst * pb;
-  for (int o = threadIdx.x * 16; o < tail * rb; o += kCT * 16) {
-    const uint4 v = ldg16(f + o);
-    *reinterpret_cast<uint4*>(t + o) = v;
-  }
+  copy_tail(c, blockIdx.y * gridDim.z + blockIdx.z, c.table[(int64_t)p * c.ld + at], c.table_out[(int64_t)j * c.ld + at], tail, kCT);
 }
 
 // ---- compaction
-__global__ __launch_bounds__(kPT) void pages_compact_kernel(const CompactCall c) {
-  extern __shared__ uint32_t bits[];  // pages in use, then the number of them before each word
+// Unit e of (move, layer, part of a page of pb bytes) by kCT threads
+Q35_DEV void copy_move(const CompactCall& c, const int32_t* holes, const int32_t* movers, int64_t e, int64_t pb, int units, int t) {
+  const int u = (int)(e % units), layer = (int)(e / units % c.P.n_layers);
+  const int m = (int)(e / units / c.P.n_layers);
+  char* base = static_cast<char*>(c.P.data) + (int64_t)layer * c.P.n_pages * pb + (int64_t)u * kUnit;
+  copy_unit(base + holes[m] * pb, base + movers[m] * pb, t);
+}
+// kOne: as pages_fork_kernel's; the lists of moves stay in LDS.
+template <bool kOne>
+__global__ __launch_bounds__(kPT) void pages_compact_kernel(const CompactCall c, int64_t pb, int units) {
+  extern __shared__ uint32_t bits[];  // pages in use, then the number of them before each word, then the moves
   __shared__ int sh[kPW];
   const int tid = threadIdx.x;
   const int np = c.P.n_pages, words = (np + 31) / 32;
   int* before = reinterpret_cast<int*>(bits + words);
+  int32_t* holes = kOne ? before + words : c.moves;  // at most half of the pages move
+  int32_t* movers = holes + (kOne ? np / 2 : np);
   const int64_t ne = (int64_t)c.B * c.ld;
+  const bool lead = !kOne || blockIdx.x == 0;
   bool bad = false;
   for (int e = tid; e < words; e += kPT) bits[e] = 0;
-  for (int e = tid; e < np; e += kPT) c.refs[e] = 0;
+  if (lead)
+    for (int e = tid; e < np; e += kPT) c.refs[e] = 0;
   __syncthreads();
   for (int64_t e = tid; e < ne; e += kPT) {
     const int v = c.table[e];
@@ -323,37 +365,47 @@ __global__ __launch_bounds__(kPT) void pages_compact_kernel(const CompactCall c)
   for (int p = tid; p < np; p += kPT) {
     const bool live = (bits[p >> 5] >> (p & 31)) & 1u;
     const int k = rank(p);
-    if (p < n && !live) c.moves[p - k] = p;
-    if (p >= n && live) c.moves[np + k - low] = p;
+    if (p < n && !live) holes[p - k] = p;
+    if (p >= n && live) movers[k - low] = p;
   }
-  if (tid == 0) *c.used = n;
+  if (tid == 0 && lead) *c.used = n;
   __syncthreads();
-  for (int64_t e = tid; e < ne; e += kPT) {
-    int v = c.table[e];
-    if ((uint32_t)v >= (uint32_t)np) v = -1;
-    else {
-      if (v >= n) v = c.moves[rank(v) - low];
-      __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (lead) {
+    for (int64_t e = tid; e < ne; e += kPT) {
+      int v = c.table[e];
+      if ((uint32_t)v >= (uint32_t)np) v = -1;
+      else {
+        if (v >= n) v = holes[rank(v) - low];
+        __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      c.table_out[e] = v;
     }
-    c.table_out[e] = v;
+    if (bad) raise_status(c.status, Q35_STATUS_ARG);
   }
-  // the copying launch reads the number of moves behind the lists
-  if (tid == 0) c.moves[2 * (int64_t)np] = n - low;
-  if (bad) raise_status(c.status, Q35_STATUS_ARG);
+  if constexpr (kOne) {
+    const int64_t all = (int64_t)(n - low) * c.P.n_layers * units;
+    constexpr int kG = kPT / kCT;
+    for (int64_t e = (int64_t)blockIdx.x * kG + tid / kCT; e < all; e += (int64_t)gridDim.x * kG)
+      copy_move(c, holes, movers, e, pb, units, tid % kCT);
+  } else {
+    // the copying launch reads the number of moves behind the lists
+    if (tid == 0) c.moves[2 * (int64_t)np] = n - low;
+  }
 }
 
 // Any number of blocks: units of (move, layer, part of the page) dealt round.
 __global__ __launch_bounds__(kCT) void pages_compact_copy_kernel(const CompactCall c, int64_t pb, int units) {
   const int np = c.P.n_pages;
   const int64_t all = (int64_t)c.moves[2 * (int64_t)np] * c.P.n_layers * units;
-  char* base = static_cast<char*>(c.P.data);
-  for (int64_t e = blockIdx.x; e < all; e += gridDim.x) {
-    const int u = (int)(e % units), layer = (int)(e / units % c.P.n_layers);
-    const int m = (int)(e / units / c.P.n_layers);
-    const int64_t off = (int64_t)layer * np * pb + (int64_t)u * kUnit;
-    copy_unit(base + off + c.moves[m] * pb, base + off + c.moves[np + m] * pb);
-  }
+  for (int64_t e = blockIdx.x; e < all; e += gridDim.x) copy_move(c, c.moves, c.moves + np, e, pb, units, threadIdx.x);
 }
+
+// One launch does everything (kOne) while the table is small, since every block reads it, and the pool's counts or
+// moves fit LDS: 8 beams 8.6 -> 7.7 us in a graph, 15.5 -> 12.6 called alone; 20 sequences compacted 22.0 -> 20.3,
+// 40 of 4000 tokens 307 -> 291.  A fork must have few copies besides: blocks of 1024 threads take one at a time (64
+// rows of 24 copies each 12.7 us as two launches, 13.0 as one; 200 rows 28 and 36).
+constexpr int kOneEntries = 16384;
+constexpr int kOneCopies = 4;  // per CU
 
 }  // namespace
 
@@ -401,9 +453,17 @@ int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t*
 }
 
 int pages_fork_launch(const ForkCall& c, hipStream_t st) {
-  const size_t lds = (size_t)fork_lds(c.P.n_pages, c.B, c.Bo).total * 4;
-  allow_lds<pages_fork_kernel>(lds);
-  hipLaunchKernelGGL(pages_fork_kernel, dim3(1), dim3(kPT), lds, st, c);
+  const int64_t parts = (int64_t)c.Bo * c.P.n_layers * 2 * c.P.kv_heads;
+  const bool one = c.P.n_pages <= kLdsRefs && c.Bo * c.ld <= kOneEntries && parts <= kOneCopies * device_cus();
+  const size_t lds = (size_t)fork_lds(c.P.n_pages, c.B, c.Bo, one).total * 4;
+  if (one) {
+    allow_lds<pages_fork_kernel<true>>(lds);
+    hipLaunchKernelGGL(pages_fork_kernel<true>, dim3((uint32_t)std::min<int64_t>(parts, device_cus())), dim3(kPT), lds, st, c);
+    Q35_HIP_TRY(hipGetLastError());
+    return Q35_OK;
+  }
+  allow_lds<pages_fork_kernel<false>>(lds);
+  hipLaunchKernelGGL(pages_fork_kernel<false>, dim3(1), dim3(kPT), lds, st, c);
   Q35_HIP_TRY(hipGetLastError());
   hipLaunchKernelGGL(pages_fork_copy_kernel, dim3(c.Bo, c.P.n_layers, 2 * c.P.kv_heads), dim3(kCT), 0, st, c);
   Q35_HIP_TRY(hipGetLastError());
@@ -412,13 +472,23 @@ int pages_fork_launch(const ForkCall& c, hipStream_t st) {
 
 int pages_compact_launch(const CompactCall& c, hipStream_t st) {
   const int words = (c.P.n_pages + 31) / 32;
-  allow_lds<pages_compact_kernel>((size_t)words * 8);
-  hipLaunchKernelGGL(pages_compact_kernel, dim3(1), dim3(kPT), (size_t)words * 8, st, c);
-  Q35_HIP_TRY(hipGetLastError());
   const int64_t pb = (int64_t)page_bytes(c.P);
   const int units = (int)(pb / kUnit);
   // at most half of the pages move
   const int64_t most = (int64_t)(c.P.n_pages / 2) * c.P.n_layers * units;
+  const int64_t ne = (int64_t)c.B * c.ld;
+  constexpr int kG = kPT / kCT;
+  if (c.P.n_pages <= kLdsRefs && ne <= kOneEntries) {
+    const size_t lds = (size_t)words * 8 + (size_t)(c.P.n_pages / 2) * 8;
+    allow_lds<pages_compact_kernel<true>>(lds);
+    const int64_t grid = std::max<int64_t>(1, std::min<int64_t>((most + kG - 1) / kG, device_cus()));
+    hipLaunchKernelGGL(pages_compact_kernel<true>, dim3((uint32_t)grid), dim3(kPT), lds, st, c, pb, units);
+    Q35_HIP_TRY(hipGetLastError());
+    return Q35_OK;
+  }
+  allow_lds<pages_compact_kernel<false>>((size_t)words * 8);
+  hipLaunchKernelGGL(pages_compact_kernel<false>, dim3(1), dim3(kPT), (size_t)words * 8, st, c, pb, units);
+  Q35_HIP_TRY(hipGetLastError());
   const int grid = (int)(most < 1 ? 1 : most > 8 * device_cus() ? 8 * device_cus() : most);
   hipLaunchKernelGGL(pages_compact_copy_kernel, dim3(grid), dim3(kCT), 0, st, c, pb, units);
   Q35_HIP_TRY(hipGetLastError());

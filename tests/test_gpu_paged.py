@@ -586,6 +586,36 @@ def test_pages_compact(dtype, page, layers, kv, seqs, tokens, n_pages):
     assert torch.equal(pool.data, want)
 
 
+@pytest.mark.parametrize("layers,seqs,tokens,n_pages,width", [(3, 40, 300, 900, 450), (1, 30, 400, 17000, 30), (1, 700, 380, 16384, 24)])
+def test_pages_compact_larger(layers, seqs, tokens, n_pages, width):
+    """Tables of more entries, pools of more pages than one launch takes, and the largest pool that it takes."""
+    table, _ = random_tables(8, seqs, tokens, 16, n_pages, width)
+    data = filled(layers, n_pages, 1, 16, "bf16")
+    pool = q35.PagePool(data.clone())
+    c = q35.pages_compact(pool, i32(table), check=True)
+    rows, refs, used, moves = R.compact(table, n_pages)
+    assert c.table.cpu().tolist() == rows and c.refs.cpu().tolist() == refs and int(c.used) == used
+    s, d = (torch.tensor(v, device="cuda") for v in zip(*moves))
+    want = data.clone()
+    want[:, d] = data[:, s]
+    assert torch.equal(pool.data, want)
+
+
+@pytest.mark.parametrize("rows,width", [(42, 10), (43, 10), (20, 820), (4096, 4), (1, 16384)])
+def test_pages_fork_one_launch_or_two(rows, width):
+    """24 copies for each partly filled page: 42 rows are one launch, 43 two; and as many entries, rows as one takes."""
+    layers, kv = (6, 2) if rows < 100 and width < 16384 else (1, 1)
+    table, lens = random_tables(12, 5, 75, 16, 40, width)
+    parents = [i % 4 for i in range(rows)]
+    n_pages = 40 + 2 * rows + (width if rows == 1 else 0)
+    grow = [(width - 6) * 16] if rows == 1 else [i % 20 for i in range(rows)]
+    if rows == 4096:
+        table, lens = [r[:4] for r in table], [min(n, 40) for n in lens]
+        n_pages = 16384
+    data = filled(layers, n_pages, kv, 16, "bf16")
+    check_fork(q35.PagePool(data.clone()), data, table, lens, parents, grow)
+
+
 def test_pages_compact_empty_and_bad_entries():
     data = filled(1, 40, 1, 16, "bf16")
     pool = q35.PagePool(data.clone())

@@ -188,6 +188,7 @@ def test_limits():
     assert ws(ctypes.byref(q35.dims_2b()), (1 << 20) + 1, 4) == 0 and ws(ctypes.byref(q35.dims_2b()), 4, (1 << 20) + 1) == 0
     assert fork(ld=65536, B=1, B_out=1025, out=A + (1 << 28)) == L.Q35_E_SHAPE
     assert fork(len_out=A + 8) == L.Q35_E_ARG  # the last of len's three
+    assert fork(parent=A + 8192) == L.Q35_E_ARG and fork(grow=A + 8192 + 16) == L.Q35_E_ARG  # len_out's place
     assert compact(ld=65536, B=1025, out=A + (1 << 30)) == L.Q35_E_SHAPE
     one = pages(n_layers=1, kv_heads=1, page=256, dtype=L.Q35_F32)  # 32 units of 16 KB per page
     assert L.lib().q35_pages_copy(one, one, A, A, 1 << 19, None, A, 1 << 40, None) == L.Q35_E_SHAPE
