@@ -155,7 +155,7 @@ def pages_fork(pool, table, lens, parents, grow=None, check=False):
         grow = _ints(grow, Bo)
     dev = table.device
     with _on(pool.data, table, lens, parents, grow):
-        res = PagesFork(torch.empty((Bo, n), dtype=torch.int32, device=dev), torch.empty(Bo, dtype=torch.int32, device=dev),
+        res = PagesFork(torch.empty((Bo, n), dtype=torch.int32, device=dev), torch.empty_like(parents),
                         torch.empty(pool.n_pages, dtype=torch.int32, device=dev))
         L.check(L.lib().q35_pages_fork(pool.desc(), table.data_ptr(), n, lens.data_ptr(), B, parents.data_ptr(),
                                        grow.data_ptr() if grow is not None else None, Bo, res.table.data_ptr(),
@@ -172,8 +172,7 @@ def pages_compact(pool, table, check=False):
     table = _ints(table, B, n)
     dev = table.device
     with _on(pool.data, table):
-        res = PagesCompact(torch.empty((B, n), dtype=torch.int32, device=dev),
-                           torch.empty(pool.n_pages, dtype=torch.int32, device=dev),
+        res = PagesCompact(torch.empty_like(table), torch.empty(pool.n_pages, dtype=torch.int32, device=dev),
                            torch.empty(1, dtype=torch.int32, device=dev))
         nbytes = L.lib().q35_pages_compact_ws_bytes(pool.n_pages)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
@@ -201,12 +200,13 @@ def token_logprobs(logits, targets=None, top=0, check=False):
         targets = _ints(targets, *lead)
     with _on(x, targets):
         logprob = rank = ids = lps = status = None
+        entropy = torch.empty(lead, dtype=f32, device=dev)
         if targets is not None:
-            logprob, rank = torch.empty(lead, dtype=f32, device=dev), torch.empty(lead, dtype=i32, device=dev)
+            logprob, rank = torch.empty_like(entropy), torch.empty_like(targets)
         if top:
-            k = (*lead, top)
-            ids, lps = torch.empty(k, dtype=i32, device=dev), torch.empty(k, dtype=f32, device=dev)
-        res = TokenLogprobs(logprob, rank, torch.empty(lead, dtype=f32, device=dev), ids, lps)
+            ids = torch.empty((*lead, top), dtype=i32, device=dev)
+            lps = torch.empty_like(ids, dtype=f32)
+        res = TokenLogprobs(logprob, rank, entropy, ids, lps)
         if M == 0:
             return res
         if check:
@@ -214,7 +214,7 @@ def token_logprobs(logits, targets=None, top=0, check=False):
         nbytes = _score_ws_bytes(M, V, top)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         L.check(L.lib().q35_token_logprobs(x.data_ptr(), dtype, M, V, x.stride(0) if M > 1 else V, _ptr(targets), top, _ptr(logprob),
-                                           _ptr(rank), res.entropy.data_ptr(), _ptr(ids), _ptr(lps), _ptr(status), ws.data_ptr(),
+                                           _ptr(rank), entropy.data_ptr(), _ptr(ids), _ptr(lps), _ptr(status), ws.data_ptr(),
                                            nbytes, _stream()))
         if check:
             L.check(L.lib().q35_status_check(status.data_ptr(), _stream()))
