@@ -29,6 +29,7 @@ constexpr int kT = 256;         // threads per block
 constexpr int kNW = kT / 64;
 constexpr int kPer = 16;        // values of a lane per chunk
 constexpr int kChunk = 64 * kPer;
+constexpr int kFewKeys = 8;    // values of the lanes that are put into the list one by one
 constexpr int kMaxSplit = 256;  // blocks per row: the joining block holds one part's sums per thread
 constexpr int kLevels = 7;      // of the join's floors: 2^6 = kMaxTop
 constexpr int kMaxCand = kLevels * kMaxTop;  // sum over i of 2^i ceil(top / 2^i), 2^i <= top
@@ -135,6 +136,18 @@ Q35_DEV void merge_keys(key_t* buf, int n, key_t& best, key_t& last, int top) {
   last = t > last ? t : last;
 }
 
+// Puts c into the sorted list that the lanes hold, if it is larger than its last wanted key.
+Q35_DEV void insert_key(key_t& best, key_t& last, key_t c, int top) {
+  if (c <= last) return;
+  // a place takes the larger of its key and of the smaller of c and the key before it
+  const key_t up = ((key_t)(uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(best >> 32), 0x138, 0xf, 0xf, false) << 32) |
+                   (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(uint32_t)best, 0x138, 0xf, 0xf, false);
+  const key_t in = up < c ? up : c;
+  best = (int)(threadIdx.x & 63) >= top ? 0 : in > best ? in : best;
+  const key_t t = lane_key(best, top - 1);
+  last = t > last ? t : last;
+}
+
 // What a key must pass, from one value of every lane (-inf or NaN: none): the r-th largest of them, without its
 // lowest 6 bits (the lane's number takes their place, so that no two are equal); that many keys do.  0 if
 // fewer lanes have one.
@@ -188,6 +201,7 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   __shared__ float stage[kNW][kPer][64];
   __shared__ float sm[kNW], ss[kNW], su[kNW];
   __shared__ int sc[kNW];
+  __shared__ key_t block_last;  // the largest of the waves' last wanted keys
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
   const int m = blockIdx.x / a.nsplit, sp = blockIdx.x % a.nsplit;
   constexpr int kEs = DT == Q35_F32 ? 4 : 2, kVec = 16 / kEs;  // values of a 16-byte load
@@ -207,40 +221,47 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   const uint32_t xb = __float_as_uint(xt + 0.0f);
   const float above = __uint_as_float(xt == 0.f ? 1u : (xb & 0x80000000u) ? xb - 1u : xb + 1u);
   Stat st = {-INFINITY, 0.f, 0.f};
-  int cnt = 0;
+  int cnt = 0;  // (the wave's)
   key_t best = 0, last = 0;  // the lane's key of the wave's list; what a value must pass to get in
-  int n = 0;                 // keys in buf
   const int top = c.top;
   const int w_first = (i0 + shift) / kVec, w_end = (i1 + shift + kVec - 1) / kVec;  // words of the split
   constexpr int kWords = kPer / kVec;
   constexpr uint32_t kAll = (1u << kPer) - 1u;
   bool first = true;
+  if (top > 0) {
+    if (tid == 0) block_last = 0;
+    __syncthreads();
+  }
   for (int w0 = w_first + wid * (kChunk / kVec); w0 < w_end; w0 += kNW * (kChunk / kVec)) {
     float x[kPer];
-    int idx0[kWords];
-    uint32_t ok = 0;  // which of the values belong to the split
+    uint32_t ok = kAll;  // which of the values belong to the split
+    const int f0 = w0 * kVec - shift;  // the chunk's first index
+    const bool whole = f0 >= i0 && f0 + kChunk <= i1;  // (uniform in the wave)
+    auto index = [&](int e) { return f0 + (e / kVec * 64 + lane) * kVec + e % kVec; };
+    if (whole) {
+      uint4 v[kWords];
 #pragma unroll
-    for (int g = 0; g < kWords; ++g) {
-      const int w = w0 + g * 64 + lane;
-      const int f = w * kVec - shift;
-      idx0[g] = f;
-      if (f >= i0 && f + kVec <= i1) {
-        const uint4 v = ldg16_nt(base + (int64_t)w * 16);
-        const uint32_t d[4] = {v.x, v.y, v.z, v.w};
+      for (int g = 0; g < kWords; ++g) v[g] = ldg16_nt(base + (int64_t)w0 * 16 + (g * 64 + lane) * 16);
+#pragma unroll
+      for (int g = 0; g < kWords; ++g) {
+        const uint32_t d[4] = {v[g].x, v[g].y, v[g].z, v[g].w};
 #pragma unroll
         for (int j = 0; j < kVec; ++j)
           x[g * kVec + j] = DT == Q35_F32 ? __uint_as_float(d[j & 3]) : half_of<DT>(d[(j >> 1) & 3], j & 1);
-        ok |= ((1u << kVec) - 1u) << (g * kVec);
-      } else {  // (the word holds others' values too)
+      }
+    } else {  // (its words may hold others' values too)
+      ok = 0;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const float v = value<DT>(row, min(max(f + j, i0), i1 - 1));
-          const bool in = f + j >= i0 && f + j < i1;
-          x[g * kVec + j] = in ? v : -INFINITY;
-          ok |= (in ? 1u : 0u) << (g * kVec + j);
-        }
+      for (int e = 0; e < kPer; ++e) {
+        const int f = index(e);
+        const float v = value<DT>(row, min(max(f, i0), i1 - 1));
+        const bool in = f >= i0 && f < i1;
+        x[e] = in ? v : -INFINITY;
+        ok |= (in ? 1u : 0u) << e;
       }
     }
+    // (a wave by itself would find one of its `top` highest values in half of the chunks of a long row)
+    const key_t bl = top > 0 ? __hip_atomic_load(&block_last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) : 0;
     float mx = x[0];
 #pragma unroll
     for (int e = 1; e < kPer; ++e) mx = fmaxf(mx, x[e]);
@@ -259,22 +280,16 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
       }
     }
     if (tgt >= 0) {
-      // a word of values whose indices all lie before the target's counts what is >= it, one behind it what
-      // is >= the next float; the word in which it lies, words with others' values and a NaN go by the keys
-      bool mixed = xt != xt || ok != kAll;
-#pragma unroll
-      for (int g = 0; g < kWords; ++g) mixed |= (uint32_t)(tgt - idx0[g]) < (uint32_t)kVec;
-      if (__ballot(mixed)) {
+      // a chunk before the target's counts what is >= it, one behind it what is >= the next float; the chunk in
+      // which it lies, chunks with others' values and a NaN go by the keys
+      if (xt != xt || !whole || (uint32_t)(tgt - f0) < (uint32_t)kChunk) {
         const key_t kt = key_of(xt, tgt);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) cnt += key_of(x[e], idx0[e / kVec] + e % kVec) > kt && ((ok >> e) & 1u) ? 1 : 0;
+        for (int e = 0; e < kPer; ++e) cnt += __popcll(__ballot(key_of(x[e], index(e)) > kt && ((ok >> e) & 1u)));
       } else {
+        const float from = f0 < tgt ? xt : above;
 #pragma unroll
-        for (int g = 0; g < kWords; ++g) {
-          const float from = idx0[g] < tgt ? xt : above;
-#pragma unroll
-          for (int j = 0; j < kVec; ++j) cnt += x[g * kVec + j] >= from ? 1 : 0;
-        }
+        for (int e = 0; e < kPer; ++e) cnt += __popcll(__ballot(x[e] >= from));
       }
     }
     if (top > 0) {
@@ -293,37 +308,48 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
           last = l2 > last ? l2 : last;
         }
       }
-      if (__ballot(asc(mx) >= (uint32_t)(last >> 32))) {
-        // values at or above the last wanted one (all, while that is nothing or NaN)
-        const float lf = from_asc((uint32_t)(last >> 32));
-        const bool open = (uint32_t)(last >> 32) == 0;
+      const key_t lb = lane_key(bl, 0);
+      if (lb > last) last = lb;
+      // values at or above the last wanted one (all, while that is nothing or NaN; a NaN always: its key decides)
+      const uint32_t la = (uint32_t)(last >> 32);
+      const float lf = la == 0 ? -INFINITY : from_asc(la);
+      if (__ballot(!(mx < lf))) {
         uint32_t left = 0;  // the lane's values to look at
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          left |= (x[e] >= lf || open ? 1u : 0u) << e;
-          stage[wid][e][lane] = x[e];
-        }
+        for (int e = kPer - 1; e >= 0; --e) left = left + left + (x[e] < lf ? 0u : 1u);
         left &= ok;
-        wave_sync();
+        // else a lane's only one is its largest (or NaN beside smaller numbers: too small either way)
+        const bool stages = !whole || __ballot((left & (left - 1)) != 0) != 0;
+        if (stages) {
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) stage[wid][e][lane] = x[e];
+          wave_sync();
+        }
+        const key_t before = last;
         // one of every lane at a time (a loop: written out for each of the 16 values, its code, which every
-        // block fetches, took 0.6 us); joined with the list whenever 64 are full
+        // block fetches, took 0.6 us): a few are put into the list one by one, many are put aside and joined
+        // with it, 64 at the most
+        int n = 0;  // keys in buf
 #pragma unroll 1
         for (;;) {
           const unsigned long long any = __ballot(left != 0);
           const int e = left != 0 ? __ffs(left) - 1 : 0;
-          const int f = (w0 + e / kVec * 64 + lane) * kVec - shift + e % kVec;
-          const key_t k = left != 0 ? key_of(stage[wid][e][lane], f) : 0;
-          const unsigned long long take = __ballot(k > last);
-          if (any ? n + __popcll(take) > 64 : n > 0) {
+          const key_t k = left != 0 ? key_of(stages ? stage[wid][e][lane] : mx, index(e)) : 0;
+          unsigned long long take = __ballot(k > last);
+          if (n == 0 && __popcll(take) <= kFewKeys) {
+            if (!any) break;
+            for (; take; take &= take - 1) insert_key(best, last, lane_key(k, (int)__builtin_ctzll(take)), top);
+            left &= left - 1;
+          } else if (any ? n + __popcll(take) > 64 : n > 0) {
             merge_keys(buf[wid], n, best, last, top);
             n = 0;  // (the same values again: fewer pass the list now)
           } else {
-            if (!any) break;
             push_keys(buf[wid], n, k, k > last);
             left &= left - 1;
           }
         }
         wave_sync();
+        if (last > before && lane == 0) __hip_atomic_fetch_max(&block_last, last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
       }
     }
   }
@@ -332,7 +358,6 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   for (int o = 32; o > 0; o >>= 1) {
     const float om = __shfl_xor(st.m, o, 64), os = __shfl_xor(st.s, o, 64), ou = __shfl_xor(st.u, o, 64);
     stat_join(st, om, os, ou);
-    cnt += __shfl_xor(cnt, o, 64);
   }
   if (lane == 0) {
     sm[wid] = st.m;

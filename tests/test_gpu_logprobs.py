@@ -117,6 +117,19 @@ def test_ascending_and_descending_rows():
     check(x, targets_of(1, 2, V), 64)
 
 
+@pytest.mark.parametrize("V", [1, 2, 5, 63, 70, 1030, 5000])
+def test_rows_of_nan_and_infinities(V):
+    """NaN, -inf, inf, few numbers in every mixture: the order of ids is still told."""
+    g = np.random.default_rng(V)
+    x = g.choice(np.array([np.nan, -np.inf, np.inf, -1.5, 2.0, 0.0, -3e38], np.float32), (24, V))
+    for m in range(7):
+        x[m] = g.choice(np.array([np.nan, -np.inf, np.inf, -1.5, 2.0, 0.0, -3e38], np.float32)[[m, (m + 1) % 7]], V)
+    x[7], x[8], x[9] = np.nan, -np.inf, -3.4e38
+    t = torch.from_numpy(g.integers(0, V, 24).astype(np.int32)).cuda()
+    for top in sorted({1, min(V, 3), min(V, 40), min(V, 64)}):
+        check(torch.from_numpy(x).cuda(), t, top)
+
+
 @pytest.mark.parametrize("top", [1, 2, 20, 33, 63, 64])
 def test_largest_values_anywhere(top):
     """The highest alternatives in one part of a long row, in a few, one in each, spread thinner and thinner; among
