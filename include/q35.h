@@ -377,7 +377,7 @@ int q35_attention_core_paged(const q35_dims* d, q35_pages pool, int32_t layer, c
  * differ in n_pages at most; they may be one pool, else they must not overlap.  A pair with an id
  * outside its pool, a destination that another pair names too, and in one pool a pair with a page that
  * is both a source and a destination are not copied (Q35_STATUS_ARG).  ws:
- * q35_pages_copy_ws_bytes(n) bytes of scratch. */
+ * q35_pages_copy_ws_bytes(n) bytes of scratch (none, and ws may be NULL, up to 256 pairs). */
 size_t q35_pages_copy_ws_bytes(int32_t n);
 int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const int32_t* dst_ids, int32_t n,
                    uint32_t* status, void* ws, size_t ws_bytes, void* stream);

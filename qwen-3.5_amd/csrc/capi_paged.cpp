@@ -102,7 +102,7 @@ int q35_attention_core_paged(const q35_dims* d, q35_pages pool, int32_t layer, c
   });
 }
 
-size_t q35_pages_copy_ws_bytes(int32_t n) { return n < 1 ? 0 : (size_t)n; }
+size_t q35_pages_copy_ws_bytes(int32_t n) { return n <= kPageFewPairs ? 0 : (size_t)n; }
 
 int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const int32_t* dst_ids, int32_t n,
                    uint32_t* status, void* ws, size_t ws_bytes, void* stream) {
@@ -121,7 +121,7 @@ int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const i
     if (n == 0) return Q35_OK;
     if (!src_ids || !dst_ids) return fail(Q35_E_ARG, "pages_copy: null pointer");
     if ((int64_t)n * (int64_t)(pb / 16384) >= kMaxGrid) return fail(Q35_E_SHAPE, "pages_copy: too many pages for one call");
-    if (!ws || ws_bytes < q35_pages_copy_ws_bytes(n)) return fail(Q35_E_WS, "pages_copy: workspace too small");
+    if (n > kPageFewPairs && (!ws || ws_bytes < q35_pages_copy_ws_bytes(n))) return fail(Q35_E_WS, "pages_copy: workspace too small");
     return pages_copy_launch(src, dst, src_ids, dst_ids, n, status, static_cast<uint8_t*>(ws), S(stream));
   });
 }

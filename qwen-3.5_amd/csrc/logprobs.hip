@@ -498,7 +498,8 @@ __global__ __launch_bounds__(kT) void score_join_kernel(const ScoreArgs a) {
 }
 
 constexpr int kBlocks = 4 * 256;
-// Blocks per row: enough to fill the chip when rows are few, of one chunk per wave at least.
+// Blocks per row: enough to fill the chip when rows are few, of one chunk per wave at least (248320 values, up to
+// 1024, 512 or 256 blocks: 64 rows 22, 25, 31 us; 400 rows 72, 77, 96; 2048 blocks: 700 rows 136 us instead of 122).
 int score_split(int M, int V) {
   const int want = (kBlocks + M - 1) / M, most = std::min(kMaxSplit, (V + kNW * kChunk - 1) / (kNW * kChunk));
   return std::max(1, std::min(want, most));

@@ -10,6 +10,7 @@ constexpr int kPageHd = 256;            // head_dim
 constexpr int kPageMaxPages = 1 << 18;  // pages of a pool that fork / compact / copy keep in LDS bitmaps
 constexpr int kPageMaxSeqs = 4096;      // rows of a table in fork
 constexpr int kPageMaxEntries = 1 << 26;  // of a page table in fork / compact (one block goes over them)
+constexpr int kPageFewPairs = 256;      // pairs of a copy that its blocks check themselves
 constexpr int kPageMaxHeads = 1024;     // query heads
 constexpr int kPageMaxRep = 16;         // query heads per kv head
 constexpr int kMaxLds = 150 * 1024;     // dynamic LDS that the kernels here ask for at most

@@ -440,7 +440,7 @@ int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t*
   a.did = did;
   a.status = status;
   a.ok = nullptr;
-  if (n > kCT) {
+  if (n > kPageFewPairs) {
     const size_t lds = ((src.n_pages + 31) / 32 + 2 * (size_t)((dst.n_pages + 31) / 32)) * 4;
     allow_lds<pages_copy_check_kernel>(lds);
     hipLaunchKernelGGL(pages_copy_check_kernel, dim3(1), dim3(kPT), lds, st, a, ok);

@@ -36,11 +36,11 @@ TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprob rank entropy to
 
 def _on(first, *tensors):
     """The tensors' device as the current one (they must share it)."""
-    dev = first.device
-    assert dev.type == "cuda", "tensors must be on the GPU"
+    dev = first.get_device()
+    assert dev >= 0, "tensors must be on the GPU"
     for t in tensors:
-        assert t is None or t.device == dev, "tensors on different devices"
-    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+        assert t is None or t.get_device() == dev, "tensors on different devices"
+    return _HERE if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _ints(t, *shape):
@@ -96,17 +96,20 @@ def attention_core_paged(dims, pool, layer, q_gate, k_new, v_new, seq_start, pos
     as they are in `out`).  check=True synchronises and raises as PagePool.check does."""
     T, B = q_gate.shape[0], pos.shape[0]
     H, KV, hd, rot, f32 = dims.attn_heads, dims.kv_heads, dims.head_dim, dims.rot_dim, torch.float32
-    for x, n in ((q_gate, 2 * H * hd), (k_new, KV * hd), (v_new, KV * hd)):
-        assert x.dtype is f32 and x.shape == (T, n) and x.stride(1) == 1, (tuple(x.shape), x.dtype, x.stride())
-    # (the stride of a single row says nothing)
-    ld_q, ld_k, ld_v = (q_gate.stride(0), k_new.stride(0), v_new.stride(0)) if T > 1 else (2 * H * hd, KV * hd, KV * hd)
+    assert q_gate.dtype is k_new.dtype is v_new.dtype is f32, (q_gate.dtype, k_new.dtype, v_new.dtype)
+    assert q_gate.shape == (T, 2 * H * hd) and k_new.shape == (T, KV * hd) == v_new.shape, \
+        (tuple(q_gate.shape), tuple(k_new.shape), tuple(v_new.shape))
+    (ld_q, cq), (ld_k, ck), (ld_v, cv) = q_gate.stride(), k_new.stride(), v_new.stride()
+    assert cq == ck == cv == 1, "rows must be contiguous"
+    if T <= 1:  # (the stride of a single row says nothing)
+        ld_q, ld_k, ld_v = 2 * H * hd, KV * hd, KV * hd
     assert ld_k == ld_v, "k_new and v_new must have one row stride"
     rows = rope_cos.shape[0]
     assert q_norm.shape == (hd,) == k_norm.shape and rope_cos.shape == (rows, rot) == rope_sin.shape
     for w in (q_norm, k_norm, rope_cos, rope_sin):
         assert w.dtype is f32 and w.is_contiguous(), (w.dtype, w.stride())
     if out is None:
-        out = torch.empty((T, H * hd), dtype=f32, device=q_gate.device)
+        out = torch.empty(T, H * hd, dtype=f32, device=q_gate.device)
     assert out.dtype is f32 and out.shape == (T, H * hd) and out.stride(1) == 1, (tuple(out.shape), out.dtype, out.stride())
     width = table.shape[1]
     seq_start, pos, table = _ints(seq_start, B + 1), _ints(pos, B), _ints(table, B, width)
@@ -134,9 +137,10 @@ def pages_copy(pool, src, dst, to=None, check=False):
     n = src.shape[0]
     src, dst = _ints(src, n), _ints(dst, n)
     with _on(pool.data, to.data, src, dst):
-        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=src.device)
+        # (up to 256 pairs need no scratch)
+        ws = torch.empty(n, dtype=torch.uint8, device=src.device) if n > 256 else None
         L.check(L.lib().q35_pages_copy(pool.desc(), to.desc(), src.data_ptr(), dst.data_ptr(), n, to.status.data_ptr(),
-                                       ws.data_ptr(), ws.numel(), _stream()))
+                                       _ptr(ws), n, _stream()))
     if check:
         to.check()
 
@@ -155,7 +159,7 @@ def pages_fork(pool, table, lens, parents, grow=None, check=False):
         grow = _ints(grow, Bo)
     dev = table.device
     with _on(pool.data, table, lens, parents, grow):
-        res = PagesFork(torch.empty((Bo, n), dtype=torch.int32, device=dev), torch.empty_like(parents),
+        res = PagesFork(torch.empty(Bo, n, dtype=torch.int32, device=dev), torch.empty_like(parents),
                         torch.empty(pool.n_pages, dtype=torch.int32, device=dev))
         L.check(L.lib().q35_pages_fork(pool.desc(), table.data_ptr(), n, lens.data_ptr(), B, parents.data_ptr(),
                                        grow.data_ptr() if grow is not None else None, Bo, res.table.data_ptr(),
@@ -200,11 +204,11 @@ def token_logprobs(logits, targets=None, top=0, check=False):
         targets = _ints(targets, *lead)
     with _on(x, targets):
         logprob = rank = ids = lps = status = None
-        entropy = torch.empty(lead, dtype=f32, device=dev)
+        entropy = torch.empty(*lead, dtype=f32, device=dev) if lead else torch.empty((), dtype=f32, device=dev)
         if targets is not None:
             logprob, rank = torch.empty_like(entropy), torch.empty_like(targets)
         if top:
-            ids = torch.empty((*lead, top), dtype=i32, device=dev)
+            ids = torch.empty(*lead, top, dtype=i32, device=dev)
             lps = torch.empty_like(ids, dtype=f32)
         res = TokenLogprobs(logprob, rank, entropy, ids, lps)
         if M == 0:

@@ -67,7 +67,7 @@ def test_copy_refusals():
     assert copy(n=0) == L.Q35_OK
     assert copy(n=-1) == L.Q35_E_SHAPE
     assert copy(s=None) == L.Q35_E_ARG and copy(d=None) == L.Q35_E_ARG
-    assert copy(ws=None) == L.Q35_E_WS and copy(nb=2) == L.Q35_E_WS
+    assert copy(n=257, ws=None, nb=300) == L.Q35_E_WS and copy(n=257, nb=256) == L.Q35_E_WS
     assert copy(n=1 << 30, nb=1 << 40) == L.Q35_E_SHAPE
     for other in (dict(dtype=L.Q35_F16), dict(n_layers=1), dict(kv_heads=1), dict(page=32)):
         assert copy(dst=pages(data=A + 4 * size, **other)) == L.Q35_E_SHAPE
