@@ -8,6 +8,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <type_traits>
 
 namespace q35 {
 
@@ -481,6 +482,16 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
           for (int w = 0; w < 2 * kW; ++w) vr[4 * hf + j][w] = ldg16_if<kStream>(p + j * kHd + w * (128 / kW));
       }
     };
+    // queries: column n; dims 32 st + 8 g .. (16-bit), 16 st + 4 g .. (f32); each wave lays out a quarter.  They are
+    // asked for first: loads arrive in order, and the operands can be laid out while keys and values are under way
+    // (one token behind 517: 8.6 -> 8.0 us).
+    const int64_t qi = (int64_t)(t.s0 + tok) * a.nh + h;
+    f4 qv[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qv[i] = *(const Q35_GLOBAL f4*)(A.q + qi * kHd + (kWide ? 16 * (4 * wid + i) + 4 * g : 32 * (2 * wid + (i >> 1)) + 8 * g + 4 * (i & 1)));
+    float qm = 0.f;
+    if constexpr (DT == Q35_F16) qm = A.qmax[qi];
     int j0 = k0 * kUnit + wid * kS, pa = 0, pb = 0;
     const int j1 = min(k1 * kUnit, end);
     if (j0 < j1) {
@@ -488,24 +499,21 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
       load_k(j0, pa, pb);
       load_v(j0, pa, pb);
     }
-    // queries: column n; dims 32 st + 8 g .. (16-bit), 16 st + 4 g .. (f32); each wave lays out a quarter
     float qscale = sl2;
     {
-      const int64_t qi = (int64_t)(t.s0 + tok) * a.nh + h;
-      const float* qp = A.q + qi * kHd;
       float fq = 1.f;
       if constexpr (DT == Q35_F16) {  // a power of two per query brings its largest value to 2^14
         float inv;
-        split_scale(A.qmax[qi], fq, inv);
+        split_scale(qm, fq, inv);
         qscale = sl2 * inv;
       }
 #pragma unroll
       for (int i = 0; i < 2 * kW; ++i) {
         const int st = 2 * kW * wid + i;
         if constexpr (kWide) {
-          qs[st * 64 + lane] = *(const Q35_GLOBAL q35_u32x4*)(qp + 16 * st + 4 * g);
+          qs[st * 64 + lane] = __builtin_bit_cast(q35_u32x4, qv[i]);
         } else {
-          const f4 v0 = *(const Q35_GLOBAL f4*)(qp + 32 * st + 8 * g), v1 = *(const Q35_GLOBAL f4*)(qp + 32 * st + 8 * g + 4);
+          const f4 v0 = qv[2 * i], v1 = qv[2 * i + 1];
           const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
           q35_u32x4 qb[3];
 #pragma unroll
@@ -527,10 +535,12 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-#pragma unroll 1
-    for (; j0 < j1; j0 += 4 * kS) {
-      const bool more = j0 + 4 * kS < j1;
-      if (more) pages(j0 + 4 * kS, pa, pb);
+    // A step waits for its keys, then its values, while the next step's are under way: that takes a loop whose every
+    // step loads, and a last step apart (at a load that only some steps make, the compiler waits for all: 33 tokens
+    // over 958 MB 175 us, 171 so; one token behind 517 9.2 and 8.6).
+    auto step = [&](auto more) {
+      constexpr bool kMore = decltype(more)::value;
+      if constexpr (kMore) pages(j0 + 4 * kS, pa, pb);
       f4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       // (two sums in turn, the halves' or even and odd dims': a product does not wait for the one before it)
 #pragma unroll
@@ -549,7 +559,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
           }
         }
       }
-      if (more) load_k(j0 + 4 * kS, pa, pb);
+      if constexpr (kMore) load_k(j0 + 4 * kS, pa, pb);
       asm volatile("" ::: "memory");
       if constexpr (kWide) sc[0] += sc[1];
       float bm = -INFINITY;
@@ -621,9 +631,12 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
           }
         }
       }
-      if (more) load_v(j0 + 4 * kS, pa, pb);
+      if constexpr (kMore) load_v(j0 + 4 * kS, pa, pb);
       asm volatile("" ::: "memory");
-    }
+    };
+#pragma unroll 1
+    for (; j0 + 4 * kS < j1; j0 += 4 * kS) step(std::true_type{});
+    if (j0 < j1) step(std::false_type{});
     __syncthreads();  // (the queries' operands are done with)
     l = add_x32(add_x16(l));
     if (n < rows) {
