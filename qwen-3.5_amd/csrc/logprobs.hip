@@ -192,7 +192,9 @@ Q35_DEV void put_top(const ScoreCall& c, int m, int i, key_t k, float mx, double
   c.top_lp[o] = mx == -INFINITY && S == 0.0 ? -INFINITY : (float)((double)(x - mx) - l);
 }
 
-// Blocks (row, split).
+// Blocks (row, split).  Bound by the stream for many rows (700 rows of 248320 f32 values, top 5: 120 us, 5.8 TB/s; 1500
+// rows 6.2; loads alone 6.7), beside 13 vector instructions per 64 values, half of them the exponential and its
+// sums; by round trips and code that every block fetches for one row (10 us).
 template <int DT>
 __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   const ScoreCall& c = a.c;
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(kT) void score_kernel(const ScoreArgs a) {
   }
 }
 
-// Block per row: joins its splits.
+// Block per row: joins its splits.  6 us (61 splits of 20 keys), round trips.
 __global__ __launch_bounds__(kT) void score_join_kernel(const ScoreArgs a) {
   const ScoreCall& c = a.c;
   __shared__ key_t cand[kMaxCand];

