@@ -328,7 +328,7 @@ size_t q35_attention_prefill_ws_bytes(const q35_dims* d, int32_t T);
  *   when they are appended; head_dim 256).
  * A page table is int32 [B][ld_table]: entry c of row b is the page that holds tokens c*page .. of
  * sequence b, or -1.  A page may stand in several rows (shared contexts); pages that a sequence is
- * about to append to must stand in its row alone, which q35_pages_fork sees to.
+ * about to append to must stand in its row alone, and once, which q35_pages_fork sees to.
  *
  * `status` (optional, NULL: not reported): a zero-initialised device word into which calls OR
  *   Q35_STATUS_ARG   a device-resident index was out of range (a page, a position, a parent, a token

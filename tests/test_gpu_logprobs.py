@@ -117,6 +117,23 @@ def test_ascending_and_descending_rows():
     check(x, targets_of(1, 2, V), 64)
 
 
+def test_one_very_long_row():
+    """20 million values: every split of the row is many chunks; the planted largest ones are told, in order."""
+    V, n = 20_000_003, 64
+    x = -torch.rand((1, V), device="cuda", generator=torch.Generator(device="cuda").manual_seed(5))
+    at = torch.randperm(V, device="cuda", generator=torch.Generator(device="cuda").manual_seed(6))[:n]
+    x[0, at] = torch.arange(n, 0, -1, device="cuda", dtype=torch.float32) * 0.25
+    t = at[40:41].int()
+    r = q35.token_logprobs(x, t, top=n)
+    assert torch.equal(r.top_ids[0].long(), at) and int(r.rank) == 40
+    lse = torch.logsumexp(x[0].double(), 0)
+    p = (x[0].double() - lse).exp()
+    ent = -(p * (x[0].double() - lse)).sum()
+    # the largest value is 16: differences of up to 17 rounded to f32, and the exponentials' own error, as in check()
+    assert abs(float(r.logprob) - float(x[0, at[40]].double() - lse)) <= 2.0 ** -21 + 2.0 ** -23 * 17
+    assert abs(float(r.entropy) - float(ent)) <= 2.0 ** -21 * (2 + float(ent)) + 2.0 ** -23 * float(ent)
+
+
 @pytest.mark.parametrize("V", [1, 2, 5, 63, 70, 1030, 5000])
 def test_rows_of_nan_and_infinities(V):
     """NaN, -inf, inf, few numbers in every mixture: the order of ids is still told."""
