@@ -9,11 +9,12 @@
 // The alternatives: a value and its index make one 64-bit key (the value's bits in ascending order,
 // then the complement of the index), so "larger value, then lower index" is one unsigned comparison
 // and every choice below is exact whatever the order of the work.  A wave keeps its best `top` keys
-// sorted, one per lane; a chunk of values costs one comparison of each lane's maximum with the
-// last wanted key, and only values above it are put aside and joined with the list, up to 64 at a time.  The
-// first chunk would put almost everything aside: the last wanted key starts at the `top`-th of the 64
-// lanes' maxima instead (that many values are at least as large), or, for more than 32, the (top / 2)-th of
-// their second largest values.
+// sorted, one per lane; a chunk of values costs one comparison of each lane's maximum with the last wanted
+// key, and only values above it are looked at: a few are put into the list one by one, many are put aside and
+// joined with it, up to 64 at a time.  The waves of a block tell each other their last wanted keys.  The first
+// chunk would have almost everything looked at: the last wanted key starts at the `top`-th of the 64 lanes'
+// maxima instead (that many values are at least as large), or, for more than 32, the (top / 2)-th of their
+// second largest values.
 // Waves, then the splits of a row (blocks), are joined by ranks: a key's place is the number of larger
 // keys.
 #include "pages.h"
