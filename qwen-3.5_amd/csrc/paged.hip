@@ -352,6 +352,22 @@ Q35_DEV Tile load_tile(const Tile* p) {  // (two 16-byte loads; a copy of the st
   return t;
 }
 
+// The same in every lane: in scalar registers
+Q35_DEV int64_t uniform(int64_t v) {
+  const int lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)hi << 32 | (uint32_t)lo;
+}
+Q35_DEV Tile uniform(Tile t) {
+  t.u0 = uniform(t.u0);
+  t.units = __builtin_amdgcn_readfirstlane(t.units);
+  t.b = __builtin_amdgcn_readfirstlane(t.b);
+  t.i = __builtin_amdgcn_readfirstlane(t.i);
+  t.s0 = __builtin_amdgcn_readfirstlane(t.s0);
+  t.n = __builtin_amdgcn_readfirstlane(t.n);
+  t.p0 = __builtin_amdgcn_readfirstlane(t.p0);
+  return t;
+}
+
 // The block's first tile, the one that holds unit u: every thread looks at some (they are few).  The first
 // ones are asked for before the plan's head has arrived.
 struct Start {
@@ -440,9 +456,9 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   constexpr int kH = kWide ? 1 : 2, kS = 16 * kH;          // keys of a wave's step
   const PagedAttn& a = A.c;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
-  int64_t u = block_u0(H, blockIdx.x);
-  const int64_t u_end = block_u0(H, blockIdx.x + 1);
-  Tile t = load_tile(&sh.t);
+  int64_t u = uniform(block_u0(H, blockIdx.x));
+  const int64_t u_end = uniform(block_u0(H, blockIdx.x + 1));
+  Tile t = uniform(load_tile(&sh.t));
   int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
   q35_u32x4* const qs = reinterpret_cast<q35_u32x4*>(os);  // [part][step][lane]
@@ -697,7 +713,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
       }
     }
     u += k1 - k0;
-    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = load_tile(&A.tiles[0][++x]);
+    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = uniform(load_tile(&A.tiles[0][++x]));
     __syncthreads();
   }
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
@@ -781,7 +797,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int64_t u_begin = block_u0(H, blockIdx.x);
   int64_t u = u_begin;
   const int64_t u_end = block_u0(H, blockIdx.x + 1);
-  Tile t = load_tile(&sh.t);
+  Tile t = uniform(load_tile(&sh.t));
   int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
   bool bad = false;
@@ -1105,7 +1121,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       }
     }
     u += k1 - k0;
-    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = load_tile(&A.tiles[1][++x]);
+    if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = uniform(load_tile(&A.tiles[1][++x]));
     __syncthreads();  // (the buffers are the next segment's)
   }
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
