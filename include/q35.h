@@ -385,9 +385,10 @@ int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const i
 /* The next page table of a set of sequences: row j of table_out [B_out][ld_table] continues sequence
  * parent[j] of table [B][ld_table] (len[b] tokens), or is empty for parent[j] = -1, with pages for grow[j]
  * more tokens (grow NULL: none).  So one call forks (a parent named several times), drops (a
- * parent not named), frees (-1) and reserves.  Full pages are shared; of a partly filled last page the
- * first child keeps the page and every other gets a new one with a copy of its tokens, in every
- * layer.  New pages are those that table_out's kept entries leave unnamed, the lowest first, dealt to
+ * parent not named), frees (-1) and reserves.  Full pages are shared; a partly filled last page stays with
+ * the first row of table_out that continues it, unless a row names it as a full page, and every other row
+ * gets a new one with a copy of its tokens, in every layer: whatever pages the rows of `table` share, a
+ * page with room stands in one row, once.  New pages are those that table_out's kept entries leave unnamed, the lowest first, dealt to
  * the rows in order; entries behind a row's pages are -1.  len_out[j] is the parent's length, refs
  * [n_pages] the number of rows of table_out that name each page.  Pages that no row names any more may
  * be overwritten, the old table is otherwise as it was: no output overlaps an input, and `table`

@@ -167,11 +167,12 @@ Q35_DEV void copy_tail(const ForkCall& c, int part, int src, int dst, int tail, 
 
 // LDS of the bookkeeping, in ints
 struct ForkLds {
-  int words, first, len, par, base, refs, fresh, total;
+  int words, first, len, par, base, tail, refs, fresh, total;
 };
 // Counts of up to this many pages are kept in LDS (64 KB); a shared prefix's counts, added to from every
 // row, otherwise wait for each other in the cache (that case: 15.8 us, 10.5 so).
 constexpr int kLdsRefs = 16384;
+constexpr int kMoved = -2;  // (-1: an entry outside the pool)
 __host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo, bool one) {
   ForkLds L;
   L.words = (n_pages + 31) / 32;
@@ -179,7 +180,8 @@ __host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo, bool one
   L.len = L.first + B;        // parent -> its first child
   L.par = L.len + Bo;         // row -> its length
   L.base = L.par + Bo;        // row -> its parent
-  L.refs = L.base + Bo + 1;   // row -> new pages before it
+  L.tail = L.base + Bo + 1;   // row -> new pages before it
+  L.refs = L.tail + Bo;       // row -> the partly filled page that it keeps (kMoved: none)
   L.fresh = L.refs + (n_pages <= kLdsRefs ? n_pages : 0);  // row -> its first new page, if the launch copies too
   L.total = L.fresh + (one ? Bo : 0);
   return L;
@@ -190,6 +192,9 @@ __host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo, bool one
 // Bound by its round trips and block-wide steps: 8 rows 7.6 us with the copies, 200 rows of 36 entries 11 without.
 // kOne: any number of blocks, which all do the bookkeeping, each for itself; the first writes it down, and then each
 // copies its share of the last pages' tokens.  That saves a launch, and a wait for it.
+// A partly filled page may be appended to, so one row may name it: the first that continues it, if no row names it as a
+// full page (as where a sequence was cut back into a prefix that others hold).  The rows' claims meet in the counts,
+// which are 0 for a page that no full entry names: the largest wins, whatever the order.
 template <bool kOne>
 __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
   extern __shared__ int lds[];
@@ -199,7 +204,8 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
   const int words = L.words;
   const bool lead = !kOne || blockIdx.x == 0;
   uint32_t* bits = reinterpret_cast<uint32_t*>(lds);
-  int *before = lds + words, *first = lds + L.first, *len = lds + L.len, *par = lds + L.par, *base = lds + L.base, *fresh = lds + L.fresh;
+  int *before = lds + words, *first = lds + L.first, *len = lds + L.len, *par = lds + L.par, *base = lds + L.base;
+  int *tail = lds + L.tail, *fresh = lds + L.fresh;
   bool bad = false;
   for (int e = tid; e < words; e += kPT) bits[e] = 0;
   int* refs = lds + L.refs;
@@ -215,14 +221,72 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
     if (lead) c.len_out[j] = n;
     len[j] = n;
     par[j] = p;
+    tail[j] = kMoved;
+    if (kOne) fresh[j] = -1;
     bad |= b;
   }
   __syncthreads();
+  // full pages, -1 behind them; a parent's partly filled page goes to its first child, which may keep it
+  const int ne = c.Bo * c.ld;  // (at most 2^26)
+  constexpr int kU = 4;  // entries of a thread in flight
+  for (int e0 = tid; e0 < ne; e0 += kU * kPT) {
+    int v[kU], kind[kU], row[kU];  // kind: 0 none, 1 behind the row's full pages, 2 full, 3 partly filled
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+      const int x = min(e0 + i * kPT, ne - 1);
+      const int j = x / c.ld, e = x - j * c.ld, n = len[j], full = n >> shift;
+      kind[i] = e < full ? 2 : e == full && (n & (page - 1)) != 0 && first[par[j]] == j ? 3 : 1;
+      if (e0 + i * kPT >= ne) kind[i] = 0;
+      v[i] = kind[i] >= 2 ? c.table[(int64_t)par[j] * c.ld + e] : -1;
+      row[i] = j;
+    }
+#pragma unroll
+    for (int i = 0; i < kU; ++i) {
+      if (kind[i] == 0) continue;
+      if (kind[i] >= 2 && (uint32_t)v[i] >= (uint32_t)np) {
+        v[i] = -1;
+        bad = true;
+      }
+      if (kind[i] == 3) {
+        tail[row[i]] = v[i];
+        v[i] = -1;
+      } else if (v[i] >= 0) {
+        atomicOr(&bits[v[i] >> 5], 1u << (v[i] & 31));
+        if (lead) {
+          if (counted) atomicAdd(&refs[v[i]], 1);
+          else __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v[i]], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+      }
+      if (lead) c.table_out[e0 + i * kPT] = v[i];
+    }
+  }
+  __syncthreads();
+  // claims of 2 and more, the lowest row's the largest; the page's count is then 1, its owner's
+  for (int j = tid; j < c.Bo; j += kPT) {
+    const int v = tail[j];
+    if (v < 0) continue;
+    if ((bits[v >> 5] >> (v & 31)) & 1u) tail[j] = kMoved;
+    else if (counted) atomicMax(&refs[v], c.Bo + 1 - j);
+    else __hip_atomic_fetch_max((Q35_GLOBAL int32_t*)&c.refs[v], c.Bo + 1 - j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  for (int j = tid; j < c.Bo; j += kPT) {
+    const int v = tail[j];
+    if (v < 0) continue;
+    const int won = counted ? __hip_atomic_load(&refs[v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)
+                            : __hip_atomic_load((Q35_GLOBAL int32_t*)&c.refs[v], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (won != c.Bo + 1 - j) {
+      tail[j] = kMoved;
+      continue;
+    }
+    if (counted) __hip_atomic_store(&refs[v], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    else __hip_atomic_store((Q35_GLOBAL int32_t*)&c.refs[v], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    atomicOr(&bits[v >> 5], 1u << (v & 31));
+    if (lead) c.table_out[(int64_t)j * c.ld + (len[j] >> shift)] = v;
+  }
+  __syncthreads();
   // entries that row j keeps
-  auto kept_of = [&](int j) {
-    const int n = len[j], p = par[j];
-    return (n >> shift) + (p >= 0 && (n & (page - 1)) != 0 && first[p] == j ? 1 : 0);
-  };
+  auto kept_of = [&](int j) { return (len[j] >> shift) + (tail[j] != kMoved ? 1 : 0); };
   int run = 0;  // new pages of the rows before this group of kPT
   for (int j0 = 0; j0 < c.Bo; j0 += kPT) {
     const int j = j0 + tid;
@@ -247,39 +311,8 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
   }
   if (tid == 0) base[c.Bo] = run;
   __syncthreads();
-  // kept entries, and -1 behind each row's pages
-  const int ne = c.Bo * c.ld;  // (at most 2^26)
-  constexpr int kU = 4;  // entries of a thread in flight
-  for (int e0 = tid; e0 < ne; e0 += kU * kPT) {
-    int v[kU], kind[kU];  // kind: 0 not written here, 1 behind the row's pages, 2 kept
-#pragma unroll
-    for (int i = 0; i < kU; ++i) {
-      const int x = min(e0 + i * kPT, ne - 1);
-      const int j = x / c.ld, e = x - j * c.ld, kept = kept_of(j);
-      kind[i] = e < kept ? 2 : e < kept + base[j + 1] - base[j] ? 0 : 1;
-      if (e0 + i * kPT >= ne) kind[i] = 0;
-      v[i] = kind[i] == 2 ? c.table[(int64_t)par[j] * c.ld + e] : -1;
-    }
-#pragma unroll
-    for (int i = 0; i < kU; ++i) {
-      if (kind[i] == 0) continue;
-      if (kind[i] == 2) {
-        if ((uint32_t)v[i] >= (uint32_t)np) {
-          v[i] = -1;
-          bad = true;
-        } else {
-          atomicOr(&bits[v[i] >> 5], 1u << (v[i] & 31));
-          if (kOne && !lead) continue;
-          if (counted) atomicAdd(&refs[v[i]], 1);
-          else __hip_atomic_fetch_add((Q35_GLOBAL int32_t*)&c.refs[v[i]], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
-      }
-      if (lead) c.table_out[e0 + i * kPT] = v[i];
-    }
-  }
-  __syncthreads();
   const int used = count_before(bits, before, words, sh);
-  // the r-th free page is the r-th new entry
+  // the r-th free page is the r-th new entry (where pages are short, the last entries stay -1)
   auto place = [&](int r, int page_id) {
     int lo = 0, hi = c.Bo;  // the row j with base[j] <= r < base[j + 1]
     while (hi - lo > 1) {
@@ -301,7 +334,6 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
       c.refs[p] = 1;
     }
   }
-  for (int r = np - used + tid; r < run; r += kPT) place(r, -1);
   if (bad && lead) raise_status(c.status, Q35_STATUS_ARG);
   if (tid == 0 && lead && run > np - used) raise_status(c.status, Q35_STATUS_FULL);
   if constexpr (kOne) {
@@ -310,7 +342,7 @@ __global__ __launch_bounds__(kPT) void pages_fork_kernel(const ForkCall c) {
     for (int i = blockIdx.x; i < c.Bo * parts; i += gridDim.x) {
       const int j = i / parts, p = par[j], n = len[j];
       // (a row that keeps its last page has no copy: its first new page, if any, is behind its tokens)
-      if (p < 0 || (n & (page - 1)) == 0 || first[p] == j) continue;
+      if (p < 0 || (n & (page - 1)) == 0 || tail[j] != kMoved) continue;
       copy_tail(c, i - j * parts, c.table[(int64_t)p * c.ld + (n >> shift)], fresh[j], n & (page - 1), kPT);
     }
   }

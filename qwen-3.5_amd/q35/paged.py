@@ -147,8 +147,8 @@ def pages_copy(pool, src, dst, to=None, check=False):
 
 def pages_fork(pool, table, lens, parents, grow=None, check=False):
     """The page table of the next set of sequences: row j continues sequence parents[j] of `table` (-1: an
-    empty row) with pages for grow[j] more tokens.  Full pages are shared; a partly filled last page stays
-    with the first child, every other child gets a copy.  table int32 [B, entries], lens int32 [B],
+    empty row) with pages for grow[j] more tokens.  Full pages are shared; a partly filled last page stays with the
+    first row that continues it, unless a row names it as a full page, and every other row gets a copy.  table int32 [B, entries], lens int32 [B],
     parents and grow int32 [B_out].  Returns PagesFork(table [B_out, entries], lens [B_out], refs [n_pages]:
     the rows that name each page).  `table` must cover every sequence that is to live on; it stays as
     it was.  check=True raises Q35Error where no page was left (Q35_E_NOMEM) or an index was out of range."""
