@@ -871,7 +871,9 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         m2 = pk_max(r32[0], r32[1]);
         split_scale(__uint_as_float(m2 << 16), fk, ik);  // (the exponent is all that counts)
         split_scale(__uint_as_float(m2 & 0xffff0000u), fv, iv);
-        iv = m2 >> 16 ? fmaxf(iv, 7.888609e-31f) : 7.888609e-31f;  // (2^-100: zeros ask for no room)
+        // (2^-100 at least: zeros ask for no room, and 2^12 over it stays finite)
+        iv = m2 >> 16 ? fmaxf(iv, 7.888609e-31f) : 7.888609e-31f;
+        fv = __uint_as_float((254u << 23) - __float_as_uint(iv));
         if (lane == 0) {
           scl[buf][0][wid] = ik;
           scl[buf][1][wid] = iv;
