@@ -359,10 +359,12 @@ int q35_status_check(uint32_t* status, void* stream);
  * of out as they were; a page outside the pool is not appended to and its tokens count as page 0's
  * (Q35_STATUS_ARG: the sequence's outputs are then invalid).  A sequence's keys and values must be
  * finite; what lies behind a sequence's last token in its last page may be anything.
- * Products and sums are f32 or their equivalent: 16-bit caches are multiplied as they are with
- * queries and weights carried whole, f32 caches in f32 or, for chunks of tokens, with every number as two
- * f16 halves (22 bits) under a power of two for every 4 keys or values: a value's error is then up to 2^-37 of
- * the largest value its chunk has met.  The keys' norms are formed in f64, so that what a 16-bit cache holds
+ * Sums are f32, products f32 or close to it: bf16 caches are multiplied with queries and weights carried whole
+ * (three bf16 parts), f16 ones with two f16 halves of a query or weight (2^-24 of it, or 2^-37 of the largest
+ * weight), f32 ones in f32 or, for chunks of tokens, as two f16 halves of either: a query, key, value or
+ * weight is off by up to 2^-24 of itself, or 2^-39 of the largest of its row, of its 4 keys, of the values that the
+ * tile of tokens (128 rows of token and head) sees, or 2^-37 of the largest weight (2^-34 within 32 tokens
+ * where values rise eightfold).  The keys' norms are formed in f64, so that what a 16-bit cache holds
  * does not hang on the order of a sum.
  * ws: q35_attention_paged_ws_bytes(d, T, B) bytes of scratch, 16-byte aligned (no zeroing needed). */
 size_t q35_attention_paged_ws_bytes(const q35_dims* d, int32_t T, int32_t B);

@@ -435,6 +435,16 @@ Q35_DEV f4 mma(q35_u32x4 x, q35_u32x4 y, f4 c) {
   if constexpr (DT == Q35_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q35_b8, x), __builtin_bit_cast(q35_b8, y), c, 0, 0, 0);
   else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q35_h8, x), __builtin_bit_cast(q35_h8, y), c, 0, 0, 0);
 }
+// y -> f16 halves (hi, lo), both to nearest: y = hi + lo to 2^-24 of y, or 2^-25 where that is more (f16's last
+// subnormal step).  What is left over has either sign; rounded toward zero it would add up over a context.
+Q35_DEV void split2_near(float y0, float y1, uint32_t& hi, uint32_t& lo) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const h2 h = __builtin_convertvector((f2{y0, y1}), h2);
+  const h2 l = __builtin_convertvector((f2{y0 - (float)h[0], y1 - (float)h[1]}), h2);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
+}
 constexpr int kFewLd = kHd + 4;
 constexpr int kFewLds = 4 * kFewRows * kFewLd * 4;
 
@@ -538,7 +548,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t p0, p1, p2 = 0;
-            if constexpr (DT == Q35_F16) split2(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
+            if constexpr (DT == Q35_F16) split2_near(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
             else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
             qb[0][j] = p0;
             qb[1][j] = p1;
@@ -610,7 +620,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
         for (int j = 0; j < 4; ++j) {
           const float p0 = sc[j >> 1][2 * (j & 1)], p1 = sc[j >> 1][2 * (j & 1) + 1];
           uint32_t w0, w1, w2 = 0;
-          if constexpr (DT == Q35_F16) split2(p0, p1, w0, w1);
+          if constexpr (DT == Q35_F16) split2_near(p0, p1, w0, w1);
           else split3(p0, p1, w0, w1, w2);
           pw[0][j] = w0;
           if constexpr (kQ > 1) pw[1][j] = w1;
@@ -747,8 +757,11 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
 // 16-byte read serves lanes 0-3, 12-15, 20-23, 24-27 at a time, then 4-11, 16-19, 28-31, and so does the
 // upper half; these places lie in different banks each time.
 // f16 caches are multiplied with 2 f16 halves of a query or weight, bf16 ones with 3 bf16 parts; f32
-// caches as 2 f16 halves with 2 (three products; what is dropped is 2^-22 of a term), under a power of
-// two for every 4 keys (a wave's share of the unit) and one for 4 values, whose inverse goes into the weights.
+// caches as 2 f16 halves with 2 (three products; what is dropped is 2^-24 of a term), under a power of
+// two for every 4 keys (a wave's share of the unit) and one for the values.  The values' power comes from the largest
+// one that the segment has met, found from 4 keys by each wave: where they differ, the weights make up for it,
+// and lose as many bits, so that a unit whose powers differ by more than 2^3 is laid out once more under their
+// largest (always under each wave's own: 10^-4 off beside values 2000 times the others).
 // Bound by the matrix cores: 2048 tokens of 8 heads behind 14336 in f32 780-860 us with the card's clock, 300-330
 // TFLOP/s of f32 products, 900-990 of f16 ones (a large f16 product of the library: 1112).
 constexpr int kMT = 512;       // threads
@@ -785,6 +798,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   // how far (log2) a score may pass the running maximum before the sums are rescaled: f16 weights
   // are kept 2^12 times larger and must stay below 2^16
   constexpr float kSlack = DT == Q35_BF16 ? 8.f : 3.f;
+  constexpr float kUneven = 0.125f;  // (the largest of 4 x 256 values of one distribution differ by less)
   typedef uint32_t u2 __attribute__((ext_vector_type(2)));
   const PagedAttn& a = A.c;
   extern __shared__ __align__(16) char lds[];  // [2 buffers][keys, values][part]
@@ -814,7 +828,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     // the first and the last token that a row of the wave sees
     const int lim0 = t.p0 + tok0 + div_rep(A, min(wid * kRowsW, rows - 1));
     const int lim1 = t.p0 + tok0 + div_rep(A, min(wid * kRowsW + kRowsW - 1, rows - 1));
-    const int end = t.p0 + t.n;
+    const int end = t.p0 + min(tok0 + A.tok_many, t.n);  // no row of the tile sees tokens from here on
     const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
     const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
     // staging registers: keys 4 wid + 2 i + hf, dims 8 n32 ..; values: keys 4 wid + i, dims 4 lane ..
@@ -835,6 +849,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
       for (int i = 0; i < 4; ++i) vr[i] = *(const Q35_GLOBAL VW*)(p + plane_elts(a) + i * kHd + 4 * lane);
     };
+    float vinv = 0.f;  // f32 caches: the power of two that brings the largest value so far to 2^14, its inverse
     auto store_unit = [&](int k, int buf) {
       if (k * kUnit + kUnit > end) {  // (uniform) rows behind the last token may hold anything
 #pragma unroll
@@ -871,9 +886,10 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         m2 = pk_max(r32[0], r32[1]);
         split_scale(__uint_as_float(m2 << 16), fk, ik);  // (the exponent is all that counts)
         split_scale(__uint_as_float(m2 & 0xffff0000u), fv, iv);
-        // (2^-100 at least: zeros ask for no room, and 2^12 over it stays finite)
-        iv = m2 >> 16 ? fmaxf(iv, 7.888609e-31f) : 7.888609e-31f;
+        // (2^-100 at least: 2^12 over it stays finite; zeros ask for nothing)
+        iv = fmaxf(fmaxf(iv, 7.888609e-31f), vinv);
         fv = __uint_as_float((254u << 23) - __float_as_uint(iv));
+        if (m2 >> 16 == 0) iv = 0.f;
         if (lane == 0) {
           scl[buf][0][wid] = ik;
           scl[buf][1][wid] = iv;
@@ -943,7 +959,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t p0, p1, p2 = 0;
-          if constexpr (kQ == 2) split2(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
+          if constexpr (kQ == 2) split2_near(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
           else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
           qb[0][st][j] = p0;
           qb[1][st][j] = p1;
@@ -956,15 +972,14 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     for (int i = 0; i < 16; ++i) o[i] = f4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     float ov = DT == Q35_BF16 ? 1.f : 4096.f;  // o is kept this much larger (f32 caches: 2^12 over the values' powers of two)
-    bool fresh = true;
     // reads: key n (+ 16), pieces 4 st + g; dim 16 dt + n, piece g
     int ka_off[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) ka_off[i] = n * 512 + ((4 * i + g) ^ n) * 16;
     const int va_off = n * 64 + ((g ^ -(n >> 2)) & 3) * 16;
     int k = ks;
-    for (int i = 0; i < k1 - k0; ++i) {
-      const int buf = i & 1;
+    for (int i = 0, turn = 0; i < k1 - k0; ++turn) {
+      const int buf = turn & 1;
       store_unit(k, buf);
       const int j0 = k * kUnit;
       k = kn;
@@ -972,49 +987,66 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
       kn = k + 1 < k1 ? k + 1 : k0;
       pg = unit_page(kn);
       __syncthreads();
-      if (!wave_on || j0 > lim1) continue;  // (uniform in the wave; the barrier above is passed by all)
+      const bool on = wave_on && j0 <= lim1;  // (uniform in the wave; the barriers are passed by all)
+      float own = 0.f;
+      if constexpr (kWide) own = scl[buf][1][lane & 7];
       const char* kb = lds + buf * 2 * kKV * kPlane;
       const char* vb = kb + kKV * kPlane;
       f4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      if (__builtin_expect(on, 1)) {
 #pragma unroll
-      for (int st = 0; st < 8; ++st) {
-        const char* src = kb + ka_off[st & 3] + (st >> 2) * 256;
-        q35_u32x4 ka[2][kKV];
+        for (int st = 0; st < 8; ++st) {
+          const char* src = kb + ka_off[st & 3] + (st >> 2) * 256;
+          q35_u32x4 ka[2][kKV];
 #pragma unroll
-        for (int w = 0; w < kKV; ++w)
+          for (int w = 0; w < kKV; ++w)
 #pragma unroll
-          for (int tl = 0; tl < 2; ++tl) ka[tl][w] = *(const q35_u32x4*)(src + tl * 16 * 512 + w * kPlane);
-        // (the two tiles in turn: a product does not wait for the one before it)
+            for (int tl = 0; tl < 2; ++tl) ka[tl][w] = *(const q35_u32x4*)(src + tl * 16 * 512 + w * kPlane);
+          // (the two tiles in turn: a product does not wait for the one before it)
 #pragma unroll
-        for (int q = 0; q < kQ; ++q)
+          for (int q = 0; q < kQ; ++q)
 #pragma unroll
-          for (int tl = 0; tl < 2; ++tl) sc[tl] = mma<DT>(ka[tl][0], qb[q][st], sc[tl]);
-        if constexpr (kWide) {
+            for (int tl = 0; tl < 2; ++tl) sc[tl] = mma<DT>(ka[tl][0], qb[q][st], sc[tl]);
+          if constexpr (kWide) {
 #pragma unroll
-          for (int tl = 0; tl < 2; ++tl) sc[tl] = mma<DT>(ka[tl][1], qb[0][st], sc[tl]);
+            for (int tl = 0; tl < 2; ++tl) sc[tl] = mma<DT>(ka[tl][1], qb[0][st], sc[tl]);
+          }
+        }
+        // operands are read kAhead steps before their products
+        constexpr int kAhead = kWide ? 1 : 2;
+        constexpr int kKr = 2 * kKV, kKm = 2 * (kWide ? 3 : kQ);  // reads and products of a step
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead * kKr, 0);
+#pragma unroll
+        for (int st = 0; st < 8 - kAhead; ++st) {
+          __builtin_amdgcn_sched_group_barrier(0x008, kKm / 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, kKr / 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, kKm / 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, kKr / 2, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kKm, 0);
+      }
+      if constexpr (kWide) {
+        // the largest of the unit's powers of two; where one is far below it, the unit is laid out again (all waves
+        // see the same numbers; then none is: at most once a unit).  Looked for behind the first products, and
+        // marked as rare, for the schedule's sake: 830 us for 2048 tokens behind 14336, 847 before them, 821 never.
+        float top = fmaxf(own, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(own), 0xB1, 0xf, 0xf, false)));
+        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x4E, 0xf, 0xf, false)));
+        top = fmaxf(top, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(top), 0x141, 0xf, 0xf, false)));
+        vinv = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(fmaxf(fmaxf(top, 7.888609e-31f), vinv))));
+        if (__builtin_expect(__ballot(own > 0.f && own < vinv * kUneven) != 0, 0)) {
+          kn = k;
+          pg = unit_page(kn);
+          k = j0 / kUnit;
+          load_unit(k, unit_page(k));
+          continue;
         }
       }
-      // operands are read kAhead steps before their products
-      constexpr int kAhead = kWide ? 1 : 2;
-      constexpr int kKr = 2 * kKV, kKm = 2 * (kWide ? 3 : kQ);  // reads and products of a step
-      __builtin_amdgcn_sched_group_barrier(0x100, kAhead * kKr, 0);
-#pragma unroll
-      for (int st = 0; st < 8 - kAhead; ++st) {
-        __builtin_amdgcn_sched_group_barrier(0x008, kKm / 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, kKr / 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, kKm / 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, kKr / 2, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, kAhead * kKm, 0);
+      ++i;
+      if (!on) continue;
       float fk[2] = {qscale, qscale}, fp[2] = {4096.f, 4096.f};
       float vscale = ov;
       if constexpr (kWide) {
-        // the outputs' power of two: 2^12 over the largest values so far
-        float iv = 0.f;
-#pragma unroll
-        for (int q = 0; q < 8; ++q) iv = fmaxf(iv, scl[buf][1][q]);
-        vscale = 4096.f * __uint_as_float((254u << 23) - __float_as_uint(iv));  // 2^12 / iv
-        if (!fresh) vscale = fminf(vscale, ov);
+        vscale = 4096.f * __uint_as_float((254u << 23) - __float_as_uint(vinv));  // the outputs': 2^12 / vinv
 #pragma unroll
         for (int tl = 0; tl < 2; ++tl) {
           fk[tl] = scl[buf][0][4 * tl + g] * qscale;
@@ -1040,7 +1072,6 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] *= al;
       }
-      fresh = false;
       const float mr = m == -INFINITY ? 0.f : m;
       q35_u32x4 pw[kQ];
 #pragma unroll
@@ -1053,7 +1084,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           p1 *= fp[e >> 2];
         }
         uint32_t w0, w1, w2 = 0;
-        if constexpr (kQ == 2) split2(p0, p1, w0, w1);
+        if constexpr (kQ == 2) split2_near(p0, p1, w0, w1);
         else split3(p0, p1, w0, w1, w2);
         pw[0][j] = w0;
         pw[1][j] = w1;
