@@ -421,7 +421,7 @@ int q35_pages_compact(q35_pages pool, const int32_t* table, int32_t ld_table, in
  *                among equal ones, and their x - lse.
  * targets NULL: no logprob and rank (both may be NULL).  A negative target scores 0 with rank -1
  * (padding); one >= V gives NaN with rank -1 (Q35_STATUS_ARG).  Rows of -inf alone: logprob -inf,
- * entropy 0.  A NaN or +inf in a row makes its logprob, entropy and top_logprobs NaN; a NaN ranks
+ * entropy 0.  No log probability is above 0, and it is 0 where no other logit is open.  A NaN or +inf in a row makes its logprob, entropy and top_logprobs NaN; a NaN ranks
  * behind every number.  ws: q35_token_logprobs_ws_bytes(M, V, top) bytes of scratch, 16-byte aligned. */
 size_t q35_token_logprobs_ws_bytes(int32_t M, int32_t V, int32_t top);
 int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, int64_t ld, const int32_t* targets,

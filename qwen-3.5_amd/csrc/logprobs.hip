@@ -162,13 +162,15 @@ Q35_DEV key_t seed_key(float v, int r) {
   return t == 0 ? 0 : ((key_t)t << 32) - 1;
 }
 
-// ln S, S a normal number: the exponent apart from the rest, whose logarithm is off by a few 2^-24 at most.
+// ln S, S >= 1 (the maximum's own term is 1): the exponent apart from the rest f in [1, 2), whose logarithm is off by a
+// few 2^-24 of itself, and what f loses in f32.  So ln 1 is 0, and no log probability comes out above 0.
 // (With the f64 functions, whose code every block fetches, and the lists asked for only when wanted, the join
 // took 7.2 us; 5.1 so.)
 Q35_DEV double ln_sum(double S) {
   int e;
-  const float f = (float)frexp(S, &e);
-  return (double)e * 0.693147180559945309 + (double)(__builtin_amdgcn_logf(f) * 0.693147180559945309f);
+  const double f = 2.0 * frexp(S, &e);
+  const float g = (float)f;
+  return ((double)(e - 1) + (double)__builtin_amdgcn_logf(g)) * 0.693147180559945309 + (double)((float)(f - (double)g) * __builtin_amdgcn_rcpf(g));
 }
 // Final numbers of row m of the call; l = ln S.
 Q35_DEV void finish_row(const ScoreCall& c, int m, float mx, double S, double U, double l, int cnt) {
