@@ -335,7 +335,8 @@ size_t q35_attention_prefill_ws_bytes(const q35_dims* d, int32_t T);
  *                    id, a pair that q35_pages_copy refuses): nothing was read or written outside
  *                    the buffers and what belongs to the index is as each entry point says;
  *   Q35_STATUS_FULL  q35_pages_fork found no free page for an entry, which is left -1.
- * q35_status_check synchronises `stream`, reads and clears it: Q35_E_RANGE for the first, Q35_E_NOMEM
+ * q35_status_check synchronises `stream`, reads the word and clears the bits that it read (one that a call on
+ * another stream sets meanwhile is told now or by the next check): Q35_E_RANGE for the first, Q35_E_NOMEM
  * for the second alone. */
 enum { Q35_F32 = 0, Q35_F16 = 1, Q35_BF16 = 2 };
 enum { Q35_STATUS_ARG = 1, Q35_STATUS_FULL = 2 };
@@ -421,8 +422,8 @@ int q35_pages_compact(q35_pages pool, const int32_t* table, int32_t ld_table, in
  *                among equal ones, and their x - lse.
  * targets NULL: no logprob and rank (both may be NULL).  A negative target scores 0 with rank -1
  * (padding); one >= V gives NaN with rank -1 (Q35_STATUS_ARG).  Rows of -inf alone: logprob -inf,
- * entropy 0.  No log probability is above 0, and it is 0 where no other logit is open.  A NaN or +inf in a row makes its logprob, entropy and top_logprobs NaN; a NaN ranks
- * behind every number.  ws: q35_token_logprobs_ws_bytes(M, V, top) bytes of scratch, 16-byte aligned. */
+ * entropy 0.  No log probability is above 0, and it is 0 where no other logit is open.  A NaN or +inf in a
+ * row makes its logprob, entropy and top_logprobs NaN; a NaN ranks behind every number.  ws: q35_token_logprobs_ws_bytes(M, V, top) bytes of scratch, 16-byte aligned. */
 size_t q35_token_logprobs_ws_bytes(int32_t M, int32_t V, int32_t top);
 int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, int64_t ld, const int32_t* targets,
                        int32_t top, float* logprob, int32_t* rank, float* entropy, int32_t* top_ids,

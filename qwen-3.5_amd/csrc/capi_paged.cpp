@@ -42,8 +42,10 @@ int q35_status_check(uint32_t* status, void* stream) {
     Q35_HIP_TRY(hipMemcpyAsync(&v, status, sizeof(v), hipMemcpyDeviceToHost, S(stream)));
     Q35_HIP_TRY(hipStreamSynchronize(S(stream)));
     if (!v) return Q35_OK;
-    const int rc = store_i32_launch(reinterpret_cast<int32_t*>(status), 0, S(stream));
+    const int rc = status_clear_launch(status, v, S(stream));
     if (rc) return rc;
+    // (a bit that is set after this call has returned must not meet the clearing)
+    Q35_HIP_TRY(hipStreamSynchronize(S(stream)));
     if (v & Q35_STATUS_ARG)
       return fail(Q35_E_RANGE, "a page, position, parent, token id or pair of pages was out of range or refused; the outputs it belongs to are invalid");
     return fail(Q35_E_NOMEM, "no free page left in the pool: entries of the page table were left -1");

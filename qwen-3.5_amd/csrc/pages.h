@@ -38,6 +38,9 @@ void allow_lds(size_t bytes) {
 
 int check_pages(const q35_pages& P, const char* what);
 
+// *status &= ~bits on the stream
+int status_clear_launch(uint32_t* status, uint32_t bits, hipStream_t st);
+
 int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t* sid, const int32_t* did, int n,
                       uint32_t* status, uint8_t* ok, hipStream_t st);
 

@@ -31,6 +31,11 @@ Q35_DEV void copy_unit(char* dst, const char* src, int t) {
   }
 }
 
+// (an atomic: calls on other streams may add bits at the same time)
+__global__ void status_clear_kernel(uint32_t* status, uint32_t bits) {
+  if (threadIdx.x == 0) __hip_atomic_fetch_and((Q35_GLOBAL uint32_t*)status, ~bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 // ---- copies
 struct CopyArgs {
   char* src;
@@ -454,6 +459,12 @@ int check_pages(const q35_pages& P, const char* what) {
   if (P.n_layers < 1 || P.n_layers > 65535 || P.n_pages < 1 || P.n_pages > kPageMaxPages || P.kv_heads < 1 || P.kv_heads > 1024)
     return no(Q35_E_SHAPE, ": layers, pages (at most 262144) and kv heads (at most 1024) must be positive");
   if ((reinterpret_cast<uintptr_t>(P.data) & 15) != 0) return no(Q35_E_ALIGN, ": pool not 16-byte aligned");
+  return Q35_OK;
+}
+
+int status_clear_launch(uint32_t* status, uint32_t bits, hipStream_t st) {
+  hipLaunchKernelGGL(status_clear_kernel, dim3(1), dim3(64), 0, st, status, bits);
+  Q35_HIP_TRY(hipGetLastError());
   return Q35_OK;
 }
 

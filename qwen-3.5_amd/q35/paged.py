@@ -14,7 +14,8 @@ sequences).  No counterparts in the reference, which decodes one sequence greedi
     pool.check()                                               # optional: raises what the kernels refused
 
 All calls are asynchronous on the current stream of their tensors' device; their scratch comes from
-torch's allocator call by call, so calls on several streams and captured graphs share nothing.
+torch's allocator call by call, so calls on several streams and captured graphs share nothing but what they are
+given: the pool's pages, and its status word, to which calls only add and from which a check takes what it read.
 """
 import collections
 import contextlib
