@@ -1232,7 +1232,9 @@ struct PagedLayout {
   size_t head, tile0, q, qmax, cut, tiles[2], ml[2], o[2];  // byte sizes
   size_t bytes;
 };
-PagedLayout paged_layout(int nh, int nkv, int T, int B) {
+// ctx_bytes: tokens that a sequence can have, times the bytes of a value; INT64_MAX for the workspace of any.
+constexpr int64_t kReread = 300000;
+PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
   PagedLayout L;
   const int rep = nh / nkv, tok_many = kManyRows / rep;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -1240,11 +1242,17 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B) {
   // 100 take 9.4 us there and 17.8 as a chunk.  16 tokens (4 tiles) take 20 us behind 200 and 98 behind 30000 in
   // f32, 32 and 47 as a chunk: every tile reads the context again.
   // Which kinds there are is the device's knowledge; what a call cannot or need not have gets no launch (an
-  // empty one takes 4 us).  If no sequence is empty, the longest has T - B + 1 tokens at most: where that is
-  // "few", all are (were all "few" up to two tokens per sequence, 63 of one token behind 2000 and one of 64
-  // behind 30000 would take 207 us, 133 so).  One sequence: its rows decide, if all rows are its.
+  // empty one takes 1.7 us, 3 where the host is behind).  If no sequence is empty, the longest has T - B + 1 tokens
+  // at most: where that is "few", all are (were all "few" up to two tokens per sequence, 63 of one token behind
+  // 2000 and one of 64 behind 30000 would take 207 us, 133 so).  But a batch of fixed slots may be one chunk and
+  // empty ones, so that holds only while the chunk's tiles could go over the longest context that the table
+  // and the rotary rows allow as cheaply as a chunk does (kReread; both ways, us: 16 tokens behind 16000 in bf16 37
+  // and 37, in f32 54 and 40; 64 behind 2000 28 and 37, 36 and 40; 256 behind 16000 272 and 112, 572 and 134).
+  // One sequence: its rows decide, if all rows are its.
   L.few_most = std::max(1, 2 * kFewRows / rep);
-  const bool few_only = T - B + 1 <= L.few_most, many_only = !few_only && B == 1;
+  const int64_t tiles = ((int64_t)T * rep + kFewRows - 1) / kFewRows * nkv;
+  const bool few_only = T <= L.few_most || (T - B + 1 <= L.few_most && ctx_bytes <= kReread / tiles);
+  const bool many_only = !few_only && B == 1;
   if (few_only) L.few_most = INT_MAX;
   if (many_only) L.few_most = 0;
   const int seqs = std::min(B, T);
@@ -1273,7 +1281,8 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B) {
 
 template <int DT>
 int launch(const PagedAttn& a, hipStream_t st) {
-  const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B);
+  const int64_t ctx = std::min<int64_t>((int64_t)a.ld_table * a.P.page, a.rope_rows);
+  const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B, ctx * elt_size(a.P.dtype));
   AttnArgs A;
   A.c = a;
   A.page_shift = __builtin_ctz((unsigned)a.P.page);
@@ -1325,7 +1334,7 @@ int launch(const PagedAttn& a, hipStream_t st) {
 
 }  // namespace
 
-size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) { return paged_layout(nh, nkv, T, B).bytes; }
+size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) { return paged_layout(nh, nkv, T, B, INT64_MAX).bytes; }
 
 int paged_attn_launch(const PagedAttn& a, hipStream_t st) {
   return a.P.dtype == Q35_F32 ? launch<Q35_F32>(a, st) : a.P.dtype == Q35_F16 ? launch<Q35_F16>(a, st) : launch<Q35_BF16>(a, st);
