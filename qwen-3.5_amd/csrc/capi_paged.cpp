@@ -24,7 +24,7 @@ inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 }
 // A launch has fewer than 2^32 threads along x: so many blocks of 256.
 constexpr int kMaxGrid = 1 << 24;
-// The paged attention's append has one block for 4 (row, query or kv head)s and one more.
+// The paged attention's append has one block for 4 (row, query or kv head)s and two more.
 inline bool rows_fit(const q35_dims* d, int32_t T) { return (int64_t)T * (d->attn_heads + d->kv_heads) < (1 << 25); }
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 

@@ -80,6 +80,7 @@ struct AttnArgs {
   int32_t few_most;       // sequences of at most this many new tokens are "few"
   int32_t max_tiles[2], max_blocks[2], part_rows[2];
   PlanHead* head;        // [2]
+  int64_t* once;         // units of "few" that no other tile reads
   float* q;              // [T][heads][256] queries after norm and rotary
   float* qmax;           // [T][heads] largest |value|
   int32_t* tile0;        // [2][B] first tile of the sequence in the list of each kind
@@ -202,6 +203,33 @@ Q35_DEV void make_plan(const AttnArgs& A) {
   }
 }
 
+// Made by another block: the units of "few" that one tile alone reads, all but what lies in pages that the sequence
+// before has at the same place (looked at in eight places) and what a sequence's second tile reads.
+Q35_DEV void count_once(const AttnArgs& A) {
+  const PagedAttn& a = A.c;
+  __shared__ int64_t sl[kT / 64];
+  if (A.max_blocks[0] == 0) return;
+  int64_t once = 0;
+  for (int b = threadIdx.x; b < a.B; b += kT) {
+    Seq s;
+    if (!load_seq(a, b, &s) || s.n == 0 || kind_of(A, s.n) != 0) continue;
+    const int ctx = s.p0 + s.n, pages = ((ctx - 1) >> A.page_shift) + 1;
+    const int32_t* row = a.table + (int64_t)b * a.ld_table;
+    int own = 8;
+    if (b > 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t c = (2 * i + 1) * (int64_t)pages >> 4;
+        own -= row[c] == row[c - a.ld_table] ? 1 : 0;
+      }
+    }
+    once += (int64_t)((ctx + kUnit - 1) / kUnit) * a.nkv * own / 8;
+  }
+  int64_t all;
+  plan_excl(once, sl, &all);
+  if (threadIdx.x == 0) *A.once = all;
+}
+
 template <int DT>
 struct Elt;
 template <>
@@ -244,19 +272,20 @@ Q35_DEV E stored(double y) {
 }
 
 // Keys and values of the new tokens into their pages, and the normalised, rotated queries (with each one's
-// largest |value|) into the workspace; a wave per (row, kv head or query head).  Block 0 makes the plan.  Bound by
+// largest |value|) into the workspace; a wave per (row, kv head or query head).  Blocks 0 and 1 make the plan.  Bound by
 // its chain of round trips (starts, table, stores) while rows are few: 4.3 us for one token, 17.6 for 2048.
 template <int DT>
 __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
   const PagedAttn& a = A.c;
   __shared__ double xs[kT / 64][kHd];
-  if (blockIdx.x == 0) {
-    make_plan(A);
+  if (blockIdx.x < 2) {
+    if (blockIdx.x == 0) make_plan(A);
+    else count_once(A);
     return;
   }
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, per = a.nkv + a.nh;
-  const int64_t item = ((int64_t)blockIdx.x - 1) * (kT / 64) + wid;
+  const int64_t item = ((int64_t)blockIdx.x - 2) * (kT / 64) + wid;
   const int64_t t = item / per;
   const int hd = (int)(item % per), g = hd, h = hd - a.nkv;  // kv head g, or query head h
   if (t >= a.T) return;
@@ -448,8 +477,6 @@ Q35_DEV void split2_near(float y0, float y1, uint32_t& hi, uint32_t& lo) {
 constexpr int kFewLd = kHd + 4;
 constexpr int kFewLds = 4 * kFewRows * kFewLd * 4;
 
-template <int DT>
-constexpr int elt_bytes() { return DT == Q35_F32 ? 4 : 2; }
 template <bool kStream>
 Q35_DEV q35_u32x4 ldg16_if(const void* p) {
   if constexpr (kStream) return __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)p);
@@ -729,17 +756,24 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   if (bad && lane == 0) raise_status(a.status, Q35_STATUS_ARG);
 }
 
+// Whether the tiles' w units are read past the 256 MB of the last-level cache: if they are more than it holds, and less
+// than an eighth of them is read by another tile too.  (us, through the cache and past it: 33 tokens over 958 MB 206
+// and 179; 40 tokens over 800 MB with a tenth shared 144 and 140, a fifth 133 and 140, half 122 and 140; 64 samples
+// of 16384 shared tokens 161 and 240; 54 tiles over 229 MB 40 and 53.)
+template <int DT>
+Q35_DEV bool past_llc(const PlanHead& H, int64_t once) {
+  return H.w > (int64_t)(256u << 20) / (kUnit * 2 * kHd * (DT == Q35_F32 ? 4 : 2)) && 8 * (H.w - once) < H.w;
+}
+
 template <int DT>
 __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
   extern __shared__ __align__(16) float os[];
   __shared__ float ms[4][kFewRows], ls[4][kFewRows];
   __shared__ Start sh;
   PlanHead H;
+  const int64_t once = *A.once;
   if (!block_start(A, 0, &H, &sh)) return;
-  // What the tiles read in all, against the 256 MB of the last-level cache: a larger stream passes it by
-  // (33 tokens over 958 MB: 179 us, 206 through it), a smaller one is found there again by sequences that
-  // share pages and by second tiles (54 tiles over 229 MB: 40 us, 53 past it).
-  if (H.w > (int64_t)(256u << 20) / (kUnit * 2 * kHd * elt_bytes<DT>())) few_run<DT, true>(A, H, sh, os, ms, ls);
+  if (past_llc<DT>(H, once)) few_run<DT, true>(A, H, sh, os, ms, ls);
   else few_run<DT, false>(A, H, sh, os, ms, ls);
 }
 
@@ -1263,7 +1297,7 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
   L.max_blocks[1] = few_only ? 0 : cus;
   L.part_rows[0] = (int)std::min<int64_t>(kFewRows, (int64_t)T * rep);
   L.part_rows[1] = (int)std::min<int64_t>(kManyRows, (int64_t)T * rep);
-  L.head = up(2 * sizeof(PlanHead));
+  L.head = up(2 * sizeof(PlanHead) + sizeof(int64_t));
   L.tile0 = up((size_t)2 * B * 4);
   L.q = up((size_t)T * nh * kHd * 4);
   L.qmax = up((size_t)T * nh * 4);
@@ -1292,6 +1326,7 @@ int launch(const PagedAttn& a, hipStream_t st) {
   A.few_most = L.few_most;
   char* p = static_cast<char*>(a.ws);
   A.head = reinterpret_cast<PlanHead*>(p);
+  A.once = reinterpret_cast<int64_t*>(A.head + 2);
   p += L.head;
   A.tile0 = reinterpret_cast<int32_t*>(p);
   p += L.tile0;
@@ -1313,7 +1348,7 @@ int launch(const PagedAttn& a, hipStream_t st) {
     p += L.o[k];
   }
   const int64_t ka = (int64_t)a.T * (a.nkv + a.nh), qa = (int64_t)a.T * a.nh;
-  hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((uint32_t)((ka + 3) / 4 + 1)), dim3(kT), 0, st, A);
+  hipLaunchKernelGGL(paged_append_kernel<DT>, dim3((uint32_t)((ka + 3) / 4 + 2)), dim3(kT), 0, st, A);
   Q35_HIP_TRY(hipGetLastError());
   if (A.max_blocks[0] > 0) {
     allow_lds<paged_few_kernel<DT>>(kFewLds);
