@@ -2,7 +2,8 @@
 // the sequences' pages, causal softmax(q K^T / 16) V with shared kv heads, sigmoid output gate.
 //
 // Launches: append (with the plan), the attention of the sequences with few new tokens, that of the
-// sequences with many, and the join of what the plan cut.
+// sequences with many (either left out where paged_layout says that no sequence needs it), and the join of what
+// the plan cut.
 #include "pages.h"
 
 #include <algorithm>
@@ -52,7 +53,7 @@ Q35_DEV bool find_seq(const PagedAttn& a, int t, Seq* s) {
 // end over all tiles of all sequences: block g of G takes the units [g W / G, (g + 1) W / G), whatever
 // tiles they belong to.  So ragged batches load every CU alike, and a few long sequences are split as
 // finely as many short ones are not.  Where a block's range cuts a tile, it leaves (max, sum, output)
-// of its part, and the merge kernel joins the parts; only the first and the last tile of a block can be
+// of its part, and paged_join_kernel joins the parts; only the first and the last tile of a block can be
 // cut, so two slots per block hold them all.
 //
 // Two kinds of tiles: sequences of few rows ("few": the cache's stream bounds them) and chunks ("many":
@@ -796,8 +797,9 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
 // one that the segment has met, found from 4 keys by each wave: where they differ, the weights make up for it,
 // and lose as many bits, so that a unit whose powers differ by more than 2^3 is laid out once more under their
 // largest (always under each wave's own: 10^-4 off beside values 2000 times the others).
-// Bound by the matrix cores: 2048 tokens of 8 heads behind 14336 in f32 780-860 us with the card's clock, 300-330
-// TFLOP/s of f32 products, 900-990 of f16 ones (a large f16 product of the library: 1112).
+// Bound by the matrix cores: 2048 tokens of 8 heads behind 14336 in f32 770-850 us with the card's clock, 300-330
+// TFLOP/s of f32 products, 900-990 of f16 ones (a large f16 product of the library: 1112); the whole call 806 us, over
+// an f16 cache (two products instead of three) 500, over bf16 (three) 617.
 constexpr int kMT = 512;       // threads
 constexpr int kRowsW = 16;     // rows of a wave
 constexpr int kPlane = 16384;  // bytes of a unit's keys (or values) of one part

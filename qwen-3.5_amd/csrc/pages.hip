@@ -1,10 +1,10 @@
 // Pages of a cache: copies, forks, compaction.
 //
-// The bookkeeping of a fork or a compaction is whole-number work on tables of a few thousand entries:
-// one block does it with a bitmap of the pool's pages in LDS, so that it needs no host round trip
-// and no order among blocks; every choice (which page is new, which page moves where) is a rank among
-// bits, hence the same on every run.  The pages themselves are then moved by a second launch over
-// the whole chip; a page of one layer is one contiguous run.
+// The bookkeeping of a fork or a compaction is whole-number work on a table of page numbers: a block does it by
+// itself with a bitmap of the pool's pages in LDS, so that it needs no host round trip and no order among
+// blocks; every choice (which page is new, which page moves where) is a rank among bits, hence the same on
+// every run.  While the table is small, every block of one launch does it and then copies its share of the
+// pages; else one block does it and a second launch copies.  A page of one layer is one contiguous run.
 #include "pages.h"
 
 #include <algorithm>
@@ -194,7 +194,8 @@ __host__ __device__ inline ForkLds fork_lds(int n_pages, int B, int Bo, bool one
 
 // Every step spreads its entries over all threads (a wave per row waited for its row's loads in turn: 35
 // instead of 17 us for 200 rows of 36 entries).
-// Bound by its round trips and block-wide steps: 8 rows 7.6 us with the copies, 200 rows of 36 entries 11 without.
+// Bound by its round trips and block-wide steps: 8 rows 7.6 us with the copies, 200 rows of 36 entries 10 without.  One
+// block's rate bounds large tables: 33 rows of 4097 entries, 29000 pages in use, 78 us, 132000 in use 250.
 // kOne: any number of blocks, which all do the bookkeeping, each for itself; the first writes it down, and then each
 // copies its share of the last pages' tokens.  That saves a launch, and a wait for it.
 // A partly filled page may be appended to, so one row may name it: the first that continues it, if no row names it as a
@@ -375,7 +376,8 @@ Q35_DEV void copy_move(const CompactCall& c, const int32_t* holes, const int32_t
   copy_unit(base + holes[m] * pb, base + movers[m] * pb, t);
 }
 // kOne: as pages_fork_kernel's; the lists of moves stay in LDS.  514 MB read and written in 101 us, 5.1 TB/s (HBM); a
-// small pool 5.6 us (round trips).
+// small pool 5.6 us (round trips).  Larger tables are one block's, a load of a thread at a time, each entry twice: 33
+// rows of 4097 entries 99 us with 29000 pages in use, 265 with 132000, beside what moves.
 template <bool kOne>
 __global__ __launch_bounds__(kPT) void pages_compact_kernel(const CompactCall c, int64_t pb, int units) {
   extern __shared__ uint32_t bits[];  // pages in use, then the number of them before each word, then the moves
