@@ -796,7 +796,7 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
 // two for every 4 keys (a wave's share of the unit) and one for the values.  The values' power comes from the largest
 // one that the segment has met, found from 4 keys by each wave: where they differ, the weights make up for it,
 // and lose as many bits, so that a unit whose powers differ by more than 2^3 is laid out once more under their
-// largest (always under each wave's own: 10^-4 off beside values 2000 times the others).
+// largest (always under each wave's own, 16384 small weights beside values 2 10^6 times the others were 4 10^-3 off).
 // Bound by the matrix cores: 2048 tokens of 8 heads behind 14336 in f32 770-850 us with the card's clock, 300-330
 // TFLOP/s of f32 products, 900-990 of f16 ones (a large f16 product of the library: 1112); the whole call 806 us, over
 // an f16 cache (two products instead of three) 500, over bf16 (three) 617.
@@ -1268,8 +1268,9 @@ struct PagedLayout {
   size_t head, tile0, q, qmax, cut, tiles[2], ml[2], o[2];  // byte sizes
   size_t bytes;
 };
-// ctx_bytes: tokens that a sequence can have, times the bytes of a value; INT64_MAX for the workspace of any.
+// What all tiles of T rows, as "few", may go over if all are one sequence's: tiles, kv heads, tokens, bytes of a value.
 constexpr int64_t kReread = 300000;
+// ctx_bytes: tokens that a sequence can have, times the bytes of a value; INT64_MAX for the workspace of any call.
 PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
   PagedLayout L;
   const int rep = nh / nkv, tok_many = kManyRows / rep;
