@@ -325,7 +325,14 @@ size_t q35_attention_prefill_ws_bytes(const q35_dims* d, int32_t T);
  * A pool of cache pages of `page` tokens (a power of two, 16..256) for n_layers attention layers:
  *   data[n_layers][n_pages][2][kv_heads][page][head_dim], plane 0 the keys (after k_norm and RoPE),
  *   plane 1 the values, 16-byte aligned, in f32, f16 or bf16 (values are rounded to nearest even
- *   when they are appended; head_dim 256).
+ *   when they are appended; head_dim 256), or in 4 bits.
+ * Q35_Q4: data[n_layers][n_pages][2][kv_heads][page] rows of 144 bytes: 256 codes of 4 bits (value d in the low
+ *   (d even) or high half of byte d / 2), then a 16-bit word, little-endian, for each 32 values: without its low
+ *   4 bits an f16 scale s, in them a zero z; code c stands for s (c - z), which is exactly an f16.  As
+ *   values y are appended (in f32, cut at +-32768), s is the smallest such scale, a number of 7 significant bits or a
+ *   multiple of 2^-20, that is not below (max(0, y) - min(0, y)) / 15 over the 32, z = -min(0, y) / s and
+ *   c = y / s + z cut to 0..15, both quotients rounded to nearest even: a value is off by s / 2 at most.  32
+ *   values one of which is infinite or NaN are all held as NaN (the word 0x7FF0).
  * A page table is int32 [B][ld_table]: entry c of row b is the page that holds tokens c*page .. of
  * sequence b, or -1.  A page may stand in several rows (shared contexts); pages that a sequence is
  * about to append to must stand in its row alone, and once, which q35_pages_fork sees to.
@@ -338,11 +345,11 @@ size_t q35_attention_prefill_ws_bytes(const q35_dims* d, int32_t T);
  * q35_status_check synchronises `stream`, reads the word and clears the bits that it read (one that a call on
  * another stream sets meanwhile is told now or by the next check): Q35_E_RANGE for the first, Q35_E_NOMEM
  * for the second alone. */
-enum { Q35_F32 = 0, Q35_F16 = 1, Q35_BF16 = 2 };
+enum { Q35_F32 = 0, Q35_F16 = 1, Q35_BF16 = 2, Q35_Q4 = 4 };
 enum { Q35_STATUS_ARG = 1, Q35_STATUS_FULL = 2 };
 typedef struct {
   void* data;
-  int32_t dtype; /* Q35_F32, Q35_F16 or Q35_BF16 */
+  int32_t dtype; /* Q35_F32, Q35_F16, Q35_BF16 or Q35_Q4 */
   int32_t n_layers, n_pages, kv_heads, page, head_dim;
 } q35_pages;
 int q35_status_check(uint32_t* status, void* stream);
@@ -361,7 +368,7 @@ int q35_status_check(uint32_t* status, void* stream);
  * (Q35_STATUS_ARG: the sequence's outputs are then invalid).  A sequence's keys and values must be
  * finite; what lies behind a sequence's last token in its last page may be anything.
  * Sums are f32, products f32 or close to it: bf16 caches are multiplied with queries and weights carried whole
- * (three bf16 parts), f16 ones with two f16 halves of a query or weight (2^-24 of it, or 2^-37 of the largest
+ * (three bf16 parts), f16 and 4-bit ones with two f16 halves of a query or weight (2^-24 of it, or 2^-37 of the largest
  * weight), f32 ones in f32 or, for chunks of tokens, as two f16 halves of either: a query, key, value or
  * weight is off by up to 2^-24 of itself, or 2^-39 of the largest of its row, of its 4 keys, of the values that the
  * tile of tokens (128 rows of token and head) sees, or 2^-37 of the largest weight (2^-34 within 32 tokens
@@ -384,6 +391,12 @@ int q35_attention_core_paged(const q35_dims* d, q35_pages pool, int32_t layer, c
 size_t q35_pages_copy_ws_bytes(int32_t n);
 int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const int32_t* dst_ids, int32_t n,
                    uint32_t* status, void* ws, size_t ws_bytes, void* stream);
+
+/* What layer `layer` of the cache holds of n tokens, as values: out[i] [2][kv_heads][256] is the key and value rows of
+ * position pos[i] of sequence row[i] of table [B][ld_table], in the pool's type (f16 for Q35_Q4, exactly).  A row, a
+ * position or a page out of range gives zeros (Q35_STATUS_ARG).  out 16-byte aligned; n kv_heads < 2^25. */
+int q35_pages_read(q35_pages pool, int32_t layer, const int32_t* table, int32_t ld_table, int32_t B,
+                   const int32_t* row, const int32_t* pos, int32_t n, void* out, uint32_t* status, void* stream);
 
 /* The next page table of a set of sequences: row j of table_out [B_out][ld_table] continues sequence
  * parent[j] of table [B][ld_table] (len[b] tokens), or is empty for parent[j] = -1, with pages for grow[j]

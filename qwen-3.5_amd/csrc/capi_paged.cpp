@@ -122,9 +122,30 @@ int q35_pages_copy(q35_pages src, q35_pages dst, const int32_t* src_ids, const i
       return fail(Q35_E_ARG, "pages_copy: two pools that overlap");
     if (n == 0) return Q35_OK;
     if (!src_ids || !dst_ids) return fail(Q35_E_ARG, "pages_copy: null pointer");
-    if ((int64_t)n * (int64_t)(pb / 16384) >= kMaxGrid) return fail(Q35_E_SHAPE, "pages_copy: too many pages for one call");
+    if ((int64_t)n * (int64_t)((pb + 16383) / 16384) >= kMaxGrid) return fail(Q35_E_SHAPE, "pages_copy: too many pages for one call");
     if (n > kPageFewPairs && (!ws || ws_bytes < q35_pages_copy_ws_bytes(n))) return fail(Q35_E_WS, "pages_copy: workspace too small");
     return pages_copy_launch(src, dst, src_ids, dst_ids, n, status, static_cast<uint8_t*>(ws), S(stream));
+  });
+}
+
+int q35_pages_read(q35_pages pool, int32_t layer, const int32_t* table, int32_t ld_table, int32_t B,
+                   const int32_t* row, const int32_t* pos, int32_t n, void* out, uint32_t* status, void* stream) {
+  return entry([&]() -> int {
+    const int rc = check_pages(pool, "pages_read");
+    if (rc) return rc;
+    if (layer < 0 || layer >= pool.n_layers) return fail(Q35_E_SHAPE, "pages_read: no such layer in the pool");
+    if (n < 0 || B < 1 || ld_table < 1 || (int64_t)n * pool.kv_heads >= (1 << 25))
+      return fail(Q35_E_SHAPE, "pages_read: n >= 0, B >= 1, ld_table >= 1 and n kv_heads < 2^25 required");
+    if (n == 0) return Q35_OK;
+    if (!table || !row || !pos || !out) return fail(Q35_E_ARG, "pages_read: null pointer");
+    if (!aligned(out, 16)) return fail(Q35_E_ALIGN, "pages_read: out not 16-byte aligned");
+    ReadCall c;
+    c.P = pool;
+    c.table = table; c.row = row; c.pos = pos;
+    c.layer = layer; c.ld = ld_table; c.B = B; c.n = n;
+    c.out = out;
+    c.status = status;
+    return pages_read_launch(c, S(stream));
   });
 }
 

@@ -245,9 +245,17 @@ template <>
 struct Elt<Q35_BF16> {
   typedef __bf16 T;
 };
+template <>
+struct Elt<Q35_Q4> {
+  typedef uint8_t T;  // (bytes)
+};
 
-Q35_DEV int64_t plane_elts(const PagedAttn& a) { return (int64_t)a.nkv * a.P.page * kHd; }
-Q35_DEV int64_t page_elts(const PagedAttn& a) { return 2 * plane_elts(a); }
+template <int DT>
+constexpr int kRow = DT == Q35_Q4 ? kQ4Row : kHd;  // elements of a token's row
+template <int DT>
+Q35_DEV int64_t plane_elts(const PagedAttn& a) { return (int64_t)a.nkv * a.P.page * kRow<DT>; }
+template <int DT>
+Q35_DEV int64_t page_elts(const PagedAttn& a) { return 2 * plane_elts<DT>(a); }
 
 // wave sum in f64, the same in every lane
 Q35_DEV double wave_sum64(double v) {
@@ -270,6 +278,80 @@ Q35_DEV E stored(double y) {
   float f = (float)y;
   asm("" : "+v"(f));
   return (E)f;
+}
+
+// ------------------------------------------------------------------ 4 bits
+// A row of a Q35_Q4 cache: a code c of 4 bits per value, and for each 32 values a word: an f16 scale s of 7 significant
+// bits (the word without its low 4 bits) and a zero z (those); the value is s (c - z).  |c - z| has 4 bits, so a value
+// is exactly an f16, and the kernels multiply f16 values, as over f16 caches, with nothing lost in between.
+// lo = min(0, the least value), hi = max(0, the largest), s the smallest such number that is not below
+// (hi - lo) / 15, z = lo / -s and c = y / s + z, both quotients rounded to nearest even: a value is off by s / 2 at
+// most.  (7 bits: s is at most 1/64 larger than it need be.)
+//
+// y / s to the nearest whole number, ties to even (|y| <= 16 s, s of 7 significant bits): an estimate, put right by its remainder, which
+// is exact (near a whole multiple of s the difference is).
+Q35_DEV float quot_even(float y, float s, float inv) {
+  float q = __builtin_rintf(y * inv);
+  const float e = __builtin_fmaf(-q, s, y), h = 0.5f * s;
+  const bool odd = (int)q & 1;
+  q += e > h || (e == h && odd) ? 1.f : e < -h || (e == -h && odd) ? -1.f : 0.f;
+  return q;
+}
+// The codes of the lane's 4 values (a group of 32 is that of 8 lanes), and the group's word
+Q35_DEV uint32_t quantise4(const float (&in)[4], uint32_t& word) {
+  float y[4], lo = 0.f, hi = 0.f;
+  bool fine = true;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    fine = fine && fabsf(in[j]) < INFINITY;
+    y[j] = fminf(fmaxf(in[j], -32768.f), 32768.f);
+    lo = fminf(lo, y[j]);
+    hi = fmaxf(hi, y[j]);
+  }
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    lo = fminf(lo, __shfl_xor(lo, o, 64));
+    hi = fmaxf(hi, __shfl_xor(hi, o, 64));
+  }
+  const unsigned long long odd = __ballot(!fine) >> (threadIdx.x & 56);
+  if (odd & 0xff) {  // a value that is no number, or infinite: none of the group's is
+    word = 0x7FF0;
+    return 0;
+  }
+  const double x = ((double)hi - (double)lo) / 15.0;
+  uint32_t b = __builtin_bit_cast(uint16_t, (_Float16)(float)x) & 0xFFF0u;
+  if ((double)(float)__builtin_bit_cast(_Float16, (uint16_t)b) < x) b += 16;
+  const float s = (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+  if (b == 0) {
+    word = 0;
+    return 0;
+  }
+  const float inv = 1.f / s, z = quot_even(-lo, s, inv);
+  word = b | (uint32_t)z;
+  uint32_t c = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c |= (uint32_t)fminf(fmaxf(quot_even(y[j], s, inv) + z, 0.f), 15.f) << (4 * j);
+  return c;
+}
+// 4 values of a group's keys or values as f16 pairs.  1024 + c and 64 + c are the bits 0x6400 | c and 0x5400 | c << 4; their
+// differences from 1024 + z and 64 + z are exact, and so is the product with s.
+struct Word2 {  // of two groups, in halves
+  uint32_t s, n0, n4;  // s, -(1024 + z), -(64 + z)
+};
+Q35_DEV Word2 word2(uint32_t w) {
+  const uint32_t z = w & 0x000F000Fu;
+  return Word2{w & 0xFFF0FFF0u, z | 0xE400E400u, z << 4 | 0xD400D400u};
+}
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+Q35_DEV uint32_t value2(uint32_t c, uint32_t n, uint32_t s) {
+  return __builtin_bit_cast(uint32_t, (h2)((__builtin_bit_cast(h2, c) + __builtin_bit_cast(h2, n)) * __builtin_bit_cast(h2, s)));
+}
+Q35_DEV uint32_t low_nibbles(uint32_t t, const Word2& w) { return value2((t & 0x000F000Fu) | 0x64006400u, w.n0, w.s); }
+Q35_DEV uint32_t high_nibbles(uint32_t t, const Word2& w) { return value2((t & 0x00F000F0u) | 0x54005400u, w.n4, w.s); }
+// 8 values (one dword of codes) as operands: values p and p + 4 in the halves of word p
+Q35_DEV q35_u32x4 values8(uint32_t c, const Word2& w) {
+  const uint32_t d = c >> 8;
+  return q35_u32x4{low_nibbles(c, w), high_nibbles(c, w), low_nibbles(d, w), high_nibbles(d, w)};
 }
 
 // Keys and values of the new tokens into their pages, and the normalised, rotated queries (with each one's
@@ -338,21 +420,36 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) x[d + j] = y[j];
   wave_lds_sync();
-  E* kr = static_cast<E*>(a.P.data) + ((int64_t)a.layer * a.P.n_pages + page) * page_elts(a) +
-          ((int64_t)g * a.P.page + (p & (a.P.page - 1))) * kHd;
-  E* vr = kr + plane_elts(a);
+  E* kr = static_cast<E*>(a.P.data) + ((int64_t)a.layer * a.P.n_pages + page) * page_elts<DT>(a) +
+          ((int64_t)g * a.P.page + (p & (a.P.page - 1))) * kRow<DT>;
+  E* vr = kr + plane_elts<DT>(a);
   const float vv[4] = {v.x, v.y, v.z, v.w};
-  E ko[4], vo[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int i = d + j;
     if (i < a.rot) y[j] = y[j] * (double)cs[i] + (i < half ? -x[i + half] : x[i - half]) * (double)sn[i];
-    ko[j] = stored<E>(y[j]);
-    vo[j] = (E)vv[j];
   }
-  typedef E E4 __attribute__((ext_vector_type(4)));
-  *reinterpret_cast<E4*>(kr + d) = E4{ko[0], ko[1], ko[2], ko[3]};
-  *reinterpret_cast<E4*>(vr + d) = E4{vo[0], vo[1], vo[2], vo[3]};
+  if constexpr (DT == Q35_Q4) {
+    const float kk[4] = {(float)y[0], (float)y[1], (float)y[2], (float)y[3]};
+    uint32_t kw, vw;
+    const uint32_t kc = quantise4(kk, kw), vc = quantise4(vv, vw);
+    *reinterpret_cast<uint16_t*>(kr + 2 * lane) = (uint16_t)kc;
+    *reinterpret_cast<uint16_t*>(vr + 2 * lane) = (uint16_t)vc;
+    if ((lane & 7) == 0) {
+      *reinterpret_cast<uint16_t*>(kr + kHd / 2 + lane / 4) = (uint16_t)kw;
+      *reinterpret_cast<uint16_t*>(vr + kHd / 2 + lane / 4) = (uint16_t)vw;
+    }
+  } else {
+    E ko[4], vo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ko[j] = stored<E>(y[j]);
+      vo[j] = (E)vv[j];
+    }
+    typedef E E4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<E4*>(kr + d) = E4{ko[0], ko[1], ko[2], ko[3]};
+    *reinterpret_cast<E4*>(vr + d) = E4{vo[0], vo[1], vo[2], vo[3]};
+  }
 }
 
 // ------------------------------------------------------------------ shared by the attention kernels
@@ -478,18 +575,18 @@ Q35_DEV void split2_near(float y0, float y1, uint32_t& hi, uint32_t& lo) {
 constexpr int kFewLd = kHd + 4;
 constexpr int kFewLds = 4 * kFewRows * kFewLd * 4;
 
-template <bool kStream>
-Q35_DEV q35_u32x4 ldg16_if(const void* p) {
-  if constexpr (kStream) return __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)p);
-  else return *(const Q35_GLOBAL q35_u32x4*)p;
+template <bool kStream, class V>
+Q35_DEV V ldg_if(const void* p) {
+  if constexpr (kStream) return __builtin_nontemporal_load((const Q35_GLOBAL V*)p);
+  else return *(const Q35_GLOBAL V*)p;
 }
 // os: the queries' operands, then the waves' outputs [wave][row][kFewLd]
 template <int DT, bool kStream>
 Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, float* os, float (&ms)[4][kFewRows],
                      float (&ls)[4][kFewRows]) {
   typedef typename Elt<DT>::T E;
-  constexpr bool kWide = DT == Q35_F32;
-  constexpr int kQ = kWide ? 1 : DT == Q35_F16 ? 2 : 3;  // parts of a query or weight
+  constexpr bool kWide = DT == Q35_F32, k4 = DT == Q35_Q4, kHalf = DT == Q35_F16 || k4;
+  constexpr int kQ = kWide ? 1 : kHalf ? 2 : 3;  // parts of a query or weight
   constexpr int kW = kWide ? 2 : 1;                       // 16-byte words of 8 values
   constexpr int kH = kWide ? 1 : 2, kS = 16 * kH;          // keys of a wave's step
   const PagedAttn& a = A.c;
@@ -512,31 +609,46 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
     const int lim = t.p0 + tok;   // the last token the lane's row sees (rows past the last one repeat it)
     const int end = t.p0 + t.n;   // tokens from here on do not exist
     const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
-    const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
+    const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts<DT>(a) + (int64_t)gk * a.P.page * kRow<DT>;
     // pages of the step's 16-key halves
     auto pages = [&](int j0, int& pa, int& pb) {
       pa = page_of(A, row, j0, &bad);
       pb = kH == 1 || a.P.page > 16 || j0 + 16 >= end ? pa : page_of(A, row, j0 + 16, &bad);
     };
-    q35_u32x4 kr[kH][8 * kW], vr[4 * kH][2 * kW];
+    q35_u32x4 kr[kH][k4 ? 2 : 8 * kW], vr[k4 ? 1 : 4 * kH][2 * kW];
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    u2 vc[k4 ? 8 : 1];               // 4 bits: codes of 16 dims of each key
+    uint32_t kw[2], vw[k4 ? 8 : 1];  // and words: of the two groups of a key's 64 dims, of a key's 16 dims
     auto load_k = [&](int j0, int pa, int pb) {
 #pragma unroll
       for (int hf = 0; hf < kH; ++hf) {
         const int slot = (j0 + 16 * hf + n) & (a.P.page - 1);
-        const E* p = base + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * g;
+        const E* p = base + (int64_t)(hf ? pb : pa) * page_elts<DT>(a) + (int64_t)slot * kRow<DT>;
+        if constexpr (k4) {
+          kr[hf][0] = ldg_if<kStream, q35_u32x4>(p + 32 * g);
+          kr[hf][1] = ldg_if<kStream, q35_u32x4>(p + 32 * g + 16);
+          kw[hf] = ldg_if<kStream, uint32_t>(p + kHd / 2 + 4 * g);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8 * kW; ++i) kr[hf][i] = ldg16_if<kStream>(p + (kWide ? 16 : 32) * i);
+          for (int i = 0; i < 8 * kW; ++i) kr[hf][i] = ldg_if<kStream, q35_u32x4>(p + (kWide ? 4 : 8) * g + (kWide ? 16 : 32) * i);
+        }
       }
     };
     auto load_v = [&](int j0, int pa, int pb) {
 #pragma unroll
       for (int hf = 0; hf < kH; ++hf) {
         const int slot = (j0 + 16 * hf + 4 * g) & (a.P.page - 1);  // 4 keys of one page
-        const E* p = base + plane_elts(a) + (int64_t)(hf ? pb : pa) * page_elts(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * n;
+        const E* p = base + plane_elts<DT>(a) + (int64_t)(hf ? pb : pa) * page_elts<DT>(a) + (int64_t)slot * kRow<DT>;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (k4) {
+            vc[4 * hf + j] = ldg_if<kStream, u2>(p + j * kRow<DT> + 8 * n);
+            vw[4 * hf + j] = ldg_if<kStream, uint16_t>(p + j * kRow<DT> + kHd / 2 + 2 * (n >> 1));
+          } else {
 #pragma unroll
-          for (int w = 0; w < 2 * kW; ++w) vr[4 * hf + j][w] = ldg16_if<kStream>(p + j * kHd + w * (128 / kW));
+            for (int w = 0; w < 2 * kW; ++w) vr[4 * hf + j][w] = ldg_if<kStream, q35_u32x4>(p + j * kHd + (kWide ? 4 : 8) * n + w * (128 / kW));
+          }
+        }
       }
     };
     // queries: column n; dims 32 st + 8 g .. (16-bit), 16 st + 4 g .. (f32); each wave lays out a quarter.  They are
@@ -546,9 +658,11 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
     f4 qv[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      qv[i] = *(const Q35_GLOBAL f4*)(A.q + qi * kHd + (kWide ? 16 * (4 * wid + i) + 4 * g : 32 * (2 * wid + (i >> 1)) + 8 * g + 4 * (i & 1)));
+      qv[i] = *(const Q35_GLOBAL f4*)(A.q + qi * kHd + (kWide ? 16 * (4 * wid + i) + 4 * g
+                                                          : k4 ? 64 * g + 8 * (2 * wid + (i >> 1)) + 4 * (i & 1)
+                                                               : 32 * (2 * wid + (i >> 1)) + 8 * g + 4 * (i & 1)));
     float qm = 0.f;
-    if constexpr (DT == Q35_F16) qm = A.qmax[qi];
+    if constexpr (kHalf) qm = A.qmax[qi];
     int j0 = k0 * kUnit + wid * kS, pa = 0, pb = 0;
     const int j1 = min(k1 * kUnit, end);
     if (j0 < j1) {
@@ -559,7 +673,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
     float qscale = sl2;
     {
       float fq = 1.f;
-      if constexpr (DT == Q35_F16) {  // a power of two per query brings its largest value to 2^14
+      if constexpr (kHalf) {  // a power of two per query brings its largest value to 2^14
         float inv;
         split_scale(qm, fq, inv);
         qscale = sl2 * inv;
@@ -576,7 +690,8 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             uint32_t p0, p1, p2 = 0;
-            if constexpr (DT == Q35_F16) split2_near(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
+            if constexpr (k4) split2_near(v[j] * fq, v[j + 4] * fq, p0, p1);  // (values8's order)
+            else if constexpr (kHalf) split2_near(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
             else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
             qb[0][j] = p0;
             qb[1][j] = p1;
@@ -607,6 +722,16 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             sc[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[0][st][e]), __uint_as_float(qv[e]), sc[e & 1], 0, 0, 0);
+        } else if constexpr (k4) {
+          q35_u32x4 kv[2];
+#pragma unroll
+          for (int hf = 0; hf < kH; ++hf) kv[hf] = values8(kr[hf][st >> 2][st & 3], word2(__builtin_amdgcn_perm(kw[hf], kw[hf], st < 4 ? 0x01000100u : 0x03020302u)));
+#pragma unroll
+          for (int q = 0; q < kQ; ++q) {
+            const q35_u32x4 qv = qs[(q * 8 + st) * 64 + lane];
+#pragma unroll
+            for (int hf = 0; hf < kH; ++hf) sc[hf] = mma<DT>(kv[hf], qv, sc[hf]);
+          }
         } else {
 #pragma unroll
           for (int q = 0; q < kQ; ++q) {
@@ -636,7 +761,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
         m = mn;
       }
       // f16 weights are kept 2^12 times larger (at most 4096), so that their halves hold 22 bits down to 2^-26
-      const float mr = (m == -INFINITY ? 0.f : m) - (DT == Q35_F16 ? 12.f : 0.f);
+      const float mr = (m == -INFINITY ? 0.f : m) - (kHalf ? 12.f : 0.f);
       q35_u32x4 pw[kQ];
 #pragma unroll
       for (int j = 0; j < 4 * kH; ++j) {
@@ -648,7 +773,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
         for (int j = 0; j < 4; ++j) {
           const float p0 = sc[j >> 1][2 * (j & 1)], p1 = sc[j >> 1][2 * (j & 1) + 1];
           uint32_t w0, w1, w2 = 0;
-          if constexpr (DT == Q35_F16) split2_near(p0, p1, w0, w1);
+          if constexpr (kHalf) split2_near(p0, p1, w0, w1);
           else split3(p0, p1, w0, w1, w2);
           pw[0][j] = w0;
           if constexpr (kQ > 1) pw[1][j] = w1;
@@ -659,10 +784,34 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
 #pragma unroll
         for (int j = 0; j < 4 * kH; ++j)
           if (j0 + 16 * (j >> 2) + 4 * g + (j & 3) >= end) {
+            if constexpr (k4) {
+              vw[j] = 0;
+            } else {
 #pragma unroll
-            for (int w = 0; w < 2 * kW; ++w) vr[j][w] = q35_u32x4{0, 0, 0, 0};
+              for (int w = 0; w < 2 * kW; ++w) vr[j][w] = q35_u32x4{0, 0, 0, 0};
+            }
           }
       }
+      // 4 bits: tile i: dims 16 (4 g + r) + i in register r
+      if constexpr (k4) {
+        Word2 w2[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w2[j] = word2(vw[2 * j] | vw[2 * j + 1] << 16);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          q35_u32x4 v[2];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {  // byte b of both keys: dims 2 b and 2 b + 1
+            const uint32_t t = __builtin_amdgcn_perm(vc[2 * j + 1][b >> 2], vc[2 * j][b >> 2], 0x0c040c00u + (b & 3) * 0x00010001u);
+            v[0][j] = low_nibbles(t, w2[j]);
+            v[1][j] = high_nibbles(t, w2[j]);
+          }
+#pragma unroll
+          for (int q = 0; q < kQ; ++q)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) o[2 * b + i] = mma<DT>(v[i], pw[q], o[2 * b + i]);
+        }
+      } else
       // tile i = w (8 / kW) + e: dims w (128 / kW) + (8 / kW) (4 g + r) + e in register r
 #pragma unroll
       for (int w = 0; w < 2 * kW; ++w) {
@@ -697,7 +846,13 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
     __syncthreads();  // (the queries' operands are done with)
     l = add_x32(add_x16(l));
     if (n < rows) {
-      float* dst = os + (wid * kFewRows + n) * kFewLd + (8 / kW) * 4 * g;
+      float* dst = os + (wid * kFewRows + n) * kFewLd + (k4 ? 64 * g : (8 / kW) * 4 * g);
+      if constexpr (k4) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) *(f4*)(dst + 16 * r + i) = f4{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]};
+      } else
 #pragma unroll
       for (int w = 0; w < 2 * kW; ++w)
 #pragma unroll
@@ -763,7 +918,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
 // of 16384 shared tokens 161 and 240; 54 tiles over 229 MB 40 and 53.)
 template <int DT>
 Q35_DEV bool past_llc(const PlanHead& H, int64_t once) {
-  return H.w > (int64_t)(256u << 20) / (kUnit * 2 * kHd * (DT == Q35_F32 ? 4 : 2)) && 8 * (H.w - once) < H.w;
+  return H.w > (int64_t)(256u << 20) / (kUnit * 2 * kRow<DT> * (int)sizeof(typename Elt<DT>::T)) && 8 * (H.w - once) < H.w;
 }
 
 template <int DT>
@@ -828,7 +983,7 @@ Q35_DEV void split2_scaled(uint32_t y0, uint32_t y1, float f, uint32_t& hi, uint
 template <int DT>
 __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_many_kernel(const AttnArgs A) {
   typedef typename Elt<DT>::T E;
-  constexpr bool kWide = DT == Q35_F32;
+  constexpr bool kWide = DT == Q35_F32, k4 = DT == Q35_Q4;
   constexpr int kQ = DT == Q35_BF16 ? 3 : 2;  // parts of a query or weight
   constexpr int kKV = kWide ? 2 : 1;          // parts of a key or value
   // how far (log2) a score may pass the running maximum before the sums are rescaled: f16 weights
@@ -866,24 +1021,41 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int lim1 = t.p0 + tok0 + div_rep(A, min(wid * kRowsW + kRowsW - 1, rows - 1));
     const int end = t.p0 + min(tok0 + A.tok_many, t.n);  // no row of the tile sees tokens from here on
     const int32_t* row = a.table + (int64_t)t.b * a.ld_table;
-    const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts(a) + (int64_t)gk * a.P.page * kHd;
+    const E* base = static_cast<const E*>(a.P.data) + (int64_t)a.layer * a.P.n_pages * page_elts<DT>(a) + (int64_t)gk * a.P.page * kRow<DT>;
     // staging registers: keys 4 wid + 2 i + hf, dims 8 n32 ..; values: keys 4 wid + i, dims 4 lane ..
-    q35_u32x4 kr[2][kKV];
-    typedef typename std::conditional<kWide, q35_u32x4, u2>::type VW;
+    typedef typename std::conditional<k4, uint32_t, q35_u32x4>::type KW;
+    KW kr[2][kKV];
+    typedef typename std::conditional<kWide, q35_u32x4, typename std::conditional<k4, uint32_t, u2>::type>::type VW;
     VW vr[4];
+    uint32_t kwd[2] = {}, vwd[4] = {};  // 4 bits: their words
     auto unit_page = [&](int k) {  // of the wave's 4 keys
       const int j0 = k * kUnit + 4 * wid;
       return page_of(A, row, j0 < end ? j0 : k * kUnit, &bad);
     };
     auto load_unit = [&](int k, int pg) {
       const int j0 = k * kUnit + 4 * wid;
-      const E* p = base + (int64_t)pg * page_elts(a) + (int64_t)(j0 & (a.P.page - 1)) * kHd;
+      const E* p = base + (int64_t)pg * page_elts<DT>(a) + (int64_t)(j0 & (a.P.page - 1)) * kRow<DT>;
+      if constexpr (k4) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 2; ++i) {
+          const E* r = p + (2 * i + hf) * kRow<DT>;
+          kr[i][0] = *(const Q35_GLOBAL uint32_t*)(r + 4 * n32);
+          kwd[i] = *(const Q35_GLOBAL uint16_t*)(r + kHd / 2 + 2 * (n32 >> 2));
+        }
 #pragma unroll
-        for (int w = 0; w < kKV; ++w) kr[i][w] = *((const Q35_GLOBAL q35_u32x4*)(p + (2 * i + hf) * kHd + 8 * n32) + w);
+        for (int i = 0; i < 4; ++i) {
+          const E* r = p + plane_elts<DT>(a) + i * kRow<DT>;
+          vr[i] = *(const Q35_GLOBAL uint16_t*)(r + 2 * lane);
+          vwd[i] = *(const Q35_GLOBAL uint16_t*)(r + kHd / 2 + 2 * (lane >> 3));
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) vr[i] = *(const Q35_GLOBAL VW*)(p + plane_elts(a) + i * kHd + 4 * lane);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int w = 0; w < kKV; ++w) kr[i][w] = *((const Q35_GLOBAL q35_u32x4*)(p + (2 * i + hf) * kHd + 8 * n32) + w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vr[i] = *(const Q35_GLOBAL VW*)(p + plane_elts<DT>(a) + i * kHd + 4 * lane);
+      }
     };
     float vinv = 0.f;  // f32 caches: the power of two that brings the largest value so far to 2^14, its inverse
     auto store_unit = [&](int k, int buf) {
@@ -891,12 +1063,16 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           if (k * kUnit + 4 * wid + 2 * i + hf >= end) {
+            kwd[i] = 0;
 #pragma unroll
-            for (int w = 0; w < kKV; ++w) kr[i][w] = q35_u32x4{0, 0, 0, 0};
+            for (int w = 0; w < kKV; ++w) kr[i][w] = KW(0);
           }
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (k * kUnit + 4 * wid + i >= end) vr[i] = VW(0);
+          if (k * kUnit + 4 * wid + i >= end) {
+            vr[i] = VW(0);
+            vwd[i] = 0;
+          }
       }
       char* kb = lds + buf * 2 * kKV * kPlane;
       char* vb = kb + kKV * kPlane;
@@ -946,6 +1122,8 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           }
           *(q35_u32x4*)dst = hi;
           *(q35_u32x4*)(dst + kPlane) = lo;
+        } else if constexpr (k4) {
+          *(q35_u32x4*)dst = values8(kr[i][0], word2(kwd[i] * 0x00010001u));
         } else {
           *(q35_u32x4*)dst = kr[i][0];
         }
@@ -960,6 +1138,10 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           split2_scaled(vr[2][e], vr[3][e], fv, b0, b1);
           *(u2*)dst = u2{a0, b0};
           *(u2*)(dst + kPlane) = u2{a1, b1};
+        } else if constexpr (k4) {
+          const uint32_t c0 = (vr[0] | vr[1] << 16) >> (e & 2) * 4, c1 = (vr[2] | vr[3] << 16) >> (e & 2) * 4;
+          const Word2 w0 = word2(vwd[0] | vwd[1] << 16), w1 = word2(vwd[2] | vwd[3] << 16);
+          *(u2*)dst = e & 1 ? u2{high_nibbles(c0, w0), high_nibbles(c1, w1)} : u2{low_nibbles(c0, w0), low_nibbles(c1, w1)};
         } else {
           const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
           *(u2*)dst = u2{__builtin_amdgcn_perm(vr[1][e >> 1], vr[0][e >> 1], sel), __builtin_amdgcn_perm(vr[3][e >> 1], vr[2][e >> 1], sel)};
@@ -995,7 +1177,8 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           uint32_t p0, p1, p2 = 0;
-          if constexpr (kQ == 2) split2_near(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
+          if constexpr (k4) split2_near(v[j] * fq, v[j + 4] * fq, p0, p1);  // (values8's order)
+          else if constexpr (kQ == 2) split2_near(v[2 * j] * fq, v[2 * j + 1] * fq, p0, p1);
           else split3(v[2 * j], v[2 * j + 1], p0, p1, p2);
           qb[0][st][j] = p0;
           qb[1][st][j] = p1;
@@ -1319,7 +1502,7 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
 template <int DT>
 int launch(const PagedAttn& a, hipStream_t st) {
   const int64_t ctx = std::min<int64_t>((int64_t)a.ld_table * a.P.page, a.rope_rows);
-  const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B, ctx * elt_size(a.P.dtype));
+  const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B, ctx * row_bytes(a.P) / kHd);
   AttnArgs A;
   A.c = a;
   A.page_shift = __builtin_ctz((unsigned)a.P.page);
@@ -1375,7 +1558,12 @@ int launch(const PagedAttn& a, hipStream_t st) {
 size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) { return paged_layout(nh, nkv, T, B, INT64_MAX).bytes; }
 
 int paged_attn_launch(const PagedAttn& a, hipStream_t st) {
-  return a.P.dtype == Q35_F32 ? launch<Q35_F32>(a, st) : a.P.dtype == Q35_F16 ? launch<Q35_F16>(a, st) : launch<Q35_BF16>(a, st);
+  switch (a.P.dtype) {
+    case Q35_F32: return launch<Q35_F32>(a, st);
+    case Q35_F16: return launch<Q35_F16>(a, st);
+    case Q35_Q4: return launch<Q35_Q4>(a, st);
+    default: return launch<Q35_BF16>(a, st);
+  }
 }
 
 }  // namespace q35

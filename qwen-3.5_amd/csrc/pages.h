@@ -16,12 +16,16 @@ constexpr int kPageMaxRep = 16;         // query heads per kv head
 constexpr int kMaxLds = 150 * 1024;     // dynamic LDS that the kernels here ask for at most
 constexpr int kMaxTop = 64;             // alternatives per row of token_logprobs
 
+constexpr int kQ4Row = kPageHd / 2 + kPageHd / 16;  // bytes of a Q35_Q4 row: codes, a word per 32 values
+
 inline int elt_size(int dtype) { return dtype == Q35_F32 ? 4 : 2; }
 
-// bytes of one page of one layer
-inline size_t page_bytes(const q35_pages& P) {
-  return (size_t)2 * P.kv_heads * P.page * P.head_dim * elt_size(P.dtype);
+// bytes that one token of one head has in a plane
+__host__ __device__ inline int row_bytes(const q35_pages& P) {
+  return P.dtype == Q35_Q4 ? kQ4Row : P.head_dim * (P.dtype == Q35_F32 ? 4 : 2);
 }
+// bytes of one page of one layer
+__host__ __device__ inline size_t page_bytes(const q35_pages& P) { return (size_t)2 * P.kv_heads * P.page * row_bytes(P); }
 
 // Lets a kernel's launches use more than 64 KB of dynamic LDS; asked once per kernel and device (the call
 // takes as long as a third of a launch).
@@ -43,6 +47,15 @@ int status_clear_launch(uint32_t* status, uint32_t bits, hipStream_t st);
 
 int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t* sid, const int32_t* did, int n,
                       uint32_t* status, uint8_t* ok, hipStream_t st);
+
+struct ReadCall {
+  q35_pages P;
+  const int32_t *table, *row, *pos;
+  int32_t layer, ld, B, n;
+  void* out;
+  uint32_t* status;
+};
+int pages_read_launch(const ReadCall& c, hipStream_t st);
 
 struct ForkCall {
   q35_pages P;

@@ -14,13 +14,17 @@ namespace q35 {
 namespace {
 
 constexpr int kCT = 256;        // threads of a copying block
-constexpr int kUnit = 16384;    // bytes a block copies at a time: 4 x 16 bytes per thread (the smallest page)
+constexpr int kUnit = 16384;    // bytes a block copies at a time: 4 x 16 bytes per thread (a page's last unit may have fewer)
 constexpr int kPT = 1024;       // threads of a bookkeeping block
 constexpr int kPW = kPT / 64;
 
-// by kCT threads, thread t of them
-Q35_DEV void copy_unit(char* dst, const char* src, int t) {
+// The `bytes` (a multiple of 16, kUnit at most) of a unit, by kCT threads, thread t of them
+Q35_DEV void copy_unit(char* dst, const char* src, int t, int64_t bytes) {
   const int o = t * 16;
+  if (bytes < kUnit) {
+    for (int i = o; i < bytes; i += 16 * kCT) *reinterpret_cast<uint4*>(dst + i) = ldg16_nt(src + i);
+    return;
+  }
   uint4 v[kUnit / (16 * kCT)];
 #pragma unroll
   for (int i = 0; i < kUnit / (16 * kCT); ++i) v[i] = ldg16_nt(src + o + i * 16 * kCT);
@@ -69,7 +73,7 @@ __global__ __launch_bounds__(kCT) void pages_copy_kernel(const CopyArgs a) {
     return;
   }
   const int64_t o = (int64_t)u * kUnit;
-  copy_unit(a.dst + layer * a.dst_layer + d * a.page + o, a.src + layer * a.src_layer + s * a.page + o, threadIdx.x);
+  copy_unit(a.dst + layer * a.dst_layer + d * a.page + o, a.src + layer * a.src_layer + s * a.page + o, threadIdx.x, a.page - o);
 }
 
 // ok[i] for many pairs: bitmaps of the pages that are a source, a destination, a destination twice.
@@ -97,6 +101,39 @@ __global__ __launch_bounds__(kPT) void pages_copy_check_kernel(const CopyArgs a,
     }
     ok[i] = good ? 1 : 0;
   }
+}
+
+// ---- rows as values
+// A wave per (token, plane and head), 4 values a lane.  Bound by its round trips (ids, table, row): 2.5 us for 33 tokens.
+__global__ __launch_bounds__(kCT) void pages_read_kernel(const ReadCall c) {
+  const int lane = threadIdx.x & 63, planes = 2 * c.P.kv_heads;
+  const int64_t item = (int64_t)blockIdx.x * (kCT / 64) + (threadIdx.x >> 6), i = item / planes;
+  if (i >= c.n) return;
+  const int ph = (int)(item - i * planes), b = c.row[i], p = c.pos[i];
+  int page = -1;
+  if ((uint32_t)b < (uint32_t)c.B && p >= 0 && p < (int64_t)c.ld * c.P.page) page = c.table[(int64_t)b * c.ld + p / c.P.page];
+  const bool ok = (uint32_t)page < (uint32_t)c.P.n_pages;
+  if (!ok && lane == 0) raise_status(c.status, Q35_STATUS_ARG);
+  const int rb = row_bytes(c.P);
+  const char* r = static_cast<const char*>(c.P.data);
+  if (ok) r += ((int64_t)c.layer * c.P.n_pages + page) * (int64_t)page_bytes(c.P) + ((int64_t)ph * c.P.page + (p & (c.P.page - 1))) * rb;
+  if (c.P.dtype == Q35_F32) {
+    const uint4 v = ok ? reinterpret_cast<const uint4*>(r)[lane] : make_uint4(0, 0, 0, 0);
+    reinterpret_cast<uint4*>(c.out)[item * 64 + lane] = v;
+    return;
+  }
+  uint2 v = make_uint2(0, 0);
+  if (ok && c.P.dtype != Q35_Q4) v = reinterpret_cast<const uint2*>(r)[lane];
+  if (ok && c.P.dtype == Q35_Q4) {
+    const uint32_t code = reinterpret_cast<const uint16_t*>(r)[lane], word = reinterpret_cast<const uint16_t*>(r + kPageHd / 2)[lane >> 3];
+    const float s = (float)__builtin_bit_cast(_Float16, (uint16_t)(word & 0xFFF0u));
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      h[j] = __builtin_bit_cast(uint16_t, (_Float16)(s * (float)((int)(code >> (4 * j) & 15) - (int)(word & 15))));
+    v = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+  }
+  reinterpret_cast<uint2*>(c.out)[item * 64 + lane] = v;
 }
 
 // ---- block-wide helpers of the bookkeeping kernels
@@ -158,7 +195,7 @@ Q35_DEV int fork_parent(const ForkCall& c, int j, int* n, bool* bad) {
 // outside the pool are left alone
 Q35_DEV void copy_tail(const ForkCall& c, int part, int src, int dst, int tail, int nt) {
   if (src == dst || (uint32_t)src >= (uint32_t)c.P.n_pages || (uint32_t)dst >= (uint32_t)c.P.n_pages) return;
-  const int rb = c.P.head_dim * (c.P.dtype == Q35_F32 ? 4 : 2), planes = 2 * c.P.kv_heads;
+  const int rb = row_bytes(c.P), planes = 2 * c.P.kv_heads;
   const int64_t head = (int64_t)c.P.page * rb, pb = head * planes;
   const int layer = part / planes, ph = part - layer * planes;
   char* base = static_cast<char*>(c.P.data) + (int64_t)layer * c.P.n_pages * pb + ph * head;
@@ -373,7 +410,7 @@ Q35_DEV void copy_move(const CompactCall& c, const int32_t* holes, const int32_t
   const int u = (int)(e % units), layer = (int)(e / units % c.P.n_layers);
   const int m = (int)(e / units / c.P.n_layers);
   char* base = static_cast<char*>(c.P.data) + (int64_t)layer * c.P.n_pages * pb + (int64_t)u * kUnit;
-  copy_unit(base + holes[m] * pb, base + movers[m] * pb, t);
+  copy_unit(base + holes[m] * pb, base + movers[m] * pb, t, pb - (int64_t)u * kUnit);
 }
 // kOne: as pages_fork_kernel's; the lists of moves stay in LDS.  514 MB read and written in 101 us, 5.1 TB/s (HBM); a
 // small pool 5.6 us (round trips).  Larger tables are one block's, a load of a thread at a time, each entry twice: 33
@@ -454,7 +491,7 @@ constexpr int kOneCopies = 4;  // per CU
 int check_pages(const q35_pages& P, const char* what) {
   auto no = [&](int code, const char* why) { return fail(code, std::string(what) + why); };
   if (!P.data) return no(Q35_E_ARG, ": null pool");
-  if (P.dtype != Q35_F32 && P.dtype != Q35_F16 && P.dtype != Q35_BF16) return no(Q35_E_ARG, ": bad pool dtype");
+  if (P.dtype != Q35_F32 && P.dtype != Q35_F16 && P.dtype != Q35_BF16 && P.dtype != Q35_Q4) return no(Q35_E_ARG, ": bad pool dtype");
   if (P.head_dim != kPageHd) return no(Q35_E_SHAPE, ": head_dim must be 256");
   if (P.page < 16 || P.page > 256 || (P.page & (P.page - 1)) != 0)
     return no(Q35_E_SHAPE, ": tokens per page must be a power of two in 16..256");
@@ -483,7 +520,7 @@ int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t*
   a.dst_pages = dst.n_pages;
   a.same = src.data == dst.data;
   a.n = n;
-  a.units = (int)(pb / kUnit);
+  a.units = (int)((pb + kUnit - 1) / kUnit);
   a.sid = sid;
   a.did = did;
   a.status = status;
@@ -496,6 +533,13 @@ int pages_copy_launch(const q35_pages& src, const q35_pages& dst, const int32_t*
     a.ok = ok;
   }
   hipLaunchKernelGGL(pages_copy_kernel, dim3(n * a.units, src.n_layers), dim3(kCT), 0, st, a);
+  Q35_HIP_TRY(hipGetLastError());
+  return Q35_OK;
+}
+
+int pages_read_launch(const ReadCall& c, hipStream_t st) {
+  const int64_t items = (int64_t)c.n * 2 * c.P.kv_heads;
+  hipLaunchKernelGGL(pages_read_kernel, dim3((uint32_t)((items + kCT / 64 - 1) / (kCT / 64))), dim3(kCT), 0, st, c);
   Q35_HIP_TRY(hipGetLastError());
   return Q35_OK;
 }
@@ -521,7 +565,7 @@ int pages_fork_launch(const ForkCall& c, hipStream_t st) {
 int pages_compact_launch(const CompactCall& c, hipStream_t st) {
   const int words = (c.P.n_pages + 31) / 32;
   const int64_t pb = (int64_t)page_bytes(c.P);
-  const int units = (int)(pb / kUnit);
+  const int units = (int)((pb + kUnit - 1) / kUnit);
   // at most half of the pages move
   const int64_t most = (int64_t)(c.P.n_pages / 2) * c.P.n_layers * units;
   const int64_t ne = (int64_t)c.B * c.ld;

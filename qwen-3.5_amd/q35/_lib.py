@@ -14,7 +14,7 @@ Q35_OK, Q35_E_SHAPE, Q35_E_ALIGN, Q35_E_HIP, Q35_E_ARG, Q35_E_WS, Q35_E_NOMEM, Q
 Q35_KN, Q35_NK, Q35_KN_TILED, Q35_KN_PANEL, Q35_KN_MB = 0, 1, 2, 3, 4
 Q35_LAUNCH_STREAM, Q35_LAUNCH_GRAPH, Q35_LAUNCH_PERSISTENT = 0, 1, 2
 Q35_PREFILL_GEMM = 0x100
-Q35_F32, Q35_F16, Q35_BF16 = 0, 1, 2
+Q35_F32, Q35_F16, Q35_BF16, Q35_Q4 = 0, 1, 2, 4
 Q35_STATUS_ARG, Q35_STATUS_FULL = 1, 2
 Q35_MB_PLAIN, Q35_MB_RMS, Q35_MB_GATED, Q35_MB_SWIGLU = 0, 1, 2, 3
 ERROR_NAMES = {1: "Q35_E_SHAPE", 2: "Q35_E_ALIGN", 3: "Q35_E_HIP", 4: "Q35_E_ARG", 5: "Q35_E_WS", 6: "Q35_E_NOMEM",
@@ -100,6 +100,7 @@ PROTOTYPES = {
                                                 c_i32, c_vp, c_vp, c_sz, c_vp]),
     "q35_pages_copy_ws_bytes": (c_sz, [c_i32]),
     "q35_pages_copy": (ctypes.c_int, [Pages, Pages, c_vp, c_vp, c_i32, c_vp, c_vp, c_sz, c_vp]),
+    "q35_pages_read": (ctypes.c_int, [Pages, c_i32, c_vp, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
     "q35_pages_fork": (ctypes.c_int, [Pages, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
     "q35_pages_compact_ws_bytes": (c_sz, [c_i32]),
     "q35_pages_compact": (ctypes.c_int, [Pages, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),

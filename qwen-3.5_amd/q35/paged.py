@@ -3,6 +3,7 @@ contexts (beam search, several samples of a prompt, drafted tokens, prompt chunk
 sequences).  No counterparts in the reference, which decodes one sequence greedily.
 
   attention_core_paged  attention_core_prefill / _decode for any mix of sequences over a PagePool
+  pages_read            what a pool holds of given tokens, as values
   pages_fork            the next page table: forked, dropped, freed and reserved sequences
   pages_copy            pages copied within a pool or between two
   pages_compact         the pages in use moved to the pool's front
@@ -28,6 +29,8 @@ from . import _lib as L
 from .kernels import _stream
 
 _DTYPES = {torch.float32: L.Q35_F32, torch.float16: L.Q35_F16, torch.bfloat16: L.Q35_BF16}
+Q4 = "q4"       # the dtype of a pool in 4 bits
+_Q4_ROW = 144   # bytes that it has for a token of a head: 256 codes, a 16-bit word for each 32
 _HERE = contextlib.nullcontext()
 
 PagesFork = collections.namedtuple("PagesFork", "table lens refs")
@@ -62,20 +65,31 @@ def _score_ws_bytes(M, V, top):
 class PagePool:
     """Pages of the attention layers' caches: data [n_layers, n_pages, 2, kv_heads, page, 256] in float32,
     float16 or bfloat16 (plane 0 the keys after norm and rotary, plane 1 the values); page a power of
-    two in 16..256.  Who owns which page is the page tables' matter (int32 [B, entries], -1 none)."""
+    two in 16..256.  Who owns which page is the page tables' matter (int32 [B, entries], -1 none).
+
+    A pool in 4 bits (dtype=q35.Q4) has uint8 rows of 144 bytes instead of 256 values: 256 codes and a 16-bit word (a scale
+    and a zero) for each 32 of them, as include/q35.h lays them out: 28% of a 16-bit pool's bytes, and each value off by
+    about 1/30 of its 32 values' range at most.  pages_read gives rows as values."""
 
     def __init__(self, data):
-        assert data.dim() == 6 and data.shape[2] == 2 and data.is_contiguous() and data.dtype in _DTYPES, \
+        q4 = data.dtype is torch.uint8
+        assert data.dim() == 6 and data.shape[2] == 2 and data.is_contiguous() and (data.dtype in _DTYPES or q4), \
             (tuple(data.shape), data.dtype)
+        assert not q4 or data.shape[5] == _Q4_ROW, tuple(data.shape)
         assert data.device.type == "cuda", "the pool must be on the GPU"
         self.data = data
         self.n_layers, self.n_pages, _, self.kv_heads, self.page, self.head_dim = data.shape
+        if q4:
+            self.head_dim = 256
         self.status = torch.zeros(1, dtype=torch.int32, device=data.device)
-        self._desc = L.Pages(data.data_ptr(), _DTYPES[data.dtype], self.n_layers, self.n_pages, self.kv_heads, self.page,
-                             self.head_dim)
+        self._desc = L.Pages(data.data_ptr(), L.Q35_Q4 if q4 else _DTYPES[data.dtype], self.n_layers, self.n_pages, self.kv_heads,
+                             self.page, self.head_dim)
 
     @classmethod
     def empty(cls, n_layers, n_pages, kv_heads=2, page=64, head_dim=256, dtype=torch.float32, device="cuda"):
+        if dtype is Q4:
+            assert head_dim == 256, head_dim
+            head_dim, dtype = _Q4_ROW, torch.uint8
         return cls(torch.empty((n_layers, n_pages, 2, kv_heads, page, head_dim), dtype=dtype, device=device))
 
     def desc(self):
@@ -144,6 +158,22 @@ def pages_copy(pool, src, dst, to=None, check=False):
                                        _ptr(ws), n, _stream()))
     if check:
         to.check()
+
+
+def pages_read(pool, layer, table, rows, pos, check=False):
+    """The keys and values that layer `layer` of the cache holds of n tokens: [n, 2, kv_heads, 256] for position pos[i] of
+    sequence rows[i] of table (int32), in the pool's type, float16 for a pool in 4 bits (exactly the values that it
+    stands for).  What is out of range gives zeros; check=True raises for it."""
+    (B, width), n = table.shape, rows.shape[0]
+    table, rows, pos = _ints(table, B, width), _ints(rows, n), _ints(pos, n)
+    with _on(pool.data, table, rows, pos):
+        out = torch.empty((n, 2, pool.kv_heads, pool.head_dim), device=table.device,
+                          dtype=torch.float16 if pool.data.dtype is torch.uint8 else pool.data.dtype)
+        L.check(L.lib().q35_pages_read(pool.desc(), layer, table.data_ptr(), width, B, rows.data_ptr(), pos.data_ptr(), n,
+                                       out.data_ptr(), pool.status.data_ptr(), _stream()))
+    if check:
+        pool.check()
+    return out
 
 
 def pages_fork(pool, table, lens, parents, grow=None, check=False):
