@@ -442,6 +442,39 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
                        int32_t top, float* logprob, int32_t* rank, float* entropy, int32_t* top_ids,
                        float* top_logprobs, uint32_t* status, void* ws, size_t ws_bytes, void* stream);
 
+/* The next beams of R groups of W beams.  Beam w of group g has score scores[g W + w] (a sum of log probabilities) and the
+ * logits of row g W + w of logits [R W][ld] (as q35_token_logprobs's); its continuation by token v scores
+ * scores[g W + w] + x[v] - ln sum e^x.  Of all continuations of a group the k (1..64) with the highest scores go, highest first,
+ * to scores_out, parents (the row g W + w, as q35_pages_fork and q35_states_fork take it) and tokens, all [R][k]; among
+ * equal ones the lowest row first, then the lowest token.
+ *   ended (int32 [R W], NULL: none): a beam with ended[row] >= 0 has ended: its only continuation is that token, at its score
+ *   as it is, and its logits are not read; a token >= V leaves it without one (Q35_STATUS_ARG).
+ * A beam whose score is not finite is dead: it has no continuation and its logits are not read (an empty slot; all but the
+ * first of a group in its first step).  Logits of -inf are never chosen, nor is any of a row with a NaN or +inf.  Where a
+ * group has fewer than k continuations the rest is score -inf, parent -1, token -1: an empty row of the next
+ * tables, a dead beam of the next step.
+ * Scores are formed in f64, from exponentials in f32 (an error of about 10^-8 in ln sum e^x), and rounded once.
+ * W <= 256, W V < 2^32, R W < 2^24, V <= 2^30; no output overlaps an input.  ws: q35_beam_select_ws_bytes bytes of scratch,
+ * 16-byte aligned. */
+size_t q35_beam_select_ws_bytes(int32_t R, int32_t W, int32_t V, int32_t k);
+int q35_beam_select(const void* logits, int32_t dtype, int32_t R, int32_t W, int32_t V, int64_t ld, const float* scores,
+                    const int32_t* ended, int32_t k, float* scores_out, int32_t* parents, int32_t* tokens,
+                    uint32_t* status, void* ws, size_t ws_bytes, void* stream);
+
+/* What q35_pages_fork does to pages, for states that are one row per sequence (conv_state, recurrent_state, contiguous
+ * caches, histories): row j of each of n states (host array) becomes what row parent[j] of it was, j < B_out.  A state's rows
+ * lie src_stride / dst_stride bytes apart and have row_bytes bytes (contiguous).  In place (every state's dst is its src, one
+ * stride) or into other buffers (no dst overlaps any src; all states alike).  parent -1 leaves row j of dst as it is; one
+ * outside [-1, B) counts as -1 (Q35_STATUS_ARG).  In place only rows that change are touched.  States of one call do not overlap each other; src has
+ * B rows and dst B_out (in place: the larger number of both).  B, B_out <= 4096. */
+typedef struct {
+  const void* src;
+  void* dst;
+  int64_t src_stride, dst_stride, row_bytes;
+} q35_state;
+int q35_states_fork(const q35_state* states_host, int32_t n, const int32_t* parent, int32_t B, int32_t B_out,
+                    uint32_t* status, void* stream);
+
 /* ---------------------------------------------------------------- model level (model.rs, main.rs) */
 
 typedef struct q35_model q35_model;

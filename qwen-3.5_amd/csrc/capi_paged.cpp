@@ -229,4 +229,64 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
   });
 }
 
+size_t q35_beam_select_ws_bytes(int32_t R, int32_t W, int32_t V, int32_t k) {
+  if (R < 1 || W < 1 || W > kMaxBeams || V < 1 || V > (1 << 30) || (int64_t)R * W >= kMaxGrid || (int64_t)W * V >= (1ll << 32) || k < 1 || k > kMaxTop) return 0;
+  return beam_ws_bytes(R, W, V, k);
+}
+
+int q35_beam_select(const void* logits, int32_t dtype, int32_t R, int32_t W, int32_t V, int64_t ld, const float* scores,
+                    const int32_t* ended, int32_t k, float* scores_out, int32_t* parents, int32_t* tokens,
+                    uint32_t* status, void* ws, size_t ws_bytes, void* stream) {
+  return entry([&]() -> int {
+    if (!logits || !scores || !scores_out || !parents || !tokens) return fail(Q35_E_ARG, "beam_select: null pointer");
+    if (dtype != Q35_F32 && dtype != Q35_F16 && dtype != Q35_BF16) return fail(Q35_E_ARG, "beam_select: bad dtype");
+    if (k < 1 || k > kMaxTop) return fail(Q35_E_SHAPE, "beam_select: k must be in 1..64");
+    const size_t need = q35_beam_select_ws_bytes(R, W, V, k);
+    if (need == 0 || ld < V) return fail(Q35_E_SHAPE, "beam_select: 1..256 beams, R W < 2^24, 1 <= V <= 2^30, W V < 2^32 and ld >= V required");
+    if (!aligned(logits, elt_size(dtype))) return fail(Q35_E_ALIGN, "beam_select: logits not aligned to their type");
+    if (!ws || ws_bytes < need) return fail(Q35_E_WS, "beam_select: workspace too small");
+    if (!aligned(ws, 16)) return fail(Q35_E_ALIGN, "beam_select: workspace not 16-byte aligned");
+    const size_t n = (size_t)R * W * 4, o = (size_t)R * k * 4;
+    const void* outs[3] = {scores_out, parents, tokens};
+    for (int i = 0; i < 3; ++i) {
+      if (overlap(outs[i], o, scores, n) || (ended && overlap(outs[i], o, ended, n)) ||
+          overlap(outs[i], o, logits, ((size_t)(R * W - 1) * ld + V) * elt_size(dtype)) || overlap(outs[i], o, outs[(i + 1) % 3], o))
+        return fail(Q35_E_ARG, "beam_select: outputs must be buffers of their own");
+    }
+    BeamCall c;
+    c.x = logits; c.dtype = dtype; c.R = R; c.W = W; c.V = V; c.k = k; c.ld = ld;
+    c.scores = scores; c.ended = ended;
+    c.scores_out = scores_out; c.parents = parents; c.tokens = tokens;
+    c.status = status;
+    c.ws = ws;
+    return beam_launch(c, S(stream));
+  });
+}
+
+int q35_states_fork(const q35_state* states, int32_t n, const int32_t* parent, int32_t B, int32_t B_out, uint32_t* status,
+                    void* stream) {
+  return entry([&]() -> int {
+    if (n < 0 || B < 1 || B > kPageMaxSeqs || B_out < 0 || B_out > kPageMaxSeqs)
+      return fail(Q35_E_SHAPE, "states_fork: n >= 0 and rows in 1..4096 required");
+    if (n == 0 || B_out == 0) return Q35_OK;
+    if (!states || !parent) return fail(Q35_E_ARG, "states_fork: null pointer");
+    int full = 0;  // (the first state that has anything)
+    while (full < n - 1 && states[full].row_bytes == 0) ++full;
+    const bool copies = states[full].src != states[full].dst;
+    for (int i = 0; i < n; ++i) {
+      const q35_state& s = states[i];
+      if (s.row_bytes == 0) continue;
+      if (!s.src || !s.dst) return fail(Q35_E_ARG, "states_fork: null pointer");
+      if (s.row_bytes < 0 || s.row_bytes > (1ll << 40) || s.src_stride < s.row_bytes || s.dst_stride < s.row_bytes ||
+          s.src_stride > (1ll << 44) || s.dst_stride > (1ll << 44))
+        return fail(Q35_E_SHAPE, "states_fork: rows of at least row_bytes apart required");
+      if ((s.src != s.dst) != copies) return fail(Q35_E_ARG, "states_fork: all states in place, or none");
+      if (!copies && s.src_stride != s.dst_stride) return fail(Q35_E_ARG, "states_fork: in place with two strides");
+      if (copies && overlap(s.src, (size_t)(B - 1) * s.src_stride + s.row_bytes, s.dst, (size_t)(B_out - 1) * s.dst_stride + s.row_bytes))
+        return fail(Q35_E_ARG, "states_fork: source and destination overlap");
+    }
+    return states_fork_launch(states, n, parent, B, B_out, copies, status, S(stream));
+  });
+}
+
 }  // extern "C"

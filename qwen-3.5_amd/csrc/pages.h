@@ -1,4 +1,4 @@
-// Paged caches and token scores: calls between the C ABI (capi_paged.cpp) and the kernels.
+// Paged caches, token scores, beams: calls between the C ABI (capi_paged.cpp) and the kernels.
 #pragma once
 #include <atomic>
 
@@ -14,7 +14,8 @@ constexpr int kPageFewPairs = 256;      // pairs of a copy that its blocks check
 constexpr int kPageMaxHeads = 1024;     // query heads
 constexpr int kPageMaxRep = 16;         // query heads per kv head
 constexpr int kMaxLds = 150 * 1024;     // dynamic LDS that the kernels here ask for at most
-constexpr int kMaxTop = 64;             // alternatives per row of token_logprobs
+constexpr int kMaxTop = 64;             // alternatives per row of token_logprobs, continuations per group of beam_select
+constexpr int kMaxBeams = 256;          // of a group
 
 constexpr int kQ4Row = kPageHd / 2 + kPageHd / 16;  // bytes of a Q35_Q4 row: codes, a word per 32 values
 
@@ -104,6 +105,24 @@ struct ScoreCall {
 };
 size_t token_logprobs_ws_bytes(int M, int V, int top);
 int token_logprobs_launch(const ScoreCall& c, hipStream_t st);
+
+struct BeamCall {
+  const void* x;
+  int32_t dtype, R, W, V, k;
+  int64_t ld;
+  const float* scores;
+  const int32_t* ended;
+  float* scores_out;
+  int32_t *parents, *tokens;
+  uint32_t* status;
+  void* ws;
+};
+size_t beam_ws_bytes(int R, int W, int V, int k);
+int beam_launch(const BeamCall& c, hipStream_t st);
+
+// states: host; copies: dst is not src
+int states_fork_launch(const q35_state* states, int n, const int32_t* parent, int B, int Bo, bool copies, uint32_t* status,
+                       hipStream_t st);
 
 Q35_DEV void raise_status(uint32_t* status, uint32_t bit) {
   if (status) __hip_atomic_fetch_or((Q35_GLOBAL uint32_t*)status, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

@@ -37,6 +37,10 @@ class Dims(ctypes.Structure):
         return {n: getattr(self, n) for n, _ in self._fields_}
 
 
+class State(ctypes.Structure):
+    _fields_ = [("src", c_vp), ("dst", c_vp)] + [(n, ctypes.c_int64) for n in ("src_stride", "dst_stride", "row_bytes")]
+
+
 class Pages(ctypes.Structure):
     _fields_ = [("data", c_vp)] + [(n, c_i32) for n in ("dtype", "n_layers", "n_pages", "kv_heads", "page", "head_dim")]
 
@@ -102,6 +106,10 @@ PROTOTYPES = {
     "q35_pages_copy": (ctypes.c_int, [Pages, Pages, c_vp, c_vp, c_i32, c_vp, c_vp, c_sz, c_vp]),
     "q35_pages_read": (ctypes.c_int, [Pages, c_i32, c_vp, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp]),
     "q35_pages_fork": (ctypes.c_int, [Pages, c_vp, c_i32, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp]),
+    "q35_beam_select_ws_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32]),
+    "q35_beam_select": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, ctypes.c_int64, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
+                                       c_sz, c_vp]),
+    "q35_states_fork": (ctypes.c_int, [ctypes.POINTER(State), c_i32, c_vp, c_i32, c_i32, c_vp, c_vp]),
     "q35_pages_compact_ws_bytes": (c_sz, [c_i32]),
     "q35_pages_compact": (ctypes.c_int, [Pages, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "q35_token_logprobs_ws_bytes": (c_sz, [c_i32, c_i32, c_i32]),

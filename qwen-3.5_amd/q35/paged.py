@@ -7,6 +7,8 @@ sequences).  No counterparts in the reference, which decodes one sequence greedi
   pages_fork            the next page table: forked, dropped, freed and reserved sequences
   pages_copy            pages copied within a pool or between two
   pages_compact         the pages in use moved to the pool's front
+  states_fork           the same for states that are one row per sequence
+  beam_select           the next beams: the highest continuations of each group of beams
   token_logprobs        log probabilities, ranks, entropy and the highest alternatives of logits
 
     pool = q35.PagePool.empty(6, 4096)
@@ -35,6 +37,7 @@ _HERE = contextlib.nullcontext()
 
 PagesFork = collections.namedtuple("PagesFork", "table lens refs")
 PagesCompact = collections.namedtuple("PagesCompact", "table refs used")
+BeamSelect = collections.namedtuple("BeamSelect", "scores parents tokens")
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprob rank entropy top_ids top_logprobs")
 
 
@@ -60,6 +63,11 @@ def _ptr(t):
 @functools.lru_cache(maxsize=1024)
 def _score_ws_bytes(M, V, top):
     return L.lib().q35_token_logprobs_ws_bytes(M, V, top)
+
+
+@functools.lru_cache(maxsize=1024)
+def _beam_ws_bytes(G, W, V, k):
+    return L.lib().q35_beam_select_ws_bytes(G, W, V, k)
 
 
 class PagePool:
@@ -254,3 +262,76 @@ def token_logprobs(logits, targets=None, top=0, check=False):
         if check:
             L.check(L.lib().q35_status_check(status.data_ptr(), _stream()))
     return res
+
+
+def beam_select(logits, scores, k, ended=None, check=False):
+    """The next beams of G groups of W beams: logits [G, W, V] or [G * W, V] (float32, float16 or bfloat16), scores float32
+    [G, W].  Of a group's continuations (beam w, token v), which score scores[g, w] + logits[g, w, v] - logsumexp of the
+    row, the k highest: BeamSelect(scores float32, parents int32, tokens int32), all [G, k], highest first; among equal ones the
+    lowest beam, then the lowest token.  parents are rows of the G * W, as pages_fork and states_fork take them.
+    ended (int32 [G * W] or [G, W]; None: none): a beam with ended >= 0 goes on as it is, with that token.  A beam whose score
+    is not finite has no continuation; a group with fewer than k is filled up with score -inf, parent -1, token -1.
+    check=True synchronises and raises Q35Error (Q35_E_RANGE) for an ended token >= V, which leaves its beam without a
+    continuation."""
+    G, W = scores.shape
+    V = logits.shape[-1]
+    dtype, dev, f32, i32 = _DTYPES.get(logits.dtype), logits.device, torch.float32, torch.int32
+    assert dtype is not None, logits.dtype
+    assert scores.dtype is f32, scores.dtype
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    assert x.shape[0] == G * W, (tuple(logits.shape), tuple(scores.shape))
+    if x.stride(1) != 1 or x.stride(0) < V:
+        x = x.contiguous()
+    scores = scores if scores.is_contiguous() else scores.contiguous()
+    if ended is not None:
+        ended = _ints(ended, *((G, W) if ended.dim() == 2 else (G * W,)))
+    with _on(x, scores, ended):
+        res = BeamSelect(torch.empty(G, k, dtype=f32, device=dev), torch.empty(G, k, dtype=i32, device=dev),
+                         torch.empty(G, k, dtype=i32, device=dev))
+        if G == 0:
+            return res
+        status = torch.zeros(1, dtype=i32, device=dev) if check else None
+        nbytes = _beam_ws_bytes(G, W, V, k)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        L.check(L.lib().q35_beam_select(x.data_ptr(), dtype, G, W, V, x.stride(0) if G * W > 1 else V, scores.data_ptr(), _ptr(ended), k,
+                                        res.scores.data_ptr(), res.parents.data_ptr(), res.tokens.data_ptr(), _ptr(status), ws.data_ptr(),
+                                        nbytes, _stream()))
+        if check:
+            L.check(L.lib().q35_status_check(status.data_ptr(), _stream()))
+    return res
+
+
+def states_fork(states, parents, out=None, check=False):
+    """Row j of every tensor of `states` becomes what its row parents[j] was (int32 [B_out]; -1: row j stays), in place, or in
+    the tensors of `out` (of the same rows, B_out of them).  The tensors [B, ...] have any type and a contiguous row; their rows
+    may lie apart (a slice of a cache's tokens).  In place B_out is at most B.  The tensors must not overlap each other.
+    Returns the tensors written.  check=True raises Q35Error (Q35_E_RANGE) for a parent outside [-1, B), which counts as -1."""
+    states = list(states)
+    dst = states if out is None else list(out)
+    assert len(dst) == len(states), (len(dst), len(states))
+    Bo = parents.shape[0]
+    parents = _ints(parents, Bo)
+    if not states:
+        return dst
+    B = states[0].shape[0]
+    desc = (L.State * len(states))()
+    for e, s, d in zip(desc, states, dst):
+        row, size = s.shape[1:], s.element_size()
+        assert s.shape[0] == B, "states of different rows"
+        assert d.dtype is s.dtype and d.shape[1:] == row and d.shape[0] >= Bo, (tuple(s.shape), tuple(d.shape), Bo)
+        n = row.numel() * size
+        e.src, e.dst, e.row_bytes, e.src_stride, e.dst_stride = s.data_ptr(), d.data_ptr(), n, _row_stride(s, n), _row_stride(d, n)
+    with _on(parents, *states, *(dst if out is not None else ())):
+        status = torch.zeros(1, dtype=torch.int32, device=parents.device) if check else None
+        L.check(L.lib().q35_states_fork(desc, len(states), parents.data_ptr(), B, Bo, _ptr(status), _stream()))
+        if check:
+            L.check(L.lib().q35_status_check(status.data_ptr(), _stream()))
+    return dst
+
+
+def _row_stride(t, row_bytes):
+    """Bytes between the rows of t, whose own values must be contiguous."""
+    if t.is_contiguous():
+        return row_bytes
+    assert t.shape[0] > 0 and t[0].is_contiguous() and t.stride(0) * t.element_size() >= row_bytes, (tuple(t.shape), t.stride())
+    return t.stride(0) * t.element_size()
