@@ -346,12 +346,22 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 Q35_DEV uint32_t value2(uint32_t c, uint32_t n, uint32_t s) {
   return __builtin_bit_cast(uint32_t, (h2)((__builtin_bit_cast(h2, c) + __builtin_bit_cast(h2, n)) * __builtin_bit_cast(h2, s)));
 }
-Q35_DEV uint32_t low_nibbles(uint32_t t, const Word2& w) { return value2((t & 0x000F000Fu) | 0x64006400u, w.n0, w.s); }
-Q35_DEV uint32_t high_nibbles(uint32_t t, const Word2& w) { return value2((t & 0x00F000F0u) | 0x54005400u, w.n4, w.s); }
+// The masks in scalar registers and the exponents in vector ones: one instruction ands and ors then (constants would be
+// literals of two).
+struct Nibbles {
+  uint32_t m0, m4, e0, e4;
+};
+Q35_DEV Nibbles nibbles() {
+  Nibbles c = {0x000F000Fu, 0x00F000F0u, 0x64006400u, 0x54005400u};
+  asm("" : "+s"(c.m0), "+s"(c.m4), "+v"(c.e0), "+v"(c.e4));
+  return c;
+}
+Q35_DEV uint32_t low_nibbles(uint32_t t, const Word2& w, const Nibbles& c) { return value2((t & c.m0) | c.e0, w.n0, w.s); }
+Q35_DEV uint32_t high_nibbles(uint32_t t, const Word2& w, const Nibbles& c) { return value2((t & c.m4) | c.e4, w.n4, w.s); }
 // 8 values (one dword of codes) as operands: values p and p + 4 in the halves of word p
-Q35_DEV q35_u32x4 values8(uint32_t c, const Word2& w) {
-  const uint32_t d = c >> 8;
-  return q35_u32x4{low_nibbles(c, w), high_nibbles(c, w), low_nibbles(d, w), high_nibbles(d, w)};
+Q35_DEV q35_u32x4 values8(uint32_t t, const Word2& w, const Nibbles& c) {
+  const uint32_t d = t >> 8;
+  return q35_u32x4{low_nibbles(t, w, c), high_nibbles(t, w, c), low_nibbles(d, w, c), high_nibbles(d, w, c)};
 }
 
 // Keys and values of the new tokens into their pages, and the normalised, rotated queries (with each one's
@@ -574,11 +584,15 @@ Q35_DEV void split2_near(float y0, float y1, uint32_t& hi, uint32_t& lo) {
 }
 constexpr int kFewLd = kHd + 4;
 constexpr int kFewLds = 4 * kFewRows * kFewLd * 4;
+// 4 bits: the queries' operands, then each wave's rows: keys of 16 tokens, of 16 more, and their values
+constexpr int kQ4Half = 16 * kQ4Row;
+constexpr int kQ4Rows = 2 * 8 * 64 * 16;
+static_assert(kQ4Rows + 4 * 4 * kQ4Half <= kFewLds);
 
-template <bool kStream, class V>
-Q35_DEV V ldg_if(const void* p) {
-  if constexpr (kStream) return __builtin_nontemporal_load((const Q35_GLOBAL V*)p);
-  else return *(const Q35_GLOBAL V*)p;
+template <bool kStream>
+Q35_DEV q35_u32x4 ldg_if(const void* p) {
+  if constexpr (kStream) return __builtin_nontemporal_load((const Q35_GLOBAL q35_u32x4*)p);
+  else return *(const Q35_GLOBAL q35_u32x4*)p;
 }
 // os: the queries' operands, then the waves' outputs [wave][row][kFewLd]
 template <int DT, bool kStream>
@@ -597,6 +611,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
   q35_u32x4* const qs = reinterpret_cast<q35_u32x4*>(os);  // [part][step][lane]
+  const Nibbles nib = nibbles();
   bool bad = false;
 #pragma unroll 1
   for (int seg = 0; u < u_end; ++seg) {
@@ -615,41 +630,44 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
       pa = page_of(A, row, j0, &bad);
       pb = kH == 1 || a.P.page > 16 || j0 + 16 >= end ? pa : page_of(A, row, j0 + 16, &bad);
     };
-    q35_u32x4 kr[kH][k4 ? 2 : 8 * kW], vr[k4 ? 1 : 4 * kH][2 * kW];
-    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    u2 vc[k4 ? 8 : 1];               // 4 bits: codes of 16 dims of each key
-    uint32_t kw[2], vw[k4 ? 8 : 1];  // and words: of the two groups of a key's 64 dims, of a key's 16 dims
+    q35_u32x4 kr[k4 ? 1 : kH][8 * kW], vr[k4 ? 1 : 4 * kH][2 * kW];
     auto load_k = [&](int j0, int pa, int pb) {
 #pragma unroll
       for (int hf = 0; hf < kH; ++hf) {
         const int slot = (j0 + 16 * hf + n) & (a.P.page - 1);
-        const E* p = base + (int64_t)(hf ? pb : pa) * page_elts<DT>(a) + (int64_t)slot * kRow<DT>;
-        if constexpr (k4) {
-          kr[hf][0] = ldg_if<kStream, q35_u32x4>(p + 32 * g);
-          kr[hf][1] = ldg_if<kStream, q35_u32x4>(p + 32 * g + 16);
-          kw[hf] = ldg_if<kStream, uint32_t>(p + kHd / 2 + 4 * g);
-        } else {
+        const E* p = base + (int64_t)(hf ? pb : pa) * page_elts<DT>(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * g;
 #pragma unroll
-          for (int i = 0; i < 8 * kW; ++i) kr[hf][i] = ldg_if<kStream, q35_u32x4>(p + (kWide ? 4 : 8) * g + (kWide ? 16 : 32) * i);
-        }
+        for (int i = 0; i < 8 * kW; ++i) kr[hf][i] = ldg_if<kStream>(p + (kWide ? 16 : 32) * i);
       }
     };
     auto load_v = [&](int j0, int pa, int pb) {
 #pragma unroll
       for (int hf = 0; hf < kH; ++hf) {
         const int slot = (j0 + 16 * hf + 4 * g) & (a.P.page - 1);  // 4 keys of one page
-        const E* p = base + plane_elts<DT>(a) + (int64_t)(hf ? pb : pa) * page_elts<DT>(a) + (int64_t)slot * kRow<DT>;
+        const E* p = base + plane_elts<DT>(a) + (int64_t)(hf ? pb : pa) * page_elts<DT>(a) + (int64_t)slot * kHd + (kWide ? 4 : 8) * n;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if constexpr (k4) {
-            vc[4 * hf + j] = ldg_if<kStream, u2>(p + j * kRow<DT> + 8 * n);
-            vw[4 * hf + j] = ldg_if<kStream, uint16_t>(p + j * kRow<DT> + kHd / 2 + 2 * (n >> 1));
-          } else {
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int w = 0; w < 2 * kW; ++w) vr[4 * hf + j][w] = ldg_if<kStream, q35_u32x4>(p + j * kHd + (kWide ? 4 : 8) * n + w * (128 / kW));
-          }
-        }
+          for (int w = 0; w < 2 * kW; ++w) vr[4 * hf + j][w] = ldg_if<kStream>(p + j * kHd + w * (128 / kW));
       }
+    };
+    // 4 bits: the rows of 16 tokens are one run of 2304 bytes, which passes LDS: read piece by piece into the
+    // operands' places, every line was asked for three times, and the L1 waited for it half of the time (33 tokens over
+    // 400 MB 104 us, %s so).  st[8]: the runs' last 256 bytes, a quarter of the wave each.
+    q35_u32x4 st[9];
+    char* const rows_lds = reinterpret_cast<char*>(os) + kQ4Rows + wid * 4 * kQ4Half;
+    auto load_rows = [&](int j0, int pa, int pb) {
+      const E* ka = base + (int64_t)pa * page_elts<DT>(a) + (int64_t)(j0 & (a.P.page - 1)) * kRow<DT>;
+      const E* kb = base + (int64_t)pb * page_elts<DT>(a) + (int64_t)((j0 + 16) & (a.P.page - 1)) * kRow<DT>;
+      const E* from[4] = {ka, kb, ka + plane_elts<DT>(a), kb + plane_elts<DT>(a)};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) st[i] = ldg_if<kStream>(from[i >> 1] + (i & 1) * 1024 + 16 * lane);
+      st[8] = ldg_if<kStream>((g < 2 ? g == 0 ? from[0] : from[1] : g == 2 ? from[2] : from[3]) + 2048 + 16 * n);
+    };
+    auto store_rows = [&]() {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *(q35_u32x4*)(rows_lds + (i >> 1) * kQ4Half + (i & 1) * 1024 + 16 * lane) = st[i];
+      *(q35_u32x4*)(rows_lds + g * kQ4Half + 2048 + 16 * n) = st[8];
     };
     // queries: column n; dims 32 st + 8 g .. (16-bit), 16 st + 4 g .. (f32); each wave lays out a quarter.  They are
     // asked for first: loads arrive in order, and the operands can be laid out while keys and values are under way
@@ -667,8 +685,12 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
     const int j1 = min(k1 * kUnit, end);
     if (j0 < j1) {
       pages(j0, pa, pb);
-      load_k(j0, pa, pb);
-      load_v(j0, pa, pb);
+      if constexpr (k4) {
+        load_rows(j0, pa, pb);
+      } else {
+        load_k(j0, pa, pb);
+        load_v(j0, pa, pb);
+      }
     }
     float qscale = sl2;
     {
@@ -713,6 +735,30 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
     auto step = [&](auto more) {
       constexpr bool kMore = decltype(more)::value;
       if constexpr (kMore) pages(j0 + 4 * kS, pa, pb);
+      typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+      q35_u32x4 kc[2][2];  // 4 bits: a key's 64 codes and two words, 8 keys' 16 codes and word
+      u2 vc[8];
+      uint32_t kw[2], vw[8];
+      if constexpr (k4) {
+        wave_lds_sync();  // (the last step's reads)
+        store_rows();
+        if constexpr (kMore) load_rows(j0 + 4 * kS, pa, pb);
+        asm volatile("" ::: "memory");
+        wave_lds_sync();
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const char* r = rows_lds + hf * kQ4Half + n * kQ4Row;
+          kc[hf][0] = *(const q35_u32x4*)(r + 32 * g);
+          kc[hf][1] = *(const q35_u32x4*)(r + 32 * g + 16);
+          kw[hf] = *(const uint32_t*)(r + kHd / 2 + 4 * g);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const char* r = rows_lds + (2 + (j >> 2)) * kQ4Half + (4 * g + (j & 3)) * kQ4Row;
+          vc[j] = *(const u2*)(r + 8 * n);
+          vw[j] = *(const uint16_t*)(r + kHd / 2 + 2 * (n >> 1));
+        }
+      }
       f4 sc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       // (two sums in turn, the halves' or even and odd dims': a product does not wait for the one before it)
 #pragma unroll
@@ -725,7 +771,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
         } else if constexpr (k4) {
           q35_u32x4 kv[2];
 #pragma unroll
-          for (int hf = 0; hf < kH; ++hf) kv[hf] = values8(kr[hf][st >> 2][st & 3], word2(__builtin_amdgcn_perm(kw[hf], kw[hf], st < 4 ? 0x01000100u : 0x03020302u)));
+          for (int hf = 0; hf < kH; ++hf) kv[hf] = values8(kc[hf][st >> 2][st & 3], word2(__builtin_amdgcn_perm(kw[hf], kw[hf], st < 4 ? 0x01000100u : 0x03020302u)), nib);
 #pragma unroll
           for (int q = 0; q < kQ; ++q) {
             const q35_u32x4 qv = qs[(q * 8 + st) * 64 + lane];
@@ -741,7 +787,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
           }
         }
       }
-      if constexpr (kMore) load_k(j0 + 4 * kS, pa, pb);
+      if constexpr (kMore && !k4) load_k(j0 + 4 * kS, pa, pb);
       asm volatile("" ::: "memory");
       if constexpr (kWide) sc[0] += sc[1];
       float bm = -INFINITY;
@@ -803,8 +849,8 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // byte b of both keys: dims 2 b and 2 b + 1
             const uint32_t t = __builtin_amdgcn_perm(vc[2 * j + 1][b >> 2], vc[2 * j][b >> 2], 0x0c040c00u + (b & 3) * 0x00010001u);
-            v[0][j] = low_nibbles(t, w2[j]);
-            v[1][j] = high_nibbles(t, w2[j]);
+            v[0][j] = low_nibbles(t, w2[j], nib);
+            v[1][j] = high_nibbles(t, w2[j], nib);
           }
 #pragma unroll
           for (int q = 0; q < kQ; ++q)
@@ -837,7 +883,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
           }
         }
       }
-      if constexpr (kMore) load_v(j0 + 4 * kS, pa, pb);
+      if constexpr (kMore && !k4) load_v(j0 + 4 * kS, pa, pb);
       asm volatile("" ::: "memory");
     };
 #pragma unroll 1
@@ -1005,6 +1051,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   Tile t = uniform(load_tile(&sh.t));
   int x = sh.x;
   const float sl2 = a.scale * 1.44269504088896341f;
+  const Nibbles nib = nibbles();
   bool bad = false;
   for (int seg = 0; u < u_end; ++seg) {
     int gk = 0;
@@ -1123,7 +1170,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           *(q35_u32x4*)dst = hi;
           *(q35_u32x4*)(dst + kPlane) = lo;
         } else if constexpr (k4) {
-          *(q35_u32x4*)dst = values8(kr[i][0], word2(kwd[i] * 0x00010001u));
+          *(q35_u32x4*)dst = values8(kr[i][0], word2(kwd[i] * 0x00010001u), nib);
         } else {
           *(q35_u32x4*)dst = kr[i][0];
         }
@@ -1141,7 +1188,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         } else if constexpr (k4) {
           const uint32_t c0 = (vr[0] | vr[1] << 16) >> (e & 2) * 4, c1 = (vr[2] | vr[3] << 16) >> (e & 2) * 4;
           const Word2 w0 = word2(vwd[0] | vwd[1] << 16), w1 = word2(vwd[2] | vwd[3] << 16);
-          *(u2*)dst = e & 1 ? u2{high_nibbles(c0, w0), high_nibbles(c1, w1)} : u2{low_nibbles(c0, w0), low_nibbles(c1, w1)};
+          *(u2*)dst = e & 1 ? u2{high_nibbles(c0, w0, nib), high_nibbles(c1, w1, nib)} : u2{low_nibbles(c0, w0, nib), low_nibbles(c1, w1, nib)};
         } else {
           const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
           *(u2*)dst = u2{__builtin_amdgcn_perm(vr[1][e >> 1], vr[0][e >> 1], sel), __builtin_amdgcn_perm(vr[3][e >> 1], vr[2][e >> 1], sel)};
