@@ -613,6 +613,13 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   q35_u32x4* const qs = reinterpret_cast<q35_u32x4*>(os);  // [part][step][lane]
   const Nibbles nib = nibbles();
   bool bad = false;
+  // 4 bits: unpacking bounds (830 instructions for 32 tokens, 130 of them for each of and / or, subtracting z and multiplying by s;
+  // with s z taken off the sums instead, 100 fewer, more registers and no faster).  Of a SIMD's two waves the older one then goes first, and the
+  // younger ends alone; a wave that is further through its steps has a lower priority (33 tokens over 400 MB 118.7
+  // -> 114.5 us of a call, 60 drafted tokens 56.0 -> 53.6).
+  const int quarter = max(1, (int)((u_end - u) >> 4));  // of a wave's steps
+  int left = 4 * quarter;
+  if constexpr (k4) __builtin_amdgcn_s_setprio(3);
 #pragma unroll 1
   for (int seg = 0; u < u_end; ++seg) {
     int gk = 0;
@@ -653,7 +660,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
     };
     // 4 bits: the rows of 16 tokens are one run of 2304 bytes, which passes LDS: read piece by piece into the
     // operands' places, every line was asked for three times, and the L1 waited for it half of the time (33 tokens over
-    // 400 MB 104 us, %s so).  st[8]: the runs' last 256 bytes, a quarter of the wave each.
+    // 400 MB 104 us, 94 so).  st[8]: the runs' last 256 bytes, a quarter of the wave each.
     q35_u32x4 st[9];
     char* const rows_lds = reinterpret_cast<char*>(os) + kQ4Rows + wid * 4 * kQ4Half;
     auto load_rows = [&](int j0, int pa, int pb) {
@@ -887,7 +894,15 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
       asm volatile("" ::: "memory");
     };
 #pragma unroll 1
-    for (; j0 + 4 * kS < j1; j0 += 4 * kS) step(std::true_type{});
+    for (; j0 + 4 * kS < j1; j0 += 4 * kS) {
+      if constexpr (k4) {
+        --left;
+        if (left == 3 * quarter) __builtin_amdgcn_s_setprio(2);
+        if (left == 2 * quarter) __builtin_amdgcn_s_setprio(1);
+        if (left == quarter) __builtin_amdgcn_s_setprio(0);
+      }
+      step(std::true_type{});
+    }
     if (j0 < j1) step(std::false_type{});
     __syncthreads();  // (the queries' operands are done with)
     l = add_x32(add_x16(l));
