@@ -18,8 +18,12 @@ namespace {
 
 constexpr int kT = 256;
 constexpr int kNW = kT / 64;
-constexpr int kMaxSplit = 256;
 constexpr int kJoinWaves = 16;
+constexpr int kBlocks = 4 * 256;  // that rows are cut into
+constexpr int kLiveMax = 4096;    // rows among which a block looks for the live ones
+constexpr int kMaxLists = 512;    // of a group
+constexpr int kListsLane = kMaxLists / 64;
+constexpr int kMaxCand = 512;     // that a group's choice ranks by comparing each with each
 
 struct alignas(16) Part {
   double s;
@@ -27,10 +31,17 @@ struct alignas(16) Part {
 };
 struct BeamArgs {
   BeamCall c;
-  int32_t nsplit, len;  // values per part
-  Part* part;           // [R W][nsplit]
-  key_t* keys;          // [R W][nsplit][k]
+  int32_t nsplit;  // parts per row; 0: the device decides, by the number of live rows (split_live)
+  int32_t most;    // parts per row at most, and that a row has room for
+  int32_t* live;   // live rows
+  Part* part;      // [row][most]
+  key_t* keys;     // [row][most][k]
 };
+// Parts of each of n live rows: enough to fill the chip, of one chunk per wave at least.
+__host__ __device__ inline int split_live(int n, int most) {
+  const int want = n > 0 ? kBlocks / n : 1;
+  return want < 1 ? 1 : want < most ? want : most;
+}
 
 // e^d for d <= 0, off by the hardware's 2^-23 at most whatever d
 Q35_DEV double exp_near(float d) {
@@ -70,6 +81,8 @@ Q35_DEV uint4 ldg16_any(const void* p) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
+// Blocks (row, part).  Bound by the stream for many rows (236 live rows of 248320 f32 values 52 us, 4.5 TB/s, the lists' first
+// chunks and the blocks' ends beside it), by round trips for few (4 rows 8.5 us).
 template <int DT>
 __global__ __launch_bounds__(kT) void beam_score_kernel(const BeamArgs a) {
   const BeamCall& c = a.c;
@@ -80,11 +93,41 @@ __global__ __launch_bounds__(kT) void beam_score_kernel(const BeamArgs a) {
   __shared__ double ss[kNW];
   __shared__ key_t block_last;
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
-  const int row_i = blockIdx.x / a.nsplit, sp = blockIdx.x % a.nsplit;
-  if (beam_state(c, row_i) != kLive) return;
+  int ns = a.nsplit, row_i;
+  if (ns > 0) {
+    row_i = blockIdx.x / ns;
+    if (beam_state(c, row_i) != kLive) return;
+  } else {
+    // Dead and ended rows leave their blocks to the others (a first step has one live beam of each group: 16 of 128 rows
+    // of 248320 f16 values 27 us in blocks of their own rows, 13.7 so).
+    __shared__ uint16_t live[kLiveMax];
+    __shared__ int count[kNW];
+    const int M = c.R * c.W;
+    int n = 0;
+    for (int r0 = 0; r0 < M; r0 += kT) {
+      const int r = r0 + tid;
+      const bool in = r < M && beam_state(c, r) == kLive;
+      const unsigned long long mask = __ballot(in);
+      if (lane == 0) count[wid] = __popcll(mask);
+      __syncthreads();
+      int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+#pragma unroll
+      for (int w = 0; w < kNW; ++w) {
+        at += w < wid ? count[w] : 0;
+        n += count[w];
+      }
+      if (in) live[at] = (uint16_t)r;
+      __syncthreads();
+    }
+    if (blockIdx.x == 0 && tid == 0) *a.live = n;
+    ns = split_live(n, a.most);
+    if ((int)(blockIdx.x / ns) >= n) return;
+    row_i = live[blockIdx.x / ns];
+  }
+  const int sp = blockIdx.x % ns, len = (c.V + ns - 1) / ns;
   constexpr int kEs = DT == Q35_F32 ? 4 : 2, kVec = 16 / kEs;
   const char* row = static_cast<const char*>(c.x) + (int64_t)row_i * c.ld * kEs;
-  const int i0 = sp * a.len, i1 = min(c.V, i0 + a.len);
+  const int i0 = min(c.V, sp * len), i1 = min(c.V, i0 + len);  // (a last part may be empty)
   const int top = c.k;
   constexpr int kWords = kPer / kVec;
   constexpr uint32_t kAll = (1u << kPer) - 1u;
@@ -148,7 +191,7 @@ __global__ __launch_bounds__(kT) void beam_score_kernel(const BeamArgs a) {
   }
   lists[wid][lane] = best;
   __syncthreads();
-  const int64_t slot = (int64_t)row_i * a.nsplit + sp;
+  const int64_t slot = (int64_t)row_i * a.most + sp;
   if (tid == 0) {
 #pragma unroll
     for (int w = 1; w < kNW; ++w) M = fmaxf(M, sm[w]);
@@ -203,43 +246,93 @@ Q35_DEV void insert_cand(Cand& best, Cand& last, const Cand& c, int top) {
   last = lane_cand(best, top - 1);
 }
 
-// Block per group.
+// The r-th largest of the wave's N values per lane without its lowest 12 bits; 0 if fewer than r are above 0.  (Two bits a
+// step, a score's 12 highest significant bits: each step waits for its counts; 32 steps of one took 3.6 us for 244 lists.)
+template <int N>
+Q35_DEV uint32_t nth_largest(const uint32_t (&v)[kListsLane], int r) {
+  uint32_t t = 0;
+#pragma unroll 1
+  for (int bit = 30; bit >= 12; bit -= 2) {
+    int n[3] = {0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+#pragma unroll
+      for (int e = 0; e < 3; ++e) n[e] += __popcll(__ballot(v[q] >= (t | (uint32_t)(e + 1) << bit)));
+    t |= (uint32_t)((n[0] >= r ? 1 : 0) + (n[1] >= r ? 1 : 0) + (n[2] >= r ? 1 : 0)) << bit;
+  }
+  return t;
+}
+
+// Block per group: the rows' logarithms, then the choice among the parts' lists.
+// If r lists have their 2^i-th continuation at or above f, and 2^i r >= k, nothing below f is chosen.  The
+// largest such f of all i (of scores as f32, which is monotonic) leaves little more than k continuations; those are
+// put into LDS, and each one's place is the number of those ahead of it.  Where many are equal and more are left than LDS
+// takes, the waves keep sorted lists instead.
+// Bound by round trips (live rows; sums and lists) and short serial steps: 11 us for 32 groups of 8 beams, with sorted
+// lists only 14.6; 6.9 for one group of 4.
 __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamArgs a) {
   const BeamCall& c = a.c;
   __shared__ double off[kMaxBeams];
   __shared__ int state[kMaxBeams];
-  __shared__ unsigned long long lhi[kJoinWaves][kMaxTop];
-  __shared__ uint32_t lix[kJoinWaves][kMaxTop];
-  __shared__ uint32_t bound;  // the highest f32 score, as bits in ascending order, that k continuations are known to reach
-  __shared__ int found[kJoinWaves];
+  __shared__ unsigned long long chi[kMaxCand];
+  __shared__ uint32_t cix[kMaxCand];
+  __shared__ uint32_t fl;
+  __shared__ int nc;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x / 64;
-  const int g = blockIdx.x, W = c.W, ns = a.nsplit, k = c.k, nl = W * ns;
+  const int g = blockIdx.x, W = c.W, k = c.k, most = a.most;
   const int64_t row0 = (int64_t)g * W;
-  constexpr int kAhead = 4;
-  const key_t* keys = a.keys + row0 * ns * k;
-  key_t pre[kAhead];
-  auto load = [&](int l, int j0) {
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) pre[e] = l < nl && j0 + e < k ? keys[(int64_t)l * k + j0 + e] : 0;
+  const key_t* keys = a.keys + row0 * most * k;
+  if (tid == 0) {
+    fl = 1;
+    nc = 0;
+  }
+  const int ns = a.nsplit > 0 ? a.nsplit : split_live(*a.live, most), nl = W * ns;
+  const int levels = 32 - __clz(k), nq = (nl + 63) / 64;
+  auto list = [&](int l, int& w, int& sp) {  // the keys of list l
+    w = l / ns;
+    sp = l - w * ns;
+    return keys + ((int64_t)w * most + sp) * k;
   };
-  load(wid * 64 + lane, 0);
-  if (tid == 0) bound = 0;
+  // Asked for together: the thread's list's first keys, the keys of the wave's level (of rows that are not live too:
+  // whatever the workspace holds, left aside below), and the sums.
+  constexpr int kFirst = 4;
+  key_t first[kFirst], level[kListsLane];
+  int my_w, my_sp;
+  const key_t* my_keys = list(min(tid, nl - 1), my_w, my_sp);
+#pragma unroll
+  for (int j = 0; j < kFirst; ++j) first[j] = tid < nl && j < k ? my_keys[j] : 0;
+  auto ask = [&](int i) {
+#pragma unroll
+    for (int q = 0; q < kListsLane; ++q) {
+      const int l = q * 64 + lane;
+      int w, sp;
+      level[q] = q < nq && l < nl ? list(l, w, sp)[(1 << i) - 1] : 0;
+    }
+  };
+  if (wid < levels) ask(wid);
+#pragma unroll 1
   for (int w = wid; w < W; w += nw) {
     const int row = (int)row0 + w, st = beam_state(c, row);
+    const Part* part = a.part + (int64_t)row * most;
+    const Part p0 = part[min(lane, ns - 1)];
     double o = c.scores[row];
     if (st == kLive) {
-      float m = -INFINITY;
-      for (int i = lane; i < ns; i += 64) m = fmaxf(m, a.part[(int64_t)row * ns + i].m);
-#pragma unroll
-      for (int e = 32; e > 0; e >>= 1) m = fmaxf(m, __shfl_xor(m, e, 64));
-      const float r = m == -INFINITY ? 0.f : m;
-      double S = 0.0;
-      for (int i = lane; i < ns; i += 64) {
-        const Part p = a.part[(int64_t)row * ns + i];
-        S += p.s * exp_near(p.m - r);
+      float m = lane < ns ? p0.m : -INFINITY;
+      double S = lane < ns ? p0.s : 0.0;
+#pragma unroll 1
+      for (int i = lane + 64; i < ns; i += 64) {
+        const Part p = part[i];
+        const float mn = fmaxf(m, p.m), r = mn == -INFINITY ? 0.f : mn;
+        S = S * exp_near(m - r) + p.s * exp_near(p.m - r);
+        m = mn;
       }
-#pragma unroll
-      for (int e = 32; e > 0; e >>= 1) S += __shfl_xor(S, e, 64);
+#pragma unroll 1
+      for (int e = 32; e > 0; e >>= 1) {
+        const float om = __shfl_xor(m, e, 64), mn = fmaxf(m, om), r = mn == -INFINITY ? 0.f : mn;
+        const double oS = __shfl_xor(S, e, 64);
+        S = S * exp_near(m - r) + oS * exp_near(om - r);
+        m = mn;
+      }
       // (NaN or +inf in the row: S is NaN; -inf alone: 0)
       o = S > 0.0 ? o - ((double)m + ln_near(S)) : -INFINITY;
     }
@@ -250,74 +343,110 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
     }
   }
   __syncthreads();
-  Cand best = {0, ~0u}, last = {0, ~0u};
-  bool seeded = false;
-  for (int l0 = wid * 64; l0 < nl; l0 += nw * 64) {
-    const int l = l0 + lane, w = l < nl ? l / ns : 0, sp = l - w * ns;
-    const int st = l < nl ? state[w] : kDead;
-    const double o = off[w];
-    if (l0 != wid * 64) load(l, 0);
-    for (int j0 = 0; j0 < k; j0 += kAhead) {
-      if (j0 > 0) load(l, j0);
-      bool more = true;
+  // continuation j of part sp of beam w, and its score's f32; 0: none
+  auto cand = [&](key_t key, int w, int sp, int j, Cand& x) {
+    const int st = state[w];
+    double s = -INFINITY;
+    uint32_t token = 0;
+    if (st == kLive && key != 0) {
+      s = off[w] + (double)from_asc((uint32_t)(key >> 32));
+      token = (uint32_t)key_index(key);
+    } else if (st == kEnded && sp == 0 && j == 0) {
+      s = off[w];
+      token = (uint32_t)c.ended[row0 + w];
+    }
+    const bool some = s > -INFINITY;
+    x = Cand{some ? asc64(s) : 0, (uint32_t)w * (uint32_t)c.V + token};
+    return some ? asc((float)s) : 0u;
+  };
+#pragma unroll 1
+  for (int i = wid; i < levels; i += nw) {
+    uint32_t v[kListsLane] = {};
+    const int j = (1 << i) - 1;
+    if (i != wid) ask(i);
 #pragma unroll
-      for (int e = 0; e < kAhead; ++e) {
-        const key_t key = pre[e];
-        double s = -INFINITY;
-        uint32_t ix = 0;
-        if (st == kLive && key != 0) {
-          s = o + (double)from_asc((uint32_t)(key >> 32));
-          ix = (uint32_t)w * (uint32_t)c.V + (uint32_t)key_index(key);
-        } else if (st == kEnded && sp == 0 && j0 + e == 0) {
-          s = o;
-          ix = (uint32_t)w * (uint32_t)c.V + (uint32_t)c.ended[row0 + w];
-        }
-        const bool some = s > -INFINITY;
-        const Cand x = {some ? asc64(s) : 0, ix};
-        const uint32_t a32 = some ? asc((float)s) : 0;
-        if (!seeded) {
-          // (float is monotonic: what is below the k-th largest of the lanes' floats is not among the k)
-          seeded = true;
-          const uint32_t t = (uint32_t)(seed_key(some ? (float)s : -INFINITY, k) >> 32) + 1u;
-          if (t > 1 && lane == 0) atomicMax(&bound, t);
-        }
-        const uint32_t b = __hip_atomic_load(&bound, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        unsigned long long take = __ballot(some && a32 >= b && ahead(x, last));
-        if (!take) {  // (lists fall: nothing behind these is wanted either)
-          more = false;
-          break;
-        }
-        for (; take; take &= take - 1) insert_cand(best, last, lane_cand(x, (int)__builtin_ctzll(take)), k);
-        if (last.hi != 0 && lane == 0) atomicMax(&bound, asc((float)from_asc64(last.hi)));
+    for (int q = 0; q < kListsLane; ++q) {
+      const int l = q * 64 + lane;
+      if (q < nq && l < nl) {
+        const int w = l / ns;
+        Cand x;
+        v[q] = cand(level[q], w, l - w * ns, j, x);
       }
-      if (!more) break;
     }
+    const int r = (k + j) >> i;
+    const uint32_t f = nq == 1 ? nth_largest<1>(v, r) : nq <= 4 ? nth_largest<4>(v, r) : nth_largest<kListsLane>(v, r);
+    if (lane == 0 && f > 1) atomicMax(&fl, f);
   }
-  if (lane < k) {
-    lhi[wid][lane] = best.hi;
-    lix[wid][lane] = best.ix;
-  }
-  const int have = __popcll(__ballot(best.hi != 0));
-  if (lane == 0) found[wid] = have;
   __syncthreads();
-  int all = 0;
-  for (int w = 0; w < nw; ++w) all += found[w];
-  if (lane < have) {
-    int place = lane;
-    for (int w = 0; w < nw; ++w) {
-      if (w == wid) continue;
-      int at = 0;
-      for (int step = 1 << (31 - __clz(k)); step > 0; step >>= 1)
-        if (at + step <= found[w] && ahead(Cand{lhi[w][at + step - 1], lix[w][at + step - 1]}, best)) at += step;
-      place += at;
+  const uint32_t floor32 = fl;
+  if (tid < nl) {
+#pragma unroll 1
+    for (int j = 0; j < k; ++j) {
+      const key_t key = j < kFirst ? first[0] : my_keys[j];
+      first[0] = first[1];
+      first[1] = first[2];
+      first[2] = first[3];
+      Cand x;
+      if (cand(key, my_w, my_sp, j, x) < floor32) break;  // (lists fall)
+      const int at = atomicAdd(&nc, 1);
+      if (at < kMaxCand) {
+        chi[at] = x.hi;
+        cix[at] = x.ix;
+      }
     }
-    if (place < k) {
-      const int64_t at = (int64_t)g * k + place;
-      const uint32_t w = best.ix / (uint32_t)c.V;
-      c.scores_out[at] = (float)from_asc64(best.hi);
-      c.parents[at] = (int32_t)(row0 + w);
-      c.tokens[at] = (int32_t)(best.ix - w * (uint32_t)c.V);
+  }
+  __syncthreads();
+  auto put = [&](const Cand& x, int place) {
+    const int64_t at = (int64_t)g * k + place;
+    const uint32_t w = x.ix / (uint32_t)c.V;
+    c.scores_out[at] = (float)from_asc64(x.hi);
+    c.parents[at] = (int32_t)(row0 + w);
+    c.tokens[at] = (int32_t)(x.ix - w * (uint32_t)c.V);
+  };
+  int all = nc;
+  if (all <= kMaxCand) {
+    for (int t = tid; t < all; t += blockDim.x) {
+      const Cand x = {chi[t], cix[t]};
+      int place = 0;
+      for (int e = 0; e < all; ++e) place += ahead(Cand{chi[e], cix[e]}, x) ? 1 : 0;
+      if (place < k) put(x, place);
     }
+  } else {
+    // lists by waves: sorted, then joined
+    __shared__ unsigned long long lhi[kJoinWaves][kMaxTop];
+    __shared__ uint32_t lix[kJoinWaves][kMaxTop];
+    Cand best = {0, ~0u}, last = {0, ~0u};
+#pragma unroll 1
+    for (int l0 = wid * 64; l0 < nl; l0 += nw * 64) {
+      int w, sp;
+      const key_t* held = list(min(l0 + lane, nl - 1), w, sp);
+#pragma unroll 1
+      for (int j = 0; j < k; ++j) {
+        Cand x = {0, ~0u};
+        const uint32_t a32 = l0 + lane < nl ? cand(held[j], w, sp, j, x) : 0;
+        unsigned long long take = __ballot(a32 >= floor32 && ahead(x, last));
+        if (!take) break;
+#pragma unroll 1
+        for (; take; take &= take - 1) insert_cand(best, last, lane_cand(x, (int)__builtin_ctzll(take)), k);
+      }
+    }
+    if (lane < k) {
+      lhi[wid][lane] = best.hi;
+      lix[wid][lane] = best.ix;
+    }
+    __syncthreads();
+    if (lane < k && best.hi != 0) {
+      int place = lane;
+#pragma unroll 1
+      for (int w = 0; w < nw; ++w) {
+        if (w == wid) continue;
+        int at = 0;
+        while (at < k && ahead(Cand{lhi[w][at], lix[w][at]}, best)) ++at;
+        place += at;
+      }
+      if (place < k) put(best, place);
+    }
+    all = k;  // (there are more)
   }
   for (int i = all + tid; i < k; i += blockDim.x) {
     const int64_t at = (int64_t)g * k + i;
@@ -327,36 +456,53 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
   }
 }
 
-// Parts per row: as token_logprobs's splits, enough to fill the chip when rows are few
-constexpr int kBlocks = 4 * 256;
-int beam_split(int M, int V) {
-  const int want = (kBlocks + M - 1) / M, most = std::min(kMaxSplit, (V + kNW * kChunk - 1) / (kNW * kChunk));
-  return std::max(1, std::min(want, most));
+struct BeamLayout {
+  int nsplit, most, blocks;  // nsplit 0: by the live rows
+  size_t live, part, keys;
+};
+BeamLayout beam_layout(int R, int W, int V, int k) {
+  const int M = R * W;
+  auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+  BeamLayout L;
+  L.most = std::max(1, std::min(kMaxLists / W, (V + kNW * kChunk - 1) / (kNW * kChunk)));
+  L.nsplit = split_live(M, L.most);
+  L.blocks = M * L.nsplit;
+  // (where all rows' parts are the smallest already, dead rows leave nothing to the others)
+  if (L.nsplit < L.most && M <= kLiveMax) {
+    L.nsplit = 0;
+    L.blocks = std::max(M, kBlocks);
+  }
+  if (L.nsplit > 0) L.most = L.nsplit;
+  L.live = L.nsplit == 0 ? 256 : 0;
+  L.part = up((size_t)M * L.most * sizeof(Part));
+  L.keys = (size_t)M * L.most * k * sizeof(key_t);
+  return L;
 }
-size_t part_bytes(int M, int ns) { return ((size_t)M * ns * sizeof(Part) + 255) & ~(size_t)255; }
 
 }  // namespace
 
 size_t beam_ws_bytes(int R, int W, int V, int k) {
-  const int ns = beam_split(R * W, V);
-  return part_bytes(R * W, ns) + (size_t)R * W * ns * k * sizeof(key_t);
+  const BeamLayout L = beam_layout(R, W, V, k);
+  return L.live + L.part + L.keys;
 }
 
 int beam_launch(const BeamCall& c, hipStream_t st) {
-  const int M = c.R * c.W;
+  const BeamLayout L = beam_layout(c.R, c.W, c.V, c.k);
   BeamArgs a;
   a.c = c;
-  a.nsplit = beam_split(M, c.V);
-  a.len = (c.V + a.nsplit - 1) / a.nsplit;
-  a.part = static_cast<Part*>(c.ws);
-  a.keys = reinterpret_cast<key_t*>(static_cast<char*>(c.ws) + part_bytes(M, a.nsplit));
-  const dim3 grid((uint32_t)M * a.nsplit);
+  a.nsplit = L.nsplit;
+  a.most = L.most;
+  char* ws = static_cast<char*>(c.ws);
+  a.live = reinterpret_cast<int32_t*>(ws);
+  a.part = reinterpret_cast<Part*>(ws + L.live);
+  a.keys = reinterpret_cast<key_t*>(ws + L.live + L.part);
+  const dim3 grid((uint32_t)L.blocks);
   if (c.dtype == Q35_F32) hipLaunchKernelGGL(beam_score_kernel<Q35_F32>, grid, dim3(kT), 0, st, a);
   else if (c.dtype == Q35_F16) hipLaunchKernelGGL(beam_score_kernel<Q35_F16>, grid, dim3(kT), 0, st, a);
   else hipLaunchKernelGGL(beam_score_kernel<Q35_BF16>, grid, dim3(kT), 0, st, a);
   Q35_HIP_TRY(hipGetLastError());
-  // a wave per 64 lists, and one per beam for the sums
-  const int waves = std::max(1, std::min(kJoinWaves, std::max(c.W, (c.W * a.nsplit + 63) / 64)));
+  // a thread per list, and a wave per beam for the sums
+  const int waves = std::max(1, std::min(kJoinWaves, std::max(c.W, (c.W * L.most + 63) / 64)));
   hipLaunchKernelGGL(beam_join_kernel, dim3(c.R), dim3(waves * 64), 0, st, a);
   Q35_HIP_TRY(hipGetLastError());
   return Q35_OK;
