@@ -42,7 +42,9 @@ struct Word<1> {
   typedef uint32_t R;
 };
 
-// All blocks find the rows that change, then take the slabs of all states in turn.
+// All blocks find the rows that change, then take the slabs of all states in turn.  Bound by HBM: 1.13 GB read and written
+// in 225 us, 5.0 TB/s, a large copy's rate (through the caches 237 us; with half the words per thread, slabs of 512
+// bytes a row, 337); 8 rows of 20 MB 13 us, 4 of 0.8 MB 6.5 us (launch, parents, a slab).
 template <int kW>
 __global__ __launch_bounds__(kT) void states_fork_kernel(const StatesArgs a) {
   typedef typename Word<kW>::M M;
@@ -98,7 +100,7 @@ __global__ __launch_bounds__(kT) void states_fork_kernel(const StatesArgs a) {
       if (i * kT < words) {
         int64_t src, dst;
         place(i, src, dst);
-        v[i] = *(const Q35_GLOBAL M*)((const char*)d.src + src);
+        v[i] = __builtin_nontemporal_load((const Q35_GLOBAL M*)((const char*)d.src + src));
       }
     }
     // every read of the slab has arrived before a write of it begins
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(kT) void states_fork_kernel(const StatesArgs a) {
     for (int i = 0; i < kPer; ++i) {
       if (i * kT < words) {
         int64_t src, dst;
-        if (place(i, src, dst)) *(Q35_GLOBAL M*)((char*)d.dst + dst) = (M)v[i];
+        if (place(i, src, dst)) __builtin_nontemporal_store((M)v[i], (Q35_GLOBAL M*)((char*)d.dst + dst));
       }
     }
   }

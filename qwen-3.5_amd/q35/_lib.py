@@ -109,7 +109,7 @@ PROTOTYPES = {
     "q35_beam_select_ws_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32]),
     "q35_beam_select": (ctypes.c_int, [c_vp, c_i32, c_i32, c_i32, c_i32, ctypes.c_int64, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp,
                                        c_sz, c_vp]),
-    "q35_states_fork": (ctypes.c_int, [ctypes.POINTER(State), c_i32, c_vp, c_i32, c_i32, c_vp, c_vp]),
+    "q35_states_fork": (ctypes.c_int, [c_vp, c_i32, c_vp, c_i32, c_i32, c_vp, c_vp]),
     "q35_pages_compact_ws_bytes": (c_sz, [c_i32]),
     "q35_pages_compact": (ctypes.c_int, [Pages, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "q35_token_logprobs_ws_bytes": (c_sz, [c_i32, c_i32, c_i32]),

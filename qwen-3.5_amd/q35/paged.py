@@ -24,6 +24,7 @@ import collections
 import contextlib
 import ctypes
 import functools
+import struct
 
 import torch
 
@@ -58,6 +59,12 @@ def _ints(t, *shape):
 
 def _ptr(t):
     return t.data_ptr() if t is not None else None
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_ws_bytes(heads, kv_heads, T, B, device):
+    """(By device: it goes by the compute units of the current one.)"""
+    return L.lib().q35_attention_paged_ws_bytes(ctypes.byref(L.make_dims(attn_heads=heads, kv_heads=kv_heads)), T, B)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -140,7 +147,7 @@ def attention_core_paged(dims, pool, layer, q_gate, k_new, v_new, seq_start, pos
         return out
     lib, d = L.lib(), ctypes.byref(dims)
     with _on(q_gate, pool.data, k_new, v_new, seq_start, pos, table, q_norm, k_norm, rope_cos, rope_sin, out):
-        nbytes = lib.q35_attention_paged_ws_bytes(d, T, B)
+        nbytes = _attention_ws_bytes(H, KV, T, B, pool.data.get_device())
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q_gate.device)
         L.check(lib.q35_attention_core_paged(
             d, pool.desc(), layer, q_gate.data_ptr(), ld_q, k_new.data_ptr(), v_new.data_ptr(), ld_k, T, seq_start.data_ptr(),
@@ -313,20 +320,32 @@ def states_fork(states, parents, out=None, check=False):
     parents = _ints(parents, Bo)
     if not states:
         return dst
-    B = states[0].shape[0]
-    desc = (L.State * len(states))()
-    for e, s, d in zip(desc, states, dst):
-        row, size = s.shape[1:], s.element_size()
-        assert s.shape[0] == B, "states of different rows"
-        assert d.dtype is s.dtype and d.shape[1:] == row and d.shape[0] >= Bo, (tuple(s.shape), tuple(d.shape), Bo)
-        n = row.numel() * size
-        e.src, e.dst, e.row_bytes, e.src_stride, e.dst_stride = s.data_ptr(), d.data_ptr(), n, _row_stride(s, n), _row_stride(d, n)
-    with _on(parents, *states, *(dst if out is not None else ())):
+    B, dev = states[0].shape[0], parents.get_device()
+    assert out is not None or Bo <= B, (Bo, B)
+    # src, dst, src_stride, dst_stride, row_bytes of every state (one by one in ctypes' fields took 40 us for 36 states)
+    flat = []
+    for s, d in zip(states, dst):
+        assert s.size(0) == B, "states of different rows"
+        n, p = s.nbytes // B, s.data_ptr()
+        ss = n if s.is_contiguous() else _row_stride(s, n)
+        assert s.get_device() == dev, "tensors on different devices"
+        if d is s:
+            flat += (p, p, ss, ss, n)
+        else:
+            assert d.dtype is s.dtype and d.shape[1:] == s.shape[1:] and d.size(0) >= Bo, (tuple(s.shape), tuple(d.shape), Bo)
+            assert d.get_device() == dev, "tensors on different devices"
+            flat += (p, d.data_ptr(), ss, _row_stride(d, n), n)
+    with _on(parents):
         status = torch.zeros(1, dtype=torch.int32, device=parents.device) if check else None
-        L.check(L.lib().q35_states_fork(desc, len(states), parents.data_ptr(), B, Bo, _ptr(status), _stream()))
+        L.check(L.lib().q35_states_fork(_words(len(flat)).pack(*flat), len(states), parents.data_ptr(), B, Bo, _ptr(status), _stream()))
         if check:
             L.check(L.lib().q35_status_check(status.data_ptr(), _stream()))
     return dst
+
+
+@functools.lru_cache(maxsize=64)
+def _words(n):
+    return struct.Struct("=%dq" % n)
 
 
 def _row_stride(t, row_bytes):
