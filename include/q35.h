@@ -654,6 +654,14 @@ int q35_batch_decode(q35_batch* b, int32_t n_steps, int32_t mode, void* stream);
  * q35_batch_reset). */
 int q35_batch_generate(q35_batch* b, const int32_t* prompts_host, const int32_t* lens_host, int32_t n_new,
                        int32_t* out_tokens_host, int32_t mode, double* decode_seconds_host, void* stream);
+/* The next set of sequences of a beam search (parents and tokens as q35_beam_select gives them, int32 [B] on the device): row j's
+ * states, caches and history become what row parent[j]'s were (q35_states_fork), and its next input token is tokens[j],
+ * which also takes its place in the history.  parent -1 leaves a row as it is; so does one outside [-1, B) or at another
+ * position than row j (Q35_STATUS_ARG).  Token -1 (an empty row) gives token 0, and so does one outside the
+ * vocabulary (Q35_STATUS_ARG).  A row whose prompt is not consumed takes its prompt's token all the same.  The rows
+ * copied are those up to the largest position at the call, so a captured fork is of that position. */
+int q35_batch_fork(q35_batch* b, const int32_t* parent, uint32_t* status, void* stream);
+int q35_batch_set_tokens(q35_batch* b, const int32_t* tokens, uint32_t* status, void* stream);
 /* Host copy of the B positions. */
 int q35_batch_position(q35_batch* b, int32_t* pos_out_host);
 /* Device pointer and bytes of a batch tensor ("layers.{i}.linear_attn.recurrent_state" [B][...],

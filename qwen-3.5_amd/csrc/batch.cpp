@@ -16,6 +16,7 @@
 // either through the decode step (rows at their own positions, ragged lengths) or through the
 // prompt path, several prompts per pass.
 #include "model_internal.h"
+#include "pages.h"
 
 #include <algorithm>
 #include <chrono>
@@ -27,6 +28,9 @@ int batch_embed_f32_launch(const int8_t* q, const float* s, int D, const int32_t
                            uint32_t* err, int B, hipStream_t st);
 int rms_step_launch(float* h, int M, int K, const float* w, float eps, float* y, const float* part, int nsplit,
                     uint32_t* err, hipStream_t st);
+int batch_parents_launch(const int32_t* parent, const int32_t* pos, int B, int32_t* checked, uint32_t* status, hipStream_t st);
+int batch_tokens_launch(const int32_t* tokens, const int32_t* pos, int B, int V, int32_t* token, int32_t* hist, int ldh, uint32_t* status,
+                        hipStream_t st);
 int batch_argmax_groups(int V);
 int batch_argmax_launch(const float* logits, int V, int B, float* pv, int32_t* pi, int32_t* token, int32_t* pos,
                         int32_t* hist, int ldh, hipStream_t st);
@@ -53,7 +57,7 @@ struct q35_batch {
   int64_t proj_n = 0;
   size_t part_floats = 0, word_floats = 0;
   uint32_t *mb_ctr = nullptr, *gdn_ctr = nullptr;
-  int32_t *token = nullptr, *pos = nullptr, *prompt = nullptr, *plen = nullptr, *hist = nullptr, *pi = nullptr;
+  int32_t *token = nullptr, *pos = nullptr, *prompt = nullptr, *plen = nullptr, *hist = nullptr, *pi = nullptr, *parents = nullptr;
   int32_t* pinned = nullptr;
   void* ws = nullptr;
   size_t ws_bytes = 0;
@@ -586,7 +590,8 @@ int q35_batch_create(q35_model* m, int32_t B, int32_t tmax, q35_batch** out) {
       (rc = balloc_t(b, "logits", (size_t)B * d.vocab, &b->logits)) || (rc = balloc_t(b, "argmax_pv", (size_t)B * G, &b->pv)) ||
       (rc = balloc_t(b, "argmax_pi", (size_t)B * G, &b->pi)) || (rc = balloc_t(b, "token", B, &b->token)) ||
       (rc = balloc_t(b, "pos", B, &b->pos)) || (rc = balloc_t(b, "prompt", (size_t)B * tmax, &b->prompt)) ||
-      (rc = balloc_t(b, "plen", B, &b->plen)) || (rc = balloc_t(b, "hist", (size_t)B * tmax, &b->hist)))
+      (rc = balloc_t(b, "plen", B, &b->plen)) || (rc = balloc_t(b, "hist", (size_t)B * tmax, &b->hist)) ||
+      (rc = balloc_t(b, "parents", B, &b->parents)))
     return bail(rc);
   b->ws_bytes = align256(attn_ws_bytes(B, ah, kvh, hd, tmax));
   if ((rc = balloc(b, "workspace", b->ws_bytes, &b->ws))) return bail(rc);
@@ -682,6 +687,43 @@ int q35_batch_generate(q35_batch* b, const int32_t* prompts_host, const int32_t*
     Q35_HIP_TRY(hipMemcpy(out_tokens_host + (size_t)r * (n_new + 1), b->hist + (size_t)r * b->tmax + start[r] + lens_host[r] - 1,
                           sizeof(int32_t) * (n_new + 1), hipMemcpyDeviceToHost));
   return Q35_OK;
+}
+
+int q35_batch_fork(q35_batch* b, const int32_t* parent, uint32_t* status, void* stream) {
+  if (!b || !parent) return fail(Q35_E_ARG, "batch_fork: null pointer");
+  try {
+    hipStream_t st = bpick(b, stream);
+    const q35_dims& d = b->m->d;
+    int rc;
+    if ((rc = batch_parents_launch(parent, b->pos, b->B, b->parents, status, st))) return rc;
+    const int64_t rows = *std::max_element(b->host_pos.begin(), b->host_pos.end());  // of a cache, at most
+    std::vector<q35_state> s;
+    auto add = [&](void* p, int64_t stride, int64_t bytes) { s.push_back({p, p, stride, stride, bytes}); };
+    for (int l = 0; l < d.n_layers; ++l) {
+      if (!b->m->layers[l].full) {
+        const int64_t conv = (int64_t)(2 * d.lin_heads * d.lin_dk + d.lin_heads * d.lin_dv) * (d.conv_k - 1) * 4;
+        const int64_t rec = (int64_t)d.lin_heads * d.lin_dk * d.lin_dv * 4;
+        add(b->conv[l], conv, conv);
+        add(b->rec[l], rec, rec);
+      } else {
+        const int64_t head = (int64_t)b->tmax * d.head_dim;
+        for (int h = 0; h < d.kv_heads; ++h) {
+          add(b->kc[l] + h * head, d.kv_heads * head * 4, rows * d.head_dim * 4);
+          add(b->vc[l] + h * head, d.kv_heads * head * 4, rows * d.head_dim * 4);
+        }
+      }
+    }
+    // (whole words of 16 bytes where the rows allow them)
+    add(b->hist, (int64_t)b->tmax * 4, 4 * (b->tmax % 4 == 0 ? (rows + 3) / 4 * 4 : rows));
+    return states_fork_launch(s.data(), (int)s.size(), b->parents, b->B, b->B, false, nullptr, st);
+  } catch (...) {
+    return Q35_E_NOMEM;
+  }
+}
+
+int q35_batch_set_tokens(q35_batch* b, const int32_t* tokens, uint32_t* status, void* stream) {
+  if (!b || !tokens) return fail(Q35_E_ARG, "batch_set_tokens: null pointer");
+  return batch_tokens_launch(tokens, b->pos, b->B, b->m->d.vocab, b->token, b->hist, b->tmax, status, bpick(b, stream));
 }
 
 int q35_batch_position(q35_batch* b, int32_t* pos_out_host) {

@@ -219,6 +219,41 @@ int rms_step_launch(float* h, int M, int K, const float* w, float eps, float* y,
   return Q35_OK;
 }
 
+// A fork's parents as they can be taken: rows of the batch at the same position; -1 for others, which are told unless they
+// are -1 already.
+__global__ __launch_bounds__(kBT) void batch_parents_kernel(const int32_t* parent, const int32_t* pos, int B, int32_t* checked, uint32_t* status) {
+  const int j = threadIdx.x;
+  if (j >= B) return;
+  const int p = parent[j];
+  const bool ok = p >= 0 && p < B && pos[p] == pos[j];
+  checked[j] = ok ? p : -1;
+  if (!ok && p != -1 && status) __hip_atomic_fetch_or((Q35_GLOBAL uint32_t*)status, (uint32_t)Q35_STATUS_ARG, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The rows' next input tokens, also as what the last step's positions were followed by; an empty row (-1) gets token 0.
+__global__ __launch_bounds__(kBT) void batch_tokens_kernel(const int32_t* tokens, const int32_t* pos, int B, int V, int32_t* token, int32_t* hist,
+                                                          int ldh, uint32_t* status) {
+  const int j = threadIdx.x;
+  if (j >= B) return;
+  const int t = tokens[j], p = pos[j], v = t >= 0 && t < V ? t : 0;
+  token[j] = v;
+  if (p >= 1 && p <= ldh) hist[(int64_t)j * ldh + p - 1] = v;
+  if (t != v && t != -1 && status) __hip_atomic_fetch_or((Q35_GLOBAL uint32_t*)status, (uint32_t)Q35_STATUS_ARG, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+int batch_parents_launch(const int32_t* parent, const int32_t* pos, int B, int32_t* checked, uint32_t* status, hipStream_t st) {
+  hipLaunchKernelGGL(batch_parents_kernel, dim3(1), dim3(kBT), 0, st, parent, pos, B, checked, status);
+  Q35_HIP_TRY(hipGetLastError());
+  return Q35_OK;
+}
+
+int batch_tokens_launch(const int32_t* tokens, const int32_t* pos, int B, int V, int32_t* token, int32_t* hist, int ldh, uint32_t* status,
+                        hipStream_t st) {
+  hipLaunchKernelGGL(batch_tokens_kernel, dim3(1), dim3(kBT), 0, st, tokens, pos, B, V, token, hist, ldh, status);
+  Q35_HIP_TRY(hipGetLastError());
+  return Q35_OK;
+}
+
 int batch_argmax_groups(int V) { return std::max(1, std::min(64, (V + 4095) / 4096)); }
 
 int batch_argmax_launch(const float* logits, int V, int B, float* pv, int32_t* pi, int32_t* token, int32_t* pos,

@@ -143,6 +143,8 @@ PROTOTYPES = {
     "q35_batch_step": (ctypes.c_int, [c_vp, c_i32, c_vp]),
     "q35_batch_decode": (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp]),
     "q35_batch_generate": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_vp, c_i32, ctypes.POINTER(ctypes.c_double), c_vp]),
+    "q35_batch_fork": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp]),
+    "q35_batch_set_tokens": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp]),
     "q35_batch_position": (ctypes.c_int, [c_vp, c_vp]),
     "q35_batch_tensor": (ctypes.c_int, [c_vp, ctypes.c_char_p, ctypes.POINTER(c_vp), ctypes.POINTER(c_sz)]),
     "q35_synth_normal": (ctypes.c_int, [c_u64, c_u64, c_i64, c_i64, c_f32, c_vp]),

@@ -269,6 +269,71 @@ class BatchDecoder:
                                            ctypes.byref(secs), stream))
         return out, secs.value
 
+    def fork(self, parents, tokens=None, status=None, stream=None):
+        """Row j goes on from row parents[j] (int32 [B] on the GPU, -1: from itself): states, caches, history; with tokens
+        (int32 [B]) as the rows' next input.  A row takes parents at its own position only; status: an int32 tensor [1]
+        that is told what was refused."""
+        st = status.data_ptr() if status is not None else None
+        for t in (parents, tokens):
+            assert t is None or (t.shape == (self.B,) and t.is_cuda and t.is_contiguous() and t.element_size() == 4), t
+        L.check(L.lib().q35_batch_fork(self.h, parents.data_ptr(), st, stream))
+        if tokens is not None:
+            L.check(L.lib().q35_batch_set_tokens(self.h, tokens.data_ptr(), st, stream))
+
+    def beam_search(self, prompts, beams, n_new, stop_ids=(), length_penalty=0.0, mode="graph"):
+        """Beam search from G = B / beams prompts (id sequences): per prompt the hypotheses (ids, score), best first, where
+        score is the sum of the ids' log probabilities over (number of ids) ** length_penalty.  A hypothesis ends with the
+        first of stop_ids or after n_new ids.  Every step: the batched decode step, beam_select over its logits, and the
+        fork of the rows' states, without a synchronisation (but every 16 steps, to end early, with stop ids)."""
+        import torch
+        from .paged import beam_select
+        G = len(prompts)
+        assert G * beams == self.B and n_new >= 1, (G, beams, self.B, n_new)
+        assert all(len(p) + n_new <= self.tmax + 1 for p in prompts), "tmax too small"
+        self.reset()
+        self.generate([p for p in prompts for _ in range(beams)], 0, mode=mode, prefill=True)
+        first = self.positions() - 1
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            logits = self._view("logits", (self.B, self.model.dims.vocab), "<f4")
+            dev = logits.device
+            scores = torch.full((G, beams), -float("inf"), device=dev)
+            scores[:, 0] = 0.0
+            stops = torch.tensor(list(stop_ids), dtype=torch.int32, device=dev)
+            ended = torch.full((self.B,), -1, dtype=torch.int32, device=dev)
+            ids = torch.zeros(self.B, dtype=torch.int32, device=dev)  # of the hypothesis so far
+            status = torch.zeros(1, dtype=torch.int32, device=dev)
+            for i in range(n_new):
+                if i > 0:
+                    self.step(mode=mode, stream=stream.cuda_stream)
+                r = beam_select(logits, scores, beams, ended=ended)
+                parents, tokens, scores = r.parents.view(-1), r.tokens.view(-1), r.scores
+                self.fork(parents, tokens, status, stream.cuda_stream)
+                old = parents.clamp(min=0).long()
+                over = (parents >= 0) & (ended[old] >= 0)
+                ids = torch.where(over, ids[old], i + 1)
+                ended = torch.where(over | ((parents >= 0) & torch.isin(tokens, stops)), tokens, -1)
+                if len(stop_ids) and i % 16 == 15 and bool(((ended >= 0) | (parents < 0)).all()):
+                    break
+            hist = self._view("hist", (self.B, self.tmax), "<i4").cpu().numpy()
+            ids, scores = ids.cpu().numpy(), scores.view(-1).cpu().numpy().astype(np.float64)
+            L.check(L.lib().q35_status_check(status.data_ptr(), stream.cuda_stream))
+        out = []
+        for g in range(G):
+            rows = [r for r in range(g * beams, (g + 1) * beams) if np.isfinite(scores[r])]
+            hyps = [(hist[r, first[r]:first[r] + ids[r]].copy(), float(scores[r] / float(ids[r]) ** length_penalty)) for r in rows]
+            out.append(sorted(hyps, key=lambda h: -h[1]))
+        return out
+
+    def _view(self, name, shape, typestr):
+        """A device tensor of the batch as torch's, without a copy (valid while the batch lives)."""
+        import torch
+        ptr, nbytes = ctypes.c_void_p(), ctypes.c_size_t()
+        L.check(L.lib().q35_batch_tensor(self.h, name.encode(), ctypes.byref(ptr), ctypes.byref(nbytes)))
+        assert int(np.prod(shape)) * 4 == nbytes.value, (name, shape, nbytes.value)
+        at = type("DeviceArray", (), {"__cuda_array_interface__": dict(shape=shape, typestr=typestr, data=(ptr.value, False), version=2)})
+        return torch.as_tensor(at(), device="cuda")
+
     def positions(self):
         out = np.zeros(self.B, np.int32)
         L.check(L.lib().q35_batch_position(self.h, out.ctypes.data))

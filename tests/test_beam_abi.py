@@ -71,3 +71,8 @@ def test_selection_by_hand():
     B.check((s.astype(np.float32), p, t), x, np.array([[-np.inf, -1.0]], np.float32), 2, np.array([-1, 2]))
     with pytest.raises(AssertionError):
         B.check((s.astype(np.float32) + 1e-4, p, t), x, np.array([[-np.inf, -1.0]], np.float32), 2, np.array([-1, 2]))
+
+
+def test_batch_forks_refuse_null_pointers():
+    lib = L.lib()
+    assert lib.q35_batch_fork(None, A, None, None) == L.Q35_E_ARG and lib.q35_batch_set_tokens(None, A, None, None) == L.Q35_E_ARG
