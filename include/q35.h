@@ -446,7 +446,7 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
  * logits of row g W + w of logits [R W][ld] (as q35_token_logprobs's); its continuation by token v scores
  * scores[g W + w] + x[v] - ln sum e^x.  Of all continuations of a group the k (1..64) with the highest scores go, highest first,
  * to scores_out, parents (the row g W + w, as q35_pages_fork and q35_states_fork take it) and tokens, all [R][k]; among
- * equal ones the lowest row first, then the lowest token.
+ * equal ones the lowest row first, and in a row the larger logit, then the lowest token.
  *   ended (int32 [R W], NULL: none): a beam with ended[row] >= 0 has ended: its only continuation is that token, at its score
  *   as it is, and its logits are not read; a token >= V leaves it without one (Q35_STATUS_ARG).
  * A beam whose score is not finite is dead: it has no continuation and its logits are not read (an empty slot; all but the
@@ -454,7 +454,7 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
  * group has fewer than k continuations the rest is score -inf, parent -1, token -1: an empty row of the next
  * tables, a dead beam of the next step.
  * Scores are formed in f64, from exponentials in f32 (an error of about 10^-8 in ln sum e^x), and rounded once.
- * W <= 256, W V < 2^32, R W < 2^24, V <= 2^30; no output overlaps an input.  ws: q35_beam_select_ws_bytes bytes of scratch,
+ * W <= 256, R W < 2^24, V <= 2^30; no output overlaps an input.  ws: q35_beam_select_ws_bytes bytes of scratch,
  * 16-byte aligned. */
 size_t q35_beam_select_ws_bytes(int32_t R, int32_t W, int32_t V, int32_t k);
 int q35_beam_select(const void* logits, int32_t dtype, int32_t R, int32_t W, int32_t V, int64_t ld, const float* scores,
@@ -465,8 +465,8 @@ int q35_beam_select(const void* logits, int32_t dtype, int32_t R, int32_t W, int
  * caches, histories): row j of each of n states (host array) becomes what row parent[j] of it was, j < B_out.  A state's rows
  * lie src_stride / dst_stride bytes apart and have row_bytes bytes (contiguous).  In place (every state's dst is its src, one
  * stride) or into other buffers (no dst overlaps any src; all states alike).  parent -1 leaves row j of dst as it is; one
- * outside [-1, B) counts as -1 (Q35_STATUS_ARG).  In place only rows that change are touched.  States of one call do not overlap each other; src has
- * B rows and dst B_out (in place: the larger number of both).  B, B_out <= 4096. */
+ * outside [-1, B) counts as -1 (Q35_STATUS_ARG).  In place only rows that change are touched.  States of one call do not overlap each
+ * other (two of one dst are refused); src has B rows and dst B_out (in place: the larger number of both).  B, B_out <= 4096. */
 typedef struct {
   const void* src;
   void* dst;

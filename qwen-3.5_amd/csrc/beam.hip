@@ -219,30 +219,35 @@ __global__ __launch_bounds__(kT) void beam_score_kernel(const BeamArgs a) {
   }
 }
 
-// A continuation: its score's bits in ascending order, and its number w V + v in the group; hi 0: none
+// A continuation: its score's bits in ascending order (0: none), its beam, and its logit and token as a list's key.  Among
+// equal scores (which two logits of a beam have where its own score is many times larger) the lower beam is first, then the larger key.
 struct Cand {
   unsigned long long hi;
-  uint32_t ix;
+  key_t key;
+  uint32_t w;
 };
-Q35_DEV bool ahead(const Cand& a, const Cand& b) { return a.hi > b.hi || (a.hi == b.hi && a.ix < b.ix); }
+Q35_DEV bool ahead(const Cand& a, const Cand& b) { return a.hi > b.hi || (a.hi == b.hi && (a.w < b.w || (a.w == b.w && a.key > b.key))); }
+constexpr uint32_t kNoBeam = ~0u;
 Q35_DEV unsigned long long asc64(double c) {
   const unsigned long long b = __builtin_bit_cast(unsigned long long, c + 0.0);
   return b >> 63 ? ~b : b | 1ull << 63;
 }
 Q35_DEV double from_asc64(unsigned long long a) { return __builtin_bit_cast(double, a >> 63 ? a & ~(1ull << 63) : ~a); }
 Q35_DEV Cand lane_cand(const Cand& c, int lane) {
-  return Cand{lane_key(c.hi, lane), (uint32_t)__builtin_amdgcn_readlane((int)c.ix, lane)};
+  return Cand{lane_key(c.hi, lane), lane_key(c.key, lane), (uint32_t)__builtin_amdgcn_readlane((int)c.w, lane)};
+}
+Q35_DEV unsigned long long lane_before(unsigned long long v) {  // (lane 0: all ones)
+  return ((unsigned long long)(uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(v >> 32), 0x138, 0xf, 0xf, false) << 32) |
+         (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(uint32_t)v, 0x138, 0xf, 0xf, false);
 }
 // Puts c (the same in every lane) into the sorted list that the lanes hold; last: its top-th
 Q35_DEV void insert_cand(Cand& best, Cand& last, const Cand& c, int top) {
   if (!ahead(c, last)) return;
-  const Cand up = {((unsigned long long)(uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(best.hi >> 32), 0x138, 0xf, 0xf, false) << 32) |
-                       (uint32_t)__builtin_amdgcn_update_dpp(-1, (int)(uint32_t)best.hi, 0x138, 0xf, 0xf, false),
-                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)best.ix, 0x138, 0xf, 0xf, false)};
+  const Cand up = {lane_before(best.hi), lane_before(best.key), (uint32_t)__builtin_amdgcn_update_dpp(0, (int)best.w, 0x138, 0xf, 0xf, false)};
   // a place takes the first of what it has and of the second of c and the one before it
   const Cand in = ahead(up, c) ? c : up;
   if (ahead(in, best)) best = in;
-  if ((int)(threadIdx.x & 63) >= top) best = Cand{0, ~0u};
+  if ((int)(threadIdx.x & 63) >= top) best = Cand{0, 0, kNoBeam};
   last = lane_cand(best, top - 1);
 }
 
@@ -274,8 +279,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
   const BeamCall& c = a.c;
   __shared__ double off[kMaxBeams];
   __shared__ int state[kMaxBeams];
-  __shared__ unsigned long long chi[kMaxCand];
-  __shared__ uint32_t cix[kMaxCand];
+  __shared__ Cand cands[kMaxCand];
   __shared__ uint32_t fl;
   __shared__ int nc;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x / 64;
@@ -347,16 +351,14 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
   auto cand = [&](key_t key, int w, int sp, int j, Cand& x) {
     const int st = state[w];
     double s = -INFINITY;
-    uint32_t token = 0;
     if (st == kLive && key != 0) {
       s = off[w] + (double)from_asc((uint32_t)(key >> 32));
-      token = (uint32_t)key_index(key);
     } else if (st == kEnded && sp == 0 && j == 0) {
       s = off[w];
-      token = (uint32_t)c.ended[row0 + w];
+      key = (uint32_t)~c.ended[row0 + w];
     }
     const bool some = s > -INFINITY;
-    x = Cand{some ? asc64(s) : 0, (uint32_t)w * (uint32_t)c.V + token};
+    x = Cand{some ? asc64(s) : 0, key, (uint32_t)w};
     return some ? asc((float)s) : 0u;
   };
 #pragma unroll 1
@@ -389,40 +391,35 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
       Cand x;
       if (cand(key, my_w, my_sp, j, x) < floor32) break;  // (lists fall)
       const int at = atomicAdd(&nc, 1);
-      if (at < kMaxCand) {
-        chi[at] = x.hi;
-        cix[at] = x.ix;
-      }
+      if (at < kMaxCand) cands[at] = x;
     }
   }
   __syncthreads();
   auto put = [&](const Cand& x, int place) {
     const int64_t at = (int64_t)g * k + place;
-    const uint32_t w = x.ix / (uint32_t)c.V;
     c.scores_out[at] = (float)from_asc64(x.hi);
-    c.parents[at] = (int32_t)(row0 + w);
-    c.tokens[at] = (int32_t)(x.ix - w * (uint32_t)c.V);
+    c.parents[at] = (int32_t)(row0 + x.w);
+    c.tokens[at] = key_index(x.key);
   };
   int all = nc;
   if (all <= kMaxCand) {
     for (int t = tid; t < all; t += blockDim.x) {
-      const Cand x = {chi[t], cix[t]};
+      const Cand x = cands[t];
       int place = 0;
-      for (int e = 0; e < all; ++e) place += ahead(Cand{chi[e], cix[e]}, x) ? 1 : 0;
+      for (int e = 0; e < all; ++e) place += ahead(cands[e], x) ? 1 : 0;
       if (place < k) put(x, place);
     }
   } else {
     // lists by waves: sorted, then joined
-    __shared__ unsigned long long lhi[kJoinWaves][kMaxTop];
-    __shared__ uint32_t lix[kJoinWaves][kMaxTop];
-    Cand best = {0, ~0u}, last = {0, ~0u};
+    __shared__ Cand sorted[kJoinWaves][kMaxTop];
+    Cand best = {0, 0, kNoBeam}, last = best;
 #pragma unroll 1
     for (int l0 = wid * 64; l0 < nl; l0 += nw * 64) {
       int w, sp;
       const key_t* held = list(min(l0 + lane, nl - 1), w, sp);
 #pragma unroll 1
       for (int j = 0; j < k; ++j) {
-        Cand x = {0, ~0u};
+        Cand x = {0, 0, kNoBeam};
         const uint32_t a32 = l0 + lane < nl ? cand(held[j], w, sp, j, x) : 0;
         unsigned long long take = __ballot(a32 >= floor32 && ahead(x, last));
         if (!take) break;
@@ -430,10 +427,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
         for (; take; take &= take - 1) insert_cand(best, last, lane_cand(x, (int)__builtin_ctzll(take)), k);
       }
     }
-    if (lane < k) {
-      lhi[wid][lane] = best.hi;
-      lix[wid][lane] = best.ix;
-    }
+    if (lane < k) sorted[wid][lane] = best;
     __syncthreads();
     if (lane < k && best.hi != 0) {
       int place = lane;
@@ -441,7 +435,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
       for (int w = 0; w < nw; ++w) {
         if (w == wid) continue;
         int at = 0;
-        while (at < k && ahead(Cand{lhi[w][at], lix[w][at]}, best)) ++at;
+        while (at < k && ahead(sorted[w][at], best)) ++at;
         place += at;
       }
       if (place < k) put(best, place);

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <vector>
 
 namespace q35 {
 namespace {
@@ -230,7 +231,7 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
 }
 
 size_t q35_beam_select_ws_bytes(int32_t R, int32_t W, int32_t V, int32_t k) {
-  if (R < 1 || W < 1 || W > kMaxBeams || V < 1 || V > (1 << 30) || (int64_t)R * W >= kMaxGrid || (int64_t)W * V >= (1ll << 32) || k < 1 || k > kMaxTop) return 0;
+  if (R < 1 || W < 1 || W > kMaxBeams || V < 1 || V > (1 << 30) || (int64_t)R * W >= kMaxGrid || k < 1 || k > kMaxTop) return 0;
   return beam_ws_bytes(R, W, V, k);
 }
 
@@ -242,7 +243,7 @@ int q35_beam_select(const void* logits, int32_t dtype, int32_t R, int32_t W, int
     if (dtype != Q35_F32 && dtype != Q35_F16 && dtype != Q35_BF16) return fail(Q35_E_ARG, "beam_select: bad dtype");
     if (k < 1 || k > kMaxTop) return fail(Q35_E_SHAPE, "beam_select: k must be in 1..64");
     const size_t need = q35_beam_select_ws_bytes(R, W, V, k);
-    if (need == 0 || ld < V) return fail(Q35_E_SHAPE, "beam_select: 1..256 beams, R W < 2^24, 1 <= V <= 2^30, W V < 2^32 and ld >= V required");
+    if (need == 0 || ld < V) return fail(Q35_E_SHAPE, "beam_select: 1..256 beams, R W < 2^24, 1 <= V <= 2^30 and ld >= V required");
     if (!aligned(logits, elt_size(dtype))) return fail(Q35_E_ALIGN, "beam_select: logits not aligned to their type");
     if (!ws || ws_bytes < need) return fail(Q35_E_WS, "beam_select: workspace too small");
     if (!aligned(ws, 16)) return fail(Q35_E_ALIGN, "beam_select: workspace not 16-byte aligned");
@@ -285,6 +286,11 @@ int q35_states_fork(const q35_state* states, int32_t n, const int32_t* parent, i
       if (copies && overlap(s.src, (size_t)(B - 1) * s.src_stride + s.row_bytes, s.dst, (size_t)(B_out - 1) * s.dst_stride + s.row_bytes))
         return fail(Q35_E_ARG, "states_fork: source and destination overlap");
     }
+    std::vector<const void*> dst;
+    for (int i = 0; i < n; ++i)
+      if (states[i].row_bytes > 0) dst.push_back(states[i].dst);
+    std::sort(dst.begin(), dst.end());
+    if (std::adjacent_find(dst.begin(), dst.end()) != dst.end()) return fail(Q35_E_ARG, "states_fork: a state named twice");
     return states_fork_launch(states, n, parent, B, B_out, copies, status, S(stream));
   });
 }

@@ -275,7 +275,7 @@ class BatchDecoder:
         that is told what was refused."""
         st = status.data_ptr() if status is not None else None
         for t in (parents, tokens):
-            assert t is None or (t.shape == (self.B,) and t.is_cuda and t.is_contiguous() and t.element_size() == 4), t
+            assert t is None or (t.shape == (self.B,) and t.is_cuda and t.is_contiguous() and str(t.dtype) == "torch.int32"), t
         L.check(L.lib().q35_batch_fork(self.h, parents.data_ptr(), st, stream))
         if tokens is not None:
             L.check(L.lib().q35_batch_set_tokens(self.h, tokens.data_ptr(), st, stream))

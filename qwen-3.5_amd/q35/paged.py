@@ -275,7 +275,7 @@ def beam_select(logits, scores, k, ended=None, check=False):
     """The next beams of G groups of W beams: logits [G, W, V] or [G * W, V] (float32, float16 or bfloat16), scores float32
     [G, W].  Of a group's continuations (beam w, token v), which score scores[g, w] + logits[g, w, v] - logsumexp of the
     row, the k highest: BeamSelect(scores float32, parents int32, tokens int32), all [G, k], highest first; among equal ones the
-    lowest beam, then the lowest token.  parents are rows of the G * W, as pages_fork and states_fork take them.
+    lowest beam, in a beam the larger logit, then the lowest token.  parents are rows of the G * W, as pages_fork and states_fork take them.
     ended (int32 [G * W] or [G, W]; None: none): a beam with ended >= 0 goes on as it is, with that token.  A beam whose score
     is not finite has no continuation; a group with fewer than k is filled up with score -inf, parent -1, token -1.
     check=True synchronises and raises Q35Error (Q35_E_RANGE) for an ended token >= V, which leaves its beam without a

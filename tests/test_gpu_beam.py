@@ -156,6 +156,31 @@ def test_scores_far_apart_and_large():
     verify(x, [[-1e6, -1e6 + 1, -1e6 - 2, -1e6], [0.0, -300.0, 5.0, -1e30]], 16)
 
 
+def test_scores_that_swallow_the_logits():
+    """A beam's score so large that all of its continuations are equal: its order is that of the logits still."""
+    x = logits(14, "bf16", 3, 5000)
+    got = run(x, [[-1e30, -1e30, -2e30]], 40)
+    order = np.lexsort((np.arange(5000), -x[0].double().cpu().numpy()))[:40]
+    assert got[1].tolist() == [[0] * 40] and got[2][0].tolist() == order.tolist() and (got[0] == np.float32(-1e30)).all()
+    got = run(x, [[-1e9, -1e9, 0.0]], 12)
+    assert got[1].tolist() == [[2] * 12]
+
+
+@pytest.mark.parametrize("W,k", [(64, 64), (8, 64), (12, 24)])
+def test_more_equal_continuations_than_the_choice_ranks(W, k):
+    """Equal logits and scores throughout, or in many rows and parts: by row, then by token."""
+    x = torch.zeros(W, 30000, device="cuda")
+    got = verify(x, np.full((1, W), -2.0), k)
+    assert got[1][0].tolist() == [0] * k and got[2][0].tolist() == list(range(k))
+    x[:, ::7] = 1.0
+    x[1] = logits(15, "f32", 1, 30000, 0.3)[0]
+    verify(x, np.full((1, W), -2.0), k)
+    half = torch.zeros(W, 30000, dtype=torch.bfloat16, device="cuda")
+    half[:, 29000:] = 0.5
+    got = verify(half, np.linspace(-2.0, -1.0, W)[None].astype(np.float32), k)
+    assert got[1][0].tolist() == [W - 1] * k and got[2][0].tolist() == list(range(29000, 29000 + k))
+
+
 def test_same_bits_on_every_run():
     x, s = logits(11, "bf16", 64, 30000), make_scores(11, 8, 8)
     first = run(x, s, 16)

@@ -157,4 +157,6 @@ def test_refusals():
         with pytest.raises(AssertionError):
             bad()
     with pytest.raises(q35.Q35Error, match="Q35_E_ARG"):
+        q35.states_fork([t, make(2, (4, 5)), t], i32([1, 0]))
+    with pytest.raises(q35.Q35Error, match="Q35_E_ARG"):
         q35.states_fork([t[:3]], i32([0, 1]), out=[t[1:]])
