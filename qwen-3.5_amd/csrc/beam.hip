@@ -279,7 +279,9 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
   const BeamCall& c = a.c;
   __shared__ double off[kMaxBeams];
   __shared__ int state[kMaxBeams];
-  __shared__ Cand cands[kMaxCand];
+  __shared__ unsigned long long chi[kMaxCand];
+  __shared__ key_t ckey[kMaxCand];
+  __shared__ uint32_t cw[kMaxCand];
   __shared__ uint32_t fl;
   __shared__ int nc;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), nw = blockDim.x / 64;
@@ -384,14 +386,18 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
   if (tid < nl) {
 #pragma unroll 1
     for (int j = 0; j < k; ++j) {
-      const key_t key = j < kFirst ? first[0] : my_keys[j];
-      first[0] = first[1];
-      first[1] = first[2];
-      first[2] = first[3];
+      const key_t key = first[0];
+#pragma unroll
+      for (int e = 1; e < kFirst; ++e) first[e - 1] = first[e];
+      first[kFirst - 1] = j + kFirst < k ? my_keys[j + kFirst] : 0;
       Cand x;
       if (cand(key, my_w, my_sp, j, x) < floor32) break;  // (lists fall)
       const int at = atomicAdd(&nc, 1);
-      if (at < kMaxCand) cands[at] = x;
+      if (at < kMaxCand) {
+        chi[at] = x.hi;
+        ckey[at] = x.key;
+        cw[at] = x.w;
+      }
     }
   }
   __syncthreads();
@@ -404,9 +410,15 @@ __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamAr
   int all = nc;
   if (all <= kMaxCand) {
     for (int t = tid; t < all; t += blockDim.x) {
-      const Cand x = cands[t];
-      int place = 0;
-      for (int e = 0; e < all; ++e) place += ahead(cands[e], x) ? 1 : 0;
+      const Cand x = {chi[t], ckey[t], cw[t]};
+      int place = 0, equal = 0;
+      for (int e = 0; e < all; ++e) {
+        place += chi[e] > x.hi ? 1 : 0;
+        equal += chi[e] == x.hi ? 1 : 0;
+      }
+      if (equal > 1) {
+        for (int e = 0; e < all; ++e) place += chi[e] == x.hi && ahead(Cand{chi[e], ckey[e], cw[e]}, x) ? 1 : 0;
+      }
       if (place < k) put(x, place);
     }
   } else {
