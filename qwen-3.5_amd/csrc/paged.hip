@@ -1529,7 +1529,8 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
   // 2000 and one of 64 behind 30000 would take 207 us, 133 so).  But a batch of fixed slots may be one chunk and
   // empty ones, so that holds only while the chunk's tiles could go over the longest context that the table
   // and the rotary rows allow as cheaply as a chunk does (kReread; both ways, us: 16 tokens behind 16000 in bf16 37
-  // and 37, in f32 54 and 40; 64 behind 2000 28 and 37, 36 and 40; 256 behind 16000 272 and 112, 572 and 134).
+  // and 37, in f32 54 and 40; 64 behind 2000 28 and 37, 36 and 40; 256 behind 16000 272 and 112, 572 and 134; in 4 bits
+  // 16 behind 60000 56 and 55, 64 behind 16000 56 and 56).
   // One sequence: its rows decide, if all rows are its.
   L.few_most = std::max(1, 2 * kFewRows / rep);
   const int64_t tiles = ((int64_t)T * rep + kFewRows - 1) / kFewRows * nkv;
