@@ -102,7 +102,7 @@ class PagePool:
 
     @classmethod
     def empty(cls, n_layers, n_pages, kv_heads=2, page=64, head_dim=256, dtype=torch.float32, device="cuda"):
-        if dtype is Q4:
+        if dtype == Q4:
             assert head_dim == 256, head_dim
             head_dim, dtype = _Q4_ROW, torch.uint8
         return cls(torch.empty((n_layers, n_pages, 2, kv_heads, page, head_dim), dtype=dtype, device=device))
