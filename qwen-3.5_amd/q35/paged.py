@@ -318,10 +318,10 @@ def states_fork(states, parents, out=None, check=False):
     assert len(dst) == len(states), (len(dst), len(states))
     Bo = parents.shape[0]
     parents = _ints(parents, Bo)
-    if not states:
+    if not states or Bo == 0:
         return dst
     B, dev = states[0].shape[0], parents.get_device()
-    assert out is not None or Bo <= B, (Bo, B)
+    assert B > 0 and (out is not None or Bo <= B), (Bo, B)
     # src, dst, src_stride, dst_stride, row_bytes of every state (one by one in ctypes' fields took 40 us for 36 states)
     flat = []
     for s, d in zip(states, dst):

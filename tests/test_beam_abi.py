@@ -4,6 +4,7 @@ import ctypes
 
 import numpy as np
 import pytest
+import torch
 
 import beam_ref as B
 import q35
@@ -77,3 +78,12 @@ def test_selection_by_hand():
 def test_batch_forks_refuse_null_pointers():
     lib = L.lib()
     assert lib.q35_batch_fork(None, A, None, None) == L.Q35_E_ARG and lib.q35_batch_set_tokens(None, A, None, None) == L.Q35_E_ARG
+
+
+def test_states_of_no_rows():
+    none, two = torch.zeros(0, 8), torch.zeros(2, 8)
+    parents = torch.zeros(0, dtype=torch.int32)
+    assert q35.states_fork([none], parents)[0] is none
+    assert q35.states_fork([none], parents, out=[two])[0] is two
+    with pytest.raises(AssertionError):
+        q35.states_fork([none], torch.full((2,), -1, dtype=torch.int32), out=[two])

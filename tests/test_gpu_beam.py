@@ -238,3 +238,16 @@ def test_refusals():
     for k in (0, 65):
         with pytest.raises((q35.Q35Error, RuntimeError)):
             q35.beam_select(x, s, k)
+
+
+@pytest.mark.parametrize("live", [0, 1, 7, 300])
+def test_many_groups_with_few_live_beams(live):
+    """600 beams of which some score: the others' logits are NaN and hold no place in the work's division."""
+    G, W, V = 150, 4, 9000
+    x = logits(11, "f16", G * W, V)
+    on = np.random.default_rng(live).permutation(G * W)[:live]
+    s = np.full(G * W, -np.inf, np.float32)
+    s[on] = make_scores(live, G, W).reshape(-1)[:live]
+    x[torch.from_numpy(np.flatnonzero(np.isinf(s))).cuda()] = float("nan")
+    got = verify(x, s.reshape(G, W), 5)
+    assert set(got[1][got[1] >= 0].tolist()) <= set(on.tolist()) and ((got[1] >= 0).sum(1) == np.where(np.isfinite(s).reshape(G, W).any(1), 5, 0)).all()

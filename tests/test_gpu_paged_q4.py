@@ -367,3 +367,30 @@ def test_pool_of_another_shape_is_refused():
     assert q35.PagePool.empty(1, 2, 3, 16, dtype=q35.Q4).data.shape == (1, 2, 2, 3, 16, ROW)
     with pytest.raises(AssertionError):
         q35.PagePool.empty(1, 2, head_dim=128, dtype=q35.Q4)
+
+
+def test_pages_beyond_32bit_offsets():
+    """A small case in the last pages of the second of two layers, 2.2 GB each."""
+    seqs = [(1, 300), (5, 70), (200, 130)]
+    c = make(12, 64, 8, 2, seqs)
+    small = d(c["pool"])
+    used, n = small.shape[1], 60000
+    pool = q35.PagePool.empty(2, n, page=64, dtype=q35.Q4)
+    assert pool.data[1, n - used:].data_ptr() - pool.data.data_ptr() > 2 ** 32
+    pool.data[1, n - used:] = small[0]
+    high = [[p + n - used if p >= 0 else -1 for p in row] for row in c["table"]]
+    out, _ = run(dict(c, layer=1, table=high), pool)
+    check(c, out, q35.PagePool(pool.data[1:, n - used:].clone()))
+    pool.check()
+    last = [(b, x + y - 1) for b, (x, y) in enumerate(seqs)]
+    rows, at = i32([b for b, _ in last]), i32([p for _, p in last])
+    got = q35.pages_read(pool, 1, i32(high), rows, at, check=True)
+    want = pool.data[1, n - used:]
+    for i, (b, p) in enumerate(last):
+        assert torch.equal(got[i].cpu(), torch.from_numpy(Q.unpack(want[c["table"][b][p // 64], :, :, p % 64].cpu().numpy())).half())
+    want = want[-2:].clone()
+    q35.pages_copy(pool, i32([n - 2, n - 1]), i32([0, 1]), check=True)
+    assert torch.equal(pool.data[1, :2], want)
+    pool.data[1, -2:] = 0
+    q35.pages_copy(pool, i32([0, 1]), i32([n - 2, n - 1]), check=True)
+    assert torch.equal(pool.data[1, -2:], want)
