@@ -55,6 +55,8 @@ Q35_DEV bool find_seq(const PagedAttn& a, int t, Seq* s) {
 // finely as many short ones are not.  Where a block's range cuts a tile, it leaves (max, sum, output)
 // of its part, and paged_join_kernel joins the parts; only the first and the last tile of a block can be
 // cut, so two slots per block hold them all.
+// A part of a second tile costs a block its queries, first loads and join once more, up to 6 us over a cache in 4 bits: there
+// "few" blocks take a part of one tile alone if that comes out even enough (kCutUnits).
 //
 // Two kinds of tiles: sequences of few rows ("few": the cache's stream bounds them) and chunks ("many":
 // the matrix cores do).
@@ -70,7 +72,8 @@ struct alignas(16) Tile {
 // The plan of one kind: block g starts at unit g q + min(g, r)
 struct PlanHead {
   int64_t w, q;  // units of all tiles
-  int32_t r, tiles, blocks, pad;
+  int32_t r, tiles, blocks;
+  int32_t whole;  // 0, or q: a (tile, kv head) is laid out over a multiple of that many units, so no block has parts of two
 };
 
 struct AttnArgs {
@@ -103,6 +106,8 @@ Q35_DEV int tile_len(const AttnArgs& A, const Seq& s, int i) {
   const int tok = kind_of(A, s.n) ? (i + 1) * A.tok_many - 1 : div_rep(A, (i + 1) * kFewRows - 1);
   return s.p0 + min(tok, s.n - 1) + 1;
 }
+// units that a (tile, kv head) of n units is laid out over
+Q35_DEV int laid_out(int n, int whole) { return whole ? (int)((uint32_t)(n + whole - 1) / (uint32_t)whole) * whole : n; }
 // first unit of block g, and the block that holds unit u
 Q35_DEV int64_t block_u0(const PlanHead& h, int g) { return h.q * g + min(g, h.r); }
 Q35_DEV int unit_block(const PlanHead& h, int64_t u) {
@@ -137,12 +142,48 @@ Q35_DEV V plan_excl(V v, V* sh, V* total) {
   return before + x - v;
 }
 
-// Made by one block: the sequences' tiles, then each tile's first unit.
+// The fewest units of a block, from `least` on, with which `most` blocks are enough for all tiles (one a thread, of `units` for
+// each kv head) if each takes a part of one (tile, kv head) alone; 0 if none of the first 64 is.  Lane c of each wave tries
+// least + c over a quarter of the tiles.
+Q35_DEV int whole_units(int units, int tiles, int nkv, int least, int most) {
+  __shared__ int n[kT], sum[kT / 64][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  n[threadIdx.x] = units;
+  __syncthreads();
+  const int per = least + lane;
+  const float inv = 1.f / (float)per;
+  int blocks = 0;
+  for (int x = w; x < tiles; x += kT / 64) {
+    int k = (int)((float)n[x] * inv);  // (off by one at most: units and quotients are below 2^22)
+    k += (k + 1) * per <= n[x] ? 1 : k * per > n[x] ? -1 : 0;
+    blocks += k + (k * per < n[x] ? 1 : 0);
+  }
+  sum[w][lane] = blocks;
+  __syncthreads();
+  blocks = 0;
+#pragma unroll
+  for (int i = 0; i < kT / 64; ++i) blocks += sum[i][lane];
+  const unsigned long long fits = __ballot(blocks <= most / nkv);
+  return fits ? least + __builtin_ctzll(fits) : 0;
+}
+
+// Blocks take whole parts while the longest has at most kCutUnits more than an even share (both ways, us of a call: 40
+// tokens behind 2048 .. 4096, 16 and 17 units, 46.6 and 44.4; 12 x 5 behind 2730 .. 8191, 20 and 21, 53.8 and 51.2; 60 of one
+// token behind 8000, 59 and 63, 93 and 91; 33 behind 16000, 65 and 72, 94 and 96; 90 behind 4000, 45 and 63, 80 and 85).
+constexpr int kCutUnits = 4;
+constexpr int kWholeMost = 1 << 22;  // units (whole_units' quotients are estimated in f32)
+
+// Made by one block: the sequences' tiles, then each tile's first unit.  kWhole: "few" blocks may take whole parts.
+template <bool kWhole>
 Q35_DEV void make_plan(const AttnArgs& A) {
   const PagedAttn& a = A.c;
   __shared__ int si[kT / 64];
   __shared__ int64_t sl[kT / 64];
+  // (up to kT sequences stay in LDS: their tiles' search and a second look at them were trips through memory)
+  __shared__ int first[2][kT];
+  __shared__ Seq seqs[kT];
   const int tid = threadIdx.x;
+  const bool held = a.B <= kT;
   int count[2] = {0, 0};
   bool bad = false, falls = false;
   for (int b0 = 0; b0 < a.B; b0 += kT) {
@@ -153,12 +194,16 @@ Q35_DEV void make_plan(const AttnArgs& A) {
       if (load_seq(a, b, &s)) nt[kind_of(A, s.n)] = tiles_of(A, s.n);
       else bad = true;
       falls |= s.n < 0;
+      if (held) seqs[b] = s;
     }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       int all;
       const int t = plan_excl(nt[k], si, &all);
-      if (b < a.B) A.tile0[(int64_t)k * a.B + b] = count[k] + t;
+      if (b < a.B) {
+        if (held) first[k][b] = count[k] + t;
+        else A.tile0[(int64_t)k * a.B + b] = count[k] + t;
+      }
       count[k] += all;
     }
   }
@@ -168,8 +213,9 @@ Q35_DEV void make_plan(const AttnArgs& A) {
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int nt = min(count[k], A.max_tiles[k]);
-    const int32_t* tile0 = A.tile0 + (int64_t)k * a.B;
-    int64_t run = 0;
+    auto tile0 = [&](int b) { return held ? first[k][b] : A.tile0[(int64_t)k * a.B + b]; };
+    int64_t run = 0, laid = 0;
+    int whole = 0;
     for (int x0 = 0; x0 < nt; x0 += kT) {
       const int x = x0 + tid;
       Tile t = {0, 0, 0, 0, 0, 0, 0};
@@ -178,13 +224,14 @@ Q35_DEV void make_plan(const AttnArgs& A) {
         int lo = 0, hi = a.B;
         while (hi - lo > 1) {
           const int m = (lo + hi) / 2;
-          if (tile0[m] <= x) lo = m;
+          if (tile0(m) <= x) lo = m;
           else hi = m;
         }
         Seq s;
-        load_seq(a, lo, &s);
+        if (held) s = seqs[lo];
+        else load_seq(a, lo, &s);
         t.b = lo;
-        t.i = x - tile0[lo];
+        t.i = x - tile0(lo);
         t.units = (tile_len(A, s, t.i) + kUnit - 1) / kUnit;
         t.s0 = s.s0;
         t.n = s.n;
@@ -192,14 +239,24 @@ Q35_DEV void make_plan(const AttnArgs& A) {
       }
       int64_t all;
       t.u0 = run + plan_excl((int64_t)t.units * a.nkv, sl, &all);
-      if (x < nt) A.tiles[k][x] = t;
       run += all;
+      laid = run;
+      if (kWhole && k == 0 && nt <= kT && nt * a.nkv <= A.max_blocks[0] && run <= (int64_t)kWholeMost) {
+        const int even = (int)((run + A.max_blocks[0] - 1) / A.max_blocks[0]);
+        const int most = whole_units(t.units, nt, a.nkv, even, A.max_blocks[0]);
+        if (most && most <= even + kCutUnits) {
+          whole = most;
+          t.u0 = plan_excl((int64_t)laid_out(t.units, whole) * a.nkv, sl, &laid);
+        }
+      }
+      if (x < nt) A.tiles[k][x] = t;
     }
     if (tid == 0) {
       // (a "many" block takes four units at least: what it leaves to the join costs about one)
       const int64_t least = k ? 4 : 1, most = (run + least - 1) / least;
       const int64_t blocks = most < A.max_blocks[k] ? most : A.max_blocks[k];
-      A.head[k] = PlanHead{run, blocks ? run / blocks : 0, blocks ? (int)(run % blocks) : 0, nt, (int)blocks, 0};
+      A.head[k] = whole ? PlanHead{run, whole, 0, nt, (int)(laid / whole), whole}
+                        : PlanHead{run, blocks ? run / blocks : 0, blocks ? (int)(run % blocks) : 0, nt, (int)blocks, 0};
     }
   }
 }
@@ -373,7 +430,7 @@ __global__ __launch_bounds__(kT) void paged_append_kernel(const AttnArgs A) {
   const PagedAttn& a = A.c;
   __shared__ double xs[kT / 64][kHd];
   if (blockIdx.x < 2) {
-    if (blockIdx.x == 0) make_plan(A);
+    if (blockIdx.x == 0) make_plan<DT == Q35_Q4>(A);
     else count_once(A);
     return;
   }
@@ -511,6 +568,7 @@ struct Start {
   Tile t;
   int x;
 };
+template <bool kWhole>
 Q35_DEV bool block_start(const AttnArgs& A, int k, PlanHead* head, Start* sh) {
   const int x0 = threadIdx.x;
   Tile t;
@@ -520,7 +578,7 @@ Q35_DEV bool block_start(const AttnArgs& A, int k, PlanHead* head, Start* sh) {
   const int64_t u = block_u0(*head, blockIdx.x);
   for (int x = x0; x < head->tiles; x += blockDim.x) {
     if (x != x0) t = load_tile(&A.tiles[k][x]);
-    if (t.u0 <= u && u < t.u0 + (int64_t)t.units * A.c.nkv) {
+    if (t.u0 <= u && u < t.u0 + (int64_t)(kWhole ? laid_out(t.units, head->whole) : t.units) * A.c.nkv) {
       sh->t = t;
       sh->x = x;
     }
@@ -624,7 +682,8 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   for (int seg = 0; u < u_end; ++seg) {
     int gk = 0;
     int64_t off = u - t.u0;
-    for (; off >= t.units; off -= t.units) ++gk;
+    const int laid = k4 ? laid_out(t.units, H.whole) : t.units;
+    for (; off >= laid; off -= laid) ++gk;
     const int k0 = (int)off, k1 = (int)min((int64_t)t.units, k0 + (u_end - u));
     const int rows = min(kFewRows, t.n * A.rep - t.i * kFewRows);
     const int pr = t.i * kFewRows + min(n, rows - 1), tok = div_rep(A, pr), h = gk * A.rep + pr - tok * A.rep;
@@ -966,7 +1025,7 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
         }
       }
     }
-    u += k1 - k0;
+    u = k4 && H.whole ? u_end : u + (k1 - k0);
     if (u < u_end && u == t.u0 + (int64_t)t.units * a.nkv) t = uniform(load_tile(&A.tiles[0][++x]));
     __syncthreads();
   }
@@ -989,7 +1048,7 @@ __global__ __launch_bounds__(kT, 2) void paged_few_kernel(const AttnArgs A) {
   __shared__ Start sh;
   PlanHead H;
   const int64_t once = *A.once;
-  if (!block_start(A, 0, &H, &sh)) return;
+  if (!block_start<DT == Q35_Q4>(A, 0, &H, &sh)) return;
   if (past_llc<DT>(H, once)) few_run<DT, true>(A, H, sh, os, ms, ls);
   else few_run<DT, false>(A, H, sh, os, ms, ls);
 }
@@ -1059,7 +1118,7 @@ __global__ __launch_bounds__(kMT) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4, n32 = lane & 31, hf = lane >> 5;
   PlanHead H;
-  if (!block_start(A, 1, &H, &sh)) return;
+  if (!block_start<false>(A, 1, &H, &sh)) return;
   const int64_t u_begin = block_u0(H, blockIdx.x);
   int64_t u = u_begin;
   const int64_t u_end = block_u0(H, blockIdx.x + 1);

@@ -394,3 +394,17 @@ def test_pages_beyond_32bit_offsets():
     pool.data[1, -2:] = 0
     q35.pages_copy(pool, i32([0, 1]), i32([n - 2, n - 1]), check=True)
     assert torch.equal(pool.data[1, -2:], want)
+
+
+@pytest.mark.parametrize("heads,kv,seqs", [
+    (8, 2, [(5, 700 + 60 * i) for i in range(12)]),               # two tiles each; a block's share is a part of one
+    (8, 2, [(1, 3000 + 130 * (i % 9)) for i in range(20)]),
+    (4, 1, [(1, 31 + 32 * (i % 5)) for i in range(200)] + [(1, 9000)]),
+    (4, 2, [(1, (37 * i) % 211) for i in range(300)]),            # more tiles than blocks
+    (4, 1, [(1, (53 * i) % 150) for i in range(257)]),            # as many as a thread of the plan each, and one
+    (16, 1, [(2, 5000), (1, 70), (2, 1)]),
+    (4, 1, [(1, 1500 if i % 2 else 2) for i in range(180)]),      # whole parts come out too uneven
+])
+def test_division_of_the_work(heads, kv, seqs):
+    c = make(len(seqs), 64, heads, kv, seqs)
+    check(c, *run(c))
