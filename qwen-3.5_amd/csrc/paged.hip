@@ -661,6 +661,10 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   constexpr int kQ = kWide ? 1 : kHalf ? 2 : 3;  // parts of a query or weight
   constexpr int kW = kWide ? 2 : 1;                       // 16-byte words of 8 values
   constexpr int kH = kWide ? 1 : 2, kS = 16 * kH;          // keys of a wave's step
+  // how far (log2) a score may pass the running maximum before the sums are rescaled (64 multiplications; in most of the first
+  // steps some row has a new maximum): 4 bits' weights are f16 of 2^15 at most then (the kernel: 33 tokens over 400 MB 98.1 -> 95.6 us,
+  // 40 over 73 MB 26.7 -> 25.2).
+  constexpr float kSlack = k4 ? 3.f : 0.f;
   const PagedAttn& a = A.c;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
   int64_t u = uniform(block_u0(H, blockIdx.x));
@@ -671,8 +675,8 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   q35_u32x4* const qs = reinterpret_cast<q35_u32x4*>(os);  // [part][step][lane]
   const Nibbles nib = nibbles();
   bool bad = false;
-  // 4 bits: unpacking bounds (830 instructions for 32 tokens, 130 of them for each of and / or, subtracting z and multiplying by s;
-  // with s z taken off the sums instead, 100 fewer, more registers and no faster).  Of a SIMD's two waves the older one then goes first, and the
+  // 4 bits: unpacking bounds (of about 710 vector instructions for 32 tokens 128 for each of and / or, subtracting z and multiplying by
+  // s; with s z taken off the sums instead, 100 fewer, more registers and no faster).  Of a SIMD's two waves the older one then goes first, and the
   // younger ends alone; a wave that is further through its steps has a lower priority (33 tokens over 400 MB 118.7
   // -> 114.5 us of a call, 60 drafted tokens 56.0 -> 53.6).
   const int quarter = max(1, (int)((u_end - u) >> 4));  // of a wave's steps
@@ -865,14 +869,14 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
       }
       bm = max_x32(max_x16(bm));
       const float mn = fmaxf(m, bm);
-      if (__ballot(mn > m)) {
+      if (__ballot(mn > m + kSlack)) {
         const float al = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
         l *= al;
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] *= al;
         m = mn;
       }
-      // f16 weights are kept 2^12 times larger (at most 4096), so that their halves hold 22 bits down to 2^-26
+      // f16 weights are kept 2^12 times larger (at most 4096, or 2^kSlack times that), so that their halves hold 22 bits down to 2^-26
       const float mr = (m == -INFINITY ? 0.f : m) - (kHalf ? 12.f : 0.f);
       q35_u32x4 pw[kQ];
 #pragma unroll

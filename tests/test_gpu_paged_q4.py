@@ -408,3 +408,17 @@ def test_pages_beyond_32bit_offsets():
 def test_division_of_the_work(heads, kv, seqs):
     c = make(len(seqs), 64, heads, kv, seqs)
     check(c, *run(c))
+
+
+@pytest.mark.parametrize("rise", [0.05, 0.5, 0.55, 4.0, -0.5])
+def test_scores_that_rise_along_the_context(rise):
+    """The running maximum is passed by little or much in every step (a step of 128 tokens rises by 23 rise / 4 powers of two)."""
+    c = make(3, 64, 8, 2, [(1, 511), (3, 400)])
+    r = np.random.default_rng(8)
+    u = r.standard_normal(HD)
+    c["qg"].reshape(4, 8, 2, HD)[:, :, 0] = u
+    c["qw"][:], c["cos"][:], c["sin"][:] = 0.0, 1.0, 0.0
+    for b, (n, ctx) in enumerate([(1, 511), (3, 400)]):
+        for t in range(ctx):
+            c["pool"][0, c["table"][b][t // 64], 0, :, t % 64] = Q.pack(u * (rise * t / 512))
+    check(c, *run(c))
