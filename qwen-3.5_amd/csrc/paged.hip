@@ -142,36 +142,42 @@ Q35_DEV V plan_excl(V v, V* sh, V* total) {
   return before + x - v;
 }
 
-// The fewest units of a block, from `least` on, with which `most` blocks are enough for all tiles (one a thread, of `units` for
-// each kv head) if each takes a part of one (tile, kv head) alone; 0 if none of the first 64 is.  Lane c of each wave tries
-// least + c over a quarter of the tiles.
-Q35_DEV int whole_units(int units, int tiles, int nkv, int least, int most) {
-  __shared__ int n[kT], sum[kT / 64][64];
+// Blocks take whole parts while the longest has at most kCutUnits more than an even share (both ways, us of a call: 40
+// tokens behind 2048 .. 4096, 16 and 17 units, 46.6 and 44.4; 12 x 5 behind 2730 .. 8191, 20 and 21, 53.8 and 51.2; 60 of one
+// token behind 8000, 59 and 63, 93 and 91; 33 behind 16000, 65 and 72, 94 and 96; 90 behind 4000, 45 and 63, 80 and 85), times the
+// tiles that an even share may have parts of (two prompts of 500 tokens, 8 and 16, tiles of 1 to 16: 89 and 47).
+constexpr int kCutUnits = 4;
+constexpr int kWholeMost = 1 << 22;  // units (quotients are estimated in f32)
+// The units of a block if each of `most` blocks at most takes a part of one (tile, kv head) alone: the fewest from `even` on, the even
+// share, with which the blocks are enough for all tiles (one a thread, of `units` for each kv head); 0 if that is none of
+// the first 64, or too many.  Lane c of each wave tries even + c over a quarter of the tiles.
+Q35_DEV int whole_units(int units, int tiles, int nkv, int even, int most) {
+  __shared__ int n[kT], sum[kT / 64][64], least[kT / 64];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   n[threadIdx.x] = units;
   __syncthreads();
-  const int per = least + lane;
+  const int per = even + lane;
   const float inv = 1.f / (float)per;
-  int blocks = 0;
+  int blocks = 0, low = n[0];
   for (int x = w; x < tiles; x += kT / 64) {
     int k = (int)((float)n[x] * inv);  // (off by one at most: units and quotients are below 2^22)
     k += (k + 1) * per <= n[x] ? 1 : k * per > n[x] ? -1 : 0;
     blocks += k + (k * per < n[x] ? 1 : 0);
+    low = min(low, n[x]);
   }
   sum[w][lane] = blocks;
+  least[w] = low;
   __syncthreads();
   blocks = 0;
 #pragma unroll
-  for (int i = 0; i < kT / 64; ++i) blocks += sum[i][lane];
+  for (int i = 0; i < kT / 64; ++i) {
+    blocks += sum[i][lane];
+    low = min(low, least[i]);
+  }
   const unsigned long long fits = __ballot(blocks <= most / nkv);
-  return fits ? least + __builtin_ctzll(fits) : 0;
+  const int more = fits ? __builtin_ctzll(fits) : 64;
+  return more < 64 && more <= kCutUnits * max(1, even / low) ? even + more : 0;
 }
-
-// Blocks take whole parts while the longest has at most kCutUnits more than an even share (both ways, us of a call: 40
-// tokens behind 2048 .. 4096, 16 and 17 units, 46.6 and 44.4; 12 x 5 behind 2730 .. 8191, 20 and 21, 53.8 and 51.2; 60 of one
-// token behind 8000, 59 and 63, 93 and 91; 33 behind 16000, 65 and 72, 94 and 96; 90 behind 4000, 45 and 63, 80 and 85).
-constexpr int kCutUnits = 4;
-constexpr int kWholeMost = 1 << 22;  // units (whole_units' quotients are estimated in f32)
 
 // Made by one block: the sequences' tiles, then each tile's first unit.  kWhole: "few" blocks may take whole parts.
 template <bool kWhole>
@@ -243,9 +249,8 @@ Q35_DEV void make_plan(const AttnArgs& A) {
       laid = run;
       if (kWhole && k == 0 && nt <= kT && nt * a.nkv <= A.max_blocks[0] && run <= (int64_t)kWholeMost) {
         const int even = (int)((run + A.max_blocks[0] - 1) / A.max_blocks[0]);
-        const int most = whole_units(t.units, nt, a.nkv, even, A.max_blocks[0]);
-        if (most && most <= even + kCutUnits) {
-          whole = most;
+        whole = whole_units(t.units, nt, a.nkv, even, A.max_blocks[0]);
+        if (whole) {
           t.u0 = plan_excl((int64_t)laid_out(t.units, whole) * a.nkv, sl, &laid);
         }
       }
@@ -1577,9 +1582,9 @@ struct PagedLayout {
   size_t bytes;
 };
 // What all tiles of T rows, as "few", may go over if all are one sequence's: tiles, kv heads, tokens, bytes of a value.
-constexpr int64_t kReread = 300000;
+constexpr int64_t kReread = 300000, kReread4 = 350000;
 // ctx_bytes: tokens that a sequence can have, times the bytes of a value; INT64_MAX for the workspace of any call.
-PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
+PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes, bool k4) {
   PagedLayout L;
   const int rep = nh / nkv, tok_many = kManyRows / rep;
   auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
@@ -1592,12 +1597,16 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
   // 2000 and one of 64 behind 30000 would take 207 us, 133 so).  But a batch of fixed slots may be one chunk and
   // empty ones, so that holds only while the chunk's tiles could go over the longest context that the table
   // and the rotary rows allow as cheaply as a chunk does (kReread; both ways, us: 16 tokens behind 16000 in bf16 37
-  // and 37, in f32 54 and 40; 64 behind 2000 28 and 37, 36 and 40; 256 behind 16000 272 and 112, 572 and 134; in 4 bits
-  // 16 behind 60000 56 and 55, 64 behind 16000 56 and 56).
+  // and 37, in f32 54 and 40; 64 behind 2000 28 and 37, 36 and 40; 256 behind 16000 272 and 112, 572 and 134).
+  // Over 4 bits, where one chunk of all rows would cost no more in tiles, any batch of several sequences goes so that has as many
+  // tiles as blocks at most (both ways, us: 16 tokens behind 60000 in a padded batch 57 and 61, 64 behind 16000 51 and 60, 256
+  // behind 5000 64 and 65, 500 behind 2000 68 and 68, behind 2600 78 and 73; 48 behind 16000 beside 12 single ones 53 and 75;
+  // 10 prompts of 100 35 and 70, 20 of 200, 1000 tiles, 153 and 108).
   // One sequence: its rows decide, if all rows are its.
   L.few_most = std::max(1, 2 * kFewRows / rep);
   const int64_t tiles = ((int64_t)T * rep + kFewRows - 1) / kFewRows * nkv;
-  const bool few_only = T <= L.few_most || (T - B + 1 <= L.few_most && ctx_bytes <= kReread / tiles);
+  const bool cheap = ctx_bytes <= (k4 ? kReread4 : kReread) / tiles;
+  const bool few_only = T <= L.few_most || (cheap && (k4 ? B > 1 && tiles <= 2 * device_cus() : T - B + 1 <= L.few_most));
   const bool many_only = !few_only && B == 1;
   if (few_only) L.few_most = INT_MAX;
   if (many_only) L.few_most = 0;
@@ -1628,7 +1637,7 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes) {
 template <int DT>
 int launch(const PagedAttn& a, hipStream_t st) {
   const int64_t ctx = std::min<int64_t>((int64_t)a.ld_table * a.P.page, a.rope_rows);
-  const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B, ctx * row_bytes(a.P) / kHd);
+  const PagedLayout L = paged_layout(a.nh, a.nkv, a.T, a.B, ctx * row_bytes(a.P) / kHd, DT == Q35_Q4);
   AttnArgs A;
   A.c = a;
   A.page_shift = __builtin_ctz((unsigned)a.P.page);
@@ -1681,7 +1690,7 @@ int launch(const PagedAttn& a, hipStream_t st) {
 
 }  // namespace
 
-size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) { return paged_layout(nh, nkv, T, B, INT64_MAX).bytes; }
+size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) { return paged_layout(nh, nkv, T, B, INT64_MAX, false).bytes; }
 
 int paged_attn_launch(const PagedAttn& a, hipStream_t st) {
   switch (a.P.dtype) {

@@ -422,3 +422,26 @@ def test_scores_that_rise_along_the_context(rise):
         for t in range(ctx):
             c["pool"][0, c["table"][b][t // 64], 0, :, t % 64] = Q.pack(u * (rise * t / 512))
     check(c, *run(c))
+
+
+@pytest.mark.parametrize("page,heads,kv,seqs", [c for c in CASES if len(c[3]) > 1 and max(n for n, _ in c[3]) * c[1] // c[2] > 32])
+def test_chunks_beside_few_tokens(page, heads, kv, seqs):
+    """The same batches under tables and rotary rows for contexts so long that a chunk would not be taken for few tokens."""
+    T = sum(n for n, _ in seqs)
+    cap = 350000 * 16 // 9 // (-(-T * heads // kv // 16) * kv) + 2 * page
+    c = make(len(seqs) + T, page, heads, kv, seqs)
+    c["table"] = [row + [-1] * (cap // page + 1 - len(row)) for row in c["table"]]
+    c["cos"], c["sin"] = (np.concatenate([x, np.zeros((cap - len(x), x.shape[1]), np.float32)]) for x in (c["cos"], c["sin"]))
+    check(c, *run(c))
+
+
+@pytest.mark.parametrize("heads,kv,seqs", [
+    (8, 2, [(500, 0), (500, 0)]),                                 # as many tiles as blocks, of 1 to 16 units
+    (8, 2, [(500, 0), (510, 0)]),                                 # one more than blocks
+    (8, 2, [(31, 200)] * 8 + [(120, 3)]),
+    (16, 1, [(128, 0)] * 4),
+    (4, 4, [(64, 700), (33, 0), (1, 0)]),
+])
+def test_prompts_as_few_tokens(heads, kv, seqs):
+    c = make(sum(n for n, _ in seqs), 64, heads, kv, seqs)
+    check(c, *run(c))
