@@ -445,3 +445,15 @@ def test_chunks_beside_few_tokens(page, heads, kv, seqs):
 def test_prompts_as_few_tokens(heads, kv, seqs):
     c = make(sum(n for n, _ in seqs), 64, heads, kv, seqs)
     check(c, *run(c))
+
+
+@pytest.mark.parametrize("heads,kv,seqs", [
+    (8, 2, [(1, 9000), (0, 5)]),                                  # 71 parts of a step of each wave
+    (8, 2, [(1, 700), (1, 3), (1, 64), (1, 2000), (3, 2500)]),
+    (4, 4, [(2, 900)] * 3),
+    (16, 1, [(1, 4097)]),
+    (4, 1, [(1, 2)] * 500 + [(1, 5000)]),
+])
+def test_parts_of_a_tile(heads, kv, seqs):
+    c = make(len(seqs), 64, heads, kv, seqs)
+    check(c, *run(c))
