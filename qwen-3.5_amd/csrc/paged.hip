@@ -1600,15 +1600,15 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes, bool 
   // empty ones, so that holds only while the chunk's tiles could go over the longest context that the table
   // and the rotary rows allow as cheaply as a chunk does (kReread; both ways, us: 16 tokens behind 16000 in bf16 37
   // and 37, in f32 54 and 40; 64 behind 2000 28 and 37, 36 and 40; 256 behind 16000 272 and 112, 572 and 134).
-  // Over 4 bits, where one chunk of all rows would cost no more in tiles, any batch of several sequences goes so that has as many
-  // tiles as blocks at most (both ways, us: 16 tokens behind 60000 in a padded batch 57 and 61, 64 behind 16000 51 and 60, 256
-  // behind 5000 64 and 65, 500 behind 2000 68 and 68, behind 2600 78 and 73; 48 behind 16000 beside 12 single ones 53 and 75;
-  // 10 prompts of 100 35 and 70, 20 of 200, 1000 tiles, 153 and 108).
-  // One sequence: its rows decide, if all rows are its.
+  // Over 4 bits, where one chunk of all rows would cost no more in tiles, any batch goes so that has as many tiles as blocks at
+  // most (both ways, us: 16 tokens behind 60000 in a padded batch 57 and 61, 64 behind 16000 51 and 60, 256 behind 5000 64 and 65,
+  // 500 behind 2000 68 and 68, behind 2600 78 and 73; 48 behind 16000 beside 12 single ones 53 and 75; 10 prompts of 100 35 and
+  // 70, 20 of 200, 1000 tiles, 153 and 108; one of 64 20 and 49, of 500 40 and 66, 500 behind 1500 63 and 64).
+  // Else, one sequence: its rows decide, if all rows are its.
   L.few_most = std::max(1, 2 * kFewRows / rep);
   const int64_t tiles = ((int64_t)T * rep + kFewRows - 1) / kFewRows * nkv;
   const bool cheap = ctx_bytes <= (k4 ? kReread4 : kReread) / tiles;
-  const bool few_only = T <= L.few_most || (cheap && (k4 ? B > 1 && tiles <= 2 * device_cus() : T - B + 1 <= L.few_most));
+  const bool few_only = T <= L.few_most || (cheap && (k4 ? tiles <= 2 * device_cus() : T - B + 1 <= L.few_most));
   const bool many_only = !few_only && B == 1;
   if (few_only) L.few_most = INT_MAX;
   if (many_only) L.few_most = 0;
@@ -1692,7 +1692,10 @@ int launch(const PagedAttn& a, hipStream_t st) {
 
 }  // namespace
 
-size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) { return paged_layout(nh, nkv, T, B, INT64_MAX, false).bytes; }
+size_t paged_attn_ws_bytes(int nh, int nkv, int T, int B) {
+  // (for any type and context: one sequence may be a chunk or few tokens)
+  return std::max(paged_layout(nh, nkv, T, B, INT64_MAX, false).bytes, paged_layout(nh, nkv, T, B, 0, true).bytes);
+}
 
 int paged_attn_launch(const PagedAttn& a, hipStream_t st) {
   switch (a.P.dtype) {

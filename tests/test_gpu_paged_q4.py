@@ -424,9 +424,9 @@ def test_scores_that_rise_along_the_context(rise):
     check(c, *run(c))
 
 
-@pytest.mark.parametrize("page,heads,kv,seqs", [c for c in CASES if len(c[3]) > 1 and max(n for n, _ in c[3]) * c[1] // c[2] > 32])
+@pytest.mark.parametrize("page,heads,kv,seqs", [c for c in CASES if max(n for n, _ in c[3]) * c[1] // c[2] > 32])
 def test_chunks_beside_few_tokens(page, heads, kv, seqs):
-    """The same batches under tables and rotary rows for contexts so long that a chunk would not be taken for few tokens."""
+    """Batches under tables and rotary rows for contexts so long that a chunk is not taken for few tokens."""
     T = sum(n for n, _ in seqs)
     cap = 350000 * 16 // 9 // (-(-T * heads // kv // 16) * kv) + 2 * page
     c = make(len(seqs) + T, page, heads, kv, seqs)
@@ -441,6 +441,8 @@ def test_chunks_beside_few_tokens(page, heads, kv, seqs):
     (8, 2, [(31, 200)] * 8 + [(120, 3)]),
     (16, 1, [(128, 0)] * 4),
     (4, 4, [(64, 700), (33, 0), (1, 0)]),
+    (8, 2, [(1000, 20)]),
+    (16, 1, [(9, 400)]),
 ])
 def test_prompts_as_few_tokens(heads, kv, seqs):
     c = make(sum(n for n, _ in seqs), 64, heads, kv, seqs)
