@@ -324,14 +324,14 @@ def states_fork(states, parents, out=None, check=False):
     assert B > 0 and (out is not None or Bo <= B), (Bo, B)
     # src, dst, src_stride, dst_stride, row_bytes of every state (one by one in ctypes' fields took 40 us for 36 states)
     flat = []
-    for s, d in zip(states, dst):
-        assert s.size(0) == B, "states of different rows"
+    for i, s in enumerate(states):
+        assert s.shape[0] == B and s.get_device() == dev, "states of different rows, or on different devices"
         n, p = s.nbytes // B, s.data_ptr()
         ss = n if s.is_contiguous() else _row_stride(s, n)
-        assert s.get_device() == dev, "tensors on different devices"
-        if d is s:
+        if out is None:
             flat += (p, p, ss, ss, n)
         else:
+            d = dst[i]
             assert d.dtype is s.dtype and d.shape[1:] == s.shape[1:] and d.size(0) >= Bo, (tuple(s.shape), tuple(d.shape), Bo)
             assert d.get_device() == dev, "tensors on different devices"
             flat += (p, d.data_ptr(), ss, _row_stride(d, n), n)

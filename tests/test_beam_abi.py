@@ -87,3 +87,10 @@ def test_states_of_no_rows():
     assert q35.states_fork([none], parents, out=[two])[0] is two
     with pytest.raises(AssertionError):
         q35.states_fork([none], torch.full((2,), -1, dtype=torch.int32), out=[two])
+
+
+def test_states_given_as_their_own_outputs_have_the_rows():
+    """(More rows out than the tensors have would be written behind them.)"""
+    s = torch.zeros(3, 8)
+    with pytest.raises(AssertionError, match="3, 8"):
+        q35.states_fork([s], torch.zeros(4, dtype=torch.int32), out=[s])
