@@ -659,7 +659,8 @@ int q35_batch_generate(q35_batch* b, const int32_t* prompts_host, const int32_t*
  * which also takes its place in the history.  parent -1 leaves a row as it is; so does one outside [-1, B) or at another
  * position than row j (Q35_STATUS_ARG).  Token -1 (an empty row) gives token 0, and so does one outside the
  * vocabulary (Q35_STATUS_ARG).  A row whose prompt is not consumed takes its prompt's token all the same.  The rows
- * copied are those up to the largest position at the call, so a captured fork is of that position. */
+ * copied are those up to the largest position at the call, so a captured fork is of that position.  stream: that of the
+ * steps (NULL: the batch's own); parent and tokens are read there, some time after the call. */
 int q35_batch_fork(q35_batch* b, const int32_t* parent, uint32_t* status, void* stream);
 int q35_batch_set_tokens(q35_batch* b, const int32_t* tokens, uint32_t* status, void* stream);
 /* Host copy of the B positions. */

@@ -272,13 +272,19 @@ class BatchDecoder:
     def fork(self, parents, tokens=None, status=None, stream=None):
         """Row j goes on from row parents[j] (int32 [B] on the GPU, -1: from itself): states, caches, history; with tokens
         (int32 [B]) as the rows' next input.  A row takes parents at its own position only; status: an int32 tensor [1]
-        that is told what was refused."""
+        that is told what was refused.  stream: that of the steps and of the tensors.  None: the batch's own, which
+        torch's knows nothing of; the call then waits for the current stream before and for the device afterwards."""
+        import torch
         st = status.data_ptr() if status is not None else None
         for t in (parents, tokens):
             assert t is None or (t.shape == (self.B,) and t.is_cuda and t.is_contiguous() and str(t.dtype) == "torch.int32"), t
+        if stream is None:
+            torch.cuda.current_stream().synchronize()
         L.check(L.lib().q35_batch_fork(self.h, parents.data_ptr(), st, stream))
         if tokens is not None:
             L.check(L.lib().q35_batch_set_tokens(self.h, tokens.data_ptr(), st, stream))
+        if stream is None:
+            torch.cuda.synchronize()
 
     def beam_search(self, prompts, beams, n_new, stop_ids=(), length_penalty=0.0, mode="graph"):
         """Beam search from G = B / beams prompts (id sequences): per prompt the hypotheses (ids, score), best first, where
@@ -288,7 +294,7 @@ class BatchDecoder:
         import torch
         from .paged import beam_select
         G = len(prompts)
-        assert G * beams == self.B and n_new >= 1, (G, beams, self.B, n_new)
+        assert G * beams == self.B and 1 <= beams <= 64 and n_new >= 1, (G, beams, self.B, n_new)
         assert all(len(p) + n_new <= self.tmax + 1 for p in prompts), "tmax too small"
         self.reset()
         self.generate([p for p in prompts for _ in range(beams)], 0, mode=mode, prefill=True)

@@ -213,3 +213,31 @@ def test_operators_together():
     assert seqs == [h[1] for h in hyps]
     # 11 sums of f32 logits of size 10 from outputs that are a few 1e-6 apart (chunks and single tokens)
     np.testing.assert_allclose(r.scores.cpu().numpy(), sc, rtol=0, atol=2e-3)
+
+
+def test_forks_without_a_stream_wait_for_the_tensors():
+    """parents and tokens are written late on torch's stream, and overwritten after the call."""
+    d = hybrid_dims()
+    m = q35.TextForCausalLM(d, seed=4, tmax=40)
+    rng = np.random.default_rng(1)
+    bt = q35.BatchDecoder(m, 4, 30)
+    bt.generate([rng.integers(0, d.vocab, 5).astype(np.int32) for _ in range(4)], 0, prefill=True)
+    name = "layers.0.linear_attn.recurrent_state"
+    before = bt.tensor(name, np.float32).reshape(4, -1)
+    parents, tokens, want, ids = i32([0, 1, 2, 3]), i32([0] * 4), i32([3, 0, 0, 1]), i32([5, 6, 7, 8])
+    big = torch.randn(8192, 8192, device="cuda", dtype=torch.float16)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        big = (big @ big).clamp(-1, 1)
+    parents.copy_(want)
+    tokens.copy_(ids)
+    bt.fork(parents, tokens)
+    parents.zero_()
+    tokens.zero_()
+    torch.cuda.synchronize()
+    after = bt.tensor(name, np.float32).reshape(4, -1)
+    for j, p in enumerate([3, 0, 0, 1]):
+        np.testing.assert_array_equal(after[j], before[p])
+    assert bt.tensor("token", np.int32).tolist() == [5, 6, 7, 8]
+    bt.close()
+    m.close()
