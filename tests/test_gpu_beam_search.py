@@ -241,3 +241,15 @@ def test_forks_without_a_stream_wait_for_the_tensors():
     assert bt.tensor("token", np.int32).tolist() == [5, 6, 7, 8]
     bt.close()
     m.close()
+
+
+def test_searches_that_do_not_fit_are_refused():
+    m = q35.TextForCausalLM(hybrid_dims(), seed=4, tmax=40)
+    bt = q35.BatchDecoder(m, 66, 12)
+    for prompts, beams, n_new in (([[1]], 66, 2), ([[1], [2]], 32, 2), ([[1], [2]], 33, 0), ([[1, 2, 3], [2]], 33, 11)):
+        with pytest.raises(AssertionError):
+            bt.beam_search(prompts, beams, n_new)
+    got = bt.beam_search([[1, 2, 3], [2]], 33, 2)
+    assert [len(g) for g in got] == [33, 33] and all(len(ids) == 2 for g in got for ids, _ in g)
+    bt.close()
+    m.close()
