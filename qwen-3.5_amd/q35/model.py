@@ -227,7 +227,8 @@ def synth_model_tensor(dims, seed, name, n):
 
 class BatchDecoder:
     """B sequences decoded together with the weights of `model` (a TextForCausalLM), each with
-    its own caches, position and history (q35_batch_*)."""
+    its own caches, position and history (q35_batch_*).  stream: the handle of a stream; None or 0 (torch's default
+    stream has that handle): the batch's own, which is not ordered with any of torch's."""
 
     def __init__(self, model, B, tmax=None):
         self.model, self.B = model, int(B)
@@ -272,18 +273,19 @@ class BatchDecoder:
     def fork(self, parents, tokens=None, status=None, stream=None):
         """Row j goes on from row parents[j] (int32 [B] on the GPU, -1: from itself): states, caches, history; with tokens
         (int32 [B]) as the rows' next input.  A row takes parents at its own position only; status: an int32 tensor [1]
-        that is told what was refused.  stream: that of the steps and of the tensors.  None: the batch's own, which
-        torch's knows nothing of; the call then waits for the current stream before and for the device afterwards."""
+        that is told what was refused.  stream: that of the steps and of the tensors.  None or 0 (the handle of torch's
+        default stream): the batch's own, which torch's streams know nothing of; the call then waits for the current stream
+        before and for the device afterwards."""
         import torch
         st = status.data_ptr() if status is not None else None
         for t in (parents, tokens):
             assert t is None or (t.shape == (self.B,) and t.is_cuda and t.is_contiguous() and str(t.dtype) == "torch.int32"), t
-        if stream is None:
+        if not stream:
             torch.cuda.current_stream().synchronize()
         L.check(L.lib().q35_batch_fork(self.h, parents.data_ptr(), st, stream))
         if tokens is not None:
             L.check(L.lib().q35_batch_set_tokens(self.h, tokens.data_ptr(), st, stream))
-        if stream is None:
+        if not stream:
             torch.cuda.synchronize()
 
     def beam_search(self, prompts, beams, n_new, stop_ids=(), length_penalty=0.0, mode="graph"):
