@@ -651,9 +651,13 @@ int q35_batch_decode(q35_batch* b, int32_t n_steps, int32_t mode, void* stream);
  * then n_new batched steps.  decode_seconds_host (optional): wall time of the batched steps.
  * Returns Q35_E_RANGE when a norm statistic or gate sum of this or an earlier q35_batch_step /
  * _decode met a non-finite or out-of-range value (the batch state is then invalid until
- * q35_batch_reset). */
+ * q35_batch_reset), as q35_batch_check does. */
 int q35_batch_generate(q35_batch* b, const int32_t* prompts_host, const int32_t* lens_host, int32_t n_new,
                        int32_t* out_tokens_host, int32_t mode, double* decode_seconds_host, void* stream);
+/* Synchronises the stream and reports, once, what the steps since the last check met: Q35_E_RANGE for a norm statistic or
+ * gate sum that was not finite or out of range (the batch state is invalid until q35_batch_reset, which also forgets what was
+ * not told yet), Q35_E_SHAPE for an attention position outside the cache.  stream: that of the steps. */
+int q35_batch_check(q35_batch* b, void* stream);
 /* The next set of sequences of a beam search (parents and tokens as q35_beam_select gives them, int32 [B] on the device): row j's
  * states, caches and history become what row parent[j]'s were (q35_states_fork), and its next input token is tokens[j],
  * which also takes its place in the history.  parent -1 leaves a row as it is; so does one outside [-1, B) or at another

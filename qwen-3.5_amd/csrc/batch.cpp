@@ -689,6 +689,12 @@ int q35_batch_generate(q35_batch* b, const int32_t* prompts_host, const int32_t*
   return Q35_OK;
 }
 
+int q35_batch_check(q35_batch* b, void* stream) {
+  if (!b) return fail(Q35_E_ARG, "batch_check: null batch");
+  Q35_HIP_TRY(hipStreamSynchronize(bpick(b, stream)));
+  return bcheck(b);
+}
+
 int q35_batch_fork(q35_batch* b, const int32_t* parent, uint32_t* status, void* stream) {
   if (!b || !parent) return fail(Q35_E_ARG, "batch_fork: null pointer");
   try {

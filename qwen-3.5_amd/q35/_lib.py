@@ -143,6 +143,7 @@ PROTOTYPES = {
     "q35_batch_step": (ctypes.c_int, [c_vp, c_i32, c_vp]),
     "q35_batch_decode": (ctypes.c_int, [c_vp, c_i32, c_i32, c_vp]),
     "q35_batch_generate": (ctypes.c_int, [c_vp, c_vp, c_vp, c_i32, c_vp, c_i32, ctypes.POINTER(ctypes.c_double), c_vp]),
+    "q35_batch_check": (ctypes.c_int, [c_vp, c_vp]),
     "q35_batch_fork": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp]),
     "q35_batch_set_tokens": (ctypes.c_int, [c_vp, c_vp, c_vp, c_vp]),
     "q35_batch_position": (ctypes.c_int, [c_vp, c_vp]),

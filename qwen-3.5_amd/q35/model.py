@@ -270,6 +270,11 @@ class BatchDecoder:
                                            ctypes.byref(secs), stream))
         return out, secs.value
 
+    def check(self, stream=None):
+        """Synchronise and raise if a step since the last check met a value out of range (Q35_E_RANGE: the batch is invalid
+        until reset).  generate checks its own steps; step and decode do not.  stream: that of the steps."""
+        L.check(L.lib().q35_batch_check(self.h, stream))
+
     def fork(self, parents, tokens=None, status=None, stream=None):
         """Row j goes on from row parents[j] (int32 [B] on the GPU, -1: from itself): states, caches, history; with tokens
         (int32 [B]) as the rows' next input.  A row takes parents at its own position only; status: an int32 tensor [1]
@@ -292,7 +297,8 @@ class BatchDecoder:
         """Beam search from G = B / beams prompts (id sequences): per prompt the hypotheses (ids, score), best first, where
         score is the sum of the ids' log probabilities over (number of ids) ** length_penalty.  A hypothesis ends with the
         first of stop_ids or after n_new ids.  Every step: the batched decode step, beam_select over its logits, and the
-        fork of the rows' states, without a synchronisation (but every 16 steps, to end early, with stop ids)."""
+        fork of the rows' states, without a synchronisation (but every 16 steps, to end early, with stop ids).  A step that
+        met a value out of range raises Q35_E_RANGE at the end, as generate does."""
         import torch
         from .paged import beam_select
         G = len(prompts)
@@ -325,6 +331,7 @@ class BatchDecoder:
                     break
             hist = self._view("hist", (self.B, self.tmax), "<i4").cpu().numpy()
             ids, scores = ids.cpu().numpy(), scores.view(-1).cpu().numpy().astype(np.float64)
+            self.check(stream.cuda_stream)
             L.check(L.lib().q35_status_check(status.data_ptr(), stream.cuda_stream))
         out = []
         for g in range(G):

@@ -51,3 +51,7 @@ def test_forks_on_the_batchs_own_stream_wait(calls, batch, stream):
 def test_forks_on_a_stream_do_not_wait(calls, batch):
     batch.fork(Rows(3), Rows(3), stream=4096)
     assert calls == [("fork", 4096), ("tokens", 4096)]
+
+
+def test_check_of_no_batch():
+    assert L.lib().q35_batch_check(None, None) == L.Q35_E_ARG and b"batch_check" in L.lib().q35_last_error()
