@@ -283,8 +283,8 @@ class BatchDecoder:
         before and for the device afterwards."""
         import torch
         st = status.data_ptr() if status is not None else None
-        for t in (parents, tokens):
-            assert t is None or (t.shape == (self.B,) and t.is_cuda and t.is_contiguous() and str(t.dtype) == "torch.int32"), t
+        for t, n in ((parents, self.B), (tokens, self.B), (status, 1)):
+            assert t is None or (t.shape == (n,) and t.is_cuda and t.is_contiguous() and t.dtype is torch.int32), t
         if not stream:
             torch.cuda.current_stream().synchronize()
         L.check(L.lib().q35_batch_fork(self.h, parents.data_ptr(), st, stream))

@@ -55,3 +55,12 @@ def test_forks_on_a_stream_do_not_wait(calls, batch):
 
 def test_check_of_no_batch():
     assert L.lib().q35_batch_check(None, None) == L.Q35_E_ARG and b"batch_check" in L.lib().q35_last_error()
+
+
+@pytest.mark.parametrize("status", [Rows(1, torch.int64), Rows(1, torch.float32), Rows(1, is_cuda=False), Rows(0)])
+def test_status_words_that_a_kernel_must_not_write_are_refused(calls, batch, status):
+    with pytest.raises(AssertionError):
+        batch.fork(Rows(3), Rows(3), status)
+    assert calls == []
+    batch.fork(Rows(3), Rows(3), Rows(1))
+    assert len(calls) == 4
