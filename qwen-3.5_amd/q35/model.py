@@ -296,12 +296,12 @@ class BatchDecoder:
     def beam_search(self, prompts, beams, n_new, stop_ids=(), length_penalty=0.0, mode="graph"):
         """Beam search from G = B / beams prompts (id sequences): per prompt the hypotheses (ids, score), best first, where
         score is the sum of the ids' log probabilities over (number of ids) ** length_penalty.  A hypothesis ends with the
-        first of stop_ids or after n_new ids.  Every step: the batched decode step, beam_select over its logits, and the
+        first of stop_ids (any iterable) or after n_new ids.  Every step: the batched decode step, beam_select over its logits, and the
         fork of the rows' states, without a synchronisation (but every 16 steps, to end early, with stop ids).  A step that
         met a value out of range raises Q35_E_RANGE at the end, as generate does."""
         import torch
         from .paged import beam_select
-        G = len(prompts)
+        G, stop_ids = len(prompts), list(stop_ids)
         assert G * beams == self.B and 1 <= beams <= 64 and n_new >= 1, (G, beams, self.B, n_new)
         assert all(len(p) + n_new <= self.tmax + 1 for p in prompts), "tmax too small"
         self.reset()
@@ -313,7 +313,7 @@ class BatchDecoder:
             dev = logits.device
             scores = torch.full((G, beams), -float("inf"), device=dev)
             scores[:, 0] = 0.0
-            stops = torch.tensor(list(stop_ids), dtype=torch.int32, device=dev)
+            stops = torch.tensor(stop_ids, dtype=torch.int32, device=dev)
             ended = torch.full((self.B,), -1, dtype=torch.int32, device=dev)
             ids = torch.zeros(self.B, dtype=torch.int32, device=dev)  # of the hypothesis so far
             status = torch.zeros(1, dtype=torch.int32, device=dev)
@@ -327,7 +327,7 @@ class BatchDecoder:
                 over = (parents >= 0) & (ended[old] >= 0)
                 ids = torch.where(over, ids[old], i + 1)
                 ended = torch.where(over | ((parents >= 0) & torch.isin(tokens, stops)), tokens, -1)
-                if len(stop_ids) and i % 16 == 15 and bool(((ended >= 0) | (parents < 0)).all()):
+                if stop_ids and i % 16 == 15 and bool(((ended >= 0) | (parents < 0)).all()):
                     break
             hist = self._view("hist", (self.B, self.tmax), "<i4").cpu().numpy()
             ids, scores = ids.cpu().numpy(), scores.view(-1).cpu().numpy().astype(np.float64)
