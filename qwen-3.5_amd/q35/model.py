@@ -326,7 +326,8 @@ class BatchDecoder:
                 old = parents.clamp(min=0).long()
                 over = (parents >= 0) & (ended[old] >= 0)
                 ids = torch.where(over, ids[old], i + 1)
-                ended = torch.where(over | ((parents >= 0) & torch.isin(tokens, stops)), tokens, -1)
+                # (not torch.isin, which sorts where the ids are many, and waits for the device)
+                ended = torch.where(over | ((parents >= 0) & (tokens[:, None] == stops).any(1)), tokens, -1)
                 if stop_ids and i % 16 == 15 and bool(((ended >= 0) | (parents < 0)).all()):
                     break
             hist = self._view("hist", (self.B, self.tmax), "<i4").cpu().numpy()

@@ -1,4 +1,6 @@
-"""Stop ids of a beam search: any iterable."""
+"""Stop ids of a beam search: any iterable, any number of them."""
+import warnings
+
 import numpy as np
 import pytest
 import torch
@@ -36,3 +38,21 @@ def test_any_iterable(batch):
     for ids in (iter([stop, 8191]), (t for t in (stop, 8191)), {stop, 8191}, np.array([stop, 8191]), torch.tensor([stop, 8191]), (stop, 8191, stop)):
         same(batch.beam_search(PROMPTS, 3, 8, stop_ids=ids), want)
     same(batch.beam_search(PROMPTS, 3, 8, stop_ids=iter(())), free)
+
+
+@pytest.mark.parametrize("n", [1, 200])
+def test_steps_do_not_synchronise(batch, n):
+    """As many waits of the host for a search of 4 steps as for one of 12 (the end that stop ids bring is looked for after 16)."""
+    def waits(n_new):
+        with warnings.catch_warnings(record=True) as told:
+            warnings.simplefilter("always")
+            torch.cuda.set_sync_debug_mode("warn")
+            try:
+                batch.beam_search(PROMPTS, 3, n_new, stop_ids=range(4000, 4000 + n))
+            finally:
+                torch.cuda.set_sync_debug_mode("default")
+        return sum("called a synchronizing" in str(w.message) for w in told)
+
+    waits(1)  # (what is made once)
+    few = waits(4)
+    assert few > 0 and waits(12) == few
