@@ -453,7 +453,9 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
  * first of a group in its first step).  Logits of -inf are never chosen, nor is any of a row with a NaN or +inf.  Where a
  * group has fewer than k continuations the rest is score -inf, parent -1, token -1: an empty row of the next
  * tables, a dead beam of the next step.
- * Scores are formed in f64, from exponentials in f32 (an error of about 10^-8 in ln sum e^x), and rounded once.
+ * Scores are formed in f64, from exponentials and sums of 16 of them in f32, and rounded once.  ln sum e^x is off by a few
+ * 10^-8 where many tokens share the probability, by up to 7 10^-7 (2 10^-7 as measured) where one to three hold it, and not
+ * at all in a row of equal logits: continuations of two beams that lie nearer to each other may change places.
  * W <= 256, R W < 2^24, V <= 2^30; no output overlaps an input.  ws: q35_beam_select_ws_bytes bytes of scratch,
  * 16-byte aligned. */
 size_t q35_beam_select_ws_bytes(int32_t R, int32_t W, int32_t V, int32_t k);
