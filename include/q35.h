@@ -374,6 +374,9 @@ int q35_status_check(uint32_t* status, void* stream);
  * tile of tokens (128 rows of token and head) sees, or 2^-37 of the largest weight (2^-34 within 32 tokens
  * where values rise eightfold).  The keys' norms are formed in f64, so that what a 16-bit cache holds
  * does not hang on the order of a sum.
+ * Positions are the device's, so which kernels a call launches goes by T, B and the tokens that the table and the rotary rows have
+ * room for: a table for many more tokens than the sequences have costs time, over 4 bits most (10 prompts of 100 tokens: 31 us
+ * under a table of two pages of 64, 64 under one of 64 pages).
  * ws: q35_attention_paged_ws_bytes(d, T, B) bytes of scratch, 16-byte aligned (no zeroing needed). */
 size_t q35_attention_paged_ws_bytes(const q35_dims* d, int32_t T, int32_t B);
 int q35_attention_core_paged(const q35_dims* d, q35_pages pool, int32_t layer, const float* q_gate, int32_t ld_qg,
@@ -454,8 +457,9 @@ int q35_token_logprobs(const void* logits, int32_t dtype, int32_t M, int32_t V, 
  * group has fewer than k continuations the rest is score -inf, parent -1, token -1: an empty row of the next
  * tables, a dead beam of the next step.
  * Scores are formed in f64, from exponentials and sums of 16 of them in f32, and rounded once.  ln sum e^x is off by a few
- * 10^-8 where many tokens share the probability, by up to 7 10^-7 (2 10^-7 as measured) where one to three hold it, and not
- * at all in a row of equal logits: continuations of two beams that lie nearer to each other may change places.
+ * 10^-8 where many tokens share the probability (2 10^-7 if the logits rise through the row), by up to 7 10^-7 (2 10^-7 as
+ * measured) where one to three hold it, and not at all in a row of equal logits: continuations of two beams that lie nearer to
+ * each other may change places.
  * W <= 256, R W < 2^24, V <= 2^30; no output overlaps an input.  ws: q35_beam_select_ws_bytes bytes of scratch,
  * 16-byte aligned. */
 size_t q35_beam_select_ws_bytes(int32_t R, int32_t W, int32_t V, int32_t k);
@@ -665,7 +669,8 @@ int q35_batch_check(q35_batch* b, void* stream);
  * which also takes its place in the history.  parent -1 leaves a row as it is; so does one outside [-1, B) or at another
  * position than row j (Q35_STATUS_ARG).  Token -1 (an empty row) gives token 0, and so does one outside the
  * vocabulary (Q35_STATUS_ARG).  A row whose prompt is not consumed takes its prompt's token all the same.  The rows
- * copied are those up to the largest position at the call, so a captured fork is of that position.  stream: that of the
+ * copied are those up to the largest position at the call (a shared prompt's too: 8 rows of the 2B shape that all move, 0.1 ms at
+ * position 500, 0.7 at 8000), so a captured fork is of that position.  stream: that of the
  * steps (NULL: the batch's own); parent and tokens are read there, some time after the call. */
 int q35_batch_fork(q35_batch* b, const int32_t* parent, uint32_t* status, void* stream);
 int q35_batch_set_tokens(q35_batch* b, const int32_t* tokens, uint32_t* status, void* stream);

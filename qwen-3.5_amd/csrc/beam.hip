@@ -48,7 +48,7 @@ __host__ __device__ inline int split_live(int n, int most) {
   return want < 1 ? 1 : want < most ? want : most;
 }
 // The same for the live rows that the device has counted: where a chunk per wave would still fill the chip with more than two
-// blocks a CU, two chunks leave half as many lists to join (16 first steps of 8 beams 27.7 -> 25.5 us).
+// blocks a CU, two chunks leave half as many lists to join (16 first steps of 8 beams 22.2 -> 20.6 us of a call among others).
 Q35_DEV int split_counted(int n, int most) {
   const int ns = split_live(n, most);
   return ns == most && n * most > kBlocks / 2 ? (most + 1) / 2 : ns;
@@ -92,8 +92,9 @@ Q35_DEV uint4 ldg16_any(const void* p) {
   return make_uint4(v.x, v.y, v.z, v.w);
 }
 
-// Blocks (row, part).  Bound by the stream for many rows (236 live rows of 248320 f32 values 52 us, 4.5 TB/s, the lists' first
-// chunks and the blocks' ends beside it), by round trips for few (4 rows 8.5 us).
+// Blocks (row, part).  Bound by the stream for many rows (236 live rows of 248320 f32 values 53 us, 4.4 TB/s, the lists' first
+// chunks and the blocks' ends beside it; in 16 bits as long, 256 rows 62 and 64 us of a call: the vector work per value), by round trips
+// for few (4 rows 8.6 us).
 template <int DT>
 __global__ __launch_bounds__(kT) void beam_score_kernel(const BeamArgs a) {
   const BeamCall& c = a.c;
@@ -109,8 +110,10 @@ __global__ __launch_bounds__(kT) void beam_score_kernel(const BeamArgs a) {
     row_i = blockIdx.x / ns;
     if (beam_state(c, row_i) != kLive) return;
   } else {
-    // Dead and ended rows leave their blocks to the others (a first step has one live beam of each group: 16 of 128 rows
-    // of 248320 f16 values 27 us in blocks of their own rows, 13.0 so).
+    // Dead and ended rows leave their blocks to the others (a first step has one live beam of each group, calls, us: 16 of 128 rows
+    // of 248320 f16 values 35 in blocks of their own rows, 20.6 so; 100 of 800 of 50257 45 and 25; 250 of 2000 of 32000 57 and 28; 1024 of
+    // 4096 84 and 52).  Where all rows live, each block's look at all of them is lost: 256 rows 60.5 and 62.2, 800 46.7 and 48.9, 2000
+    // 58 and 66, 4096 85 and 116.
     __shared__ uint16_t live[kLiveMax];
     __shared__ int count[kNW];
     const int M = c.R * c.W;
@@ -285,7 +288,7 @@ Q35_DEV uint32_t nth_largest(const uint32_t (&v)[kListsLane], int r) {
 // put into LDS, and each one's place is the number of those ahead of it.  Where many are equal and more are left than LDS
 // takes, the waves keep sorted lists instead.
 // Bound by round trips (live rows; sums and lists) and short serial steps: 11 us for 32 groups of 8 beams, with sorted
-// lists only 14.6; 6.9 for one group of 4.
+// lists only 14.6; 6.6 for one group of 4.
 __global__ __launch_bounds__(kJoinWaves * 64) void beam_join_kernel(const BeamArgs a) {
   const BeamCall& c = a.c;
   __shared__ double off[kMaxBeams];

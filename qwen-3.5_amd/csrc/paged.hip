@@ -142,10 +142,10 @@ Q35_DEV V plan_excl(V v, V* sh, V* total) {
   return before + x - v;
 }
 
-// Blocks take whole parts while the longest has at most kCutUnits more than an even share (both ways, us of a call: 40
-// tokens behind 2048 .. 4096, 16 and 17 units, 46.6 and 44.4; 12 x 5 behind 2730 .. 8191, 20 and 21, 53.8 and 51.2; 60 of one
-// token behind 8000, 59 and 63, 93 and 91; 33 behind 16000, 65 and 72, 94 and 96; 90 behind 4000, 45 and 63, 80 and 85), times the
-// tiles that an even share may have parts of (two prompts of 500 tokens, 8 and 16, tiles of 1 to 16: 89 and 47).
+// Blocks take whole parts while the longest has at most kCutUnits more than an even share (both ways, us of a call among others: 40
+// tokens behind 2048 .. 4096, 16 and 17 units, 37.0 and 35.2; 12 x 5 behind 2730 .. 8191, 20 and 21, 39.5 and 37.6; 60 of one
+// token behind 8000, 59 and 63, 76 and 76; 33 behind 16000, 65 and 72, 78.8 and 79.8; 90 behind 4000, 45 and 63, 60.5 and 70.5), times the
+// tiles that an even share may have parts of (two prompts of 500 tokens, 8 and 16, tiles of 1 to 16: 83 and 40).
 constexpr int kCutUnits = 4;
 constexpr int kWholeMost = 1 << 22;  // units (quotients are estimated in f32)
 // The units of a block if each of `most` blocks at most takes a part of one (tile, kv head) alone: the fewest from `even` on, the even
@@ -249,7 +249,7 @@ Q35_DEV void make_plan(const AttnArgs& A) {
       laid = run;
       if (kWhole && k == 0 && nt <= kT && nt * a.nkv <= A.max_blocks[0] && run <= (int64_t)kWholeMost) {
         // (a step of each wave at least: it takes as long as one wave's, and there are fewer parts to join: one token behind 8000
-        // 27.0 -> 21.9 us of a call, 100 x 2 tokens behind 120 30.3 -> 23.2)
+        // 21.9 -> 16.8 us of a call, 100 x 2 tokens behind 120 24.8 -> 18.0)
         const int even = max(kT / 64, (int)((run + A.max_blocks[0] - 1) / A.max_blocks[0]));
         whole = whole_units(t.units, nt, a.nkv, even, A.max_blocks[0]);
         if (whole) {
@@ -669,8 +669,8 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   constexpr int kW = kWide ? 2 : 1;                       // 16-byte words of 8 values
   constexpr int kH = kWide ? 1 : 2, kS = 16 * kH;          // keys of a wave's step
   // how far (log2) a score may pass the running maximum before the sums are rescaled (64 multiplications; in most of the first
-  // steps some row has a new maximum): 4 bits' weights are f16 of 2^15 at most then (the kernel: 33 tokens over 400 MB 98.1 -> 95.6 us,
-  // 40 over 73 MB 26.7 -> 25.2).
+  // steps some row has a new maximum): 4 bits' weights are f16 of 2^15 at most then (calls, us: 33 tokens behind 16000 80.1 -> 78.3,
+  // 60 behind 8000 77.2 -> 75.5, 40 behind 2048 .. 4096 36.0 -> 35.2).
   constexpr float kSlack = k4 ? 3.f : 0.f;
   const PagedAttn& a = A.c;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6), n = lane & 15, g = lane >> 4;
@@ -684,8 +684,8 @@ Q35_DEV void few_run(const AttnArgs& A, const PlanHead& H, const Start& sh, floa
   bool bad = false;
   // 4 bits: unpacking bounds (of about 710 vector instructions for 32 tokens 128 for each of and / or, subtracting z and multiplying by
   // s; with s z taken off the sums instead, 100 fewer, more registers and no faster).  Of a SIMD's two waves the older one then goes first, and the
-  // younger ends alone; a wave that is further through its steps has a lower priority (33 tokens over 400 MB 118.7
-  // -> 114.5 us of a call, 60 drafted tokens 56.0 -> 53.6).
+  // younger ends alone; a wave that is further through its steps has a lower priority (calls, us: 33 tokens behind 16000 80.9 ->
+  // 78.3, behind 20000 96.2 -> 94.3; short streams as they were).
   const int quarter = max(1, (int)((u_end - u) >> 4));  // of a wave's steps
   int left = 4 * quarter;
   if constexpr (k4) __builtin_amdgcn_s_setprio(3);
@@ -1601,9 +1601,10 @@ PagedLayout paged_layout(int nh, int nkv, int T, int B, int64_t ctx_bytes, bool 
   // and the rotary rows allow as cheaply as a chunk does (kReread; both ways, us: 16 tokens behind 16000 in bf16 37
   // and 37, in f32 54 and 40; 64 behind 2000 28 and 37, 36 and 40; 256 behind 16000 272 and 112, 572 and 134).
   // Over 4 bits, where one chunk of all rows would cost no more in tiles, any batch goes so that has as many tiles as blocks at
-  // most (both ways, us: 16 tokens behind 60000 in a padded batch 57 and 61, 64 behind 16000 51 and 60, 256 behind 5000 64 and 65,
-  // 500 behind 2000 68 and 68, behind 2600 78 and 73; 48 behind 16000 beside 12 single ones 53 and 75; 10 prompts of 100 35 and
-  // 70, 20 of 200, 1000 tiles, 153 and 108; one of 64 20 and 49, of 500 40 and 66, 500 behind 1500 63 and 64).
+  // most (both ways, us: 16 tokens behind 60000 in a padded batch 48 and 53, 64 behind 16000 46 and 54, 256 behind 5000 60 and 60,
+  // 500 behind 2000 63 and 63, behind 2600 73 and 69; 48 behind 16000 beside 12 single ones 49 and 70; 10 prompts of 100 31 and
+  // 64, 20 of 200, 1000 tiles, 148 and 102; one of 64 16 and 45, of 500 35 and 63, 500 behind 1500 57 and 57).  What counts is what
+  // the table and the rotary rows could hold: under ones for 4096 tokens 10 prompts of 100 take 64, for 32768 one of 64 takes 45.
   // Else, one sequence: its rows decide, if all rows are its.
   L.few_most = std::max(1, 2 * kFewRows / rep);
   const int64_t tiles = ((int64_t)T * rep + kFewRows - 1) / kFewRows * nkv;

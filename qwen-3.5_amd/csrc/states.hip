@@ -43,8 +43,8 @@ struct Word<1> {
 };
 
 // All blocks find the rows that change, then take the slabs of all states in turn.  Bound by HBM: 1.13 GB read and written
-// in 225 us, 5.0 TB/s, a large copy's rate (through the caches 237 us; with half the words per thread, slabs of 512
-// bytes a row, 337); 8 rows of 20 MB 13 us, 4 of 0.8 MB 6.5 us (launch, parents, a slab).
+// in 220 us, 5.1 TB/s, a large copy's rate (through the caches 12 more; with half the words per thread, slabs of 512
+// bytes a row, half as long again); 8 rows of 20 MB 13 us, 4 of 0.8 MB 6.7 us (launch, parents, a slab).  Into other tensors 5.7 TB/s.
 template <int kW>
 __global__ __launch_bounds__(kT) void states_fork_kernel(const StatesArgs a) {
   typedef typename Word<kW>::M M;

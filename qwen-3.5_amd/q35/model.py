@@ -296,9 +296,10 @@ class BatchDecoder:
     def beam_search(self, prompts, beams, n_new, stop_ids=(), length_penalty=0.0, mode="graph"):
         """Beam search from G = B / beams prompts (id sequences): per prompt the hypotheses (ids, score), best first, where
         score is the sum of the ids' log probabilities over (number of ids) ** length_penalty.  A hypothesis ends with the
-        first of stop_ids (any iterable) or after n_new ids.  Every step: the batched decode step, beam_select over its logits, and the
-        fork of the rows' states, without a synchronisation (but every 16 steps, to end early, with stop ids).  A step that
-        met a value out of range raises Q35_E_RANGE at the end, as generate does."""
+        first of stop_ids (any iterable) or after n_new ids.  The batch's sequences are reset first and are the search's
+        afterwards; every row of a group runs through its prompt.  Every step: the batched decode step, beam_select over its
+        logits, and the fork of the rows' states, without a synchronisation (but every 16 steps, to end early, with stop ids).
+        A step that met a value out of range raises Q35_E_RANGE at the end, as generate does."""
         import torch
         from .paged import beam_select
         G, stop_ids = len(prompts), list(stop_ids)

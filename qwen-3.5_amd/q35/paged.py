@@ -123,7 +123,8 @@ def attention_core_paged(dims, pool, layer, q_gate, k_new, v_new, seq_start, pos
     sequences: rows seq_start[b] .. seq_start[b+1]-1 (int32 [B+1]) are sequence b's, at positions pos[b] ..
     (int32 [B]: tokens cached before); table int32 [B, entries].  q_gate [T, heads*512]; k_new / v_new
     [T, kv_heads*256]; rotary tables [rows, rot_dim]; returns [T, heads*256] (rows of no sequence are left
-    as they are in `out`).  check=True synchronises and raises as PagePool.check does."""
+    as they are in `out`).  The kernels are chosen by what `table` and the rotary tables have room for: give those of the longest
+    sequence, not of the longest possible, where that is known.  check=True synchronises and raises as PagePool.check does."""
     T, B = q_gate.shape[0], pos.shape[0]
     H, KV, hd, rot, f32 = dims.attn_heads, dims.kv_heads, dims.head_dim, dims.rot_dim, torch.float32
     assert q_gate.dtype is k_new.dtype is v_new.dtype is f32, (q_gate.dtype, k_new.dtype, v_new.dtype)
